@@ -111,6 +111,10 @@ const char *gphq_error_string(int status) {
         return "qwen3: empty calibration set";
     case GPHQ_ERR_CALIBRATION_SHAPE:
         return "qwen3: calibration sequences take 1 to 256 tokens each and 4096 in all";
+    case GPHQ_ERR_PAGED_SHAPE:
+        return "gphq: sizes, strides or alignment of the paged cache, batch or buffers do not fit";
+    case GPHQ_ERR_PAGED_BATCH:
+        return "gphq: a sequence, page number or position of the batch is out of bounds";
     }
     return "gphq: unknown status";
 }

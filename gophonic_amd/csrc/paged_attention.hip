@@ -1,0 +1,221 @@
+// gphq_paged_attention: argument checks, the cut of a batch into tiles and splits, and the
+// join of split results. Kernels: paged_rows.hip and paged_chunk.hip.
+#include "paged_attention.h"
+
+namespace gphq {
+
+int paged_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, PagedPool &pool, PagedBatch &batch) {
+    if (!kv || !b) return GPHQ_ERR_PAGED_SHAPE;
+    if (kv->dtype != GPHQ_DTYPE_F32 && kv->dtype != GPHQ_DTYPE_F16 && kv->dtype != GPHQ_DTYPE_BF16)
+        return GPHQ_ERR_UNSUPPORTED;
+    if (kv->head_dim != 64 && kv->head_dim != 128) return GPHQ_ERR_UNSUPPORTED;
+    if (kv->page_tokens < 16 || kv->page_tokens > GPHQ_PAGED_MAX_PAGE_TOKENS ||
+        (kv->page_tokens & (kv->page_tokens - 1)))
+        return GPHQ_ERR_UNSUPPORTED;
+    if (kv->pages < 1 || kv->pages > INT32_MAX || kv->kv_heads < 1 || kv->kv_heads > GPHQ_PAGED_MAX_HEADS)
+        return GPHQ_ERR_PAGED_SHAPE;
+    const int64_t size = kv->dtype == GPHQ_DTYPE_F32 ? 4 : 2, unit = 16 / size;
+    for (const int64_t s : {kv->page_stride, kv->token_stride, kv->head_stride})
+        if (s < kv->head_dim || s % unit || s > INT64_MAX / (size * kv->pages)) return GPHQ_ERR_PAGED_SHAPE;
+    if (!kv->k_dev || !kv->v_dev || (uintptr_t)kv->k_dev % 16 || (uintptr_t)kv->v_dev % 16)
+        return GPHQ_ERR_PAGED_SHAPE;
+    if (b->seqs < 0 || b->seqs > GPHQ_PAGED_MAX_SEQS || b->rows < 0 || b->rows > GPHQ_PAGED_MAX_ROWS ||
+        b->max_rows < 0 || b->max_len < 0 || b->max_len > GPHQ_PAGED_MAX_LEN || b->table_stride < 0)
+        return GPHQ_ERR_PAGED_SHAPE;
+    if (b->table_stride < (b->max_len + kv->page_tokens - 1) / kv->page_tokens || b->table_stride > INT32_MAX)
+        return GPHQ_ERR_PAGED_SHAPE;
+    if (b->seqs && (!b->starts_dev || !b->lens_dev || (b->table_stride && !b->table_dev))) return GPHQ_ERR_PAGED_SHAPE;
+    if (((uintptr_t)b->starts_dev | (uintptr_t)b->lens_dev | (uintptr_t)b->table_dev | (uintptr_t)b->bad_dev) % 4)
+        return GPHQ_ERR_PAGED_SHAPE;
+    pool = PagedPool{kv->k_dev,       kv->v_dev,
+                     kv->page_stride, kv->token_stride,
+                     kv->head_stride, (int)kv->pages,
+                     __builtin_ctzll((uint64_t)kv->page_tokens), (int)kv->kv_heads};
+    batch = PagedBatch{b->starts_dev, b->lens_dev,  b->table_dev, b->bad_dev,
+                       b->table_stride, (int)b->seqs, (int)b->rows, (int)std::min(b->max_rows, b->rows),
+                       (int)b->max_len};
+    if (batch.seqs == 0 || batch.max_rows == 0) batch.rows = 0;  // nothing to do
+    return GPHQ_OK;
+}
+
+namespace {
+
+// How a call is cut: which kernels run, over how many tiles and splits.
+struct AttnPlan {
+    int small_cols, small_tiles, small_splits, small_len;  // small_tiles per sequence; 0: the row kernel is not run
+    int big_tiles, big_splits, big_len;                    // big_tiles in all; 0: the chunk kernel is not run
+    int parts;
+};
+
+// Keys per split of `span` keys and how many splits that makes, for about `want` of them.
+void cut(int64_t span, int64_t want, int &len, int &splits) {
+    const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);
+    const int64_t n = std::min(std::max<int64_t>(want, 1), steps);
+    len = (int)((steps + n - 1) / n * 128);
+    splits = (int)((span + len - 1) / len);
+    if (splits < 1) splits = 1;
+}
+
+// From host numbers alone, so a captured call keeps its cut whatever the lengths become.
+AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window) {
+    AttnPlan p{};
+    const int64_t cus = device_cus(), rows = b.rows, cols = (int64_t)b.max_rows * group;
+    // Sequences of up to 32 columns run in the row kernel, in tiles of 16; a call of one
+    // sequence runs in one kernel only.
+    p.small_cols = cols > 32 && b.seqs == 1 ? 0 : 32;
+    auto span = [&](int64_t tile) {  // keys a tile of that many columns may see, from a multiple of 32
+        return window > 0 ? std::min<int64_t>(b.max_len, (int64_t)window + tile / group + 33) : (int64_t)b.max_len;
+    };
+    if (p.small_cols) {
+        p.small_tiles = (int)((std::min<int64_t>(cols, p.small_cols) + kSmallTile - 1) / kSmallTile);
+        const int64_t units = std::min<int64_t>(b.seqs, rows) * p.small_tiles * kv_heads;
+        cut(span(kSmallTile), (2 * cus + units - 1) / units, p.small_len, p.small_splits);
+    }
+    if (cols > p.small_cols) {
+        const int64_t all = rows * group;
+        p.big_tiles = (int)(all / kBigTile + std::min<int64_t>(b.seqs, all / (p.small_cols + 1)));
+        const int64_t units = (int64_t)p.big_tiles * kv_heads;
+        cut(span(kBigTile), units >= cus ? 1 : (2 * cus + units - 1) / units, p.big_len, p.big_splits);
+    }
+    p.parts = std::max(p.small_tiles ? p.small_splits : 1, p.big_tiles ? p.big_splits : 1);
+    return p;
+}
+
+int64_t work_bytes_of(const AttnPlan &p, int64_t rows, int64_t heads, int64_t hd) {
+    return p.parts > 1 ? rows * heads * p.parts * (hd + 2) * 4 : 0;
+}
+
+// Adds the split results of one (row, head) per wavefront, in the splits' order:
+// o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, M = max m_i. Rows whose tile had one
+// split were written by the tile itself.
+template <typename RT, int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
+    constexpr int E = HD / 64;
+    const int lane = threadIdx.x & 63;
+    const int unit = uniform((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const int row = unit / a.heads, head = unit - row * a.heads;
+    if (row >= a.b.rows) return;
+    const SeqRow s = find_seq(a.b, row);
+    if (row < s.start || row >= s.end || !seq_ok(a.b, s.start, s.end, s.len)) return;
+    const int n = s.end - s.start, i = row - s.start, cols = n * a.group;
+    const bool small = cols <= a.small_cols;
+    const int tm = small ? kSmallTile : kBigTile, c0 = (i * a.group + head % a.group) / tm * tm;
+    const TileKeys k = tile_keys(n, s.len, c0 / a.group, min((c0 + tm - 1) / a.group, n - 1), a.window);
+    const int splits = tile_splits(k, small ? a.split_small : a.split_big);
+    if (splits == 1) return;
+    const int64_t at = (int64_t)unit * a.parts;
+    float M = -INFINITY;
+    for (int j = lane; j < splits; j += 64) M = fmaxf(M, a.part_ml[2 * (at + j)]);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d));
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f, o[E] = {};
+    for (int j0 = 0; j0 < splits; j0 += 64) {
+        const int j = min(j0 + lane, splits - 1);
+        const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + j)] - ref), l = a.part_ml[2 * (at + j) + 1];
+        const int m = min(64, splits - j0);
+#pragma unroll 4
+        for (int u = 0; u < m; ++u) {
+            const float wu = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), u));
+            const float lu = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), u));
+            float v[E];
+            load_vec(a.part_o + (at + j0 + u) * HD + E * lane, v);
+            L += wu * lu;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += wu * v[e];
+        }
+    }
+    const bool empty = s.len - n + i < 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = empty ? 0.0f : o[e] / L;
+    store_vec((RT *)a.out + (int64_t)row * a.out_stride + head * HD + E * lane, o);
+}
+
+template <typename RT, typename CT>
+int attend(const AttnArgs &a, const AttnPlan &p, int hd, hipStream_t st) {
+    if (p.big_tiles) GPHQ_TRY((attn_chunk_launch<RT, CT>(a, hd, p.big_splits, p.big_tiles, st)));
+    if (p.small_tiles) GPHQ_TRY((attn_rows_launch<RT, CT>(a, hd, p.small_splits, p.small_tiles, st)));
+    if (p.parts == 1) return GPHQ_OK;
+    const unsigned blocks = (unsigned)(((int64_t)a.b.rows * a.heads + 3) / 4);
+    if (hd == 128)
+        hipLaunchKernelGGL((paged_join_kernel<RT, 128>), dim3(blocks), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((paged_join_kernel<RT, 64>), dim3(blocks), dim3(256), 0, st, a);
+    return launch_status();
+}
+
+// The checks that the attention and its workspace size share.
+int attn_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, int row_dtype, int64_t heads, int64_t window,
+              AttnArgs &a) {
+    GPHQ_TRY(paged_args(kv, b, a.pool, a.b));
+    if (row_dtype != GPHQ_DTYPE_F32 && row_dtype != kv->dtype) return GPHQ_ERR_UNSUPPORTED;
+    if (heads < 1 || heads > GPHQ_PAGED_MAX_HEADS || heads % kv->kv_heads || window < 0) return GPHQ_ERR_PAGED_SHAPE;
+    a.heads = (int)heads;
+    a.group = (int)(heads / kv->kv_heads);
+    a.window = window >= b->max_len ? 0 : (int)window;  // a window as long as any sequence hides nothing
+    return GPHQ_OK;
+}
+
+}  // namespace
+}  // namespace gphq
+
+using namespace gphq;
+
+extern "C" {
+
+int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype,
+                                             int64_t heads, int64_t window) {
+    AttnArgs a{};
+    GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
+    if (a.b.rows == 0) return 0;
+    return work_bytes_of(attn_plan(a.b, a.pool.kv_heads, a.group, a.window), a.b.rows, heads, kv->head_dim);
+}
+
+int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
+                         int64_t q_stride, int64_t heads, double scale, int64_t window, void *out, int64_t out_stride,
+                         void *work, int64_t work_bytes, void *stream) {
+    AttnArgs a{};
+    GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
+    const int64_t hd = kv->head_dim, size = row_dtype == GPHQ_DTYPE_F32 ? 4 : 2;
+    if (q_stride < heads * hd || out_stride < heads * hd || q_stride * size % 16 || out_stride * size % 16)
+        return GPHQ_ERR_PAGED_SHAPE;
+    if (a.b.rows == 0) return GPHQ_OK;
+    if (!q || !out || ((uintptr_t)q | (uintptr_t)out) % 16) return GPHQ_ERR_PAGED_SHAPE;
+    if (spans_overlap(q, span_bytes(a.b.rows, q_stride, heads * hd, size), out,
+                      span_bytes(a.b.rows, out_stride, heads * hd, size)))
+        return GPHQ_ERR_OVERLAP;
+    const AttnPlan p = attn_plan(a.b, a.pool.kv_heads, a.group, a.window);
+    if (p.parts > 1 && (!work || (uintptr_t)work % 16 || work_bytes < work_bytes_of(p, a.b.rows, heads, hd)))
+        return GPHQ_ERR_PAGED_SHAPE;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.parts = p.parts;
+    a.part_o = (float *)work;
+    a.part_ml = (float *)work + (int64_t)a.b.rows * heads * p.parts * hd;
+    a.small_cols = p.small_cols;
+    a.split_small = p.small_len;
+    a.split_big = p.big_len;
+    a.scale_log2 = (float)(scale * 1.4426950408889634);
+    hipStream_t st = (hipStream_t)stream;
+    if (row_dtype == GPHQ_DTYPE_F32) {
+        if (kv->dtype == GPHQ_DTYPE_F32) return attend<float, float>(a, p, (int)hd, st);
+        if (kv->dtype == GPHQ_DTYPE_F16) return attend<float, f16>(a, p, (int)hd, st);
+        return attend<float, bf16>(a, p, (int)hd, st);
+    }
+    if (kv->dtype == GPHQ_DTYPE_F16) return attend<f16, f16>(a, p, (int)hd, st);
+    return attend<bf16, bf16>(a, p, (int)hd, st);
+}
+
+int gphq_paged_check(int32_t *bad_dev, void *stream) {
+    if (!bad_dev) return GPHQ_ERR_PAGED_SHAPE;
+    GPHQ_TRY(hip_status(hipStreamSynchronize((hipStream_t)stream)));
+    int32_t bad = 0;
+    GPHQ_TRY(hip_status(hipMemcpy(&bad, bad_dev, 4, hipMemcpyDeviceToHost)));
+    if (!bad) return GPHQ_OK;
+    GPHQ_TRY(hip_status(hipMemset(bad_dev, 0, 4)));
+    return GPHQ_ERR_PAGED_BATCH;
+}
+
+}  // extern "C"

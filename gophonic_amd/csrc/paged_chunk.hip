@@ -1,0 +1,506 @@
+// Paged attention of many query rows: the chunk kernel of gphq_paged_attention (prompt
+// chunks). See paged_attention.h for the mathematics and the tiling.
+#include "paged_attention.h"
+
+namespace gphq {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// One block's tile: 128 columns of a sequence and KV head, 32 to each of four wavefronts,
+// over the keys [k0, k1).
+struct ChunkTile {
+    int seq, g, n, len, start, splits, split;
+    int lo, hi, k0, k1;
+    // this wavefront's rows and their keys [w_lo, w_hi)
+    int r0, r1, p0, p1, w_lo, w_hi;
+    // this lane's column
+    int row, head, pos, first;
+    bool live;
+};
+
+// The block's tile among those of the sequences that are not the row kernel's, counted by
+// 64 lanes over 64 sequences at a time. Tiles are dealt out from the back: a sequence's last
+// rows see most keys, so the long tiles start first. False where there is no such tile.
+__device__ __forceinline__ bool chunk_tile(const AttnArgs &a, int tiles, int splits, ChunkTile &t) {
+    int u = blockIdx.x;
+    t.g = u % a.pool.kv_heads;
+    u /= a.pool.kv_heads;
+    t.split = u % splits;
+    const int want = tiles - 1 - u / splits;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    int before = 0, tile = -1;
+    for (int s0 = 0; s0 < a.b.seqs; s0 += 64) {
+        const int s = min(s0 + lane, a.b.seqs - 1);
+        const int start = a.b.starts[s], end = a.b.starts[s + 1], len = a.b.lens[s];
+        const bool ok = seq_ok(a.b, start, end, len);
+        if (!ok) paged_flag(a.b, PAGED_BAD_SEQ);
+        const int cols = ok ? (end - start) * a.group : 0;
+        const int mine = s0 + lane < a.b.seqs && cols > a.small_cols ? (cols + kBigTile - 1) / kBigTile : 0;
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int v = __shfl_up(sum, d);
+            sum += lane >= d ? v : 0;
+        }
+        const int total = __builtin_amdgcn_readlane(sum, 63);
+        if (want < before + total) {
+            const int at = __builtin_ctzll(__ballot(want < before + sum));
+            t.seq = s0 + at;
+            tile = want - before - __builtin_amdgcn_readlane(sum - mine, at);
+            t.start = __builtin_amdgcn_readlane(start, at);
+            t.n = __builtin_amdgcn_readlane(end, at) - t.start;
+            t.len = __builtin_amdgcn_readlane(len, at);
+            break;
+        }
+        before += total;
+    }
+    if (tile < 0) return false;
+    const int cols = t.n * a.group, c0 = tile * kBigTile, off = t.len - t.n;
+    const TileKeys k =
+        tile_keys(t.n, t.len, c0 / a.group, min((c0 + kBigTile - 1) / a.group, t.n - 1), a.window);
+    t.lo = k.lo;
+    t.hi = k.hi;
+    t.splits = tile_splits(k, a.split_big);
+    if (t.split >= t.splits) return false;
+    t.k0 = k.from + t.split * a.split_big;
+    t.k1 = min(t.k0 + a.split_big, k.hi);
+    const int w0 = c0 + 32 * wave;
+    t.r0 = min(w0 / a.group, t.n - 1);
+    t.r1 = min((w0 + 31) / a.group, t.n - 1);
+    t.p0 = off + t.r0;
+    t.p1 = off + t.r1;
+    const TileKeys w = tile_keys(t.n, t.len, t.r0, t.r1, a.window);
+    t.w_lo = w.lo;
+    t.w_hi = w0 < cols ? w.hi : 0;  // a wavefront without columns sees no key
+    const int col = w0 + (lane & 31);
+    t.live = col < cols;
+    t.row = t.live ? col / a.group : t.r1;
+    t.head = t.g * a.group + (t.live ? col - t.row * a.group : 0);
+    t.pos = off + t.row;
+    t.first = a.window > 0 ? t.pos - a.window + 1 : 0;
+    return true;
+}
+
+// As the row kernel's: the pool offset of the 16 keys from kt on.
+__device__ __forceinline__ int64_t chunk_keys(const AttnArgs &a, const ChunkTile &t, int kt, bool &ok) {
+    int page = 0;
+    ok = kt < t.hi && kt + 16 > t.lo;
+    if (ok) {
+        page = uniform(a.b.table[t.seq * a.b.table_stride + (kt >> a.pool.shift)]);
+        if (page < 0 || page >= a.pool.pages) {
+            paged_flag(a.b, PAGED_BAD_PAGE);
+            page = 0;
+            ok = false;
+        }
+    }
+    return page * a.pool.page_stride + (kt & ((1 << a.pool.shift) - 1)) * a.pool.token_stride +
+           t.g * a.pool.head_stride;
+}
+
+// One step's exponentials over N 32-key score tiles: s[h][r] is key kt + 32 h + 8 (r / 4) +
+// 4 hi + r % 4; as the row kernel's softmax_step. ok: a bit per 16 keys.
+template <int N>
+__device__ __forceinline__ float chunk_softmax(const ChunkTile &t, f32x16 (&s)[N], float fac, bool masked, int kt,
+                                               unsigned ok, float &m, float &l, bool &moved) {
+    const int hi = (threadIdx.x & 63) >> 5;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < N; ++h) s[h] *= fac;
+    if (masked) {
+#pragma unroll
+        for (int h = 0; h < N; ++h)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int key = kt + 32 * h + 8 * (r >> 2) + 4 * hi + (r & 3);
+                if (key > t.pos || key < t.first || !(ok >> (2 * h + (r >> 3)) & 1)) s[h][r] = -INFINITY;
+            }
+    }
+#pragma unroll
+    for (int h = 0; h < N; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[h][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const bool grew = mx > m + kLag;
+    const float mn = grew ? mx : m;
+    const float ref = mn == -INFINITY ? 0.0f : mn - kLift;
+    const float corr = __builtin_amdgcn_exp2f((m == -INFINITY ? m : m - kLift) - ref);
+    m = mn;
+    float sum = 0.0f;
+#pragma unroll
+    for (int h = 0; h < N; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[h][r] = __builtin_amdgcn_exp2f(s[h][r] - ref);
+            sum += s[h][r];
+        }
+    l = l * corr + sum;
+    moved = __any(grew);
+    return corr;
+}
+
+// Writes a lane's column, or its split result: o(d0) gives four values of consecutive dims
+// from d0 on, the lane holding the dims of every 8 that start at 4 hi.
+template <typename RT, int HD, typename F>
+__device__ __forceinline__ void chunk_finish(const AttnArgs &a, const ChunkTile &t, float m, float l, F &&o) {
+    const int hi = (threadIdx.x & 63) >> 5;
+    l += __shfl_xor(l, 32);
+    if (!t.live) return;
+    if (t.splits == 1) {
+        const float inv = 1.0f / l;
+        RT *out = (RT *)a.out + (int64_t)(t.start + t.row) * a.out_stride + t.head * HD;
+#pragma unroll
+        for (int d = 0; d < HD; d += 8) {
+            const f32x4 v = o(d / 8);
+            const float w[4] = {t.pos < 0 ? 0.0f : v[0] * inv, t.pos < 0 ? 0.0f : v[1] * inv,
+                                t.pos < 0 ? 0.0f : v[2] * inv, t.pos < 0 ? 0.0f : v[3] * inv};
+            store_vec(out + d + 4 * hi, w);
+        }
+        return;
+    }
+    const int64_t at = ((int64_t)(t.start + t.row) * a.heads + t.head) * a.parts + t.split;
+#pragma unroll
+    for (int d = 0; d < HD; d += 8) *(f32x4 *)(a.part_o + at * HD + d + 4 * hi) = o(d / 8);
+    if (hi == 0) {
+        a.part_ml[2 * at] = m;
+        a.part_ml[2 * at + 1] = l;
+    }
+}
+
+// 16-bit pages. Each step's 64 keys are staged once for the block's 128 columns: K as rows,
+// V transposed, [dim][key], by exchanging 16-bit halves between the four keys that a thread
+// loads; both with their 16-byte pieces permuted within a row, so that the fragment reads
+// of 16 consecutive rows and the stores fall on all banks. On v_mfma_f32_32x32x16:
+//   S^T (32 keys x 32 columns) = K . Q^T;
+//   O^T (32 dims x 32 columns) += V^T . P^T, the score registers being P^T's fragment: in
+//     each 16 keys a lane of the lower half holds keys 0-3 and 8-11, of the upper half 4-7
+//     and 12-15, and V^T's rows are stored in that order.
+// Two LDS buffers, one barrier a step: step u + 1 is loaded into registers while step u is
+// multiplied.
+template <typename RT, typename CT, int HD>
+__global__ __launch_bounds__(256) void attn_chunk16_kernel(const AttnArgs a, int tiles, int splits) {
+    typedef Half<CT> H;
+    typedef typename H::vec8 vec8;
+    constexpr int NP = kPieces<RT, CT>, KB = 64, QC = HD / 16, DT = HD / 32, VD = HD / 16, VW = VD / 2;
+    constexpr int KI = KB * HD / 8 / 256;   // 16-byte pieces of K per thread
+    constexpr int KP = HD / 8;              // pieces per key
+    __shared__ CT Ks[2][KB * HD];
+    __shared__ CT Vt[2][HD * KB];
+    ChunkTile t;
+    if (!chunk_tile(a, tiles, splits, t)) return;
+    const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, q = lane & 31, hi = lane >> 5;
+    const CT *kp = (const CT *)a.pool.k, *vp = (const CT *)a.pool.v;
+
+    float fac = a.scale_log2;
+    vec8 qf[NP][QC];
+    {
+        const RT *src = (const RT *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 8 * hi;
+        float inverse = 1.0f, up = 1.0f;
+        if (NP == 2) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2 * QC; ++i) {
+                float x[4];
+                load_vec(src + 16 * (i >> 1) + 4 * (i & 1), x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[e]));
+            }
+            m = fmaxf(m, __shfl_xor(m, 32));
+            up = f16_scale(m, inverse);
+            fac *= inverse;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * QC; ++i) {
+            float x[4];
+            load_vec(src + 16 * (i >> 1) + 4 * (i & 1), x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                CT pc[NP];
+                split_pieces(x[e] * up, pc);
+#pragma unroll
+                for (int k = 0; k < NP; ++k) qf[k][i >> 1][4 * (i & 1) + e] = pc[k];
+            }
+        }
+    }
+
+    typedef int vrow __attribute__((ext_vector_type(VW)));
+    i32x4 kr[KI];
+    vrow vr[4];
+    const int krow = tid / KP, kpc = tid % KP;    // K: piece kpc of keys krow + i * (256 / KP)
+    const int vkg = tid >> 4, vdg = tid & 15;     // V: keys 4 vkg .. 4 vkg + 3 of dims VD vdg ..
+    auto load = [&](int kt) __attribute__((always_inline)) -> unsigned {
+        bool ok[4];
+        int64_t at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at[i] = chunk_keys(a, t, kt + 16 * i, ok[i]);
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+            const int64_t base = KI == 4 ? at[i] : wave < 2 ? at[2 * i % 4] : at[(2 * i + 1) % 4];
+            kr[i] = *(const i32x4 *)(kp + base + (krow & 15) * a.pool.token_stride + 8 * kpc);
+        }
+        const int64_t base = wave == 0 ? at[0] : wave == 1 ? at[1] : wave == 2 ? at[2] : at[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            vr[i] = *(const vrow *)(vp + base + (4 * (vkg & 3) + i) * a.pool.token_stride + VD * vdg);
+        return (unsigned)ok[0] | (unsigned)ok[1] << 1 | (unsigned)ok[2] << 2 | (unsigned)ok[3] << 3;
+    };
+    auto store = [&](int kt, unsigned ok, int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+            const int row = krow + i * (256 / KP);
+            const int pc = HD == 128 ? kpc ^ (row & 15) : kpc ^ ((row >> 1) & 7);
+            *(i32x4 *)(Ks[buf] + row * HD + 8 * pc) = kr[i];
+        }
+        if (kt < t.lo || kt + KB > t.hi || ok != 15) {
+            // What no row of the tile sees may hold anything: 0 times it must stay 0.
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int key = kt + 4 * vkg + i;
+                if (key < t.lo || key >= t.hi || !(ok >> wave & 1)) vr[i] = vrow{};
+            }
+        }
+        // Key group vkg goes to position group {0, 2, 1, 3}[vkg % 4] of its 16 keys.
+        const int pg = (vkg & ~3) + ((vkg & 3) == 1 ? 2 : (vkg & 3) == 2 ? 1 : vkg & 3);
+#pragma unroll
+        for (int e = 0; e < VD; ++e) {
+            const int sel = e % 2 ? 0x07060302 : 0x05040100, d = VD * vdg + e;
+            typedef int i32x2 __attribute__((ext_vector_type(2)));
+            const i32x2 x = {(int)__builtin_amdgcn_perm(vr[1][e / 2], vr[0][e / 2], sel),
+                             (int)__builtin_amdgcn_perm(vr[3][e / 2], vr[2][e / 2], sel)};
+            const int unit = (pg >> 1) ^ (((d >> 1) ^ (d >> 4)) & 7);
+            *(i32x2 *)(Vt[buf] + d * KB + 8 * unit + 4 * (pg & 1)) = x;
+        }
+    };
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = f32x16{};
+    float m = -INFINITY, l = 0.0f;
+    unsigned ok = t.k0 < t.k1 ? load(t.k0) : 0;
+    int buf = 0;
+    for (int kt = t.k0; kt < t.k1; kt += KB, buf ^= 1) {
+        store(kt, ok, buf);
+        __syncthreads();
+        const unsigned okc = ok;
+        if (kt + KB < t.k1) ok = load(kt + KB);
+        if (kt >= t.w_hi || kt + KB <= t.w_lo) continue;
+        f32x16 s[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+        for (int i = 0; i < QC; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = 32 * h + q;
+                const int pc = HD == 128 ? (2 * i + hi) ^ (row & 15) : (2 * i + hi) ^ ((row >> 1) & 7);
+                const vec8 kf = *(const vec8 *)(Ks[buf] + row * HD + 8 * pc);
+#pragma unroll
+                for (int k = 0; k < NP; ++k) s[h] = H::mfma32(kf, qf[k][i], s[h]);
+            }
+        const bool masked =
+            kt + KB - 1 > t.p0 || kt < t.w_lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 15;
+        bool moved;
+        const float corr = chunk_softmax(t, s, fac, masked, kt, okc, m, l, moved);
+        if (moved) {
+#pragma unroll
+            for (int i = 0; i < DT; ++i) o[i] *= corr;
+        }
+        const bool check = masked && t.r0 != t.r1;
+#pragma unroll
+        for (int ks = 0; ks < KB / 16; ++ks) {
+            vec8 pf[NP];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                CT pc[NP];
+                split_pieces(s[ks >> 1][8 * (ks & 1) + i], pc);
+#pragma unroll
+                for (int k = 0; k < NP; ++k) pf[k][i] = pc[k];
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const int dim = 32 * d + q;
+                const int unit = (2 * ks + hi) ^ (((dim >> 1) ^ (dim >> 4)) & 7);
+                const i32x4 f = *(const i32x4 *)(Vt[buf] + dim * KB + 8 * unit);
+                bool odd = false;  // a value that is not finite, which a row must not meet
+                if (check) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) odd |= pair_not_finite<CT>(f[j]);
+                    odd = __any(odd);
+                }
+                if (!odd) {
+#pragma unroll
+                    for (int k = 0; k < NP; ++k) o[d] = H::mfma32(__builtin_bit_cast(vec8, f), pf[k], o[d]);
+                    continue;
+                }
+                // Row by row, with the values its own mask leaves.
+                for (int r = t.r0; r <= t.r1; ++r) {
+                    const int pos = t.len - t.n + r, first = a.window > 0 ? pos - a.window + 1 : 0;
+                    i32x4 fr;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int k0 = kt + 16 * ks + 8 * (j >> 1) + 4 * hi + 2 * (j & 1);
+                        fr[j] = f[j] & ((k0 <= pos && k0 >= first ? 0xFFFF : 0) |
+                                        (k0 + 1 <= pos && k0 + 1 >= first ? 0xFFFF0000 : 0));
+                    }
+                    f32x16 add{};
+#pragma unroll
+                    for (int k = 0; k < NP; ++k) add = H::mfma32(__builtin_bit_cast(vec8, fr), pf[k], add);
+                    if (t.row == r) o[d] += add;
+                }
+            }
+        }
+    }
+    chunk_finish<RT, HD>(a, t, m, l, [&](int i) {
+        const f32x16 &v = o[i / 4];
+        const int r = 4 * (i % 4);
+        return f32x4{v[r], v[r + 1], v[r + 2], v[r + 3]};
+    });
+}
+
+// fp32 pages, the same walk in 32-key steps on v_mfma_f32_32x32x2_f32. Its operands are one
+// fp32 value a lane, so V is staged as rows; a lane takes HD / 32 neighbouring dims of V at
+// once, one for each of its output tiles: tile d holds dims HD/32 * i + d.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_chunk32_kernel(const AttnArgs a, int tiles, int splits) {
+    constexpr int KB = 32, QC = HD / 8, DT = HD / 32;
+    constexpr int KP = HD / 4, KI = KB * KP / 256;  // 16-byte pieces per key, per thread
+    __shared__ float Ks[2][KB * HD];
+    __shared__ float Vs[2][KB * HD];
+    ChunkTile t;
+    if (!chunk_tile(a, tiles, splits, t)) return;
+    const int tid = threadIdx.x, lane = tid & 63, q = lane & 31, hi = lane >> 5;
+    const float *kp = (const float *)a.pool.k, *vp = (const float *)a.pool.v;
+    f32x4 qf[QC];
+    {
+        const float *src = (const float *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 4 * hi;
+#pragma unroll
+        for (int i = 0; i < QC; ++i) qf[i] = *(const f32x4 *)(src + 8 * i);
+    }
+    f32x4 kr[KI], vr[KI];
+    const int krow = tid / KP, kpc = tid % KP;
+    auto load = [&](int kt) __attribute__((always_inline)) -> unsigned {
+        bool ok[2];
+        int64_t at[2];
+        at[0] = chunk_keys(a, t, kt, ok[0]);
+        at[1] = chunk_keys(a, t, kt + 16, ok[1]);
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+            const int row = krow + i * (256 / KP);
+            const int64_t off = at[i * (256 / KP) / 16] + (row & 15) * a.pool.token_stride + 4 * kpc;
+            kr[i] = *(const f32x4 *)(kp + off);
+            vr[i] = *(const f32x4 *)(vp + off);
+        }
+        return (unsigned)ok[0] | (unsigned)ok[1] << 1;
+    };
+    auto store = [&](int kt, unsigned ok, int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < KI; ++i) {
+            const int row = krow + i * (256 / KP), key = kt + row;
+            *(f32x4 *)(Ks[buf] + row * HD + 4 * (kpc ^ (row & 15))) = kr[i];
+            // What no row of the tile sees may hold anything: 0 times it must stay 0.
+            if (key < t.lo || key >= t.hi || !(ok >> (row >> 4) & 1)) vr[i] = f32x4{};
+            *(f32x4 *)(Vs[buf] + row * HD + 4 * kpc) = vr[i];
+        }
+    };
+    f32x16 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = f32x16{};
+    float m = -INFINITY, l = 0.0f;
+    unsigned ok = t.k0 < t.k1 ? load(t.k0) : 0;
+    int buf = 0;
+    for (int kt = t.k0; kt < t.k1; kt += KB, buf ^= 1) {
+        store(kt, ok, buf);
+        __syncthreads();
+        const unsigned okc = ok;
+        if (kt + KB < t.k1) ok = load(kt + KB);
+        if (kt >= t.w_hi || kt + KB <= t.w_lo) continue;
+        f32x16 s[1] = {f32x16{}};
+#pragma unroll
+        for (int i = 0; i < QC; ++i) {
+            const f32x4 kf = *(const f32x4 *)(Ks[buf] + q * HD + 4 * ((2 * i + hi) ^ (q & 15)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], qf[i][e], s[0], 0, 0, 0);
+        }
+        const bool masked =
+            kt + KB - 1 > t.p0 || kt < t.w_lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 3;
+        bool moved;
+        const float corr = chunk_softmax(t, s, a.scale_log2, masked, kt, okc, m, l, moved);
+        if (moved) {
+#pragma unroll
+            for (int i = 0; i < DT; ++i) o[i] *= corr;
+        }
+        const bool check = masked && t.r0 != t.r1;
+        typedef float vdim __attribute__((ext_vector_type(DT)));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int key = kt + 8 * (r >> 2) + 4 * hi + (r & 3);
+            const vdim v = *(const vdim *)(Vs[buf] + (key - kt) * HD + DT * q);
+            bool odd = false;  // a value that is not finite, which a row must not meet
+            if (check) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) odd |= !(fabsf(v[d]) < INFINITY);
+                odd = __any(odd);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                if (!odd) {
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[d], s[0][r], o[d], 0, 0, 0);
+                    continue;
+                }
+                // Row by row, with the values its own mask leaves.
+                for (int i = t.r0; i <= t.r1; ++i) {
+                    const int pos = t.len - t.n + i, first = a.window > 0 ? pos - a.window + 1 : 0;
+                    f32x16 add{};
+                    add = __builtin_amdgcn_mfma_f32_32x32x2f32(key <= pos && key >= first ? v[d] : 0.0f, s[0][r], add,
+                                                               0, 0, 0);
+                    if (t.row == i) o[d] += add;
+                }
+            }
+        }
+    }
+    // Output register r of tile d is dim DT * (8 (r / 4) + 4 hi + r % 4) + d: DT rows of four
+    // consecutive registers hold 4 DT consecutive dims, starting at 4 DT (2 (r / 4) + hi).
+    l += __shfl_xor(l, 32);
+    if (!t.live) return;
+    const float inv = 1.0f / l;
+    float *out = (float *)a.out + (int64_t)(t.start + t.row) * a.out_stride + t.head * HD;
+    const int64_t at = ((int64_t)(t.start + t.row) * a.heads + t.head) * a.parts + t.split;
+    typedef float vdim __attribute__((ext_vector_type(DT)));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int d0 = DT * (8 * (r >> 2) + 4 * hi + (r & 3));
+        vdim v;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) v[d] = t.splits > 1 ? o[d][r] : t.pos < 0 ? 0.0f : o[d][r] * inv;
+        *(vdim *)((t.splits > 1 ? a.part_o + at * HD : out) + d0) = v;
+    }
+    if (t.splits > 1 && hi == 0) {
+        a.part_ml[2 * at] = m;
+        a.part_ml[2 * at + 1] = l;
+    }
+}
+
+}  // namespace
+
+template <typename RT, typename CT>
+int attn_chunk_launch(const AttnArgs &a, int hd, int splits, int tiles, hipStream_t st) {
+    const unsigned blocks = (unsigned)tiles * (unsigned)splits * (unsigned)a.pool.kv_heads;
+    if constexpr (std::is_same<CT, float>::value) {
+        if (hd == 128)
+            hipLaunchKernelGGL((attn_chunk32_kernel<128>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+        else
+            hipLaunchKernelGGL((attn_chunk32_kernel<64>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+    } else {
+        if (hd == 128)
+            hipLaunchKernelGGL((attn_chunk16_kernel<RT, CT, 128>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+        else
+            hipLaunchKernelGGL((attn_chunk16_kernel<RT, CT, 64>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+    }
+    return launch_status();
+}
+
+template int attn_chunk_launch<float, float>(const AttnArgs &, int, int, int, hipStream_t);
+template int attn_chunk_launch<float, f16>(const AttnArgs &, int, int, int, hipStream_t);
+template int attn_chunk_launch<float, bf16>(const AttnArgs &, int, int, int, hipStream_t);
+template int attn_chunk_launch<f16, f16>(const AttnArgs &, int, int, int, hipStream_t);
+template int attn_chunk_launch<bf16, bf16>(const AttnArgs &, int, int, int, hipStream_t);
+
+}  // namespace gphq

@@ -1,0 +1,432 @@
+// Paged attention of few query rows: the row kernel of gphq_paged_attention
+// (single tokens, and sequences of a few rows). See paged_attention.h for the
+// mathematics and the tiling.
+#include "paged_attention.h"
+
+namespace gphq {
+namespace {
+
+// One block's tile: 16 columns of a sequence and KV head over the keys [k0, k1).
+struct RowTile {
+    int seq, g, n, len, start, r0, r1, splits, split;
+    int lo, hi, k0, k1, p0, p1;  // p0, p1: positions of the tile's first and last row
+    // this lane's column
+    int row, head, pos, first;
+    bool live;
+};
+
+// False where this block has nothing to do.
+__device__ __forceinline__ bool row_tile(const AttnArgs &a, int tiles, int splits, RowTile &t) {
+    int u = blockIdx.x;
+    t.g = u % a.pool.kv_heads;
+    u /= a.pool.kv_heads;
+    t.split = u % splits;
+    u /= splits;
+    const int ct = u % tiles;
+    t.seq = u / tiles;
+    t.start = a.b.starts[t.seq];
+    const int end = a.b.starts[t.seq + 1];
+    t.len = a.b.lens[t.seq];
+    if (!seq_ok(a.b, t.start, end, t.len)) {
+        if (threadIdx.x == 0) paged_flag(a.b, PAGED_BAD_SEQ);
+        return false;
+    }
+    t.n = end - t.start;
+    const int cols = t.n * a.group;
+    if (cols > a.small_cols || ct * kSmallTile >= cols) return false;
+    t.r0 = ct * kSmallTile / a.group;
+    t.r1 = min((ct * kSmallTile + kSmallTile - 1) / a.group, t.n - 1);
+    const TileKeys k = tile_keys(t.n, t.len, t.r0, t.r1, a.window);
+    t.lo = k.lo;
+    t.hi = k.hi;
+    t.splits = tile_splits(k, a.split_small);
+    if (t.split >= t.splits) return false;
+    t.k0 = k.from + t.split * a.split_small;
+    t.k1 = min(t.k0 + a.split_small, k.hi);
+    t.p0 = t.len - t.n + t.r0;
+    t.p1 = t.len - t.n + t.r1;
+    const int col = ct * kSmallTile + (threadIdx.x & 15);
+    t.live = col < cols;
+    t.row = t.live ? col / a.group : t.r1;
+    t.head = t.g * a.group + (t.live ? col - t.row * a.group : 0);
+    t.pos = t.len - t.n + t.row;
+    t.first = a.window > 0 ? t.pos - a.window + 1 : 0;
+    return true;
+}
+
+// Where the 16 keys from kt on lie: the pool offset of key kt and KV head t.g. Not ok for
+// keys that no row of the tile sees (their table entry may be unset) and for a page number
+// outside the pool, which is flagged; the offset is then page 0's, which can be read.
+__device__ __forceinline__ int64_t key_tile(const AttnArgs &a, const RowTile &t, int kt, bool &ok) {
+    int page = 0;
+    ok = kt < t.hi && kt + 16 > t.lo;
+    if (ok) {
+        page = uniform(a.b.table[t.seq * a.b.table_stride + (kt >> a.pool.shift)]);
+        if (page < 0 || page >= a.pool.pages) {
+            paged_flag(a.b, PAGED_BAD_PAGE);
+            page = 0;
+            ok = false;
+        }
+    }
+    return page * a.pool.page_stride + (kt & ((1 << a.pool.shift) - 1)) * a.pool.token_stride +
+           t.g * a.pool.head_stride;
+}
+
+// One 32-key step's exponentials: s[0], s[1] are the scores (times fac: in log2) of keys
+// kt + 4 g4 + r and kt + 16 + 4 g4 + r; those that the lane's column does not see are left
+// out. p[8] are 2^(x - m + 7), m and l the running reference and this lane's running sum;
+// returns what o is to be multiplied by, and whether any lane's reference moved.
+__device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)[2], float fac, bool masked, int kt,
+                                              bool ok0, bool ok1, float (&p)[8], float &m, float &l, bool &moved) {
+    const int g4 = (threadIdx.x & 63) >> 4;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * fac;
+    if (masked) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
+            if (key > t.pos || key < t.first || !(i < 4 ? ok0 : ok1)) x[i] = -INFINITY;
+        }
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const bool grew = mx > m + kLag;
+    const float mn = grew ? mx : m;
+    const float ref = mn == -INFINITY ? 0.0f : mn - kLift;
+    const float corr = __builtin_amdgcn_exp2f((m == -INFINITY ? m : m - kLift) - ref);
+    m = mn;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+        sum += p[i];
+    }
+    l = l * corr + sum;
+    moved = __any(grew);
+    return corr;
+}
+
+// Joins the four wavefronts' (m, l, o) of a tile and writes the tile's rows, or its split
+// results. o[t][r] is column lane % 16, dim VD * (4 g4 + r) + t.
+template <typename RT, int HD>
+__device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t, float m, float l,
+                                            const f32x4 (&o)[HD / 16]) {
+    constexpr int VD = HD / 16, LD = HD + 4;
+    __shared__ float so[4][16][LD];
+    __shared__ float sm[4][16], sl[4][16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g4 == 0) {
+        sm[wave][c] = m;
+        sl[wave][c] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int v = 0; v < VD; v += 4)
+            *(f32x4 *)&so[wave][c][VD * (4 * g4 + r) + v] =
+                f32x4{o[v][r], o[v + 1][r], o[v + 2][r], o[v + 3][r]};
+    // The column of thread i is i / 16: this lane's own numbers come from the lane holding it.
+    const int col = threadIdx.x >> 4, d = (threadIdx.x & 15) * VD;
+    const int from = col;  // lanes 0..15 of any wavefront hold columns 0..15
+    const int row = __shfl(t.row, from), head = __shfl(t.head, from), pos = __shfl(t.pos, from);
+    const bool live = __shfl((int)t.live, from) != 0;
+    __syncthreads();
+    if (!live) return;
+    float M = sm[0][col];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) M = fmaxf(M, sm[w][col]);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f, v[VD];
+#pragma unroll
+    for (int i = 0; i < VD; ++i) v[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float e = __builtin_amdgcn_exp2f(sm[w][col] - ref);
+        L += e * sl[w][col];
+#pragma unroll
+        for (int i = 0; i < VD; ++i) v[i] += e * so[w][col][d + i];
+    }
+    if (t.splits == 1) {
+        const float inv = 1.0f / L;
+        RT *out = (RT *)a.out + (int64_t)(t.start + row) * a.out_stride + head * HD + d;
+#pragma unroll
+        for (int i = 0; i < VD; i += 4) {
+            float w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = pos < 0 ? 0.0f : v[i + k] * inv;
+            store_vec(out + i, w);
+        }
+        return;
+    }
+    const int64_t at = ((int64_t)(t.start + row) * a.heads + head) * a.parts + t.split;
+#pragma unroll
+    for (int i = 0; i < VD; i += 4) *(f32x4 *)(a.part_o + at * HD + d + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    if (d == 0) {
+        a.part_ml[2 * at] = M;
+        a.part_ml[2 * at + 1] = L;
+    }
+}
+
+// 16-bit pages. Four wavefronts take the tile's 32-key steps in turn, each on its own:
+// everything goes from memory to registers, nothing through LDS. On
+// v_mfma_f32_16x16x32:
+//   S^T (16 keys x 16 columns) = K . Q^T, K's fragment as it lies in the page;
+//   O^T (16 dims x 16 columns) += V^T . P^T: the score registers are P^T's fragment as they
+//     stand (keys 4 g4 + 0..3 of both 16-key tiles); a lane loads those eight keys of V at
+//     HD/16 neighbouring dims, and 16-bit halves exchanged between the eight registers make
+//     the fragments of V^T for HD/16 tiles of dims HD/16 apart.
+template <typename RT, typename CT, int HD>
+__global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int tiles, int splits) {
+    typedef Half<CT> H;
+    typedef typename H::vec8 vec8;
+    constexpr int NP = kPieces<RT, CT>, KC = HD / 32, VD = HD / 16, VW = VD / 2;  // VW: dwords of V per key
+    RowTile t;
+    if (!row_tile(a, tiles, splits, t)) return;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
+    const CT *kp = (const CT *)a.pool.k, *vp = (const CT *)a.pool.v;
+
+    float fac = a.scale_log2;
+    vec8 qf[NP][KC];
+    {
+        const RT *q = (const RT *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 8 * g4;
+        float x[KC][8], inverse = 1.0f, up = 1.0f;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+            float lo[4], hi[4];
+            load_vec(q + 32 * i, lo);
+            load_vec(q + 32 * i + 4, hi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i][e] = lo[e], x[i][4 + e] = hi[e];
+        }
+        if (NP == 2) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KC; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[i][e]));
+            m = fmaxf(m, __shfl_xor(m, 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            up = f16_scale(m, inverse);
+            fac *= inverse;
+        }
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                CT pc[NP];
+                split_pieces(x[i][e] * up, pc);
+#pragma unroll
+                for (int k = 0; k < NP; ++k) qf[k][i][e] = pc[k];
+            }
+    }
+    f32x4 o[VD];
+#pragma unroll
+    for (int i = 0; i < VD; ++i) o[i] = f32x4{};
+    float m = -INFINITY, l = 0.0f;
+    for (int kt = t.k0 + 32 * wave; kt < t.k1; kt += 128) {
+        bool ok0, ok1;
+        const int64_t at0 = key_tile(a, t, kt, ok0), at1 = key_tile(a, t, kt + 16, ok1);
+        vec8 kf[2][KC];
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+            kf[0][i] = *(const vec8 *)(kp + at0 + c * a.pool.token_stride + 32 * i + 8 * g4);
+            kf[1][i] = *(const vec8 *)(kp + at1 + c * a.pool.token_stride + 32 * i + 8 * g4);
+        }
+        typedef int vrow __attribute__((ext_vector_type(VW)));
+        vrow v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = *(const vrow *)(vp + (i < 4 ? at0 : at1) + (4 * g4 + (i & 3)) * a.pool.token_stride + VD * c);
+        f32x4 s[2] = {f32x4{}, f32x4{}};
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+                s[0] = H::mfma16(kf[0][i], qf[k][i], s[0]);
+                s[1] = H::mfma16(kf[1][i], qf[k][i], s[1]);
+            }
+        // Whether some column does not see some key of the step.
+        const bool masked = kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || !ok0 || !ok1;
+        float p[8];
+        bool moved;
+        const float corr = softmax_step(t, s, fac, masked, kt, ok0, ok1, p, m, l, moved);
+        bool odd = false;  // a value that is not finite, which a row of the tile must not meet
+        if (masked) {
+            // What no row of the tile sees may hold anything: 0 times it must stay 0.
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
+                if (key >= t.hi || key < t.lo || !(i < 4 ? ok0 : ok1)) v[i] = vrow{};
+#pragma unroll
+                for (int w = 0; w < VW; ++w) odd |= pair_not_finite<CT>(v[i][w]);
+            }
+            odd = t.r0 != t.r1 && __any(odd);
+        }
+        vec8 pf[NP];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            CT pc[NP];
+            split_pieces(p[i], pc);
+#pragma unroll
+            for (int k = 0; k < NP; ++k) pf[k][i] = pc[k];
+        }
+        if (moved) {
+#pragma unroll
+            for (int i = 0; i < VD; ++i) o[i] *= corr;
+        }
+#pragma unroll
+        for (int d = 0; d < VD; ++d) {
+            i32x4 f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                f[j] = __builtin_amdgcn_perm(v[2 * j + 1][d / 2], v[2 * j][d / 2], d % 2 ? 0x07060302 : 0x05040100);
+            if (!odd) {
+#pragma unroll
+                for (int k = 0; k < NP; ++k) o[d] = H::mfma16(__builtin_bit_cast(vec8, f), pf[k], o[d]);
+                continue;
+            }
+            // Row by row, with the values its own mask leaves.
+            for (int r = t.r0; r <= t.r1; ++r) {
+                const int pos = t.len - t.n + r, first = a.window > 0 ? pos - a.window + 1 : 0;
+                i32x4 fr;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int k0 = kt + 16 * (j >> 1) + 4 * g4 + 2 * (j & 1);
+                    fr[j] = f[j] & ((k0 <= pos && k0 >= first ? 0xFFFF : 0) |
+                                    (k0 + 1 <= pos && k0 + 1 >= first ? 0xFFFF0000 : 0));
+                }
+                f32x4 add{};
+#pragma unroll
+                for (int k = 0; k < NP; ++k) add = H::mfma16(__builtin_bit_cast(vec8, fr), pf[k], add);
+                if (t.row == r) o[d] += add;
+            }
+        }
+    }
+    rows_finish<RT, HD>(a, t, m, l, o);
+}
+
+// fp32 pages, the same walk on v_mfma_f32_16x16x4_f32: its operands are one fp32 value a
+// lane, so V needs no exchange between registers, and a lane's 16-byte pieces of K and Q
+// hold the same dims (16 i + 4 g4 ..), in whatever order they are multiplied.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int tiles, int splits) {
+    constexpr int KC = HD / 16, VD = HD / 16;
+    RowTile t;
+    if (!row_tile(a, tiles, splits, t)) return;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
+    const float *kp = (const float *)a.pool.k, *vp = (const float *)a.pool.v;
+    f32x4 qf[KC];
+    {
+        const float *q = (const float *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 4 * g4;
+#pragma unroll
+        for (int i = 0; i < KC; ++i) qf[i] = *(const f32x4 *)(q + 16 * i);
+    }
+    f32x4 o[VD];
+#pragma unroll
+    for (int i = 0; i < VD; ++i) o[i] = f32x4{};
+    float m = -INFINITY, l = 0.0f;
+    for (int kt = t.k0 + 32 * wave; kt < t.k1; kt += 128) {
+        bool ok[2];
+        int64_t at[2];
+        at[0] = key_tile(a, t, kt, ok[0]);
+        at[1] = key_tile(a, t, kt + 16, ok[1]);
+        f32x4 kf[2][KC];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < KC; ++i)
+                kf[h][i] = *(const f32x4 *)(kp + at[h] + c * a.pool.token_stride + 16 * i + 4 * g4);
+        f32x4 v[8][VD / 4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int w = 0; w < VD / 4; ++w)
+                v[i][w] = *(const f32x4 *)(vp + at[i >> 2] + (4 * g4 + (i & 3)) * a.pool.token_stride + VD * c + 4 * w);
+        f32x4 s[2] = {f32x4{}, f32x4{}};
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[0][i][e], qf[i][e], s[0], 0, 0, 0);
+                s[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[1][i][e], qf[i][e], s[1], 0, 0, 0);
+            }
+        const bool masked =
+            kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || !ok[0] || !ok[1];
+        float p[8];
+        bool moved;
+        const float corr = softmax_step(t, s, a.scale_log2, masked, kt, ok[0], ok[1], p, m, l, moved);
+        bool odd = false;
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
+                const bool none = key >= t.hi || key < t.lo || !ok[i >> 2];
+#pragma unroll
+                for (int w = 0; w < VD / 4; ++w) {
+                    if (none) v[i][w] = f32x4{};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd |= !(fabsf(v[i][w][e]) < INFINITY);
+                }
+            }
+            odd = t.r0 != t.r1 && __any(odd);
+        }
+        if (moved) {
+#pragma unroll
+            for (int i = 0; i < VD; ++i) o[i] *= corr;
+        }
+#pragma unroll
+        for (int d = 0; d < VD; ++d) {
+            if (!odd) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d / 4][d % 4], p[i], o[d], 0, 0, 0);
+                continue;
+            }
+            for (int r = t.r0; r <= t.r1; ++r) {
+                const int pos = t.len - t.n + r, first = a.window > 0 ? pos - a.window + 1 : 0;
+                f32x4 add{};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
+                    const float x = key <= pos && key >= first ? v[i][d / 4][d % 4] : 0.0f;
+                    add = __builtin_amdgcn_mfma_f32_16x16x4f32(x, p[i], add, 0, 0, 0);
+                }
+                if (t.row == r) o[d] += add;
+            }
+        }
+    }
+    rows_finish<float, HD>(a, t, m, l, o);
+}
+
+}  // namespace
+
+template <typename RT, typename CT>
+int attn_rows_launch(const AttnArgs &a, int hd, int splits, int tiles, hipStream_t st) {
+    const unsigned blocks = (unsigned)(a.b.seqs * tiles) * (unsigned)splits * (unsigned)a.pool.kv_heads;
+    if constexpr (std::is_same<CT, float>::value) {
+        if (hd == 128)
+            hipLaunchKernelGGL((attn_rows32_kernel<128>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+        else
+            hipLaunchKernelGGL((attn_rows32_kernel<64>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+    } else {
+        if (hd == 128)
+            hipLaunchKernelGGL((attn_rows16_kernel<RT, CT, 128>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+        else
+            hipLaunchKernelGGL((attn_rows16_kernel<RT, CT, 64>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+    }
+    return launch_status();
+}
+
+template int attn_rows_launch<float, float>(const AttnArgs &, int, int, int, hipStream_t);
+template int attn_rows_launch<float, f16>(const AttnArgs &, int, int, int, hipStream_t);
+template int attn_rows_launch<float, bf16>(const AttnArgs &, int, int, int, hipStream_t);
+template int attn_rows_launch<f16, f16>(const AttnArgs &, int, int, int, hipStream_t);
+template int attn_rows_launch<bf16, bf16>(const AttnArgs &, int, int, int, hipStream_t);
+
+}  // namespace gphq

@@ -56,10 +56,13 @@ ERR_READ_RANGE = -40
 ERR_GPTQ_WIDTH = -41
 ERR_CALIBRATION_EMPTY = -42
 ERR_CALIBRATION_SHAPE = -43
+ERR_PAGED_SHAPE = -44
+ERR_PAGED_BATCH = -45
 TAIL_MAX_ROWS = 256
 
 FMT_Q4, FMT_Q8, FMT_Q8B, FMT_Q8B_F32 = 4, 8, 9, 10
 PASS_FP16, PASS_INT8 = 0, 1  # gphq_prefill_set_arith
+DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 1, 2, 3
 
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
@@ -195,6 +198,15 @@ SIGNATURES = {
     "gphq_prefill_batch": (ctypes.c_int, [_vp, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp]),
     "gphq_q8b_quantize": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp]),
     "gphq_q8b_gemm": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "gphq_paged_append": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _i64, _i64, _vp, _vp, ctypes.c_double, _vp, _vp,
+                                         _i64, ctypes.c_double, _vp, _i64, _vp]),
+    "gphq_paged_attention_workspace_bytes": (_i64, [_vp, _vp, ctypes.c_int, _i64, _i64]),
+    "gphq_paged_attention": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _i64, _i64, ctypes.c_double, _i64, _vp, _i64,
+                                            _vp, _i64, _vp]),
+    "gphq_paged_check": (ctypes.c_int, [_vp, _vp]),
+    "gphq_lora_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "gphq_lora_add": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64,
+                                     _i64, _i64, _vp, _i64, _vp]),
     "gphq_prefill_check": (ctypes.c_int, [_vp, _vp]),
     "gphq_prefill_set_arith": (ctypes.c_int, [_vp, ctypes.c_int]),
     "gphq_prefill_arith": (ctypes.c_int, [_vp]),
@@ -995,6 +1007,176 @@ def lm_random(geom_kwargs, fmt, seed, device="cuda", host=False):
         stored.update(embed=emb.cpu().numpy().view(np.uint16), final_norm=final_norm, head=(hc, hs))
     torch.cuda.synchronize()
     return lm, weight_bytes, stored
+
+
+# ---- paged K/V cache (gphq_paged_*) and low-rank adapters (gphq_lora_*) ---------
+
+
+class PagedKvDesc(ctypes.Structure):
+    _fields_ = [("k_dev", ctypes.c_void_p), ("v_dev", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("pages", ctypes.c_int64),
+                ("page_tokens", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class PagedBatchDesc(ctypes.Structure):
+    _fields_ = [("starts_dev", ctypes.c_void_p), ("lens_dev", ctypes.c_void_p), ("table_dev", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("seqs", ctypes.c_int64), ("rows", ctypes.c_int64),
+                ("max_rows", ctypes.c_int64), ("max_len", ctypes.c_int64), ("bad_dev", ctypes.c_void_p)]
+
+
+def _dtype(t):
+    """The GPHQ_DTYPE_* code of a torch dtype; ERR_UNSUPPORTED for one without."""
+    import torch
+
+    code = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}.get(t)
+    return check(ERR_UNSUPPORTED) if code is None else code
+
+
+def _rows2(t, rows, width, err):
+    """The row stride of a 2-D tensor of at least `rows` rows of `width` neighbouring values."""
+    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1):
+        check(err)
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _ints(t, n):
+    """A contiguous int32 tensor of at least n values (None if n is 0 and there is none)."""
+    import torch
+
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n:
+        check(ERR_PAGED_SHAPE)
+    return t
+
+
+def _here(*tensors):
+    """Refuses tensors that are not in the current device's memory, where the call's stream runs."""
+    import torch
+
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            check(ERR_PAGED_SHAPE)
+
+
+class PagedKv:
+    """gphq_paged_kv over two torch tensors seen as [pages][page tokens][KV
+    heads][head dim] with the same strides, of any page order (token-major as
+    created, head-major through transpose(1, 2)); kept alive by this object."""
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
+            check(ERR_PAGED_SHAPE)
+        self.k, self.v, self.dtype = k, v, k.dtype
+        pages, tokens, heads, hd = k.shape
+        # The stride of a dimension of one is never taken: one that the checks allow.
+        ps, ts, hs = (s if n > 1 else hd for s, n in zip(k.stride()[:3], k.shape[:3]))
+        self.desc = PagedKvDesc(ptr(k), ptr(v), ps, ts, hs, pages, tokens, heads, hd, _dtype(k.dtype), 0)
+        self.kv_heads, self.head_dim = heads, hd
+
+
+class PagedBatch:
+    """gphq_paged_batch: the sequences of one step. starts int32 [seqs + 1],
+    lens int32 [seqs] and table int32 [seqs][entries] are device tensors, read
+    when the work runs (their values may change between calls); rows is what
+    the row buffers hold, max_rows and max_len bound one sequence's rows and
+    lens. check() waits and raises for values out of bounds that a call met."""
+
+    def __init__(self, starts, lens, table, rows, max_rows, max_len):
+        import torch
+
+        seqs = lens.numel()
+        if table.dim() != 2 or table.shape[0] != seqs:
+            check(ERR_PAGED_SHAPE)
+        self.starts, self.lens, self.table = _ints(starts, seqs + 1), _ints(lens, seqs), _ints(table, 0)
+        self.bad = torch.zeros(1, dtype=torch.int32, device=lens.device)
+        self.rows = rows
+        self.desc = PagedBatchDesc(ptr(starts), ptr(lens), ptr(table), table.shape[1], seqs, rows, max_rows, max_len,
+                                   ptr(self.bad))
+
+    def check(self, stream=None):
+        return check(load().gphq_paged_check(ptr(self.bad), stream_handle(stream)))
+
+
+def paged_append(kv, batch, qkv, q, heads, q_norm=None, k_norm=None, eps=1e-6, cos=None, sin=None, q_scale=1.0,
+                 stream=None):
+    """gphq_paged_append: qkv [rows][(heads + 2 KV heads) head_dim] rows to
+    prepared queries q [rows][heads head_dim] and keys and values in the pages.
+    q_norm, k_norm float32 [head_dim]; cos, sin float32 [positions][head_dim / 2]."""
+    import torch
+
+    _here(kv.k, batch.lens, qkv, q, q_norm, k_norm, cos, sin)
+    if qkv.dtype != q.dtype or (cos is None) != (sin is None):
+        check(ERR_PAGED_SHAPE)
+    for t, n in ((q_norm, kv.head_dim), (k_norm, kv.head_dim), (cos, 0), (sin, 0)):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n):
+            check(ERR_PAGED_SHAPE)
+    if cos is not None and (cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != kv.head_dim // 2):
+        check(ERR_PAGED_SHAPE)
+    qs = _rows2(qkv, batch.rows, (heads + 2 * kv.kv_heads) * kv.head_dim, ERR_PAGED_SHAPE)
+    os_ = _rows2(q, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
+    return check(load().gphq_paged_append(ctypes.byref(kv.desc), ctypes.byref(batch.desc), _dtype(qkv.dtype), ptr(qkv),
+                                          qs, heads, ptr(q_norm), ptr(k_norm), eps, ptr(cos), ptr(sin),
+                                          0 if cos is None else cos.shape[0], q_scale, ptr(q), os_,
+                                          stream_handle(stream)))
+
+
+def paged_attention_workspace_bytes(kv, batch, dtype, heads, window=0):
+    n = load().gphq_paged_attention_workspace_bytes(ctypes.byref(kv.desc), ctypes.byref(batch.desc), _dtype(dtype),
+                                                    heads, window)
+    return n if n >= 0 else check(n)
+
+
+def _work(need, device):
+    import torch
+
+    return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+
+
+def paged_attention(kv, batch, q, out, heads, scale, window=0, work=None, stream=None):
+    """gphq_paged_attention: out [rows][heads head_dim] = causal attention of
+    the rows q over their sequences' pages. work: a uint8 device tensor of
+    paged_attention_workspace_bytes, or None for one of this call's own."""
+    _here(kv.k, batch.lens, q, out, work)
+    if q.dtype != out.dtype:
+        check(ERR_PAGED_SHAPE)
+    qs = _rows2(q, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
+    os_ = _rows2(out, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
+    if work is None:
+        work = _work(paged_attention_workspace_bytes(kv, batch, q.dtype, heads, window), q.device)
+    return check(load().gphq_paged_attention(ctypes.byref(kv.desc), ctypes.byref(batch.desc), _dtype(q.dtype), ptr(q),
+                                             qs, heads, scale, window, ptr(out), os_, ptr(work),
+                                             work.numel() * work.element_size(), stream_handle(stream)))
+
+
+def lora_workspace_bytes(rows, k, max_rank):
+    n = load().gphq_lora_workspace_bytes(rows, k, max_rank)
+    return n if n >= 0 else check(n)
+
+
+def lora_add(a, b, x, y, row_slots, ranks=None, scales=None, work=None, stream=None):
+    """gphq_lora_add: y[r] += scales[s] * b[s] (a[s] x[r]), s = row_slots[r],
+    for the rows with a slot in 0 .. slots - 1. a [slots][max_rank][k] and
+    b [slots][n][max_rank]; x [rows][k] and y [rows][n] float32; row_slots and
+    ranks int32, scales float32."""
+    import torch
+
+    _here(a, b, x, y, row_slots, ranks, scales, work)
+    if a.dim() != 3 or b.dim() != 3 or a.dtype != b.dtype or not a.is_contiguous() or not b.is_contiguous():
+        check(ERR_DIMENSIONS)
+    slots, max_rank, k = a.shape
+    n, rows = b.shape[1], x.shape[0] if x.dim() == 2 else -1
+    if b.shape != (slots, n, max_rank) or x.dtype != torch.float32 or y.dtype != torch.float32 or rows < 0:
+        check(ERR_DIMENSIONS)
+    for t, count, dt in ((row_slots, rows, torch.int32), (ranks, slots, torch.int32), (scales, slots, torch.float32)):
+        if t is not None and (t.dtype != dt or not t.is_contiguous() or t.numel() < count):
+            check(ERR_DIMENSIONS)
+    xs, ys = _rows2(x, rows, k, ERR_DIMENSIONS), _rows2(y, rows, n, ERR_DIMENSIONS)
+    if work is None:
+        work = _work(lora_workspace_bytes(rows, k, max_rank), x.device)
+    return check(load().gphq_lora_add(_dtype(a.dtype), ptr(a), ptr(b), ptr(ranks), ptr(scales), slots, max_rank,
+                                      ptr(row_slots), ptr(x), xs, ptr(y), ys, rows, k, n, ptr(work),
+                                      work.numel() * work.element_size(), stream_handle(stream)))
 
 
 # ---- weight preparation (gphq_prepare_projection) ----------------------------

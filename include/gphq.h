@@ -111,6 +111,9 @@ extern "C" {
 #define GPHQ_ERR_CALIBRATION_EMPTY (-42) /* gptq.go:324-326 "qwen3: empty calibration set" */
 #define GPHQ_ERR_CALIBRATION_SHAPE (-43) /* a sequence outside 1..256 tokens (gptqMaxSeq) or more than 4096 rows
                                             (gptqMaxRows); the reference's own sequence builder never makes one */
+/* Paged cache, paged attention and adapters: no reference counterpart. */
+#define GPHQ_ERR_PAGED_SHAPE (-44) /* a pool, batch or buffer whose sizes, strides or alignment do not fit */
+#define GPHQ_ERR_PAGED_BATCH (-45) /* found on the device: a sequence, page number or position out of bounds */
 
 /* The reference message for a status code ("" for GPHQ_OK). Static storage. */
 const char *gphq_error_string(int status);
@@ -527,6 +530,118 @@ int gphq_decode_batch_logits(gphq_decode_batch *ws, const float *hidden_dev, int
  * the last check produced a non-finite hidden value (the reference's error,
  * gpu_darwin.go:1245-1249, which it raises before returning). */
 int gphq_decode_batch_check(gphq_decode_batch *ws, void *stream);
+
+/* ---- paged K/V cache ---------------------------------------------------------
+ * No counterpart in the reference, whose prefixes (gphq_prefix) are private and
+ * contiguous. A pool is memory for `pages` pages of page_tokens tokens of one
+ * layer's keys and values: element (page, token, KV head, dim) of either is at
+ * page * page_stride + token * token_stride + head * head_stride + dim, so the
+ * memory may be in token order ([page][token][head][dim], a prefix's row order)
+ * or in head order ([page][head][token][dim], where a head's keys stand
+ * together), or a view of a larger pool. The caller hands pages out and owns
+ * the memory. dtype: GPHQ_DTYPE_F32, _F16 or _BF16. head_dim: 64 or 128;
+ * page_tokens: a power of two from 16 to GPHQ_PAGED_MAX_PAGE_TOKENS; strides in
+ * elements, multiples of 16 bytes; both pointers 16-byte aligned. */
+#define GPHQ_PAGED_MAX_PAGE_TOKENS 4096
+#define GPHQ_PAGED_MAX_HEADS 1024
+#define GPHQ_PAGED_MAX_SEQS 65536
+#define GPHQ_PAGED_MAX_ROWS (1 << 20)
+#define GPHQ_PAGED_MAX_LEN (1 << 30)
+typedef struct gphq_paged_kv {
+    void *k_dev, *v_dev;
+    int64_t page_stride, token_stride, head_stride;
+    int64_t pages, page_tokens, kv_heads, head_dim;
+    int32_t dtype, reserved;
+} gphq_paged_kv;
+
+/* The sequences of one step, ragged: sequence s brings the rows
+ * starts[s] .. starts[s + 1] - 1 of the call's row buffers, its last tokens of
+ * lens[s] in all (so row i of its n rows is the token at position
+ * lens[s] - n + i), and token p of it lies in slot p % page_tokens of page
+ * table[s * table_stride + p / page_tokens]. All three are device arrays of
+ * int32, read when the work runs: a captured call may be replayed with other
+ * values. rows is what the row buffers hold; rows behind starts[seqs] are left
+ * as they are. max_rows and max_len bound the rows of one sequence and lens;
+ * the work is cut by these bounds, so tight ones are faster. Table entries
+ * that no token of the call needs may hold anything.
+ * The device checks what it reads. A sequence whose starts descend or leave
+ * the rows, with more than max_rows rows, or with lens outside 0 .. max_len is
+ * skipped whole (and where starts descend, others may be with it); a needed page number outside the pool stores nothing and
+ * reads as masked keys; each also sets a bit of *bad_dev (may be NULL), which
+ * gphq_paged_check waits for, reports as GPHQ_ERR_PAGED_BATCH and clears. */
+typedef struct gphq_paged_batch {
+    const int32_t *starts_dev; /* [seqs + 1], ascending */
+    const int32_t *lens_dev;   /* [seqs] */
+    const int32_t *table_dev;  /* [seqs][table_stride] */
+    int64_t table_stride;      /* >= ceil(max_len / page_tokens) */
+    int64_t seqs, rows, max_rows, max_len;
+    int32_t *bad_dev;
+} gphq_paged_batch;
+
+/* What a pass does between the QKV projection and the attention
+ * (gphq_prefill_project proj 0 makes such rows): of each row [heads | KV heads |
+ * KV heads][head_dim] every query and key head is RMS-normalized with weight
+ * q_norm / k_norm (device f32[head_dim]; NULL: not normalized) and rotated by
+ * its position, value l with value l + head_dim / 2 (cos, sin: device
+ * f32[rope_rows][head_dim / 2]; both NULL: not rotated), queries are multiplied
+ * by q_scale and written to q [rows][q_stride], keys and values stored in their
+ * pages. fp32 arithmetic, one rounding per stored value. row_dtype (of qkv and
+ * q): GPHQ_DTYPE_F32, or the pool's. q may be qkv itself (the same address and
+ * stride: queries replace queries), and else must not overlap it. A row whose
+ * position is past the cos table, or before token 0 (lens[s] < its rows), is
+ * skipped and sets *bad_dev. Two rows of one call must not name the same slot
+ * of the same page: sequences may share pages of tokens before the call's.
+ * Rows 16-byte aligned, strides multiples of 16 bytes. */
+int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *qkv_dev,
+                      int64_t qkv_stride, int64_t heads, const float *q_norm_dev, const float *k_norm_dev, double eps,
+                      const float *cos_dev, const float *sin_dev, int64_t rope_rows, double q_scale, void *q_dev,
+                      int64_t q_stride, void *stream);
+
+/* Causal attention of each row over its sequence's pages, the call's own tokens
+ * among them (append them first):
+ *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j][h / (heads / kv_heads)]) v[j][...]
+ * over the tokens j of row i's sequence up to its position p, and with
+ * window > 0 only those past p - window. A row before token 0 sees none and
+ * becomes 0. What a row does not see, whatever it holds (NaN included), does
+ * not reach it. Any number of rows per sequence: prompt chunks and single
+ * tokens may stand in one call. fp32 rows are multiplied to fp32 accuracy
+ * whatever the pool's type; 16-bit rows (the pool's type) round probabilities
+ * to that type before the product with the values. out may not overlap q. work
+ * (16-byte aligned) of at least gphq_paged_attention_workspace_bytes for the
+ * same pool, batch, row type, heads and window; its contents need not be kept
+ * between calls, and calls that may run at the same time need one each. Sums
+ * are taken in a fixed order: the same call gives the same bits. */
+int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype,
+                                             int64_t heads, int64_t window);
+int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q_dev,
+                         int64_t q_stride, int64_t heads, double scale, int64_t window, void *out_dev,
+                         int64_t out_stride, void *work_dev, int64_t work_bytes, void *stream);
+/* Waits for the stream; GPHQ_ERR_PAGED_BATCH if *bad_dev was set, which is then
+ * cleared. */
+int gphq_paged_check(int32_t *bad_dev, void *stream);
+
+/* ---- low-rank adapters beside a shared projection ------------------------------
+ * No counterpart in the reference. After a projection of many requests' rows
+ * (gphq_gemv_vec, gphq_mm, gphq_prefill_project) the adapters that some of them
+ * carry:
+ *   y[r] += scales[s] * B[s] (A[s] x[r]),  s = row_slots[r]
+ * x fp32 [rows][x_stride], y fp32 [rows][y_stride]; A [slots][max_rank][k] and
+ * B [slots][n][max_rank] of dtype (GPHQ_DTYPE_*), adapter s using its first
+ * ranks[s] of max_rank (device int32[slots], taken into 0 .. max_rank; NULL: all;
+ * the rest of its memory is not used) and scales[s] (device f32[slots]; NULL: 1).
+ * row_slots: device int32[rows]; a row whose slot is outside 0 .. slots - 1 has
+ * no adapter and is left as it is. Rows may come in any order; neighbouring rows
+ * of one adapter are fastest. fp32 products and sums in a fixed order.
+ * k % 32 == 0, max_rank % 8 == 0 up to GPHQ_LORA_MAX_RANK, x_stride % 4 == 0;
+ * A, B, x and work 16-byte aligned; y_stride and y are best multiples of 16
+ * bytes. y must not overlap x. work: gphq_lora_workspace_bytes, one per call
+ * that may run at the same time. */
+#define GPHQ_LORA_MAX_RANK 128
+int64_t gphq_lora_workspace_bytes(int64_t rows, int64_t k, int64_t max_rank);
+int gphq_lora_add(int dtype, const void *a_dev, const void *b_dev, const int32_t *ranks_dev, const float *scales_dev,
+                  int64_t slots, int64_t max_rank, const int32_t *row_slots_dev, const float *x_dev, int64_t x_stride,
+                  float *y_dev, int64_t y_stride, int64_t rows, int64_t k, int64_t n, void *work_dev,
+                  int64_t work_bytes, void *stream);
 
 /* ---- weight preparation (prepareGPU's jobs) ---------------------------------
  * Replaces the body of one gpuJob of qwen3lm's prepareGPU

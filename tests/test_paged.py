@@ -1,0 +1,152 @@
+"""CPU checks of the paged cache's and the adapters' entry points: bad arguments are refused before any device work."""
+import ctypes
+
+import pytest
+
+from gophonic_amd import gphq
+
+P = 4096  # a non-null, aligned address that is never read
+
+
+def kv(**over):
+    d = dict(k_dev=P, v_dev=P, page_stride=2048, token_stride=128, head_stride=128, pages=4, page_tokens=16, kv_heads=1,
+             head_dim=128, dtype=gphq.DTYPE_F16, reserved=0)
+    d.update(over)
+    return gphq.PagedKvDesc(*[d[n] for n, _ in gphq.PagedKvDesc._fields_])
+
+
+def batch(**over):
+    d = dict(starts_dev=P, lens_dev=P, table_dev=P, table_stride=4, seqs=2, rows=8, max_rows=4, max_len=64, bad_dev=None)
+    d.update(over)
+    return gphq.PagedBatchDesc(*[d[n] for n, _ in gphq.PagedBatchDesc._fields_])
+
+
+def append(k=None, b=None, **over):
+    d = dict(dtype=gphq.DTYPE_F32, qkv=P, qkv_stride=4 * 128, heads=2, qn=P, kn=P, eps=1e-6, cos=P, sin=P, rope=64,
+             scale=1.0, q=P, q_stride=256)
+    d.update(over)
+    return gphq.load().gphq_paged_append(ctypes.byref(k or kv()), ctypes.byref(b or batch()), *d.values(), None)
+
+
+def attend(k=None, b=None, **over):
+    d = dict(dtype=gphq.DTYPE_F32, q=P, q_stride=256, heads=2, scale=1.0, window=0, out=P + (1 << 20), out_stride=256,
+             work=P, bytes=1 << 30)
+    d.update(over)
+    return gphq.load().gphq_paged_attention(ctypes.byref(k or kv()), ctypes.byref(b or batch()), *d.values(), None)
+
+
+BAD_KV = [
+    (dict(dtype=7), gphq.ERR_UNSUPPORTED), (dict(head_dim=96), gphq.ERR_UNSUPPORTED),
+    (dict(page_tokens=8), gphq.ERR_UNSUPPORTED), (dict(page_tokens=48), gphq.ERR_UNSUPPORTED),
+    (dict(page_tokens=8192), gphq.ERR_UNSUPPORTED), (dict(pages=0), gphq.ERR_PAGED_SHAPE),
+    (dict(pages=1 << 31), gphq.ERR_PAGED_SHAPE), (dict(kv_heads=0), gphq.ERR_PAGED_SHAPE),
+    (dict(token_stride=64), gphq.ERR_PAGED_SHAPE), (dict(token_stride=132), gphq.ERR_PAGED_SHAPE),
+    (dict(page_stride=-2048), gphq.ERR_PAGED_SHAPE), (dict(head_stride=0), gphq.ERR_PAGED_SHAPE),
+    (dict(page_stride=1 << 61), gphq.ERR_PAGED_SHAPE), (dict(k_dev=None), gphq.ERR_PAGED_SHAPE),
+    (dict(v_dev=P + 8), gphq.ERR_PAGED_SHAPE),
+]
+BAD_BATCH = [
+    (dict(seqs=-1), gphq.ERR_PAGED_SHAPE), (dict(rows=-1), gphq.ERR_PAGED_SHAPE),
+    (dict(rows=(1 << 20) + 1), gphq.ERR_PAGED_SHAPE), (dict(seqs=1 << 20), gphq.ERR_PAGED_SHAPE),
+    (dict(max_rows=-1), gphq.ERR_PAGED_SHAPE), (dict(max_len=-1), gphq.ERR_PAGED_SHAPE),
+    (dict(max_len=65), gphq.ERR_PAGED_SHAPE), (dict(table_stride=3), gphq.ERR_PAGED_SHAPE),
+    (dict(table_stride=1 << 31), gphq.ERR_PAGED_SHAPE), (dict(starts_dev=None), gphq.ERR_PAGED_SHAPE),
+    (dict(lens_dev=None), gphq.ERR_PAGED_SHAPE), (dict(table_dev=None), gphq.ERR_PAGED_SHAPE),
+    (dict(bad_dev=P + 2), gphq.ERR_PAGED_SHAPE), (dict(table_dev=P + 2), gphq.ERR_PAGED_SHAPE),
+]
+
+
+@pytest.mark.parametrize("over,want", BAD_KV, ids=lambda v: str(v))
+def test_bad_pools_are_refused(over, want):
+    assert append(kv(**over)) == want
+    assert attend(kv(**over)) == want
+
+
+@pytest.mark.parametrize("over,want", BAD_BATCH, ids=lambda v: str(v))
+def test_bad_batches_are_refused(over, want):
+    assert append(b=batch(**over)) == want
+    assert attend(b=batch(**over)) == want
+
+
+@pytest.mark.parametrize("over,want", [
+    (dict(dtype=gphq.DTYPE_BF16), gphq.ERR_UNSUPPORTED), (dict(dtype=0), gphq.ERR_UNSUPPORTED),
+    (dict(heads=0), gphq.ERR_PAGED_SHAPE), (dict(heads=1025), gphq.ERR_PAGED_SHAPE),
+    (dict(qkv_stride=508), gphq.ERR_PAGED_SHAPE), (dict(qkv_stride=514), gphq.ERR_PAGED_SHAPE),
+    (dict(q_stride=252), gphq.ERR_PAGED_SHAPE), (dict(cos=None), gphq.ERR_PAGED_SHAPE),
+    (dict(sin=None), gphq.ERR_PAGED_SHAPE), (dict(rope=0), gphq.ERR_PAGED_SHAPE), (dict(eps=-1.0), gphq.ERR_PAGED_SHAPE),
+    (dict(eps=float("nan")), gphq.ERR_PAGED_SHAPE), (dict(qkv=None), gphq.ERR_PAGED_SHAPE),
+    (dict(q=P + 4), gphq.ERR_PAGED_SHAPE), (dict(qn=P + 8), gphq.ERR_PAGED_SHAPE),
+], ids=lambda v: str(v))
+def test_append_refuses(over, want):
+    assert append(**over) == want
+
+
+def test_append_refuses_queries_laid_over_other_rows():
+    assert append(q=P + 64, q_stride=512) == gphq.ERR_OVERLAP
+    assert append(q=P, q_stride=256) == gphq.ERR_OVERLAP  # the same address with another stride
+
+
+@pytest.mark.parametrize("over,want", [
+    (dict(dtype=gphq.DTYPE_BF16), gphq.ERR_UNSUPPORTED), (dict(heads=0), gphq.ERR_PAGED_SHAPE),
+    (dict(window=-1), gphq.ERR_PAGED_SHAPE), (dict(q_stride=252), gphq.ERR_PAGED_SHAPE),
+    (dict(out_stride=258), gphq.ERR_PAGED_SHAPE), (dict(q=None), gphq.ERR_PAGED_SHAPE),
+    (dict(out=P + (1 << 20) + 8), gphq.ERR_PAGED_SHAPE), (dict(out=P), gphq.ERR_OVERLAP),
+    (dict(out=P + 1024), gphq.ERR_OVERLAP),
+], ids=lambda v: str(v))
+def test_attention_refuses(over, want):
+    assert attend(**over) == want
+
+
+def test_attention_refuses_a_short_workspace():
+    lib = gphq.load()
+    k, b = kv(pages=1 << 16), batch(max_len=1 << 16, table_stride=1 << 12)
+    need = lib.gphq_paged_attention_workspace_bytes(ctypes.byref(k), ctypes.byref(b), gphq.DTYPE_F32, 2, 0)
+    assert need > 0
+    assert attend(k, b, bytes=need - 1) == gphq.ERR_PAGED_SHAPE
+    assert attend(k, b, work=None) == gphq.ERR_PAGED_SHAPE
+    assert attend(k, b, work=P + 8) == gphq.ERR_PAGED_SHAPE
+    for over in (dict(dtype=gphq.DTYPE_BF16), dict(heads=0), dict(window=-1)):
+        d = dict(dtype=gphq.DTYPE_F32, heads=2, window=0)
+        d.update(over)
+        assert lib.gphq_paged_attention_workspace_bytes(ctypes.byref(k), ctypes.byref(b), *d.values()) < 0
+
+
+def test_null_descriptions_are_refused():
+    lib = gphq.load()
+    assert lib.gphq_paged_attention_workspace_bytes(None, ctypes.byref(batch()), 3, 2, 0) == gphq.ERR_PAGED_SHAPE
+    assert lib.gphq_paged_attention_workspace_bytes(ctypes.byref(kv()), None, 3, 2, 0) == gphq.ERR_PAGED_SHAPE
+    assert lib.gphq_paged_check(None, None) == gphq.ERR_PAGED_SHAPE
+
+
+@pytest.mark.parametrize("over", [dict(seqs=0), dict(rows=0), dict(max_rows=0)], ids=lambda v: str(v))
+def test_an_empty_batch_is_no_work(over):
+    b = batch(starts_dev=P, **over)
+    assert append(b=b) == gphq.OK
+    assert attend(b=b) == gphq.OK
+    assert gphq.load().gphq_paged_attention_workspace_bytes(ctypes.byref(kv()), ctypes.byref(b), 3, 2, 0) == 0
+
+
+def lora(**over):
+    d = dict(dtype=gphq.DTYPE_BF16, a=P, b=P, ranks=P, scales=P, slots=2, max_rank=16, row_slots=P, x=P, x_stride=64,
+             y=P + (1 << 20), y_stride=40, rows=3, k=64, n=40, work=P, bytes=1 << 24)
+    d.update(over)
+    return gphq.load().gphq_lora_add(*d.values(), None)
+
+
+@pytest.mark.parametrize("over,want", [
+    (dict(dtype=9), gphq.ERR_UNSUPPORTED), (dict(slots=-1), gphq.ERR_DIMENSIONS), (dict(max_rank=12), gphq.ERR_DIMENSIONS),
+    (dict(max_rank=136), gphq.ERR_DIMENSIONS), (dict(k=48), gphq.ERR_DIMENSIONS), (dict(k=-32), gphq.ERR_DIMENSIONS),
+    (dict(n=-1), gphq.ERR_DIMENSIONS), (dict(rows=-1), gphq.ERR_DIMENSIONS), (dict(x_stride=60), gphq.ERR_DIMENSIONS),
+    (dict(x_stride=66), gphq.ERR_DIMENSIONS), (dict(y_stride=39), gphq.ERR_DIMENSIONS), (dict(a=None), gphq.ERR_DIMENSIONS),
+    (dict(row_slots=None), gphq.ERR_DIMENSIONS), (dict(x=P + 8), gphq.ERR_DIMENSIONS), (dict(b=P + 8), gphq.ERR_DIMENSIONS),
+    (dict(work=None), gphq.ERR_DIMENSIONS), (dict(bytes=191), gphq.ERR_DIMENSIONS), (dict(y=P + 2), gphq.ERR_DIMENSIONS),
+    (dict(y=P), gphq.ERR_OVERLAP),
+], ids=lambda v: str(v))
+def test_lora_refuses(over, want):
+    assert lora(**over) == want
+
+
+@pytest.mark.parametrize("over", [dict(rows=0), dict(n=0), dict(slots=0), dict(max_rank=0), dict(k=0, x_stride=0)],
+                         ids=lambda v: str(v))
+def test_lora_without_work_is_ok(over):
+    assert lora(**over) == gphq.OK
