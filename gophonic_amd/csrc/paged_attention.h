@@ -30,11 +30,13 @@ struct AttnArgs {
     int heads, group, window;
     int parts;             // split slots per (row, head) in the workspace
     int small_cols;        // sequences of at most this many columns are the row kernel's
+    int big_tile;          // columns of the chunk kernel's tiles
+    float q_sign;          // the sign of scale (0 if scale is 0), applied to the queries
     int split_small, split_big;  // keys per split in each kernel, multiples of 128
-    float scale_log2;
+    float scale_log2;      // |scale| log2(e) (1 if scale is 0): positive, so the largest score stays the largest
 };
 
-constexpr int kSmallTile = 16, kBigTile = 128;
+constexpr int kSmallTile = 16;
 constexpr float kLag = 8.0f;    // the reference maximum may be passed by this much (in log2)
 constexpr float kLift = 7.0f;   // exponentials are 2^(x - m + 7): at most 2^15, so that FP16
                                 // probabilities keep 2^-24 of a 2^7 .. 2^15 maximum, not of 1
@@ -55,6 +57,11 @@ __device__ __forceinline__ TileKeys tile_keys(int n, int len, int r0, int r1, in
 __device__ __forceinline__ int tile_splits(const TileKeys &t, int split_len) {
     return t.hi > t.lo ? (t.hi - t.from + split_len - 1) / split_len : 1;
 }
+
+// A key that some rows of a tile see and others do not may hold values that are not finite,
+// and a masked probability times one is NaN, not 0. So in a step with such keys V's values
+// that are not finite are taken out of the products, and added to the columns that do see
+// their key (a probability is positive) in a loop over the keys that have any.
 
 // 16-bit types: conversion, matrix instructions, packed tests.
 template <typename T>
@@ -101,6 +108,9 @@ __device__ __forceinline__ void split_pieces(float v, CT (&out)[NP]) {
     }
 }
 
+// A positive factor of the scores that -inf times it stays -inf.
+__device__ __forceinline__ float score_factor(float f) { return fmaxf(f, 0x1p-126f); }
+
 // 2^e that brings a largest magnitude m into [2^13, 2^14) (1 for 0, Inf and NaN), with
 // both it and its inverse normal.
 __device__ __forceinline__ float f16_scale(float m, float &inverse) {
@@ -109,12 +119,19 @@ __device__ __forceinline__ float f16_scale(float m, float &inverse) {
     return __builtin_amdgcn_ldexpf(1.0f, e);
 }
 
-// Whether either half of a packed pair has an all-ones exponent (Inf or NaN).
+// A value that is not finite, 0 for one that is.
+__device__ __forceinline__ float not_finite(float v) { return fabsf(v) < INFINITY ? 0.0f : v; }
+
+// Of a packed pair, the halves with an all-ones exponent (Inf or NaN), as a mask.
 template <typename T>
-__device__ __forceinline__ bool pair_not_finite(int x) {
+__device__ __forceinline__ int pair_not_finite(int x) {
     constexpr int e = Half<T>::kExp;
-    return (x & e) == e || (x & (e << 16)) == (e << 16);
+    return ((x & e) == e ? 0xFFFF : 0) | ((x & (e << 16)) == (e << 16) ? 0xFFFF0000 : 0);
 }
+
+// Wavefronts, of 32 columns each, in a block of the chunk kernel.
+template <typename RT, typename CT>
+constexpr int kChunkWaves = kPieces<RT, CT> > 1 ? 8 : 4;
 
 template <typename RT, typename CT>
 int attn_rows_launch(const AttnArgs &a, int hd, int splits, int tiles, hipStream_t st);

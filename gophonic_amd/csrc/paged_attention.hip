@@ -1,5 +1,7 @@
 // gphq_paged_attention: argument checks, the cut of a batch into tiles and splits, and the
 // join of split results. Kernels: paged_rows.hip and paged_chunk.hip.
+#include <math.h>
+
 #include "paged_attention.h"
 
 namespace gphq {
@@ -57,7 +59,7 @@ void cut(int64_t span, int64_t want, int &len, int &splits) {
 }
 
 // From host numbers alone, so a captured call keeps its cut whatever the lengths become.
-AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window) {
+AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int big_tile) {
     AttnPlan p{};
     const int64_t cus = device_cus(), rows = b.rows, cols = (int64_t)b.max_rows * group;
     // Sequences of up to 32 columns run in the row kernel, in tiles of 16; a call of one
@@ -73,9 +75,9 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window) {
     }
     if (cols > p.small_cols) {
         const int64_t all = rows * group;
-        p.big_tiles = (int)(all / kBigTile + std::min<int64_t>(b.seqs, all / (p.small_cols + 1)));
+        p.big_tiles = (int)(all / big_tile + std::min<int64_t>(b.seqs, all / (p.small_cols + 1)));
         const int64_t units = (int64_t)p.big_tiles * kv_heads;
-        cut(span(kBigTile), units >= cus ? 1 : (2 * cus + units - 1) / units, p.big_len, p.big_splits);
+        cut(span(big_tile), units >= cus ? 1 : (2 * cus + units - 1) / units, p.big_len, p.big_splits);
     }
     p.parts = std::max(p.small_tiles ? p.small_splits : 1, p.big_tiles ? p.big_splits : 1);
     return p;
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
     if (row < s.start || row >= s.end || !seq_ok(a.b, s.start, s.end, s.len)) return;
     const int n = s.end - s.start, i = row - s.start, cols = n * a.group;
     const bool small = cols <= a.small_cols;
-    const int tm = small ? kSmallTile : kBigTile, c0 = (i * a.group + head % a.group) / tm * tm;
+    const int tm = small ? kSmallTile : a.big_tile, c0 = (i * a.group + head % a.group) / tm * tm;
     const TileKeys k = tile_keys(n, s.len, c0 / a.group, min((c0 + tm - 1) / a.group, n - 1), a.window);
     const int splits = tile_splits(k, small ? a.split_small : a.split_big);
     if (splits == 1) return;
@@ -153,6 +155,10 @@ int attn_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, int row_dtype,
     a.heads = (int)heads;
     a.group = (int)(heads / kv->kv_heads);
     a.window = window >= b->max_len ? 0 : (int)window;  // a window as long as any sequence hides nothing
+    const bool f16c = kv->dtype == GPHQ_DTYPE_F16;
+    a.big_tile = 32 * (kv->dtype == GPHQ_DTYPE_F32 ? kChunkWaves<float, float>
+                       : row_dtype == kv->dtype    ? (f16c ? kChunkWaves<f16, f16> : kChunkWaves<bf16, bf16>)
+                                                   : (f16c ? kChunkWaves<float, f16> : kChunkWaves<float, bf16>));
     return GPHQ_OK;
 }
 
@@ -168,7 +174,7 @@ int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq
     AttnArgs a{};
     GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
     if (a.b.rows == 0) return 0;
-    return work_bytes_of(attn_plan(a.b, a.pool.kv_heads, a.group, a.window), a.b.rows, heads, kv->head_dim);
+    return work_bytes_of(attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile), a.b.rows, heads, kv->head_dim);
 }
 
 int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
@@ -177,14 +183,14 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     AttnArgs a{};
     GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
     const int64_t hd = kv->head_dim, size = row_dtype == GPHQ_DTYPE_F32 ? 4 : 2;
-    if (q_stride < heads * hd || out_stride < heads * hd || q_stride * size % 16 || out_stride * size % 16)
+    if (!(fabs(scale) <= 1e30) || q_stride < heads * hd || out_stride < heads * hd || q_stride * size % 16 || out_stride * size % 16)
         return GPHQ_ERR_PAGED_SHAPE;
     if (a.b.rows == 0) return GPHQ_OK;
     if (!q || !out || ((uintptr_t)q | (uintptr_t)out) % 16) return GPHQ_ERR_PAGED_SHAPE;
     if (spans_overlap(q, span_bytes(a.b.rows, q_stride, heads * hd, size), out,
                       span_bytes(a.b.rows, out_stride, heads * hd, size)))
         return GPHQ_ERR_OVERLAP;
-    const AttnPlan p = attn_plan(a.b, a.pool.kv_heads, a.group, a.window);
+    const AttnPlan p = attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile);
     if (p.parts > 1 && (!work || (uintptr_t)work % 16 || work_bytes < work_bytes_of(p, a.b.rows, heads, hd)))
         return GPHQ_ERR_PAGED_SHAPE;
     a.q = q;
@@ -197,7 +203,8 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     a.small_cols = p.small_cols;
     a.split_small = p.small_len;
     a.split_big = p.big_len;
-    a.scale_log2 = (float)(scale * 1.4426950408889634);
+    a.q_sign = scale > 0 ? 1.0f : scale < 0 ? -1.0f : 0.0f;
+    a.scale_log2 = scale == 0 ? 1.0f : (float)(fabs(scale) * 1.4426950408889634);
     hipStream_t st = (hipStream_t)stream;
     if (row_dtype == GPHQ_DTYPE_F32) {
         if (kv->dtype == GPHQ_DTYPE_F32) return attend<float, float>(a, p, (int)hd, st);

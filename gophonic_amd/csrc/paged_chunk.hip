@@ -7,11 +7,11 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// One block's tile: 128 columns of a sequence and KV head, 32 to each of four wavefronts,
-// over the keys [k0, k1).
+// One block's tile: TM columns of a sequence and KV head, 32 to each wavefront, over the keys [k0, k1).
 struct ChunkTile {
     int seq, g, n, len, start, splits, split;
     int lo, hi, k0, k1;
+    int b_p0, b_p1;  // positions of the tile's first and last row
     // this wavefront's rows and their keys [w_lo, w_hi)
     int r0, r1, p0, p1, w_lo, w_hi;
     // this lane's column
@@ -22,6 +22,7 @@ struct ChunkTile {
 // The block's tile among those of the sequences that are not the row kernel's, counted by
 // 64 lanes over 64 sequences at a time. Tiles are dealt out from the back: a sequence's last
 // rows see most keys, so the long tiles start first. False where there is no such tile.
+template <int TM>
 __device__ __forceinline__ bool chunk_tile(const AttnArgs &a, int tiles, int splits, ChunkTile &t) {
     int u = blockIdx.x;
     t.g = u % a.pool.kv_heads;
@@ -36,7 +37,7 @@ __device__ __forceinline__ bool chunk_tile(const AttnArgs &a, int tiles, int spl
         const bool ok = seq_ok(a.b, start, end, len);
         if (!ok) paged_flag(a.b, PAGED_BAD_SEQ);
         const int cols = ok ? (end - start) * a.group : 0;
-        const int mine = s0 + lane < a.b.seqs && cols > a.small_cols ? (cols + kBigTile - 1) / kBigTile : 0;
+        const int mine = s0 + lane < a.b.seqs && cols > a.small_cols ? (cols + TM - 1) / TM : 0;
         int sum = mine;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -56,11 +57,13 @@ __device__ __forceinline__ bool chunk_tile(const AttnArgs &a, int tiles, int spl
         before += total;
     }
     if (tile < 0) return false;
-    const int cols = t.n * a.group, c0 = tile * kBigTile, off = t.len - t.n;
+    const int cols = t.n * a.group, c0 = tile * TM, off = t.len - t.n;
     const TileKeys k =
-        tile_keys(t.n, t.len, c0 / a.group, min((c0 + kBigTile - 1) / a.group, t.n - 1), a.window);
+        tile_keys(t.n, t.len, c0 / a.group, min((c0 + TM - 1) / a.group, t.n - 1), a.window);
     t.lo = k.lo;
     t.hi = k.hi;
+    t.b_p0 = off + c0 / a.group;
+    t.b_p1 = off + min((c0 + TM - 1) / a.group, t.n - 1);
     t.splits = tile_splits(k, a.split_big);
     if (t.split >= t.splits) return false;
     t.k0 = k.from + t.split * a.split_big;
@@ -98,6 +101,11 @@ __device__ __forceinline__ int64_t chunk_keys(const AttnArgs &a, const ChunkTile
            t.g * a.pool.head_stride;
 }
 
+// A step that holds keys which some row of the tile does not see.
+__device__ __forceinline__ bool chunk_edge(const AttnArgs &a, const ChunkTile &t, int kt, int keys) {
+    return kt + keys - 1 > t.b_p0 || kt < t.lo || (a.window > 0 && kt < t.b_p1 - a.window + 1);
+}
+
 // One step's exponentials over N 32-key score tiles: s[h][r] is key kt + 32 h + 8 (r / 4) +
 // 4 hi + r % 4; as the row kernel's softmax_step. ok: a bit per 16 keys.
 template <int N>
@@ -105,8 +113,6 @@ __device__ __forceinline__ float chunk_softmax(const ChunkTile &t, f32x16 (&s)[N
                                                unsigned ok, float &m, float &l, bool &moved) {
     const int hi = (threadIdx.x & 63) >> 5;
     float mx = -INFINITY;
-#pragma unroll
-    for (int h = 0; h < N; ++h) s[h] *= fac;
     if (masked) {
 #pragma unroll
         for (int h = 0; h < N; ++h)
@@ -120,7 +126,7 @@ __device__ __forceinline__ float chunk_softmax(const ChunkTile &t, f32x16 (&s)[N
     for (int h = 0; h < N; ++h)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[h][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mx = fmaxf(mx, __shfl_xor(mx, 32)) * fac;
     const bool grew = mx > m + kLag;
     const float mn = grew ? mx : m;
     const float ref = mn == -INFINITY ? 0.0f : mn - kLift;
@@ -131,7 +137,7 @@ __device__ __forceinline__ float chunk_softmax(const ChunkTile &t, f32x16 (&s)[N
     for (int h = 0; h < N; ++h)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[h][r] = __builtin_amdgcn_exp2f(s[h][r] - ref);
+            s[h][r] = __builtin_amdgcn_exp2f(fmaf(s[h][r], fac, -ref));
             sum += s[h][r];
         }
     l = l * corr + sum;
@@ -167,7 +173,7 @@ __device__ __forceinline__ void chunk_finish(const AttnArgs &a, const ChunkTile 
     }
 }
 
-// 16-bit pages. Each step's 64 keys are staged once for the block's 128 columns: K as rows,
+// 16-bit pages. Each step's 64 keys are staged once for the block's 32 NW columns: K as rows,
 // V transposed, [dim][key], by exchanging 16-bit halves between the four keys that a thread
 // loads; both with their 16-byte pieces permuted within a row, so that the fragment reads
 // of 16 consecutive rows and the stores fall on all banks. On v_mfma_f32_32x32x16:
@@ -177,21 +183,22 @@ __device__ __forceinline__ void chunk_finish(const AttnArgs &a, const ChunkTile 
 //     and 12-15, and V^T's rows are stored in that order.
 // Two LDS buffers, one barrier a step: step u + 1 is loaded into registers while step u is
 // multiplied.
-template <typename RT, typename CT, int HD>
-__global__ __launch_bounds__(256) void attn_chunk16_kernel(const AttnArgs a, int tiles, int splits) {
+template <typename RT, typename CT, int HD, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs a, int tiles, int splits) {
     typedef Half<CT> H;
     typedef typename H::vec8 vec8;
-    constexpr int NP = kPieces<RT, CT>, KB = 64, QC = HD / 16, DT = HD / 32, VD = HD / 16, VW = VD / 2;
-    constexpr int KI = KB * HD / 8 / 256;   // 16-byte pieces of K per thread
-    constexpr int KP = HD / 8;              // pieces per key
+    constexpr int NT = 64 * NW, NP = kPieces<RT, CT>, KB = 64, QC = HD / 16, DT = HD / 32;
+    constexpr int KP = HD / 8, KI = KB * KP / NT;        // 16-byte pieces of K per key, per thread
+    constexpr int DG = NT / 16, VD = HD / DG, VW = VD / 2;  // V: dim groups, dims and dwords of each per thread
     __shared__ CT Ks[2][KB * HD];
     __shared__ CT Vt[2][HD * KB];
+    __shared__ int odd[2][KB];  // for each key of a buffer, the step (its first key) whose V[key] is not all finite
     ChunkTile t;
-    if (!chunk_tile(a, tiles, splits, t)) return;
+    if (!chunk_tile<32 * NW>(a, tiles, splits, t)) return;
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, q = lane & 31, hi = lane >> 5;
     const CT *kp = (const CT *)a.pool.k, *vp = (const CT *)a.pool.v;
 
-    float fac = a.scale_log2;
+    float fac = score_factor(a.scale_log2);
     vec8 qf[NP][QC];
     {
         const RT *src = (const RT *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 8 * hi;
@@ -207,8 +214,9 @@ __global__ __launch_bounds__(256) void attn_chunk16_kernel(const AttnArgs a, int
             }
             m = fmaxf(m, __shfl_xor(m, 32));
             up = f16_scale(m, inverse);
-            fac *= inverse;
+            fac = score_factor(fac * inverse);
         }
+        up *= a.q_sign;
 #pragma unroll
         for (int i = 0; i < 2 * QC; ++i) {
             float x[4];
@@ -226,37 +234,43 @@ __global__ __launch_bounds__(256) void attn_chunk16_kernel(const AttnArgs a, int
     typedef int vrow __attribute__((ext_vector_type(VW)));
     i32x4 kr[KI];
     vrow vr[4];
-    const int krow = tid / KP, kpc = tid % KP;    // K: piece kpc of keys krow + i * (256 / KP)
-    const int vkg = tid >> 4, vdg = tid & 15;     // V: keys 4 vkg .. 4 vkg + 3 of dims VD vdg ..
+    const int krow = tid / KP, kpc = tid % KP;  // K: piece kpc of keys krow + i * (NT / KP)
+    const int vkg = tid / DG, vdg = tid % DG;   // V: keys 4 vkg .. 4 vkg + 3 of dims VD vdg ..
+    const int vtile = wave * (64 / DG) / 4;     // the 16 keys that vkg lies in
     auto load = [&](int kt) __attribute__((always_inline)) -> unsigned {
         bool ok[4];
         int64_t at[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) at[i] = chunk_keys(a, t, kt + 16 * i, ok[i]);
+        auto pick = [&](int i) { return i == 0 ? at[0] : i == 1 ? at[1] : i == 2 ? at[2] : at[3]; };
 #pragma unroll
-        for (int i = 0; i < KI; ++i) {
-            const int64_t base = KI == 4 ? at[i] : wave < 2 ? at[2 * i % 4] : at[(2 * i + 1) % 4];
-            kr[i] = *(const i32x4 *)(kp + base + (krow & 15) * a.pool.token_stride + 8 * kpc);
-        }
-        const int64_t base = wave == 0 ? at[0] : wave == 1 ? at[1] : wave == 2 ? at[2] : at[3];
+        for (int i = 0; i < KI; ++i)
+            kr[i] = *(const i32x4 *)(kp + pick((wave * 64 + i * NT) / KP / 16) + (krow + i * (NT / KP)) % 16 * a.pool.token_stride + 8 * kpc);
+        const CT *src = vp + pick(vtile) + 4 * (vkg & 3) * a.pool.token_stride + VD * vdg;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            vr[i] = *(const vrow *)(vp + base + (4 * (vkg & 3) + i) * a.pool.token_stride + VD * vdg);
+        for (int i = 0; i < 4; ++i) vr[i] = *(const vrow *)(src + i * a.pool.token_stride);
         return (unsigned)ok[0] | (unsigned)ok[1] << 1 | (unsigned)ok[2] << 2 | (unsigned)ok[3] << 3;
     };
     auto store = [&](int kt, unsigned ok, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < KI; ++i) {
-            const int row = krow + i * (256 / KP);
+            const int row = krow + i * (NT / KP);
             const int pc = HD == 128 ? kpc ^ (row & 15) : kpc ^ ((row >> 1) & 7);
             *(i32x4 *)(Ks[buf] + row * HD + 8 * pc) = kr[i];
         }
-        if (kt < t.lo || kt + KB > t.hi || ok != 15) {
-            // What no row of the tile sees may hold anything: 0 times it must stay 0.
+        if (chunk_edge(a, t, kt, KB) || ok != 15) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int key = kt + 4 * vkg + i;
-                if (key < t.lo || key >= t.hi || !(ok >> wave & 1)) vr[i] = vrow{};
+                if (key < t.lo || key >= t.hi || !(ok >> vtile & 1)) vr[i] = vrow{};  // no row of the tile sees it
+                int any = 0;
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    const int out = pair_not_finite<CT>(vr[i][w]);
+                    vr[i][w] &= ~out;
+                    any |= out;
+                }
+                if (any) odd[buf][key - kt] = kt;
             }
         }
         // Key group vkg goes to position group {0, 2, 1, 3}[vkg % 4] of its 16 keys.
@@ -271,13 +285,20 @@ __global__ __launch_bounds__(256) void attn_chunk16_kernel(const AttnArgs a, int
             *(i32x2 *)(Vt[buf] + d * KB + 8 * unit + 4 * (pg & 1)) = x;
         }
     };
+    auto v_frag = [&](int buf, int ks, int d) __attribute__((always_inline)) {
+        const int dim = 32 * d + q;
+        const int unit = (2 * ks + hi) ^ (((dim >> 1) ^ (dim >> 4)) & 7);
+        return *(const i32x4 *)(Vt[buf] + dim * KB + 8 * unit);
+    };
 
     f32x16 o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = f32x16{};
     float m = -INFINITY, l = 0.0f;
+    if (tid < 2 * KB) (&odd[0][0])[tid] = -1;
     unsigned ok = t.k0 < t.k1 ? load(t.k0) : 0;
     int buf = 0;
+    __syncthreads();
     for (int kt = t.k0; kt < t.k1; kt += KB, buf ^= 1) {
         store(kt, ok, buf);
         __syncthreads();
@@ -303,7 +324,6 @@ __global__ __launch_bounds__(256) void attn_chunk16_kernel(const AttnArgs a, int
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] *= corr;
         }
-        const bool check = masked && t.r0 != t.r1;
 #pragma unroll
         for (int ks = 0; ks < KB / 16; ++ks) {
             vec8 pf[NP];
@@ -316,36 +336,28 @@ __global__ __launch_bounds__(256) void attn_chunk16_kernel(const AttnArgs a, int
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const int dim = 32 * d + q;
-                const int unit = (2 * ks + hi) ^ (((dim >> 1) ^ (dim >> 4)) & 7);
-                const i32x4 f = *(const i32x4 *)(Vt[buf] + dim * KB + 8 * unit);
-                bool odd = false;  // a value that is not finite, which a row must not meet
-                if (check) {
+                const int dim = 32 * d + q, unit = (2 * ks + hi) ^ (((dim >> 1) ^ (dim >> 4)) & 7);
+                const vec8 f = *(const vec8 *)(Vt[buf] + dim * KB + 8 * unit);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) odd |= pair_not_finite<CT>(f[j]);
-                    odd = __any(odd);
-                }
-                if (!odd) {
-#pragma unroll
-                    for (int k = 0; k < NP; ++k) o[d] = H::mfma32(__builtin_bit_cast(vec8, f), pf[k], o[d]);
-                    continue;
-                }
-                // Row by row, with the values its own mask leaves.
-                for (int r = t.r0; r <= t.r1; ++r) {
-                    const int pos = t.len - t.n + r, first = a.window > 0 ? pos - a.window + 1 : 0;
-                    i32x4 fr;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int k0 = kt + 16 * ks + 8 * (j >> 1) + 4 * hi + 2 * (j & 1);
-                        fr[j] = f[j] & ((k0 <= pos && k0 >= first ? 0xFFFF : 0) |
-                                        (k0 + 1 <= pos && k0 + 1 >= first ? 0xFFFF0000 : 0));
-                    }
-                    f32x16 add{};
-#pragma unroll
-                    for (int k = 0; k < NP; ++k) add = H::mfma32(__builtin_bit_cast(vec8, fr), pf[k], add);
-                    if (t.row == r) o[d] += add;
-                }
+                for (int k = 0; k < NP; ++k) o[d] = H::mfma32(f, pf[k], o[d]);
             }
+        }
+        if (!chunk_edge(a, t, kt, KB) && okc == 15) continue;
+        for (uint64_t left = __ballot(odd[buf][lane] == kt); left; left &= left - 1) {
+            const int key = kt + __builtin_ctzll(left);
+            bool in;
+            const CT *v = vp + chunk_keys(a, t, key & ~15, in) + (key & 15) * a.pool.token_stride;
+            const bool sees = key <= t.pos && key >= t.first;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float x[4];
+                    load_vec(v + 32 * d + 8 * j + 4 * hi, x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[d][4 * j + e] += sees ? not_finite(x[e]) : 0.0f;
+                    asm volatile("" ::: "memory");  // few values at a time: this must not cost registers
+                }
         }
     }
     chunk_finish<RT, HD>(a, t, m, l, [&](int i) {
@@ -358,22 +370,24 @@ __global__ __launch_bounds__(256) void attn_chunk16_kernel(const AttnArgs a, int
 // fp32 pages, the same walk in 32-key steps on v_mfma_f32_32x32x2_f32. Its operands are one
 // fp32 value a lane, so V is staged as rows; a lane takes HD / 32 neighbouring dims of V at
 // once, one for each of its output tiles: tile d holds dims HD/32 * i + d.
-template <int HD>
-__global__ __launch_bounds__(256) void attn_chunk32_kernel(const AttnArgs a, int tiles, int splits) {
-    constexpr int KB = 32, QC = HD / 8, DT = HD / 32;
-    constexpr int KP = HD / 4, KI = KB * KP / 256;  // 16-byte pieces per key, per thread
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a, int tiles, int splits) {
+    constexpr int NT = 64 * NW, KB = 32, QC = HD / 8, DT = HD / 32;
+    constexpr int KP = HD / 4, KI = KB * KP / NT;  // 16-byte pieces per key, per thread
     __shared__ float Ks[2][KB * HD];
     __shared__ float Vs[2][KB * HD];
+    __shared__ int odd[2][KB];  // for each key of a buffer, the step (its first key) whose V[key] is not all finite
     ChunkTile t;
-    if (!chunk_tile(a, tiles, splits, t)) return;
-    const int tid = threadIdx.x, lane = tid & 63, q = lane & 31, hi = lane >> 5;
+    if (!chunk_tile<32 * NW>(a, tiles, splits, t)) return;
+    const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, q = lane & 31, hi = lane >> 5;
     const float *kp = (const float *)a.pool.k, *vp = (const float *)a.pool.v;
     f32x4 qf[QC];
     {
         const float *src = (const float *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 4 * hi;
 #pragma unroll
-        for (int i = 0; i < QC; ++i) qf[i] = *(const f32x4 *)(src + 8 * i);
+        for (int i = 0; i < QC; ++i) qf[i] = *(const f32x4 *)(src + 8 * i) * a.q_sign;
     }
+    typedef float vdim __attribute__((ext_vector_type(DT)));
     f32x4 kr[KI], vr[KI];
     const int krow = tid / KP, kpc = tid % KP;
     auto load = [&](int kt) __attribute__((always_inline)) -> unsigned {
@@ -383,20 +397,28 @@ __global__ __launch_bounds__(256) void attn_chunk32_kernel(const AttnArgs a, int
         at[1] = chunk_keys(a, t, kt + 16, ok[1]);
 #pragma unroll
         for (int i = 0; i < KI; ++i) {
-            const int row = krow + i * (256 / KP);
-            const int64_t off = at[i * (256 / KP) / 16] + (row & 15) * a.pool.token_stride + 4 * kpc;
+            const int row = krow + i * (NT / KP);
+            const int64_t base = (wave * 64 + i * NT) / KP < 16 ? at[0] : at[1];  // the same for a wavefront's rows
+            const int64_t off = base + (row & 15) * a.pool.token_stride + 4 * kpc;
             kr[i] = *(const f32x4 *)(kp + off);
             vr[i] = *(const f32x4 *)(vp + off);
         }
         return (unsigned)ok[0] | (unsigned)ok[1] << 1;
     };
     auto store = [&](int kt, unsigned ok, int buf) __attribute__((always_inline)) {
+        const bool edge = chunk_edge(a, t, kt, KB) || ok != 3;
 #pragma unroll
         for (int i = 0; i < KI; ++i) {
-            const int row = krow + i * (256 / KP), key = kt + row;
+            const int row = krow + i * (NT / KP), key = kt + row;
             *(f32x4 *)(Ks[buf] + row * HD + 4 * (kpc ^ (row & 15))) = kr[i];
-            // What no row of the tile sees may hold anything: 0 times it must stay 0.
-            if (key < t.lo || key >= t.hi || !(ok >> (row >> 4) & 1)) vr[i] = f32x4{};
+            if (edge) {
+                if (key < t.lo || key >= t.hi || !(ok >> (row >> 4) & 1)) vr[i] = f32x4{};  // no row of the tile sees it
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!(fabsf(vr[i][e]) < INFINITY)) vr[i][e] = 0.0f, any = true;
+                if (any) odd[buf][row] = kt;
+            }
             *(f32x4 *)(Vs[buf] + row * HD + 4 * kpc) = vr[i];
         }
     };
@@ -404,8 +426,10 @@ __global__ __launch_bounds__(256) void attn_chunk32_kernel(const AttnArgs a, int
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = f32x16{};
     float m = -INFINITY, l = 0.0f;
+    if (tid < 2 * KB) (&odd[0][0])[tid] = -1;
     unsigned ok = t.k0 < t.k1 ? load(t.k0) : 0;
     int buf = 0;
+    __syncthreads();
     for (int kt = t.k0; kt < t.k1; kt += KB, buf ^= 1) {
         store(kt, ok, buf);
         __syncthreads();
@@ -422,37 +446,29 @@ __global__ __launch_bounds__(256) void attn_chunk32_kernel(const AttnArgs a, int
         const bool masked =
             kt + KB - 1 > t.p0 || kt < t.w_lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 3;
         bool moved;
-        const float corr = chunk_softmax(t, s, a.scale_log2, masked, kt, okc, m, l, moved);
+        const float corr = chunk_softmax(t, s, score_factor(a.scale_log2), masked, kt, okc, m, l, moved);
         if (moved) {
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] *= corr;
         }
-        const bool check = masked && t.r0 != t.r1;
-        typedef float vdim __attribute__((ext_vector_type(DT)));
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int key = kt + 8 * (r >> 2) + 4 * hi + (r & 3);
-            const vdim v = *(const vdim *)(Vs[buf] + (key - kt) * HD + DT * q);
-            bool odd = false;  // a value that is not finite, which a row must not meet
-            if (check) {
+            const vdim v = *(const vdim *)(Vs[buf] + (8 * (r >> 2) + 4 * hi + (r & 3)) * HD + DT * q);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) odd |= !(fabsf(v[d]) < INFINITY);
-                odd = __any(odd);
-            }
+            for (int d = 0; d < DT; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[d], s[0][r], o[d], 0, 0, 0);
+        }
+        if (!chunk_edge(a, t, kt, KB) && okc == 3) continue;
+        for (uint64_t left = __ballot(lane < KB && odd[buf][lane % KB] == kt); left; left &= left - 1) {
+            const int key = kt + __builtin_ctzll(left);
+            bool in;
+            const float *v = vp + chunk_keys(a, t, key & ~15, in) + (key & 15) * a.pool.token_stride;
+            const bool sees = key <= t.pos && key >= t.first;
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                if (!odd) {
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[d], s[0][r], o[d], 0, 0, 0);
-                    continue;
-                }
-                // Row by row, with the values its own mask leaves.
-                for (int i = t.r0; i <= t.r1; ++i) {
-                    const int pos = t.len - t.n + i, first = a.window > 0 ? pos - a.window + 1 : 0;
-                    f32x16 add{};
-                    add = __builtin_amdgcn_mfma_f32_32x32x2f32(key <= pos && key >= first ? v[d] : 0.0f, s[0][r], add,
-                                                               0, 0, 0);
-                    if (t.row == i) o[d] += add;
-                }
+            for (int r = 0; r < 16; ++r) {
+                const vdim x = *(const vdim *)(v + DT * (8 * (r >> 2) + 4 * hi + (r & 3)));
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d][r] += sees ? not_finite(x[d]) : 0.0f;
+                asm volatile("" ::: "memory");  // few values at a time: this must not cost registers
             }
         }
     }
@@ -463,7 +479,6 @@ __global__ __launch_bounds__(256) void attn_chunk32_kernel(const AttnArgs a, int
     const float inv = 1.0f / l;
     float *out = (float *)a.out + (int64_t)(t.start + t.row) * a.out_stride + t.head * HD;
     const int64_t at = ((int64_t)(t.start + t.row) * a.heads + t.head) * a.parts + t.split;
-    typedef float vdim __attribute__((ext_vector_type(DT)));
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         const int d0 = DT * (8 * (r >> 2) + 4 * hi + (r & 3));
@@ -483,16 +498,19 @@ __global__ __launch_bounds__(256) void attn_chunk32_kernel(const AttnArgs a, int
 template <typename RT, typename CT>
 int attn_chunk_launch(const AttnArgs &a, int hd, int splits, int tiles, hipStream_t st) {
     const unsigned blocks = (unsigned)tiles * (unsigned)splits * (unsigned)a.pool.kv_heads;
+    constexpr int NW = kChunkWaves<RT, CT>;
     if constexpr (std::is_same<CT, float>::value) {
         if (hd == 128)
-            hipLaunchKernelGGL((attn_chunk32_kernel<128>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+            hipLaunchKernelGGL((attn_chunk32_kernel<128, NW>), dim3(blocks), dim3(64 * NW), 0, st, a, tiles, splits);
         else
-            hipLaunchKernelGGL((attn_chunk32_kernel<64>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+            hipLaunchKernelGGL((attn_chunk32_kernel<64, NW>), dim3(blocks), dim3(64 * NW), 0, st, a, tiles, splits);
     } else {
         if (hd == 128)
-            hipLaunchKernelGGL((attn_chunk16_kernel<RT, CT, 128>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+            hipLaunchKernelGGL((attn_chunk16_kernel<RT, CT, 128, NW>), dim3(blocks), dim3(64 * NW), 0, st, a, tiles,
+                               splits);
         else
-            hipLaunchKernelGGL((attn_chunk16_kernel<RT, CT, 64>), dim3(blocks), dim3(256), 0, st, a, tiles, splits);
+            hipLaunchKernelGGL((attn_chunk16_kernel<RT, CT, 64, NW>), dim3(blocks), dim3(64 * NW), 0, st, a, tiles,
+                               splits);
     }
     return launch_status();
 }

@@ -72,7 +72,7 @@ __device__ __forceinline__ int64_t key_tile(const AttnArgs &a, const RowTile &t,
            t.g * a.pool.head_stride;
 }
 
-// One 32-key step's exponentials: s[0], s[1] are the scores (times fac: in log2) of keys
+// One 32-key step's exponentials: s[0], s[1] are the scores (fac times them in log2) of keys
 // kt + 4 g4 + r and kt + 16 + 4 g4 + r; those that the lane's column does not see are left
 // out. p[8] are 2^(x - m + 7), m and l the running reference and this lane's running sum;
 // returns what o is to be multiplied by, and whether any lane's reference moved.
@@ -81,7 +81,7 @@ __device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)
     const int g4 = (threadIdx.x & 63) >> 4;
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * fac;
+    for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3];
     if (masked) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -93,7 +93,7 @@ __device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)
 #pragma unroll
     for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mx = fmaxf(mx, __shfl_xor(mx, 32)) * fac;
     const bool grew = mx > m + kLag;
     const float mn = grew ? mx : m;
     const float ref = mn == -INFINITY ? 0.0f : mn - kLift;
@@ -102,12 +102,36 @@ __device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(x[i] - ref);
+        p[i] = __builtin_amdgcn_exp2f(fmaf(x[i], fac, -ref));
         sum += p[i];
     }
     l = l * corr + sum;
     moved = __any(grew);
     return corr;
+}
+
+// Adds what was taken out of a step's values: odd has a bit for each of the lane's eight keys.
+template <typename CT, int HD>
+__device__ __forceinline__ void add_not_finite(const RowTile &t, const CT *vp, int64_t at0, int64_t at1,
+                                               int64_t token_stride, int kt, unsigned odd, f32x4 (&o)[HD / 16]) {
+    constexpr int VD = HD / 16;
+    const int g4 = (threadIdx.x & 63) >> 4;
+#pragma unroll 1
+    for (int n = 0; n < 32; ++n) {  // key kt + n is key 4 (n / 16) + n % 4 of the lanes of group n / 4 % 4
+        if (!(__ballot(odd >> (4 * (n >> 4) + (n & 3)) & 1) >> (16 * (n >> 2 & 3)) & 0xFFFF)) continue;
+        const CT *v = vp + (n < 16 ? at0 : at1) + (n & 15) * token_stride + VD * 4 * g4;
+        const bool sees = kt + n <= t.pos && kt + n >= t.first;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int d = 0; d < VD; d += 4) {
+                float x[4];
+                load_vec(v + VD * r + d, x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[d + e][r] += sees ? not_finite(x[e]) : 0.0f;
+                asm volatile("" ::: "memory");  // few values at a time: this must not cost registers
+            }
+    }
 }
 
 // Joins the four wavefronts' (m, l, o) of a tile and writes the tile's rows, or its split
@@ -191,7 +215,7 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
     const CT *kp = (const CT *)a.pool.k, *vp = (const CT *)a.pool.v;
 
-    float fac = a.scale_log2;
+    float fac = score_factor(a.scale_log2);
     vec8 qf[NP][KC];
     {
         const RT *q = (const RT *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 8 * g4;
@@ -213,8 +237,9 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
             m = fmaxf(m, __shfl_xor(m, 16));
             m = fmaxf(m, __shfl_xor(m, 32));
             up = f16_scale(m, inverse);
-            fac *= inverse;
+            fac = score_factor(fac * inverse);
         }
+        up *= a.q_sign;
 #pragma unroll
         for (int i = 0; i < KC; ++i)
 #pragma unroll
@@ -256,17 +281,21 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
         float p[8];
         bool moved;
         const float corr = softmax_step(t, s, fac, masked, kt, ok0, ok1, p, m, l, moved);
-        bool odd = false;  // a value that is not finite, which a row of the tile must not meet
+        unsigned odd = 0;  // of this lane's eight keys, those with a value that is not finite
         if (masked) {
-            // What no row of the tile sees may hold anything: 0 times it must stay 0.
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
-                if (key >= t.hi || key < t.lo || !(i < 4 ? ok0 : ok1)) v[i] = vrow{};
+                if (key >= t.hi || key < t.lo || !(i < 4 ? ok0 : ok1)) v[i] = vrow{};  // no row of the tile sees it
+                int any = 0;
 #pragma unroll
-                for (int w = 0; w < VW; ++w) odd |= pair_not_finite<CT>(v[i][w]);
+                for (int w = 0; w < VW; ++w) {
+                    const int out = pair_not_finite<CT>(v[i][w]);
+                    v[i][w] &= ~out;
+                    any |= out;
+                }
+                odd |= any ? 1u << i : 0u;
             }
-            odd = t.r0 != t.r1 && __any(odd);
         }
         vec8 pf[NP];
 #pragma unroll
@@ -286,27 +315,10 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 f[j] = __builtin_amdgcn_perm(v[2 * j + 1][d / 2], v[2 * j][d / 2], d % 2 ? 0x07060302 : 0x05040100);
-            if (!odd) {
 #pragma unroll
-                for (int k = 0; k < NP; ++k) o[d] = H::mfma16(__builtin_bit_cast(vec8, f), pf[k], o[d]);
-                continue;
-            }
-            // Row by row, with the values its own mask leaves.
-            for (int r = t.r0; r <= t.r1; ++r) {
-                const int pos = t.len - t.n + r, first = a.window > 0 ? pos - a.window + 1 : 0;
-                i32x4 fr;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int k0 = kt + 16 * (j >> 1) + 4 * g4 + 2 * (j & 1);
-                    fr[j] = f[j] & ((k0 <= pos && k0 >= first ? 0xFFFF : 0) |
-                                    (k0 + 1 <= pos && k0 + 1 >= first ? 0xFFFF0000 : 0));
-                }
-                f32x4 add{};
-#pragma unroll
-                for (int k = 0; k < NP; ++k) add = H::mfma16(__builtin_bit_cast(vec8, fr), pf[k], add);
-                if (t.row == r) o[d] += add;
-            }
+            for (int k = 0; k < NP; ++k) o[d] = H::mfma16(__builtin_bit_cast(vec8, f), pf[k], o[d]);
         }
+        if (__any(odd)) add_not_finite<CT, HD>(t, vp, at0, at1, a.pool.token_stride, kt, odd, o);
     }
     rows_finish<RT, HD>(a, t, m, l, o);
 }
@@ -325,7 +337,7 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
     {
         const float *q = (const float *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 4 * g4;
 #pragma unroll
-        for (int i = 0; i < KC; ++i) qf[i] = *(const f32x4 *)(q + 16 * i);
+        for (int i = 0; i < KC; ++i) qf[i] = *(const f32x4 *)(q + 16 * i) * a.q_sign;
     }
     f32x4 o[VD];
 #pragma unroll
@@ -360,46 +372,33 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
             kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || !ok[0] || !ok[1];
         float p[8];
         bool moved;
-        const float corr = softmax_step(t, s, a.scale_log2, masked, kt, ok[0], ok[1], p, m, l, moved);
-        bool odd = false;
+        const float corr = softmax_step(t, s, score_factor(a.scale_log2), masked, kt, ok[0], ok[1], p, m, l, moved);
+        unsigned odd = 0;  // of this lane's eight keys, those with a value that is not finite
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
-                const bool none = key >= t.hi || key < t.lo || !ok[i >> 2];
+                const bool none = key >= t.hi || key < t.lo || !ok[i >> 2];  // no row of the tile sees it
 #pragma unroll
-                for (int w = 0; w < VD / 4; ++w) {
-                    if (none) v[i][w] = f32x4{};
+                for (int w = 0; w < VD / 4; ++w)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) odd |= !(fabsf(v[i][w][e]) < INFINITY);
-                }
+                    for (int e = 0; e < 4; ++e) {
+                        const bool out = !(fabsf(v[i][w][e]) < INFINITY);
+                        if (out || none) v[i][w][e] = 0.0f;
+                        odd |= out && !none ? 1u << i : 0u;
+                    }
             }
-            odd = t.r0 != t.r1 && __any(odd);
         }
         if (moved) {
 #pragma unroll
             for (int i = 0; i < VD; ++i) o[i] *= corr;
         }
 #pragma unroll
-        for (int d = 0; d < VD; ++d) {
-            if (!odd) {
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d / 4][d % 4], p[i], o[d], 0, 0, 0);
-                continue;
-            }
-            for (int r = t.r0; r <= t.r1; ++r) {
-                const int pos = t.len - t.n + r, first = a.window > 0 ? pos - a.window + 1 : 0;
-                f32x4 add{};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
-                    const float x = key <= pos && key >= first ? v[i][d / 4][d % 4] : 0.0f;
-                    add = __builtin_amdgcn_mfma_f32_16x16x4f32(x, p[i], add, 0, 0, 0);
-                }
-                if (t.row == r) o[d] += add;
-            }
-        }
+            for (int d = 0; d < VD; ++d)
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d / 4][d % 4], p[i], o[d], 0, 0, 0);
+        if (__any(odd)) add_not_finite<float, HD>(t, vp, at[0], at[1], a.pool.token_stride, kt, odd, o);
     }
     rows_finish<float, HD>(a, t, m, l, o);
 }
