@@ -11,7 +11,7 @@
 // A query tile is TM columns of one sequence and one KV head: column c is query
 // row c / group, query head KV head * group + c % group, so all heads that share
 // the KV head, and rows behind one another, share one read of its keys. A tile's
-// keys start at a multiple of 32 (tile_keys) and are cut every split_len keys;
+// keys start at a multiple of 64 (tile_keys) and are cut every split_len keys;
 // where that gives more than one piece, each writes its unnormalized output, its
 // reference and its sum, and paged_join_kernel adds them in order.
 #pragma once
@@ -42,7 +42,7 @@ constexpr float kLift = 7.0f;   // exponentials are 2^(x - m + 7): at most 2^15,
                                 // probabilities keep 2^-24 of a 2^7 .. 2^15 maximum, not of 1
 
 // The keys [lo, hi) that rows r0 .. r1 of a sequence of n rows and len keys see, and the
-// 32-aligned key that its splits count from.
+// key, a multiple of 64, that its splits count from.
 struct TileKeys {
     int lo, hi, from;
 };
@@ -51,11 +51,74 @@ __device__ __forceinline__ TileKeys tile_keys(int n, int len, int r0, int r1, in
     t.hi = max(len - n + r1 + 1, 0);
     t.lo = window > 0 ? max(len - n + r0 - window + 1, 0) : 0;
     t.lo = min(t.lo, t.hi);
-    t.from = t.lo & ~31;
+    t.from = t.lo & ~63;
     return t;
 }
 __device__ __forceinline__ int tile_splits(const TileKeys &t, int split_len) {
     return t.hi > t.lo ? (t.hi - t.from + split_len - 1) / split_len : 1;
+}
+
+// The pages of a tile's keys [lo, hi): lane i of a wavefront holds where entry first + i of
+// the sequence's table lies, so that a step finds its pages without waiting for memory.
+// Entries no row of the tile needs may be unset: numbers outside lo .. hi stand for the
+// nearest that is needed. An entry that names no page of the pool is flagged and becomes
+// page 0, which can be read; its keys are bad (a bit per lane) and are masked.
+struct PageWalk {
+    int first, lo_entry, hi_entry;
+    uint64_t bad;
+    int at_lo, at_hi;  // byte offset of the entry's page and KV head, in two halves
+};
+
+template <typename CT>
+__device__ __forceinline__ void pages_fill(const AttnArgs &a, PageWalk &w, int seq, int g, int first) {
+    const int lane = threadIdx.x & 63;
+    w.first = first;
+    const int e = min(max(first + lane, w.lo_entry), w.hi_entry);
+    int page = a.b.table[seq * a.b.table_stride + e];
+    const bool bad = page < 0 || page >= a.pool.pages;
+    if (bad) {
+        paged_flag(a.b, PAGED_BAD_PAGE);
+        page = 0;
+    }
+    w.bad = __ballot(bad);
+    const int64_t at = (page * a.pool.page_stride + g * a.pool.head_stride) * (int64_t)sizeof(CT);
+    w.at_lo = (int)at;
+    w.at_hi = (int)(at >> 32);
+}
+
+template <typename CT>
+__device__ __forceinline__ void pages_start(const AttnArgs &a, PageWalk &w, int seq, int g, int lo, int hi, int kt) {
+    w.lo_entry = lo >> a.pool.shift;
+    w.hi_entry = (hi - 1) >> a.pool.shift;
+    pages_fill<CT>(a, w, seq, g, kt >> a.pool.shift);
+}
+
+// Byte offsets of the 16-key groups kt, kt + 16, ... of a step; a bit per group that is not bad.
+template <typename CT, int N>
+__device__ __forceinline__ unsigned pages_step(const AttnArgs &a, PageWalk &w, int seq, int g, int kt,
+                                               int64_t (&at)[N]) {
+    const int shift = a.pool.shift, ts = (int)(a.pool.token_stride * sizeof(CT)), mask = (1 << shift) - 1;
+    if (((kt + 16 * N - 1) >> shift) - w.first >= 64) pages_fill<CT>(a, w, seq, g, kt >> shift);
+    auto get = [&](int key, bool &bad) {
+        const int i = (key >> shift) - w.first;
+        bad = w.bad >> i & 1;
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(w.at_hi, i) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane(w.at_lo, i)) + (int64_t)((key & mask) * ts);
+    };
+    unsigned ok = 0;
+    bool bad;
+    if (16 * N <= mask + 1) {  // steps of 16 N keys start at multiples of 16 N: one page
+        at[0] = get(kt, bad);
+#pragma unroll
+        for (int i = 1; i < N; ++i) at[i] = at[0] + (int64_t)i * 16 * ts;
+        return bad ? 0 : (1u << N) - 1;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        at[i] = get(kt + 16 * i, bad);
+        ok |= bad ? 0 : 1u << i;
+    }
+    return ok;
 }
 
 // A key that some rows of a tile see and others do not may hold values that are not finite,

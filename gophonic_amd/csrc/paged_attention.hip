@@ -19,6 +19,7 @@ int paged_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, PagedPool &po
     const int64_t size = kv->dtype == GPHQ_DTYPE_F32 ? 4 : 2, unit = 16 / size;
     for (const int64_t s : {kv->page_stride, kv->token_stride, kv->head_stride})
         if (s < kv->head_dim || s % unit || s > INT64_MAX / (size * kv->pages)) return GPHQ_ERR_PAGED_SHAPE;
+    if (kv->token_stride > INT32_MAX / (kv->page_tokens * size)) return GPHQ_ERR_PAGED_SHAPE;  // a page under 2 GiB
     if (!kv->k_dev || !kv->v_dev || (uintptr_t)kv->k_dev % 16 || (uintptr_t)kv->v_dev % 16)
         return GPHQ_ERR_PAGED_SHAPE;
     if (b->seqs < 0 || b->seqs > GPHQ_PAGED_MAX_SEQS || b->rows < 0 || b->rows > GPHQ_PAGED_MAX_ROWS ||
@@ -65,8 +66,8 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
     // Sequences of up to 32 columns run in the row kernel, in tiles of 16; a call of one
     // sequence runs in one kernel only.
     p.small_cols = cols > 32 && b.seqs == 1 ? 0 : 32;
-    auto span = [&](int64_t tile) {  // keys a tile of that many columns may see, from a multiple of 32
-        return window > 0 ? std::min<int64_t>(b.max_len, (int64_t)window + tile / group + 33) : (int64_t)b.max_len;
+    auto span = [&](int64_t tile) {  // keys a tile of that many columns may see, from a multiple of 64
+        return window > 0 ? std::min<int64_t>(b.max_len, (int64_t)window + tile / group + 65) : (int64_t)b.max_len;
     };
     if (p.small_cols) {
         p.small_tiles = (int)((std::min<int64_t>(cols, p.small_cols) + kSmallTile - 1) / kSmallTile);

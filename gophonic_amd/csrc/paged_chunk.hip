@@ -85,22 +85,6 @@ __device__ __forceinline__ bool chunk_tile(const AttnArgs &a, int tiles, int spl
     return true;
 }
 
-// As the row kernel's: the pool offset of the 16 keys from kt on.
-__device__ __forceinline__ int64_t chunk_keys(const AttnArgs &a, const ChunkTile &t, int kt, bool &ok) {
-    int page = 0;
-    ok = kt < t.hi && kt + 16 > t.lo;
-    if (ok) {
-        page = uniform(a.b.table[t.seq * a.b.table_stride + (kt >> a.pool.shift)]);
-        if (page < 0 || page >= a.pool.pages) {
-            paged_flag(a.b, PAGED_BAD_PAGE);
-            page = 0;
-            ok = false;
-        }
-    }
-    return page * a.pool.page_stride + (kt & ((1 << a.pool.shift) - 1)) * a.pool.token_stride +
-           t.g * a.pool.head_stride;
-}
-
 // A step that holds keys which some row of the tile does not see.
 __device__ __forceinline__ bool chunk_edge(const AttnArgs &a, const ChunkTile &t, int kt, int keys) {
     return kt + keys - 1 > t.b_p0 || kt < t.lo || (a.window > 0 && kt < t.b_p1 - a.window + 1);
@@ -196,7 +180,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
     ChunkTile t;
     if (!chunk_tile<32 * NW>(a, tiles, splits, t)) return;
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, q = lane & 31, hi = lane >> 5;
-    const CT *kp = (const CT *)a.pool.k, *vp = (const CT *)a.pool.v;
+    const char *kp = (const char *)a.pool.k, *vp = (const char *)a.pool.v;
+    const int ts = (int)(a.pool.token_stride * sizeof(CT));
 
     float fac = score_factor(a.scale_log2);
     vec8 qf[NP][QC];
@@ -237,19 +222,20 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
     const int krow = tid / KP, kpc = tid % KP;  // K: piece kpc of keys krow + i * (NT / KP)
     const int vkg = tid / DG, vdg = tid % DG;   // V: keys 4 vkg .. 4 vkg + 3 of dims VD vdg ..
     const int vtile = wave * (64 / DG) / 4;     // the 16 keys that vkg lies in
+    PageWalk w;
     auto load = [&](int kt) __attribute__((always_inline)) -> unsigned {
-        bool ok[4];
         int64_t at[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) at[i] = chunk_keys(a, t, kt + 16 * i, ok[i]);
+        const unsigned ok = pages_step<CT>(a, w, t.seq, t.g, kt, at);
         auto pick = [&](int i) { return i == 0 ? at[0] : i == 1 ? at[1] : i == 2 ? at[2] : at[3]; };
 #pragma unroll
         for (int i = 0; i < KI; ++i)
-            kr[i] = *(const i32x4 *)(kp + pick((wave * 64 + i * NT) / KP / 16) + (krow + i * (NT / KP)) % 16 * a.pool.token_stride + 8 * kpc);
-        const CT *src = vp + pick(vtile) + 4 * (vkg & 3) * a.pool.token_stride + VD * vdg;
+            kr[i] = *(const i32x4 *)(kp + pick((wave * 64 + i * NT) / KP / 16) +
+                                     (unsigned)((krow + i * (NT / KP)) % 16 * ts + 16 * kpc));
+        const char *src = vp + pick(vtile);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vr[i] = *(const vrow *)(src + i * a.pool.token_stride);
-        return (unsigned)ok[0] | (unsigned)ok[1] << 1 | (unsigned)ok[2] << 2 | (unsigned)ok[3] << 3;
+        for (int i = 0; i < 4; ++i)
+            vr[i] = *(const vrow *)(src + i * ts + (unsigned)(4 * (vkg & 3) * ts + 2 * VD * vdg));
+        return ok;
     };
     auto store = [&](int kt, unsigned ok, int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -296,7 +282,11 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
     for (int i = 0; i < DT; ++i) o[i] = f32x16{};
     float m = -INFINITY, l = 0.0f;
     if (tid < 2 * KB) (&odd[0][0])[tid] = -1;
-    unsigned ok = t.k0 < t.k1 ? load(t.k0) : 0;
+    unsigned ok = 0;
+    if (t.k0 < t.k1) {
+        pages_start<CT>(a, w, t.seq, t.g, t.lo, t.hi, t.k0);
+        ok = load(t.k0);
+    }
     int buf = 0;
     __syncthreads();
     for (int kt = t.k0; kt < t.k1; kt += KB, buf ^= 1) {
@@ -345,8 +335,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
         if (!chunk_edge(a, t, kt, KB) && okc == 15) continue;
         for (uint64_t left = __ballot(odd[buf][lane] == kt); left; left &= left - 1) {
             const int key = kt + __builtin_ctzll(left);
-            bool in;
-            const CT *v = vp + chunk_keys(a, t, key & ~15, in) + (key & 15) * a.pool.token_stride;
+            const int page = a.b.table[t.seq * a.b.table_stride + (key >> a.pool.shift)];  // a good one: V was kept
+            const CT *v = (const CT *)a.pool.v + page * a.pool.page_stride +
+                          (key & ((1 << a.pool.shift) - 1)) * a.pool.token_stride + t.g * a.pool.head_stride;
             const bool sees = key <= t.pos && key >= t.first;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -380,7 +371,8 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
     ChunkTile t;
     if (!chunk_tile<32 * NW>(a, tiles, splits, t)) return;
     const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, q = lane & 31, hi = lane >> 5;
-    const float *kp = (const float *)a.pool.k, *vp = (const float *)a.pool.v;
+    const char *kp = (const char *)a.pool.k, *vp = (const char *)a.pool.v;
+    const int ts = (int)(a.pool.token_stride * sizeof(float));
     f32x4 qf[QC];
     {
         const float *src = (const float *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 4 * hi;
@@ -390,20 +382,18 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
     typedef float vdim __attribute__((ext_vector_type(DT)));
     f32x4 kr[KI], vr[KI];
     const int krow = tid / KP, kpc = tid % KP;
+    PageWalk w;
     auto load = [&](int kt) __attribute__((always_inline)) -> unsigned {
-        bool ok[2];
         int64_t at[2];
-        at[0] = chunk_keys(a, t, kt, ok[0]);
-        at[1] = chunk_keys(a, t, kt + 16, ok[1]);
+        const unsigned ok = pages_step<float>(a, w, t.seq, t.g, kt, at);
 #pragma unroll
         for (int i = 0; i < KI; ++i) {
-            const int row = krow + i * (NT / KP);
             const int64_t base = (wave * 64 + i * NT) / KP < 16 ? at[0] : at[1];  // the same for a wavefront's rows
-            const int64_t off = base + (row & 15) * a.pool.token_stride + 4 * kpc;
-            kr[i] = *(const f32x4 *)(kp + off);
-            vr[i] = *(const f32x4 *)(vp + off);
+            const unsigned off = (krow + i * (NT / KP)) % 16 * ts + 16 * kpc;
+            kr[i] = *(const f32x4 *)(kp + base + off);
+            vr[i] = *(const f32x4 *)(vp + base + off);
         }
-        return (unsigned)ok[0] | (unsigned)ok[1] << 1;
+        return ok;
     };
     auto store = [&](int kt, unsigned ok, int buf) __attribute__((always_inline)) {
         const bool edge = chunk_edge(a, t, kt, KB) || ok != 3;
@@ -427,7 +417,11 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
     for (int i = 0; i < DT; ++i) o[i] = f32x16{};
     float m = -INFINITY, l = 0.0f;
     if (tid < 2 * KB) (&odd[0][0])[tid] = -1;
-    unsigned ok = t.k0 < t.k1 ? load(t.k0) : 0;
+    unsigned ok = 0;
+    if (t.k0 < t.k1) {
+        pages_start<float>(a, w, t.seq, t.g, t.lo, t.hi, t.k0);
+        ok = load(t.k0);
+    }
     int buf = 0;
     __syncthreads();
     for (int kt = t.k0; kt < t.k1; kt += KB, buf ^= 1) {
@@ -460,8 +454,9 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
         if (!chunk_edge(a, t, kt, KB) && okc == 3) continue;
         for (uint64_t left = __ballot(lane < KB && odd[buf][lane % KB] == kt); left; left &= left - 1) {
             const int key = kt + __builtin_ctzll(left);
-            bool in;
-            const float *v = vp + chunk_keys(a, t, key & ~15, in) + (key & 15) * a.pool.token_stride;
+            const int page = a.b.table[t.seq * a.b.table_stride + (key >> a.pool.shift)];  // a good one: V was kept
+            const float *v = (const float *)a.pool.v + page * a.pool.page_stride +
+                             (key & ((1 << a.pool.shift) - 1)) * a.pool.token_stride + t.g * a.pool.head_stride;
             const bool sees = key <= t.pos && key >= t.first;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {

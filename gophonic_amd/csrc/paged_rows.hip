@@ -54,30 +54,12 @@ __device__ __forceinline__ bool row_tile(const AttnArgs &a, int tiles, int split
     return true;
 }
 
-// Where the 16 keys from kt on lie: the pool offset of key kt and KV head t.g. Not ok for
-// keys that no row of the tile sees (their table entry may be unset) and for a page number
-// outside the pool, which is flagged; the offset is then page 0's, which can be read.
-__device__ __forceinline__ int64_t key_tile(const AttnArgs &a, const RowTile &t, int kt, bool &ok) {
-    int page = 0;
-    ok = kt < t.hi && kt + 16 > t.lo;
-    if (ok) {
-        page = uniform(a.b.table[t.seq * a.b.table_stride + (kt >> a.pool.shift)]);
-        if (page < 0 || page >= a.pool.pages) {
-            paged_flag(a.b, PAGED_BAD_PAGE);
-            page = 0;
-            ok = false;
-        }
-    }
-    return page * a.pool.page_stride + (kt & ((1 << a.pool.shift) - 1)) * a.pool.token_stride +
-           t.g * a.pool.head_stride;
-}
-
 // One 32-key step's exponentials: s[0], s[1] are the scores (fac times them in log2) of keys
 // kt + 4 g4 + r and kt + 16 + 4 g4 + r; those that the lane's column does not see are left
 // out. p[8] are 2^(x - m + 7), m and l the running reference and this lane's running sum;
 // returns what o is to be multiplied by, and whether any lane's reference moved.
 __device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)[2], float fac, bool masked, int kt,
-                                              bool ok0, bool ok1, float (&p)[8], float &m, float &l, bool &moved) {
+                                              unsigned ok, float (&p)[8], float &m, float &l, bool &moved) {
     const int g4 = (threadIdx.x & 63) >> 4;
     float x[8];
 #pragma unroll
@@ -86,7 +68,7 @@ __device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
-            if (key > t.pos || key < t.first || !(i < 4 ? ok0 : ok1)) x[i] = -INFINITY;
+            if (key > t.pos || key < t.first || !(ok >> (i >> 2) & 1)) x[i] = -INFINITY;
         }
     }
     float mx = x[0];
@@ -112,21 +94,21 @@ __device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)
 
 // Adds what was taken out of a step's values: odd has a bit for each of the lane's eight keys.
 template <typename CT, int HD>
-__device__ __forceinline__ void add_not_finite(const RowTile &t, const CT *vp, int64_t at0, int64_t at1,
-                                               int64_t token_stride, int kt, unsigned odd, f32x4 (&o)[HD / 16]) {
+__device__ __forceinline__ void add_not_finite(const RowTile &t, const char *v, const int64_t (&at)[2], int ts,
+                                               int kt, unsigned odd, f32x4 (&o)[HD / 16]) {
     constexpr int VD = HD / 16;
     const int g4 = (threadIdx.x & 63) >> 4;
 #pragma unroll 1
     for (int n = 0; n < 32; ++n) {  // key kt + n is key 4 (n / 16) + n % 4 of the lanes of group n / 4 % 4
         if (!(__ballot(odd >> (4 * (n >> 4) + (n & 3)) & 1) >> (16 * (n >> 2 & 3)) & 0xFFFF)) continue;
-        const CT *v = vp + (n < 16 ? at0 : at1) + (n & 15) * token_stride + VD * 4 * g4;
+        const CT *row = (const CT *)(v + (n < 16 ? at[0] : at[1]) + (n & 15) * ts) + VD * 4 * g4;
         const bool sees = kt + n <= t.pos && kt + n >= t.first;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int d = 0; d < VD; d += 4) {
                 float x[4];
-                load_vec(v + VD * r + d, x);
+                load_vec(row + VD * r + d, x);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[d + e][r] += sees ? not_finite(x[e]) : 0.0f;
                 asm volatile("" ::: "memory");  // few values at a time: this must not cost registers
@@ -213,7 +195,9 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
     RowTile t;
     if (!row_tile(a, tiles, splits, t)) return;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
-    const CT *kp = (const CT *)a.pool.k, *vp = (const CT *)a.pool.v;
+    const char *kp = (const char *)a.pool.k, *vp = (const char *)a.pool.v;
+    const int ts = (int)(a.pool.token_stride * sizeof(CT));
+    const unsigned ko = c * ts + 16 * g4, vo = 4 * g4 * ts + 2 * VD * c;  // this lane's bytes within 16 keys
 
     float fac = score_factor(a.scale_log2);
     vec8 qf[NP][KC];
@@ -254,20 +238,23 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
 #pragma unroll
     for (int i = 0; i < VD; ++i) o[i] = f32x4{};
     float m = -INFINITY, l = 0.0f;
-    for (int kt = t.k0 + 32 * wave; kt < t.k1; kt += 128) {
-        bool ok0, ok1;
-        const int64_t at0 = key_tile(a, t, kt, ok0), at1 = key_tile(a, t, kt + 16, ok1);
+    int kt = t.k0 + 32 * wave;
+    PageWalk w;
+    if (kt < t.k1) pages_start<CT>(a, w, t.seq, t.g, t.lo, t.hi, kt);
+    for (; kt < t.k1; kt += 128) {
+        int64_t at[2];
+        const unsigned ok = pages_step<CT>(a, w, t.seq, t.g, kt, at);
         vec8 kf[2][KC];
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
-            kf[0][i] = *(const vec8 *)(kp + at0 + c * a.pool.token_stride + 32 * i + 8 * g4);
-            kf[1][i] = *(const vec8 *)(kp + at1 + c * a.pool.token_stride + 32 * i + 8 * g4);
+            kf[0][i] = *(const vec8 *)(kp + at[0] + (ko + 64 * i));
+            kf[1][i] = *(const vec8 *)(kp + at[1] + (ko + 64 * i));
         }
         typedef int vrow __attribute__((ext_vector_type(VW)));
         vrow v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            v[i] = *(const vrow *)(vp + (i < 4 ? at0 : at1) + (4 * g4 + (i & 3)) * a.pool.token_stride + VD * c);
+            v[i] = *(const vrow *)(vp + at[i >> 2] + (i & 3) * ts + vo);
         f32x4 s[2] = {f32x4{}, f32x4{}};
 #pragma unroll
         for (int i = 0; i < KC; ++i)
@@ -277,16 +264,16 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
                 s[1] = H::mfma16(kf[1][i], qf[k][i], s[1]);
             }
         // Whether some column does not see some key of the step.
-        const bool masked = kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || !ok0 || !ok1;
+        const bool masked = kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || ok != 3;
         float p[8];
         bool moved;
-        const float corr = softmax_step(t, s, fac, masked, kt, ok0, ok1, p, m, l, moved);
+        const float corr = softmax_step(t, s, fac, masked, kt, ok, p, m, l, moved);
         unsigned odd = 0;  // of this lane's eight keys, those with a value that is not finite
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
-                if (key >= t.hi || key < t.lo || !(i < 4 ? ok0 : ok1)) v[i] = vrow{};  // no row of the tile sees it
+                if (key >= t.hi || key < t.lo || !(ok >> (i >> 2) & 1)) v[i] = vrow{};  // no row of the tile sees it
                 int any = 0;
 #pragma unroll
                 for (int w = 0; w < VW; ++w) {
@@ -318,7 +305,7 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
 #pragma unroll
             for (int k = 0; k < NP; ++k) o[d] = H::mfma16(__builtin_bit_cast(vec8, f), pf[k], o[d]);
         }
-        if (__any(odd)) add_not_finite<CT, HD>(t, vp, at0, at1, a.pool.token_stride, kt, odd, o);
+        if (__any(odd)) add_not_finite<CT, HD>(t, vp, at, ts, kt, odd, o);
     }
     rows_finish<RT, HD>(a, t, m, l, o);
 }
@@ -332,7 +319,9 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
     RowTile t;
     if (!row_tile(a, tiles, splits, t)) return;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
-    const float *kp = (const float *)a.pool.k, *vp = (const float *)a.pool.v;
+    const char *kp = (const char *)a.pool.k, *vp = (const char *)a.pool.v;
+    const int ts = (int)(a.pool.token_stride * sizeof(float));
+    const unsigned ko = c * ts + 16 * g4, vo = 4 * g4 * ts + 4 * VD * c;  // this lane's bytes within 16 keys
     f32x4 qf[KC];
     {
         const float *q = (const float *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 4 * g4;
@@ -343,23 +332,24 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
 #pragma unroll
     for (int i = 0; i < VD; ++i) o[i] = f32x4{};
     float m = -INFINITY, l = 0.0f;
-    for (int kt = t.k0 + 32 * wave; kt < t.k1; kt += 128) {
-        bool ok[2];
+    int kt = t.k0 + 32 * wave;
+    PageWalk w;
+    if (kt < t.k1) pages_start<float>(a, w, t.seq, t.g, t.lo, t.hi, kt);
+    for (; kt < t.k1; kt += 128) {
         int64_t at[2];
-        at[0] = key_tile(a, t, kt, ok[0]);
-        at[1] = key_tile(a, t, kt + 16, ok[1]);
+        const unsigned ok = pages_step<float>(a, w, t.seq, t.g, kt, at);
         f32x4 kf[2][KC];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < KC; ++i)
-                kf[h][i] = *(const f32x4 *)(kp + at[h] + c * a.pool.token_stride + 16 * i + 4 * g4);
+                kf[h][i] = *(const f32x4 *)(kp + at[h] + (ko + 64 * i));
         f32x4 v[8][VD / 4];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int w = 0; w < VD / 4; ++w)
-                v[i][w] = *(const f32x4 *)(vp + at[i >> 2] + (4 * g4 + (i & 3)) * a.pool.token_stride + VD * c + 4 * w);
+            for (int u = 0; u < VD / 4; ++u)
+                v[i][u] = *(const f32x4 *)(vp + at[i >> 2] + (i & 3) * ts + (vo + 16 * u));
         f32x4 s[2] = {f32x4{}, f32x4{}};
 #pragma unroll
         for (int i = 0; i < KC; ++i)
@@ -369,22 +359,22 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
                 s[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[1][i][e], qf[i][e], s[1], 0, 0, 0);
             }
         const bool masked =
-            kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || !ok[0] || !ok[1];
+            kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || ok != 3;
         float p[8];
         bool moved;
-        const float corr = softmax_step(t, s, score_factor(a.scale_log2), masked, kt, ok[0], ok[1], p, m, l, moved);
+        const float corr = softmax_step(t, s, score_factor(a.scale_log2), masked, kt, ok, p, m, l, moved);
         unsigned odd = 0;  // of this lane's eight keys, those with a value that is not finite
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
-                const bool none = key >= t.hi || key < t.lo || !ok[i >> 2];  // no row of the tile sees it
+                const bool none = key >= t.hi || key < t.lo || !(ok >> (i >> 2) & 1);  // no row of the tile sees it
 #pragma unroll
-                for (int w = 0; w < VD / 4; ++w)
+                for (int u = 0; u < VD / 4; ++u)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const bool out = !(fabsf(v[i][w][e]) < INFINITY);
-                        if (out || none) v[i][w][e] = 0.0f;
+                        const bool out = !(fabsf(v[i][u][e]) < INFINITY);
+                        if (out || none) v[i][u][e] = 0.0f;
                         odd |= out && !none ? 1u << i : 0u;
                     }
             }
@@ -398,7 +388,7 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
 #pragma unroll
             for (int d = 0; d < VD; ++d)
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d / 4][d % 4], p[i], o[d], 0, 0, 0);
-        if (__any(odd)) add_not_finite<float, HD>(t, vp, at[0], at[1], a.pool.token_stride, kt, odd, o);
+        if (__any(odd)) add_not_finite<float, HD>(t, vp, at, ts, kt, odd, o);
     }
     rows_finish<float, HD>(a, t, m, l, o);
 }
