@@ -121,6 +121,15 @@ __device__ __forceinline__ unsigned pages_step(const AttnArgs &a, PageWalk &w, i
     return ok;
 }
 
+// One 16-byte-per-lane load straight to LDS, lane l's from base + off to lds + 16 l. Unlike
+// lds_dma16 the compiler does not know of it, and so does not wait for it at the next LDS
+// read, whatever that reads: the caller waits (vmcnt) and has a barrier before the data's use.
+__device__ __forceinline__ void dma16(const char *base, unsigned off, void *lds) {
+    const int at = uniform((int)(uintptr_t)(__attribute__((address_space(3))) void *)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base)
+                 : "memory", "m0");
+}
+
 // A key that some rows of a tile see and others do not may hold values that are not finite,
 // and a masked probability times one is NaN, not 0. So in a step with such keys V's values
 // that are not finite are taken out of the products, and added to the columns that do see

@@ -157,25 +157,24 @@ __device__ __forceinline__ void chunk_finish(const AttnArgs &a, const ChunkTile 
     }
 }
 
-// 16-bit pages. Each step's 64 keys are staged once for the block's 32 NW columns: K as rows,
-// V transposed, [dim][key], by exchanging 16-bit halves between the four keys that a thread
-// loads; both with their 16-byte pieces permuted within a row, so that the fragment reads
-// of 16 consecutive rows and the stores fall on all banks. On v_mfma_f32_32x32x16:
+// 16-bit pages. Each step's 64 keys are brought from the pages straight to LDS, once for the
+// block's 32 NW columns, both K and V as rows. A row's 16-byte pieces are permuted (by the
+// source address: the LDS side of such a load is linear), so that the fragment reads below
+// fall on all banks. On v_mfma_f32_32x32x16:
 //   S^T (32 keys x 32 columns) = K . Q^T;
 //   O^T (32 dims x 32 columns) += V^T . P^T, the score registers being P^T's fragment: in
 //     each 16 keys a lane of the lower half holds keys 0-3 and 8-11, of the upper half 4-7
-//     and 12-15, and V^T's rows are stored in that order.
-// Two LDS buffers, one barrier a step: step u + 1 is loaded into registers while step u is
-// multiplied.
+//     and 12-15; V^T's fragment comes from two transposing LDS reads, in each of which 16
+//     lanes read 4 keys x 16 dims and a lane gets the 4 keys of one dim.
+// Two LDS buffers, one barrier a step: step u + 1 is on its way while step u is multiplied.
 template <typename RT, typename CT, int HD, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs a, int tiles, int splits) {
     typedef Half<CT> H;
     typedef typename H::vec8 vec8;
     constexpr int NT = 64 * NW, NP = kPieces<RT, CT>, KB = 64, QC = HD / 16, DT = HD / 32;
-    constexpr int KP = HD / 8, KI = KB * KP / NT;        // 16-byte pieces of K per key, per thread
-    constexpr int DG = NT / 16, VD = HD / DG, VW = VD / 2;  // V: dim groups, dims and dwords of each per thread
-    __shared__ CT Ks[2][KB * HD];
-    __shared__ CT Vt[2][HD * KB];
+    constexpr int KP = HD / 8, RI = 64 / KP, KI = KB / RI / NW;  // pieces per key; keys per load, loads per wavefront
+    __shared__ __attribute__((aligned(16))) CT Ks[2][KB * HD];
+    __shared__ __attribute__((aligned(16))) CT Vs[2][KB * HD];
     __shared__ int odd[2][KB];  // for each key of a buffer, the step (its first key) whose V[key] is not all finite
     ChunkTile t;
     if (!chunk_tile<32 * NW>(a, tiles, splits, t)) return;
@@ -216,65 +215,63 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
         }
     }
 
-    typedef int vrow __attribute__((ext_vector_type(VW)));
-    i32x4 kr[KI];
-    vrow vr[4];
-    const int krow = tid / KP, kpc = tid % KP;  // K: piece kpc of keys krow + i * (NT / KP)
-    const int vkg = tid / DG, vdg = tid % DG;   // V: keys 4 vkg .. 4 vkg + 3 of dims VD vdg ..
-    const int vtile = wave * (64 / DG) / 4;     // the 16 keys that vkg lies in
+    // Load j of a wavefront brings keys row0 + RI j .. of the step, lane l piece l % KP of key l / KP.
+    const int row0 = wave * KI * RI, lrow = lane / KP, lpc = lane % KP;
+    auto k_swz = [](int row) { return HD == 128 ? row & 15 : row >> 1 & 7; };
+    auto v_swz = [](int row) { return HD == 128 ? 4 * (row & 3) : 4 * (row >> 1 & 1); };
     PageWalk w;
-    auto load = [&](int kt) __attribute__((always_inline)) -> unsigned {
+    auto load = [&](int kt, int buf) __attribute__((always_inline)) -> unsigned {
         int64_t at[4];
         const unsigned ok = pages_step<CT>(a, w, t.seq, t.g, kt, at);
-        auto pick = [&](int i) { return i == 0 ? at[0] : i == 1 ? at[1] : i == 2 ? at[2] : at[3]; };
 #pragma unroll
-        for (int i = 0; i < KI; ++i)
-            kr[i] = *(const i32x4 *)(kp + pick((wave * 64 + i * NT) / KP / 16) +
-                                     (unsigned)((krow + i * (NT / KP)) % 16 * ts + 16 * kpc));
-        const char *src = vp + pick(vtile);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            vr[i] = *(const vrow *)(src + i * ts + (unsigned)(4 * (vkg & 3) * ts + 2 * VD * vdg));
+        for (int j = 0; j < KI; ++j) {
+            const int row = row0 + RI * j, n = row >> 4, r = (row & 15) + lrow;
+            const int64_t base = n == 0 ? at[0] : n == 1 ? at[1] : n == 2 ? at[2] : at[3];
+            dma16(kp + base, r * ts + 16 * (lpc ^ k_swz(r)), Ks[buf] + row * HD);
+            dma16(vp + base, r * ts + 16 * (lpc ^ v_swz(r)), Vs[buf] + row * HD);
+        }
         return ok;
     };
-    auto store = [&](int kt, unsigned ok, int buf) __attribute__((always_inline)) {
+    // In a step with keys that some row of the tile does not see: what no row sees becomes 0
+    // (it may hold anything, and 0 times it must stay 0), what is not finite is taken out.
+    // Each wavefront mends what it has loaded itself.
+    auto mend = [&](int kt, unsigned ok, int buf) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < KI; ++i) {
-            const int row = krow + i * (NT / KP);
-            const int pc = HD == 128 ? kpc ^ (row & 15) : kpc ^ ((row >> 1) & 7);
-            *(i32x4 *)(Ks[buf] + row * HD + 8 * pc) = kr[i];
-        }
-        if (chunk_edge(a, t, kt, KB) || ok != 15) {
+        for (int j = 0; j < KI; ++j) {
+            const int row = row0 + RI * j + lrow, key = kt + row;
+            i32x4 *p = (i32x4 *)(Vs[buf] + (row0 + RI * j) * HD) + lane;
+            i32x4 v = *p;
+            if (key < t.lo || key >= t.hi || !(ok >> (row >> 4) & 1)) v = i32x4{};
+            int any = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = kt + 4 * vkg + i;
-                if (key < t.lo || key >= t.hi || !(ok >> vtile & 1)) vr[i] = vrow{};  // no row of the tile sees it
-                int any = 0;
-#pragma unroll
-                for (int w = 0; w < VW; ++w) {
-                    const int out = pair_not_finite<CT>(vr[i][w]);
-                    vr[i][w] &= ~out;
-                    any |= out;
-                }
-                if (any) odd[buf][key - kt] = kt;
+            for (int e = 0; e < 4; ++e) {
+                const int out = pair_not_finite<CT>(v[e]);
+                v[e] &= ~out;
+                any |= out;
             }
-        }
-        // Key group vkg goes to position group {0, 2, 1, 3}[vkg % 4] of its 16 keys.
-        const int pg = (vkg & ~3) + ((vkg & 3) == 1 ? 2 : (vkg & 3) == 2 ? 1 : vkg & 3);
-#pragma unroll
-        for (int e = 0; e < VD; ++e) {
-            const int sel = e % 2 ? 0x07060302 : 0x05040100, d = VD * vdg + e;
-            typedef int i32x2 __attribute__((ext_vector_type(2)));
-            const i32x2 x = {(int)__builtin_amdgcn_perm(vr[1][e / 2], vr[0][e / 2], sel),
-                             (int)__builtin_amdgcn_perm(vr[3][e / 2], vr[2][e / 2], sel)};
-            const int unit = (pg >> 1) ^ (((d >> 1) ^ (d >> 4)) & 7);
-            *(i32x2 *)(Vt[buf] + d * KB + 8 * unit + 4 * (pg & 1)) = x;
+            if (any) odd[buf][row] = kt;
+            *p = v;
         }
     };
+
+    // This lane's part of the transposing reads, for each 32 dims.
+    const int s16 = lane & 15;
+    int v_at[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+        const int row = 4 * hi + (s16 >> 2), pc = 4 * d + 2 * (lane >> 4 & 1) + (s16 >> 1 & 1);
+        v_at[d] = row * HD + 8 * (pc ^ v_swz(row)) + 4 * (s16 & 1);
+    }
     auto v_frag = [&](int buf, int ks, int d) __attribute__((always_inline)) {
-        const int dim = 32 * d + q;
-        const int unit = (2 * ks + hi) ^ (((dim >> 1) ^ (dim >> 4)) & 7);
-        return *(const i32x4 *)(Vt[buf] + dim * KB + 8 * unit);
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4 lds_s4;
+        union {
+            s4 h[2];
+            vec8 v;
+        } f;
+        f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(Vs[buf] + v_at[d] + 16 * ks * HD));
+        f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(Vs[buf] + v_at[d] + (16 * ks + 8) * HD));
+        return f.v;
     };
 
     f32x16 o[DT];
@@ -282,18 +279,20 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
     for (int i = 0; i < DT; ++i) o[i] = f32x16{};
     float m = -INFINITY, l = 0.0f;
     if (tid < 2 * KB) (&odd[0][0])[tid] = -1;
+    __syncthreads();
     unsigned ok = 0;
     if (t.k0 < t.k1) {
         pages_start<CT>(a, w, t.seq, t.g, t.lo, t.hi, t.k0);
-        ok = load(t.k0);
+        ok = load(t.k0, 0);
     }
     int buf = 0;
-    __syncthreads();
     for (int kt = t.k0; kt < t.k1; kt += KB, buf ^= 1) {
-        store(kt, ok, buf);
-        __syncthreads();
+        wait_vm_lgkm0<0>();
         const unsigned okc = ok;
-        if (kt + KB < t.k1) ok = load(kt + KB);
+        const bool edge = chunk_edge(a, t, kt, KB) || okc != 15;
+        if (edge) mend(kt, okc, buf);
+        __syncthreads();  // the step is here, and the other buffer has been read
+        if (kt + KB < t.k1) ok = load(kt + KB, buf ^ 1);
         if (kt >= t.w_hi || kt + KB <= t.w_lo) continue;
         f32x16 s[2] = {f32x16{}, f32x16{}};
 #pragma unroll
@@ -301,8 +300,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int row = 32 * h + q;
-                const int pc = HD == 128 ? (2 * i + hi) ^ (row & 15) : (2 * i + hi) ^ ((row >> 1) & 7);
-                const vec8 kf = *(const vec8 *)(Ks[buf] + row * HD + 8 * pc);
+                const vec8 kf = *(const vec8 *)(Ks[buf] + row * HD + 8 * ((2 * i + hi) ^ k_swz(row & 15)));
 #pragma unroll
                 for (int k = 0; k < NP; ++k) s[h] = H::mfma32(kf, qf[k][i], s[h]);
             }
@@ -326,13 +324,12 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const int dim = 32 * d + q, unit = (2 * ks + hi) ^ (((dim >> 1) ^ (dim >> 4)) & 7);
-                const vec8 f = *(const vec8 *)(Vt[buf] + dim * KB + 8 * unit);
+                const vec8 f = v_frag(buf, ks, d);
 #pragma unroll
                 for (int k = 0; k < NP; ++k) o[d] = H::mfma32(f, pf[k], o[d]);
             }
         }
-        if (!chunk_edge(a, t, kt, KB) && okc == 15) continue;
+        if (!edge) continue;
         for (uint64_t left = __ballot(odd[buf][lane] == kt); left; left &= left - 1) {
             const int key = kt + __builtin_ctzll(left);
             const int page = a.b.table[t.seq * a.b.table_stride + (key >> a.pool.shift)];  // a good one: V was kept
