@@ -175,6 +175,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
     constexpr int KP = HD / 8, RI = 64 / KP, KI = KB / RI / NW;  // pieces per key; keys per load, loads per wavefront
     __shared__ __attribute__((aligned(16))) CT Ks[2][KB * HD];
     __shared__ __attribute__((aligned(16))) CT Vs[2][KB * HD];
+    // Of three pieces of Q the last stays in LDS, read again each step: three do not fit the registers.
+    constexpr int NR = HD == 128 && NP == 3 ? 2 : NP;
+    __shared__ vec8 ql[NR < NP ? NW : 1][QC][NR < NP ? 64 : 1];
     __shared__ int odd[2][KB];  // for each key of a buffer, the step (its first key) whose V[key] is not all finite
     ChunkTile t;
     if (!chunk_tile<32 * NW>(a, tiles, splits, t)) return;
@@ -183,7 +186,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
     const int ts = (int)(a.pool.token_stride * sizeof(CT));
 
     float fac = score_factor(a.scale_log2);
-    vec8 qf[NP][QC];
+    vec8 qf[NR][QC];
     {
         const RT *src = (const RT *)a.q + (int64_t)(t.start + t.row) * a.q_stride + t.head * HD + 8 * hi;
         float inverse = 1.0f, up = 1.0f;
@@ -210,7 +213,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
                 CT pc[NP];
                 split_pieces(x[e] * up, pc);
 #pragma unroll
-                for (int k = 0; k < NP; ++k) qf[k][i >> 1][4 * (i & 1) + e] = pc[k];
+                for (int k = 0; k < NR; ++k) qf[k][i >> 1][4 * (i & 1) + e] = pc[k];
+                if (NR < NP) ql[wave][i >> 1][lane][4 * (i & 1) + e] = pc[NP - 1];
             }
         }
     }
@@ -295,6 +299,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
         if (kt + KB < t.k1) ok = load(kt + KB, buf ^ 1);
         if (kt >= t.w_hi || kt + KB <= t.w_lo) continue;
         f32x16 s[2] = {f32x16{}, f32x16{}};
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < QC; ++i)
 #pragma unroll
@@ -302,8 +307,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
                 const int row = 32 * h + q;
                 const vec8 kf = *(const vec8 *)(Ks[buf] + row * HD + 8 * ((2 * i + hi) ^ k_swz(row & 15)));
 #pragma unroll
-                for (int k = 0; k < NP; ++k) s[h] = H::mfma32(kf, qf[k][i], s[h]);
+                for (int k = 0; k < NR; ++k) s[h] = H::mfma32(kf, qf[k][i], s[h]);
+                if (NR < NP) s[h] = H::mfma32(kf, ql[wave][i][lane], s[h]);
             }
+        __builtin_amdgcn_s_setprio(0);
         const bool masked =
             kt + KB - 1 > t.p0 || kt < t.w_lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 15;
         bool moved;

@@ -188,7 +188,7 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t,
 //     HD/16 neighbouring dims, and 16-bit halves exchanged between the eight registers make
 //     the fragments of V^T for HD/16 tiles of dims HD/16 apart.
 template <typename RT, typename CT, int HD>
-__global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int tiles, int splits) {
+__global__ __launch_bounds__(256, 2) void attn_rows16_kernel(const AttnArgs a, int tiles, int splits) {
     typedef Half<CT> H;
     typedef typename H::vec8 vec8;
     constexpr int NP = kPieces<RT, CT>, KC = HD / 32, VD = HD / 16, VW = VD / 2;  // VW: dwords of V per key
@@ -238,23 +238,25 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
 #pragma unroll
     for (int i = 0; i < VD; ++i) o[i] = f32x4{};
     float m = -INFINITY, l = 0.0f;
-    int kt = t.k0 + 32 * wave;
+    typedef int vrow __attribute__((ext_vector_type(VW)));
+    vec8 kf[2][KC];
+    vrow v[8];
+    int64_t at[2];
     PageWalk w;
-    if (kt < t.k1) pages_start<CT>(a, w, t.seq, t.g, t.lo, t.hi, kt);
-    for (; kt < t.k1; kt += 128) {
-        int64_t at[2];
-        const unsigned ok = pages_step<CT>(a, w, t.seq, t.g, kt, at);
-        vec8 kf[2][KC];
+    auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
             kf[0][i] = *(const vec8 *)(kp + at[0] + (ko + 64 * i));
             kf[1][i] = *(const vec8 *)(kp + at[1] + (ko + 64 * i));
         }
-        typedef int vrow __attribute__((ext_vector_type(VW)));
-        vrow v[8];
+    };
+    auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = *(const vrow *)(vp + at[i >> 2] + (i & 3) * ts + vo);
+        for (int i = 0; i < 8; ++i) v[i] = *(const vrow *)(vp + at[i >> 2] + (i & 3) * ts + vo);
+    };
+    // One step, of keys kt .. kt + 31, whose K and V are in registers; more: the step after it
+    // is loaded into them as they become free.
+    auto step = [&](int kt, unsigned &ok, auto more) __attribute__((always_inline)) {
         f32x4 s[2] = {f32x4{}, f32x4{}};
 #pragma unroll
         for (int i = 0; i < KC; ++i)
@@ -263,22 +265,28 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
                 s[0] = H::mfma16(kf[0][i], qf[k][i], s[0]);
                 s[1] = H::mfma16(kf[1][i], qf[k][i], s[1]);
             }
+        const unsigned okc = ok;
+        const int64_t now[2] = {at[0], at[1]};
+        if (more) {
+            ok = pages_step<CT>(a, w, t.seq, t.g, kt + 128, at);
+            load_k();
+        }
         // Whether some column does not see some key of the step.
-        const bool masked = kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || ok != 3;
+        const bool masked = kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 3;
         float p[8];
         bool moved;
-        const float corr = softmax_step(t, s, fac, masked, kt, ok, p, m, l, moved);
+        const float corr = softmax_step(t, s, fac, masked, kt, okc, p, m, l, moved);
         unsigned odd = 0;  // of this lane's eight keys, those with a value that is not finite
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
-                if (key >= t.hi || key < t.lo || !(ok >> (i >> 2) & 1)) v[i] = vrow{};  // no row of the tile sees it
+                if (key >= t.hi || key < t.lo || !(okc >> (i >> 2) & 1)) v[i] = vrow{};  // no row of the tile sees it
                 int any = 0;
 #pragma unroll
-                for (int w = 0; w < VW; ++w) {
-                    const int out = pair_not_finite<CT>(v[i][w]);
-                    v[i][w] &= ~out;
+                for (int u = 0; u < VW; ++u) {
+                    const int out = pair_not_finite<CT>(v[i][u]);
+                    v[i][u] &= ~out;
                     any |= out;
                 }
                 odd |= any ? 1u << i : 0u;
@@ -305,7 +313,17 @@ __global__ __launch_bounds__(256) void attn_rows16_kernel(const AttnArgs a, int 
 #pragma unroll
             for (int k = 0; k < NP; ++k) o[d] = H::mfma16(__builtin_bit_cast(vec8, f), pf[k], o[d]);
         }
-        if (__any(odd)) add_not_finite<CT, HD>(t, vp, at, ts, kt, odd, o);
+        if (more) load_v();
+        if (__any(odd)) add_not_finite<CT, HD>(t, vp, now, ts, kt, odd, o);
+    };
+    int kt = t.k0 + 32 * wave;
+    if (kt < t.k1) {
+        pages_start<CT>(a, w, t.seq, t.g, t.lo, t.hi, kt);
+        unsigned ok = pages_step<CT>(a, w, t.seq, t.g, kt, at);
+        load_k();
+        load_v();
+        for (; kt + 128 < t.k1; kt += 128) step(kt, ok, std::true_type{});
+        step(kt, ok, std::false_type{});
     }
     rows_finish<RT, HD>(a, t, m, l, o);
 }
@@ -332,24 +350,23 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
 #pragma unroll
     for (int i = 0; i < VD; ++i) o[i] = f32x4{};
     float m = -INFINITY, l = 0.0f;
-    int kt = t.k0 + 32 * wave;
+    f32x4 kf[2][KC], v[8][VD / 4];
+    int64_t at[2];
     PageWalk w;
-    if (kt < t.k1) pages_start<float>(a, w, t.seq, t.g, t.lo, t.hi, kt);
-    for (; kt < t.k1; kt += 128) {
-        int64_t at[2];
-        const unsigned ok = pages_step<float>(a, w, t.seq, t.g, kt, at);
-        f32x4 kf[2][KC];
+    auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < KC; ++i)
-                kf[h][i] = *(const f32x4 *)(kp + at[h] + (ko + 64 * i));
-        f32x4 v[8][VD / 4];
+            for (int i = 0; i < KC; ++i) kf[h][i] = *(const f32x4 *)(kp + at[h] + (ko + 64 * i));
+    };
+    auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
             for (int u = 0; u < VD / 4; ++u)
                 v[i][u] = *(const f32x4 *)(vp + at[i >> 2] + (i & 3) * ts + (vo + 16 * u));
+    };
+    auto step = [&](int kt, unsigned &ok, auto more) __attribute__((always_inline)) {
         f32x4 s[2] = {f32x4{}, f32x4{}};
 #pragma unroll
         for (int i = 0; i < KC; ++i)
@@ -358,17 +375,22 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
                 s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[0][i][e], qf[i][e], s[0], 0, 0, 0);
                 s[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[1][i][e], qf[i][e], s[1], 0, 0, 0);
             }
-        const bool masked =
-            kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || ok != 3;
+        const unsigned okc = ok;
+        const int64_t now[2] = {at[0], at[1]};
+        if (more) {
+            ok = pages_step<float>(a, w, t.seq, t.g, kt + 128, at);
+            load_k();
+        }
+        const bool masked = kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 3;
         float p[8];
         bool moved;
-        const float corr = softmax_step(t, s, score_factor(a.scale_log2), masked, kt, ok, p, m, l, moved);
+        const float corr = softmax_step(t, s, score_factor(a.scale_log2), masked, kt, okc, p, m, l, moved);
         unsigned odd = 0;  // of this lane's eight keys, those with a value that is not finite
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
-                const bool none = key >= t.hi || key < t.lo || !(ok >> (i >> 2) & 1);  // no row of the tile sees it
+                const bool none = key >= t.hi || key < t.lo || !(okc >> (i >> 2) & 1);  // no row of the tile sees it
 #pragma unroll
                 for (int u = 0; u < VD / 4; ++u)
 #pragma unroll
@@ -388,7 +410,17 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
 #pragma unroll
             for (int d = 0; d < VD; ++d)
                 o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][d / 4][d % 4], p[i], o[d], 0, 0, 0);
-        if (__any(odd)) add_not_finite<float, HD>(t, vp, at, ts, kt, odd, o);
+        if (more) load_v();
+        if (__any(odd)) add_not_finite<float, HD>(t, vp, now, ts, kt, odd, o);
+    };
+    int kt = t.k0 + 32 * wave;
+    if (kt < t.k1) {
+        pages_start<float>(a, w, t.seq, t.g, t.lo, t.hi, kt);
+        unsigned ok = pages_step<float>(a, w, t.seq, t.g, kt, at);
+        load_k();
+        load_v();
+        for (; kt + 128 < t.k1; kt += 128) step(kt, ok, std::true_type{});
+        step(kt, ok, std::false_type{});
     }
     rows_finish<float, HD>(a, t, m, l, o);
 }

@@ -281,8 +281,9 @@ def ptr(t):
 def stream_handle(stream=None):
     import torch
 
-    s = torch.cuda.current_stream() if stream is None else stream
-    return s.cuda_stream
+    if stream is None:  # the current stream's handle, without a Stream object (2.7 us less a call)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return stream.cuda_stream
 
 
 def q8gemv_mul_into(x, q, scales, dst, k, n, stream=None):
@@ -1025,28 +1026,30 @@ class PagedBatchDesc(ctypes.Structure):
                 ("max_rows", ctypes.c_int64), ("max_len", ctypes.c_int64), ("bad_dev", ctypes.c_void_p)]
 
 
+_DTYPES = {}
+
+
 def _dtype(t):
     """The GPHQ_DTYPE_* code of a torch dtype; ERR_UNSUPPORTED for one without."""
-    import torch
+    if not _DTYPES:
+        import torch
 
-    code = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}.get(t)
-    return check(ERR_UNSUPPORTED) if code is None else code
+        _DTYPES.update({torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32})
+    return _DTYPES.get(t) or check(ERR_UNSUPPORTED)
 
 
 def _rows2(t, rows, width, err):
     """The row stride of a 2-D tensor of at least `rows` rows of `width` neighbouring values."""
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] < rows or shape[1] < width or (stride[1] != 1 and shape[1] > 1):
         check(err)
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return stride[0] if shape[0] > 1 else max(stride[0], shape[1])
 
 
-def _ints(t, n):
-    """A contiguous int32 tensor of at least n values (None if n is 0 and there is none)."""
-    import torch
-
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n:
-        check(ERR_PAGED_SHAPE)
-    return t
+def _values(t, dtype, n, err):
+    """Refuses a tensor that is not n or more contiguous values of a type."""
+    if t is not None and (t.dtype != dtype or not t.is_contiguous() or t.numel() < n):
+        check(err)
 
 
 def _here(*tensors):
@@ -1088,7 +1091,9 @@ class PagedBatch:
         seqs = lens.numel()
         if table.dim() != 2 or table.shape[0] != seqs:
             check(ERR_PAGED_SHAPE)
-        self.starts, self.lens, self.table = _ints(starts, seqs + 1), _ints(lens, seqs), _ints(table, 0)
+        for v, n in ((starts, seqs + 1), (lens, seqs), (table, 0)):
+            _values(v, torch.int32, n, ERR_PAGED_SHAPE)
+        self.starts, self.lens, self.table = starts, lens, table
         self.bad = torch.zeros(1, dtype=torch.int32, device=lens.device)
         self.rows = rows
         self.desc = PagedBatchDesc(ptr(starts), ptr(lens), ptr(table), table.shape[1], seqs, rows, max_rows, max_len,
@@ -1109,8 +1114,7 @@ def paged_append(kv, batch, qkv, q, heads, q_norm=None, k_norm=None, eps=1e-6, c
     if qkv.dtype != q.dtype or (cos is None) != (sin is None):
         check(ERR_PAGED_SHAPE)
     for t, n in ((q_norm, kv.head_dim), (k_norm, kv.head_dim), (cos, 0), (sin, 0)):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n):
-            check(ERR_PAGED_SHAPE)
+        _values(t, torch.float32, n, ERR_PAGED_SHAPE)
     if cos is not None and (cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != kv.head_dim // 2):
         check(ERR_PAGED_SHAPE)
     qs = _rows2(qkv, batch.rows, (heads + 2 * kv.kv_heads) * kv.head_dim, ERR_PAGED_SHAPE)
@@ -1169,8 +1173,7 @@ def lora_add(a, b, x, y, row_slots, ranks=None, scales=None, work=None, stream=N
     if b.shape != (slots, n, max_rank) or x.dtype != torch.float32 or y.dtype != torch.float32 or rows < 0:
         check(ERR_DIMENSIONS)
     for t, count, dt in ((row_slots, rows, torch.int32), (ranks, slots, torch.int32), (scales, slots, torch.float32)):
-        if t is not None and (t.dtype != dt or not t.is_contiguous() or t.numel() < count):
-            check(ERR_DIMENSIONS)
+        _values(t, dt, count, ERR_DIMENSIONS)
     xs, ys = _rows2(x, rows, k, ERR_DIMENSIONS), _rows2(y, rows, n, ERR_DIMENSIONS)
     if work is None:
         work = _work(lora_workspace_bytes(rows, k, max_rank), x.device)
