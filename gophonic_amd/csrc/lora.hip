@@ -18,6 +18,7 @@
 namespace gphq {
 namespace {
 
+constexpr int kFewRows = 256;  // up to here a tile's adapters go to blocks of their own
 constexpr int kShrinkRows = 32;  // two 16-row tiles share the weights' fragments
 
 struct LoraArgs {
@@ -217,8 +218,11 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraArgs a) {
 
 // y[r][n0 .. n0 + n_block) += scale * B t[r] of the tile's 16 RH rows: D (16 rows x 16
 // columns) = T . B^T, four column tiles at once, tile j holding columns 4 i + j, so that a
-// lane has four neighbouring columns of y. The sums start from y.
-template <typename W, int RH>
+// lane has four neighbouring columns of y. EARLY: y is read before the products, so that the
+// two reads are on their way together, at the price of registers and so of wavefronts at once
+// (4814 rows beside 6144 columns: 106 us, 125 without; 32 rows of eight adapters beside 24576
+// columns, whose blocks have one adapter each and are many: 25 us, 21 without).
+template <typename W, int RH, bool EARLY>
 __global__ __launch_bounds__(256) void lora_expand_kernel(const LoraArgs a) {
     typedef Frag<W> F;
     extern __shared__ char lds[];  // T's fragments: [row tile][32 ranks][piece][lane], 16 bytes each
@@ -261,23 +265,6 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(const LoraArgs a) {
     __syncthreads();
     for (int n = n0 + 64 * wave; n < n1; n += 256) {
         const int at = n + 4 * c;  // lane (c, g) holds rows r0 + 16 h + 4 g + i at columns at .. at + 3
-        f32x4 acc[RH][4];
-        const bool whole = a.vec && at + 4 <= n1;
-#pragma unroll
-        for (int h = 0; h < RH; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                acc[h][i] = f32x4{};
-                if (!(live >> (16 * h + 4 * g + i) & 1)) continue;
-                const float *y = a.y + (int64_t)(r0 + 16 * h + 4 * g + i) * a.y_stride + at;
-                if (whole)
-                    acc[h][i] = *(const f32x4 *)y;
-                else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (at + j < n1) acc[h][i][j] = y[j];
-                }
-            }
         each_slot(slot, 0, 1, [&](int s, unsigned long long mine) {
             const int rank = lora_rank(a, s);
             const W *w = (const W *)a.b + (int64_t)s * a.n * a.max_rank;
@@ -286,6 +273,25 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(const LoraArgs a) {
             for (int h = 0; h < RH; ++h)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) d[h][j] = f32x4{};
+            auto own = [&](int h, int i) { return (mine >> (16 * h + 4 * g + i) & 1) != 0; };
+            auto y_of = [&](int h, int i) { return a.y + (int64_t)(r0 + 16 * h + 4 * g + i) * a.y_stride + at; };
+            const bool whole = a.vec && at + 4 <= n1;
+            f32x4 y[RH][4];
+            auto load_y = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int h = 0; h < RH; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (!own(h, i)) continue;
+                        if (whole)
+                            y[h][i] = *(const f32x4 *)y_of(h, i);
+                        else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) y[h][i][j] = at + j < n1 ? y_of(h, i)[j] : 0.0f;
+                        }
+                    }
+            };
+            if (EARLY) load_y();
 #pragma unroll 2
             for (int r = 0; r < rank; r += 32) {
                 typename F::weight wv[4];
@@ -315,29 +321,23 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(const LoraArgs a) {
                     for (int j = 0; j < 4; ++j) d[h][j] = product(tv, wv[j], d[h][j]);
                 }
             }
+            if (!EARLY) load_y();
+            // Rows of other adapters are left out here: a row has one adapter, so each is written once.
 #pragma unroll
             for (int h = 0; h < RH; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const bool own = mine >> (16 * h + 4 * g + i) & 1;
+                    if (!own(h, i)) continue;
+                    y[h][i] += f32x4{d[h][0][i], d[h][1][i], d[h][2][i], d[h][3][i]};
+                    if (whole)
+                        *(f32x4 *)y_of(h, i) = y[h][i];
+                    else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[h][i][j] += own ? d[h][j][i] : 0.0f;
+                        for (int j = 0; j < 4; ++j)
+                            if (at + j < n1) y_of(h, i)[j] = y[h][i][j];
+                    }
                 }
         });
-#pragma unroll
-        for (int h = 0; h < RH; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (!(live >> (16 * h + 4 * g + i) & 1)) continue;
-                float *y = a.y + (int64_t)(r0 + 16 * h + 4 * g + i) * a.y_stride + at;
-                if (whole)
-                    *(f32x4 *)y = acc[h][i];
-                else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (at + j < n1) y[j] = acc[h][i][j];
-                }
-            }
     }
 }
 
@@ -358,11 +358,11 @@ void lora_plan(int64_t rows, int64_t k, int64_t n, LoraArgs &a) {
     a.n_block = (int)std::min<int64_t>(1024, std::max<int64_t>(256, ((n + blocks - 1) / blocks + 255) / 256 * 256));
 }
 
-template <typename W, int RH>
+template <typename W, int RH, bool EARLY>
 int expand_launch(const LoraArgs &a, hipStream_t st) {
     const unsigned tiles = (unsigned)((a.rows + 16 * RH - 1) / (16 * RH)), nb = (unsigned)((a.n + a.n_block - 1) / a.n_block);
     const unsigned lds = (unsigned)(RH * ((a.max_rank + 31) / 32) * (sizeof(W) == 2 ? 3 : 2) * 1024);
-    hipLaunchKernelGGL((lora_expand_kernel<W, RH>), dim3(tiles * nb * (unsigned)a.passes), dim3(256), lds, st, a);
+    hipLaunchKernelGGL((lora_expand_kernel<W, RH, EARLY>), dim3(tiles * nb * (unsigned)a.passes), dim3(256), lds, st, a);
     return launch_status();
 }
 
@@ -380,7 +380,8 @@ int lora_run(const LoraArgs &a, hipStream_t st) {
         hipLaunchKernelGGL((lora_shrink_kernel<W, 8>), grid, dim3(256), 0, st, a);
     GPHQ_TRY(launch_status());
     const int rows = expand_rows(a.rows);
-    return rows == 16 ? expand_launch<W, 1>(a, st) : expand_launch<W, 2>(a, st);
+    if (rows == 16) return expand_launch<W, 1, false>(a, st);
+    return a.rows <= kFewRows ? expand_launch<W, 2, false>(a, st) : expand_launch<W, 2, true>(a, st);
 }
 
 }  // namespace
@@ -435,7 +436,7 @@ int gphq_lora_add(int dtype, const void *a_dev, const void *b_dev, const int32_t
     p.vec = y_stride % 4 == 0 && (uintptr_t)y % 16 == 0;
     lora_plan(rows, k, n, p);
     // Few tiles: the adapters of a tile go to blocks of their own.
-    p.passes = rows <= 256 ? (int)std::min<int64_t>(std::min<int64_t>(slots, rows), 16) : 1;
+    p.passes = rows <= kFewRows ? (int)std::min<int64_t>(std::min<int64_t>(slots, rows), 16) : 1;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == GPHQ_DTYPE_F32) return lora_run<float>(p, st);
     if (dtype == GPHQ_DTYPE_F16) return lora_run<f16>(p, st);
