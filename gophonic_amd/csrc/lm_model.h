@@ -34,6 +34,14 @@ struct gphq_prefix {
     uint64_t gen = 0;
 };
 
+// gphq_paged_pool: one allocation each for keys and values, [layers][pages][kv_heads][page_tokens][head_dim].
+struct gphq_paged_pool {
+    const gphq_lm *lm;
+    char *k = nullptr, *v = nullptr;
+    int64_t pages = 0, page_tokens = 0, layer_bytes = 0;
+    int dtype = 0;
+};
+
 namespace gphq {
 
 constexpr int kLmHeadDim = 128;

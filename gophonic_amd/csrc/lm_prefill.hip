@@ -27,6 +27,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "common.h"
@@ -57,6 +58,9 @@ struct gphq_prefill {
     int32_t *rowpos, *rowstart;  // packed passes: each row's position and its sequence's first row
     float *okc = nullptr, *ovc = nullptr;  // packed passes' own K/V [layers][rows][kv_dim], on first use
     _Float16 *kv16;  // FP16 K and V^T of the pass's 32-row cache tiles, per layer (lm_kv_half_kernel)
+    int32_t *seqs = nullptr;  // paged passes: starts, lens, then the page table, grown on demand
+    void *attn = nullptr;     // paged passes: the attention's workspace, grown on demand
+    size_t seqs_bytes = 0, attn_bytes = 0;
     int arith = GPHQ_PASS_FP16;
     int8_t *a8 = nullptr;  // int8 route: activations in 16-row tiles and their row scales, on first use
     float *s8 = nullptr;
@@ -71,6 +75,12 @@ enum { EPI_STORE = 0, EPI_ADD = 1, EPI_SWIGLU = 2 };
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// What a paged pass attends to: its batch, and the pool's layer 0.
+struct PassPaged {
+    const gphq_paged_pool *pool;
+    gphq_paged_batch batch;
+};
 
 struct RopeArgs {
     float *qkv;             // [rows][qkvw]
@@ -751,9 +761,42 @@ struct PassKV {
     const int32_t *rowpos, *rowstart;  // packed pass: per-row position and sequence start (device)
 };
 
+// A paged pass's layer between its QKV and O projections: queries prepared in place, keys
+// and values into the pages, attention over them.
+int paged_layer(gphq_prefill *ws, const PassPaged &p, int layer, hipStream_t st) {
+    const gphq_lm *lm = ws->lm;
+    const int64_t qkvw = lm->qd + 2 * lm->kvd;
+    gphq_paged_kv kv;
+    GPHQ_TRY(gphq_paged_pool_layer(p.pool, layer, &kv));
+    const float *norms = lm->norms + (size_t)layer * 2 * kHeadDim;
+    GPHQ_TRY(gphq_paged_append(&kv, &p.batch, GPHQ_DTYPE_F32, ws->qkv, qkvw, lm->cfg.heads, norms, norms + kHeadDim,
+                               lm->cfg.eps, lm->rope, lm->rope + lm->positions * 64, lm->positions,
+                               (float)(1.0 / sqrt((double)lm->cfg.head_dim)), ws->qkv, qkvw, st));
+    return gphq_paged_attention(&kv, &p.batch, GPHQ_DTYPE_F32, ws->qkv, qkvw, lm->cfg.heads, 1.0, 0, ws->ctx, lm->qd,
+                                ws->attn, (int64_t)ws->attn_bytes, st);
+}
+
+// Device memory of at least n bytes in *p, contents lost when it grows.
+template <typename T>
+int grow(T *&p, size_t &have, size_t n) {
+    if (n <= have) return GPHQ_OK;
+    if (p) (void)hipFree(p);
+    p = nullptr;
+    have = 0;
+    const hipError_t e = hipMalloc((void **)&p, n);
+    if (e != hipSuccess) {
+        p = nullptr;
+        return hip_status(e);
+    }
+    have = n;
+    return GPHQ_OK;
+}
+
 // One pass: R tokens already in ws->tok, at cache rows base.. of kv.kc (or,
-// packed, at rows 0..R-1 with per-row positions).
-int encode_pass(gphq_prefill *ws, const PassKV &kv, int base, int R, hipStream_t st, const float *splice = nullptr) {
+// packed, at rows 0..R-1 with per-row positions; or, paged, in the pages of
+// paged's batch).
+int encode_pass(gphq_prefill *ws, const PassKV &kv, int base, int R, hipStream_t st, const float *splice = nullptr,
+                const PassPaged *paged = nullptr) {
     const gphq_lm *lm = ws->lm;
     const gphq_lm_config &c = lm->cfg;
     const int64_t H = c.hidden, I = c.intermediate, qd = lm->qd, kvd = lm->kvd, qkvw = qd + 2 * kvd;
@@ -790,23 +833,27 @@ int encode_pass(gphq_prefill *ws, const PassKV &kv, int base, int R, hipStream_t
         const gphq_lm_layer &L = lm->layers[layer];
         const uint8_t *buf = (const uint8_t *)L.buf_dev;
         GPHQ_TRY(project(ws, R, PRO_NORM, EPI_STORE, buf, L.qkv, L.qkv_scale, ws->h, H, ws->qkv, qkvw, qkvw, st));
-        const size_t off = (size_t)layer * kv.cap * kvd;
-        ra.kc = kv.kc + off;
-        ra.vc = kv.vc + off;
-        if (kv.plen > 0) {
-            fa.pkc = kv.pkc + (size_t)layer * kv.pcap * kvd;
-            fa.pvc = kv.pvc + (size_t)layer * kv.pcap * kvd;
+        if (paged) {
+            GPHQ_TRY(paged_layer(ws, *paged, layer, st));
+        } else {
+            const size_t off = (size_t)layer * kv.cap * kvd;
+            ra.kc = kv.kc + off;
+            ra.vc = kv.vc + off;
+            if (kv.plen > 0) {
+                fa.pkc = kv.pkc + (size_t)layer * kv.pcap * kvd;
+                fa.pvc = kv.pvc + (size_t)layer * kv.pcap * kvd;
+            }
+            ra.qn = lm->norms + (size_t)layer * 2 * kHeadDim;
+            ra.kn = ra.qn + kHeadDim;
+            hipLaunchKernelGGL(lm_qk_rope16_kernel, dim3((unsigned)R), dim3(256), 0, st, ra);
+            GPHQ_TRY(launch_status());
+            fa.kc = ra.kc;
+            fa.vc = ra.vc;
+            hipLaunchKernelGGL(lm_kv_half_kernel, dim3((unsigned)kvTiles, (unsigned)c.kv_heads), dim3(256), 0, st, fa.kc,
+                               fa.vc, (int)kvd, fa.k0, kvEnd, ws->kv16);
+            GPHQ_TRY(launch_status());
+            GPHQ_TRY(launch_flash((int)lm->group, fa, (int)c.kv_heads, st));
         }
-        ra.qn = lm->norms + (size_t)layer * 2 * kHeadDim;
-        ra.kn = ra.qn + kHeadDim;
-        hipLaunchKernelGGL(lm_qk_rope16_kernel, dim3((unsigned)R), dim3(256), 0, st, ra);
-        GPHQ_TRY(launch_status());
-        fa.kc = ra.kc;
-        fa.vc = ra.vc;
-        hipLaunchKernelGGL(lm_kv_half_kernel, dim3((unsigned)kvTiles, (unsigned)c.kv_heads), dim3(256), 0, st, fa.kc,
-                           fa.vc, (int)kvd, fa.k0, kvEnd, ws->kv16);
-        GPHQ_TRY(launch_status());
-        GPHQ_TRY(launch_flash((int)lm->group, fa, (int)c.kv_heads, st));
         GPHQ_TRY(project(ws, R, PRO_PLAIN, EPI_ADD, buf, L.o, L.o_scale, ws->ctx, qd, ws->h, H, H, st));
         GPHQ_TRY(project(ws, R, PRO_NORM, EPI_SWIGLU, buf, L.gu, L.gu_scale, ws->h, H, ws->act, I, 2 * I, st));
         GPHQ_TRY(project(ws, R, PRO_PLAIN, EPI_ADD, buf, L.d, L.d_scale, ws->act, I, ws->h, H, H, st, true));
@@ -816,6 +863,8 @@ int encode_pass(gphq_prefill *ws, const PassKV &kv, int base, int R, hipStream_t
 
 void free_prefill(gphq_prefill *ws) {
     for (void *p : ws->allocs) (void)hipFree(p);
+    if (ws->seqs) (void)hipFree(ws->seqs);
+    if (ws->attn) (void)hipFree(ws->attn);
     delete ws;
 }
 
@@ -1089,6 +1138,101 @@ int gphq_prefill_batch(gphq_prefill *ws, const gphq_prefix *shared, int64_t past
         GPHQ_TRY(hip_status(hipStreamSynchronize(st)));
         t0 += R;
         q0 = q1;
+    }
+    return GPHQ_OK;
+}
+
+int gphq_prefill_paged(gphq_prefill *ws, gphq_paged_pool *pool, const int32_t *tokens, const int64_t *lens,
+                       const int64_t *past, int64_t count, const int32_t *table, int64_t table_stride,
+                       float *hidden_dev, int64_t hidden_len, void *stream) {
+    if (!ws || !ws->lm) return GPHQ_ERR_WORKSPACE;
+    const gphq_lm *lm = ws->lm;
+    const gphq_lm_config &c = lm->cfg;
+    if (!pool || pool->lm != lm) return GPHQ_ERR_FOREIGN_PREFIX;
+    if (count < 1 || count > GPHQ_PAGED_MAX_SEQS || !lens || !past) return GPHQ_ERR_SEQUENCE_COUNT;
+    const int64_t H = c.hidden, page = pool->page_tokens;
+    int64_t total = 0;
+    for (int64_t q = 0; q < count; ++q) {
+        const int64_t n = lens[q];
+        if (past[q] < 0) return GPHQ_ERR_KEEP_RANGE;
+        if (n < 1 || !tokens) return GPHQ_ERR_EMPTY_SEQUENCE;
+        if (n > lm->positions || past[q] > lm->positions || past[q] + n > c.max_positions || past[q] + n > lm->positions)
+            return GPHQ_ERR_CONTEXT;
+        if (!hidden_dev || hidden_len != count * H) return GPHQ_ERR_DEST_WIDTH;
+        for (int64_t i = 0; i < n; ++i)
+            if (tokens[total + i] < 0 || tokens[total + i] >= c.vocab) return GPHQ_ERR_TOKEN_VOCAB;
+        total += n;
+    }
+    if (!table || table_stride < 1) return GPHQ_ERR_PAGED_SHAPE;
+    std::vector<char> written((size_t)pool->pages, 0);
+    for (int64_t q = 0; q < count; ++q) {
+        const int64_t last = past[q] + lens[q] - 1;
+        if (last / page >= table_stride) return GPHQ_ERR_PAGED_SHAPE;
+        for (int64_t e = 0; e <= last / page; ++e) {
+            const int32_t p = table[q * table_stride + e];
+            if (p < 0 || p >= pool->pages) return GPHQ_ERR_PAGED_BATCH;
+            if (e < past[q] / page) continue;
+            if (written[p]) return GPHQ_ERR_PAGED_BATCH;
+            written[p] = 1;
+        }
+    }
+    hipStream_t st = (hipStream_t)stream;
+    // Consecutive passes of up to the workspace's rows; a sequence may continue in the next.
+    std::vector<int32_t> ints;
+    std::vector<std::pair<int64_t, int64_t>> ends;  // (sequence, its last row) where a sequence ends
+    int64_t q0 = 0, done = 0, t0 = 0;               // first unfinished sequence, its tokens so far, tokens so far
+    while (q0 < count) {
+        int64_t R = 0, q1 = q0, off = done, max_rows = 0, max_len = 0;
+        ends.clear();
+        std::vector<int64_t> n, len;
+        while (q1 < count && R < ws->rows) {
+            const int64_t m = std::min<int64_t>(lens[q1] - off, ws->rows - R);
+            n.push_back(m);
+            len.push_back(past[q1] + off + m);
+            max_rows = std::max(max_rows, m);
+            max_len = std::max(max_len, len.back());
+            R += m;
+            off += m;
+            if (off < lens[q1]) break;
+            ends.push_back({q1, R - 1});
+            off = 0;
+            ++q1;
+        }
+        const int64_t seqs = (int64_t)n.size(), entries = (max_len + page - 1) / page;
+        ints.assign((size_t)(2 * seqs + 1 + seqs * entries), 0);
+        for (int64_t s = 0; s < seqs; ++s) {
+            ints[s + 1] = ints[s] + (int32_t)n[s];
+            ints[seqs + 1 + s] = (int32_t)len[s];
+            for (int64_t e = 0; e < (len[s] + page - 1) / page; ++e)
+                ints[2 * seqs + 1 + s * entries + e] = table[(q0 + s) * table_stride + e];
+        }
+        GPHQ_TRY(grow(ws->seqs, ws->seqs_bytes, ints.size() * 4));
+        PassPaged paged{};
+        paged.pool = pool;
+        paged.batch.starts_dev = ws->seqs;
+        paged.batch.lens_dev = ws->seqs + seqs + 1;
+        paged.batch.table_dev = ws->seqs + 2 * seqs + 1;
+        paged.batch.table_stride = entries;
+        paged.batch.seqs = seqs;
+        paged.batch.rows = R;
+        paged.batch.max_rows = max_rows;
+        paged.batch.max_len = max_len;
+        gphq_paged_kv kv;
+        GPHQ_TRY(gphq_paged_pool_layer(pool, 0, &kv));
+        const int64_t need = gphq_paged_attention_workspace_bytes(&kv, &paged.batch, GPHQ_DTYPE_F32, c.heads, 0);
+        if (need < 0) return (int)need;
+        GPHQ_TRY(grow(ws->attn, ws->attn_bytes, (size_t)need));
+        GPHQ_TRY(hip_status(hipMemcpyAsync(ws->seqs, ints.data(), ints.size() * 4, hipMemcpyHostToDevice, st)));
+        GPHQ_TRY(hip_status(hipMemcpyAsync(ws->tok, tokens + t0, R * 4, hipMemcpyHostToDevice, st)));
+        GPHQ_TRY(encode_pass(ws, PassKV{}, 0, (int)R, st, nullptr, &paged));
+        for (const auto &e : ends)
+            GPHQ_TRY(lm_final_launch(lm, ws->h + (size_t)e.second * H, 1, hidden_dev + e.first * H, ws->hn,
+                                     ws->nonfinite, st));
+        // The host arrays are read before the next pass rewrites them.
+        GPHQ_TRY(hip_status(hipStreamSynchronize(st)));
+        t0 += R;
+        q0 = q1;
+        done = off;
     }
     return GPHQ_OK;
 }

@@ -2,6 +2,7 @@
 // join of split results. Kernels: paged_rows.hip and paged_chunk.hip.
 #include <math.h>
 
+#include "lm_model.h"
 #include "paged_attention.h"
 
 namespace gphq {
@@ -255,6 +256,58 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     }
     if (kv->dtype == GPHQ_DTYPE_F16) return attend<f16, f16>(a, p, (int)hd, st);
     return attend<bf16, bf16>(a, p, (int)hd, st);
+}
+
+int gphq_paged_pool_new(const gphq_lm *lm, int64_t pages, int64_t page_tokens, int dtype, gphq_paged_pool **out) {
+    if (!out) return GPHQ_ERR_DIMENSIONS;
+    *out = nullptr;
+    if (!lm) return GPHQ_ERR_WORKSPACE;
+    if (dtype != GPHQ_DTYPE_F32 && dtype != GPHQ_DTYPE_F16 && dtype != GPHQ_DTYPE_BF16) return GPHQ_ERR_UNSUPPORTED;
+    if (page_tokens < 16 || page_tokens > GPHQ_PAGED_MAX_PAGE_TOKENS || (page_tokens & (page_tokens - 1)))
+        return GPHQ_ERR_UNSUPPORTED;
+    if (pages < 1 || pages > INT32_MAX) return GPHQ_ERR_PAGED_SHAPE;
+    const gphq_lm_config &c = lm->cfg;
+    const int64_t token = lm->kvd * (dtype == GPHQ_DTYPE_F32 ? 4 : 2);
+    if (pages > INT64_MAX / (token * page_tokens * c.layers)) return GPHQ_ERR_PAGED_SHAPE;
+    gphq_paged_pool *p = new gphq_paged_pool();
+    p->lm = lm;
+    p->pages = pages;
+    p->page_tokens = page_tokens;
+    p->dtype = dtype;
+    p->layer_bytes = token * page_tokens * pages;
+    hipError_t e = hipMalloc((void **)&p->k, (size_t)(p->layer_bytes * c.layers));
+    if (e == hipSuccess) e = hipMalloc((void **)&p->v, (size_t)(p->layer_bytes * c.layers));
+    if (e != hipSuccess) {
+        gphq_paged_pool_free(p);
+        return hip_status(e);
+    }
+    *out = p;
+    return GPHQ_OK;
+}
+
+void gphq_paged_pool_free(gphq_paged_pool *p) {
+    if (!p) return;
+    if (p->k) (void)hipFree(p->k);
+    if (p->v) (void)hipFree(p->v);
+    delete p;
+}
+
+int gphq_paged_pool_layer(const gphq_paged_pool *p, int64_t layer, gphq_paged_kv *out) {
+    if (!p || !out) return GPHQ_ERR_PAGED_SHAPE;
+    const gphq_lm_config &c = p->lm->cfg;
+    if (layer < 0 || layer >= c.layers) return GPHQ_ERR_PAGED_SHAPE;
+    out->k_dev = p->k + layer * p->layer_bytes;
+    out->v_dev = p->v + layer * p->layer_bytes;
+    out->token_stride = c.head_dim;
+    out->head_stride = p->page_tokens * c.head_dim;
+    out->page_stride = c.kv_heads * p->page_tokens * c.head_dim;
+    out->pages = p->pages;
+    out->page_tokens = p->page_tokens;
+    out->kv_heads = c.kv_heads;
+    out->head_dim = c.head_dim;
+    out->dtype = p->dtype;
+    out->reserved = 0;
+    return GPHQ_OK;
 }
 
 int gphq_paged_check(int32_t *bad_dev, void *stream) {

@@ -203,6 +203,10 @@ SIGNATURES = {
     "gphq_paged_attention_workspace_bytes": (_i64, [_vp, _vp, ctypes.c_int, _i64, _i64]),
     "gphq_paged_attention": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _i64, _i64, ctypes.c_double, _i64, _vp, _i64,
                                             _vp, _i64, _vp]),
+    "gphq_paged_pool_new": (ctypes.c_int, [_vp, _i64, _i64, ctypes.c_int, _vpp]),
+    "gphq_paged_pool_free": (None, [_vp]),
+    "gphq_paged_pool_layer": (ctypes.c_int, [_vp, _i64, _vp]),
+    "gphq_prefill_paged": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "gphq_paged_check": (ctypes.c_int, [_vp, _vp]),
     "gphq_lora_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "gphq_lora_add": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64,
@@ -873,6 +877,24 @@ class Prefill:
                                         len(seqs), ptr(hidden), 0 if hidden is None else hidden.numel(),
                                         stream_handle(stream)))
 
+    def paged(self, pool, seqs, past, table, hidden, stream=None):
+        """gphq_prefill_paged: seqs a list of host token lists (prompt chunks or
+        single tokens), past the tokens each sequence's pages hold already,
+        table host page numbers [len(seqs)][entries]; hidden [len(seqs), hidden]
+        device tensor receives each sequence's last-token state."""
+        import numpy as np
+
+        lens, lp = _host([len(q) for q in seqs], np.int64)
+        old, op = _host(past, np.int64)
+        tab, tp = _host(table, np.int32)
+        if tab.ndim != 2 or tab.shape[0] != len(seqs) or old.size != len(seqs):
+            check(ERR_PAGED_SHAPE)
+        flat = np.ascontiguousarray(np.concatenate([np.asarray(q, np.int64) for q in seqs]) if len(seqs) else
+                                    np.zeros(0), dtype=np.int32)
+        check(load().gphq_prefill_paged(self.h, pool.h if pool is not None else None,
+                                        flat.ctypes.data if flat.size else None, lp, op, len(seqs), tp, tab.shape[1],
+                                        ptr(hidden), 0 if hidden is None else hidden.numel(), stream_handle(stream)))
+
     def check(self, stream=None):
         return check(load().gphq_prefill_check(self.h, stream_handle(stream)))
 
@@ -1151,6 +1173,47 @@ def paged_attention(kv, batch, q, out, heads, scale, window=0, work=None, stream
     return check(load().gphq_paged_attention(ctypes.byref(kv.desc), ctypes.byref(batch.desc), _dtype(q.dtype), ptr(q),
                                              qs, heads, scale, window, ptr(out), os_, ptr(work),
                                              work.numel() * work.element_size(), stream_handle(stream)))
+
+
+class _PoolMemory:
+    """Device memory of a paged pool. A tensor made from it keeps this object, and so the pool, alive."""
+
+    def __init__(self, pool, address, shape, typestr):
+        self.pool = pool
+        self.__cuda_array_interface__ = dict(shape=shape, typestr=typestr, data=(address, False), version=2)
+
+
+class PagedPool:
+    """gphq_paged_pool: a model's layers' pages, for Prefill.paged and, layer
+    by layer, for paged_append and paged_attention."""
+
+    def __init__(self, lm, pages, page_tokens, dtype):
+        h = ctypes.c_void_p()
+        check(load().gphq_paged_pool_new(lm.h, pages, page_tokens, _dtype(dtype), ctypes.byref(h)))
+        self.h, self.lm, self.dtype = h, lm, dtype
+
+    def close(self):
+        if self.h:
+            load().gphq_paged_pool_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def layer(self, i):
+        """PagedKv of layer i, its tensors views of the pool's memory."""
+        import torch
+
+        d = PagedKvDesc()
+        check(load().gphq_paged_pool_layer(self.h, i, ctypes.byref(d)))
+        shape = (d.pages, d.kv_heads, d.page_tokens, d.head_dim)
+        name = {DTYPE_F32: "<f4"}.get(d.dtype, "<i2")
+        k, v = (torch.as_tensor(_PoolMemory(self, a, shape, name), device="cuda").view(self.dtype).transpose(1, 2)
+                for a in (d.k_dev, d.v_dev))
+        return PagedKv(k, v)
 
 
 def lora_workspace_bytes(rows, k, max_rank):

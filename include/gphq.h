@@ -620,6 +620,15 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
  * cleared. */
 int gphq_paged_check(int32_t *bad_dev, void *stream);
 
+/* A pool of one model's layers: `pages` pages of page_tokens tokens of every
+ * layer, keys and values in head order, dtype as gphq_paged_kv. The caller
+ * hands its page numbers out; page p of every layer belongs to the same tokens.
+ * gphq_paged_pool_layer describes one layer's pages for the calls above. */
+typedef struct gphq_paged_pool gphq_paged_pool;
+int gphq_paged_pool_new(const gphq_lm *lm, int64_t pages, int64_t page_tokens, int dtype, gphq_paged_pool **out);
+void gphq_paged_pool_free(gphq_paged_pool *pool);
+int gphq_paged_pool_layer(const gphq_paged_pool *pool, int64_t layer, gphq_paged_kv *out);
+
 /* ---- low-rank adapters beside a shared projection ------------------------------
  * No counterpart in the reference. After a projection of many requests' rows
  * (gphq_gemv_vec, gphq_mm, gphq_prefill_project) the adapters that some of them
@@ -789,6 +798,22 @@ int gphq_prefill_extend_embed(gphq_prefill *ws, gphq_prefix *kv, int64_t stored,
  * order, before any device work. */
 int gphq_prefill_batch(gphq_prefill *ws, const gphq_prefix *shared, int64_t past, const int32_t *tokens,
                        const int64_t *lens, int64_t count, float *hidden_dev, int64_t hidden_len, void *stream);
+/* The batched pass over a paged cache (no reference counterpart): `count`
+ * sequences of one step, each bringing lens[s] >= 1 tokens, a prompt chunk or
+ * the one token of a decode step, to the past[s] its pages hold; `tokens` (host)
+ * are theirs concatenated, table (host [count][table_stride]) their pages. Per
+ * layer the pass projects, appends (gphq_paged_append with the layer's norms and
+ * the model's rotation) and attends (gphq_paged_attention). Row s of hidden_dev
+ * [count][hidden] receives the post-final-norm state of sequence s's last
+ * token. Tokens beyond the workspace's rows run as consecutive passes, in
+ * order. Validation as gphq_prefill_batch's per sequence, then the table: a
+ * needed entry outside the pool, or a page that would be written through two
+ * entries, is GPHQ_ERR_PAGED_BATCH; before any device work. Sequences may share
+ * pages of earlier tokens, which are only read. Waits for each pass's host
+ * arrays to be consumed. gphq_prefill_check reports a non-finite state. */
+int gphq_prefill_paged(gphq_prefill *ws, gphq_paged_pool *pool, const int32_t *tokens, const int64_t *lens,
+                       const int64_t *past, int64_t count, const int32_t *table, int64_t table_stride,
+                       float *hidden_dev, int64_t hidden_len, void *stream);
 /* Waits for the stream; GPHQ_ERR_NON_FINITE_STATE if an extension since the
  * last check produced a non-finite hidden value. */
 int gphq_prefill_check(gphq_prefill *ws, void *stream);

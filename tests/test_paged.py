@@ -150,3 +150,14 @@ def test_lora_refuses(over, want):
                          ids=lambda v: str(v))
 def test_lora_without_work_is_ok(over):
     assert lora(**over) == gphq.OK
+
+
+def test_pool_and_paged_pass_refuse_null_handles():
+    lib = gphq.load()
+    h = ctypes.c_void_p(1)
+    assert lib.gphq_paged_pool_new(None, 4, 16, gphq.DTYPE_F32, ctypes.byref(h)) == gphq.ERR_WORKSPACE
+    assert not h.value
+    assert lib.gphq_paged_pool_new(None, 4, 16, gphq.DTYPE_F32, None) == gphq.ERR_DIMENSIONS
+    assert lib.gphq_paged_pool_layer(None, 0, ctypes.byref(kv())) == gphq.ERR_PAGED_SHAPE
+    assert lib.gphq_prefill_paged(None, None, None, None, None, 1, None, 1, None, 0, None) == gphq.ERR_WORKSPACE
+    lib.gphq_paged_pool_free(None)
