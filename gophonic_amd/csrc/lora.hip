@@ -171,21 +171,18 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraArgs a) {
             const int only = use[0] ? 0 : 1;
 #pragma unroll 2
             for (int k = k0 + 32 * wave; k < k1; k += 128) {
-                float v[8];
-                typename F::value xv[2];
-                load8(both ? x[0] + k : x[only] + k, v);
-                xv[0] = F::values(v);
-                if (both) {
-                    load8(x[1] + k, v);
-                    xv[1] = F::values(v);
-                }
+                // Ranks past the last are the last again (and become 0 below), so no load waits for a test.
+                float v0[8], v1[8], u[RT][8];
+                load8(both ? x[0] + k : x[only] + k, v0);
+                if (both) load8(x[1] + k, v1);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) load8(w[i] + k, u[i]);
+                const typename F::value x0 = F::values(v0), x1 = F::values(both ? v1 : v0);
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
-                    if (16 * i >= rank) break;
-                    load8(w[i] + k, v);
-                    const typename F::weight wv = F::weights(v);
-                    acc[0][i] = product(wv, xv[0], acc[0][i]);
-                    if (both) acc[1][i] = product(wv, xv[1], acc[1][i]);
+                    const typename F::weight wv = F::weights(u[i]);
+                    acc[0][i] = product(wv, x0, acc[0][i]);
+                    if (both) acc[1][i] = product(wv, x1, acc[1][i]);
                 }
             }
             if (!both && only == 1) {
