@@ -60,8 +60,8 @@ void cut(int64_t span, int64_t want, int &len, int &splits) {
     if (splits < 1) splits = 1;
 }
 
-// From host numbers alone, so a captured call keeps its cut whatever the lengths become.
-AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int big_tile) {
+// wide: fp32 pages. From host numbers alone, so a captured call keeps its cut whatever the lengths become.
+AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int big_tile, bool wide) {
     AttnPlan p{};
     const int64_t cus = device_cus(), rows = b.rows, cols = (int64_t)b.max_rows * group;
     // Sequences of up to 32 columns run in the row kernel, in tiles of 16; a call of one
@@ -73,7 +73,14 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
     if (p.small_cols) {
         p.small_tiles = (int)((std::min<int64_t>(cols, p.small_cols) + kSmallTile - 1) / kSmallTile);
         const int64_t units = std::min<int64_t>(b.seqs, rows) * p.small_tiles * kv_heads;
-        cut(span(kSmallTile), (2 * cus + units - 1) / units, p.small_len, p.small_splits);
+        // As many splits as leave one block on a CU: its four wavefronts keep enough loads in
+        // flight, and a round more, begun or whole, costs more than it hides (16 bfloat16 rows of
+        // 2000 to 4095 tokens, eight KV heads: 39.4 us with one block a CU, 41.4 with two, 46.8
+        // with one and a half; fp32: 71.5, 74.7, 89.7). Short rows take no split: the second
+        // launch costs more than the steps it saves up to 512 keys of 16 bits (one row: 8.2 us,
+        // split 9.4; 768 keys: 10.3 and 9.3) and 256 of 32 (10.6 and 11.0; 384: 13.4 and 11.1).
+        const bool brief = span(kSmallTile) <= (wide ? 256 : 512);
+        cut(span(kSmallTile), brief ? 1 : cus / units, p.small_len, p.small_splits);
     }
     if (cols > p.small_cols) {
         const int64_t all = rows * group;
@@ -217,7 +224,7 @@ int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq
     AttnArgs a{};
     GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
     if (a.b.rows == 0) return 0;
-    return work_bytes_of(attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile), a.b.rows, heads, kv->head_dim);
+    return work_bytes_of(attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile, kv->dtype == GPHQ_DTYPE_F32), a.b.rows, heads, kv->head_dim);
 }
 
 int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
@@ -233,7 +240,7 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     if (spans_overlap(q, span_bytes(a.b.rows, q_stride, heads * hd, size), out,
                       span_bytes(a.b.rows, out_stride, heads * hd, size)))
         return GPHQ_ERR_OVERLAP;
-    const AttnPlan p = attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile);
+    const AttnPlan p = attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile, kv->dtype == GPHQ_DTYPE_F32);
     if (p.parts > 1 && (!work || (uintptr_t)work % 16 || work_bytes < work_bytes_of(p, a.b.rows, heads, hd)))
         return GPHQ_ERR_PAGED_SHAPE;
     a.q = q;

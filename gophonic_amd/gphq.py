@@ -241,11 +241,12 @@ class GphqError(RuntimeError):
 
 
 _lib = None
+_torch = None  # set by load(): an import statement in a call costs it about 0.3 us
 
 
 def load():
     """Loads libgphq.so (raises if it has not been built)."""
-    global _lib
+    global _lib, _torch
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(f"{LIB_PATH} is missing: run `python -m gophonic_amd.build` first")
@@ -253,8 +254,9 @@ def load():
         # The first one loaded serves the whole process, so load torch's before
         # libgphq: the binding hands torch streams and device pointers to the
         # library, and both sides must then talk to one HIP runtime.
-        import torch  # noqa: F401
+        import torch
 
+        _torch = torch
         lib = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(lib, name)
@@ -283,10 +285,9 @@ def ptr(t):
 
 
 def stream_handle(stream=None):
-    import torch
-
     if stream is None:  # the current stream's handle, without a Stream object (2.7 us less a call)
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+        load()
+        return _torch._C._cuda_getCurrentRawStream(_torch.cuda.current_device())
     return stream.cuda_stream
 
 
@@ -1076,9 +1077,7 @@ def _values(t, dtype, n, err):
 
 def _here(*tensors):
     """Refuses tensors that are not in the current device's memory, where the call's stream runs."""
-    import torch
-
-    dev = torch.cuda.current_device()
+    dev = _torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
             check(ERR_PAGED_SHAPE)
@@ -1097,6 +1096,7 @@ class PagedKv:
         # The stride of a dimension of one is never taken: one that the checks allow.
         ps, ts, hs = (s if n > 1 else hd for s, n in zip(k.stride()[:3], k.shape[:3]))
         self.desc = PagedKvDesc(ptr(k), ptr(v), ps, ts, hs, pages, tokens, heads, hd, _dtype(k.dtype), 0)
+        self.ref = ctypes.byref(self.desc)
         self.kv_heads, self.head_dim = heads, hd
 
 
@@ -1120,6 +1120,7 @@ class PagedBatch:
         self.rows = rows
         self.desc = PagedBatchDesc(ptr(starts), ptr(lens), ptr(table), table.shape[1], seqs, rows, max_rows, max_len,
                                    ptr(self.bad))
+        self.ref = ctypes.byref(self.desc)
 
     def check(self, stream=None):
         return check(load().gphq_paged_check(ptr(self.bad), stream_handle(stream)))
@@ -1130,26 +1131,23 @@ def paged_append(kv, batch, qkv, q, heads, q_norm=None, k_norm=None, eps=1e-6, c
     """gphq_paged_append: qkv [rows][(heads + 2 KV heads) head_dim] rows to
     prepared queries q [rows][heads head_dim] and keys and values in the pages.
     q_norm, k_norm float32 [head_dim]; cos, sin float32 [positions][head_dim / 2]."""
-    import torch
-
+    lib = load()
     _here(kv.k, batch.lens, qkv, q, q_norm, k_norm, cos, sin)
     if qkv.dtype != q.dtype or (cos is None) != (sin is None):
         check(ERR_PAGED_SHAPE)
     for t, n in ((q_norm, kv.head_dim), (k_norm, kv.head_dim), (cos, 0), (sin, 0)):
-        _values(t, torch.float32, n, ERR_PAGED_SHAPE)
+        _values(t, _torch.float32, n, ERR_PAGED_SHAPE)
     if cos is not None and (cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != kv.head_dim // 2):
         check(ERR_PAGED_SHAPE)
     qs = _rows2(qkv, batch.rows, (heads + 2 * kv.kv_heads) * kv.head_dim, ERR_PAGED_SHAPE)
     os_ = _rows2(q, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
-    return check(load().gphq_paged_append(ctypes.byref(kv.desc), ctypes.byref(batch.desc), _dtype(qkv.dtype), ptr(qkv),
-                                          qs, heads, ptr(q_norm), ptr(k_norm), eps, ptr(cos), ptr(sin),
-                                          0 if cos is None else cos.shape[0], q_scale, ptr(q), os_,
-                                          stream_handle(stream)))
+    return check(lib.gphq_paged_append(kv.ref, batch.ref, _dtype(qkv.dtype), ptr(qkv), qs, heads, ptr(q_norm),
+                                       ptr(k_norm), eps, ptr(cos), ptr(sin), 0 if cos is None else cos.shape[0],
+                                       q_scale, ptr(q), os_, stream_handle(stream)))
 
 
 def paged_attention_workspace_bytes(kv, batch, dtype, heads, window=0):
-    n = load().gphq_paged_attention_workspace_bytes(ctypes.byref(kv.desc), ctypes.byref(batch.desc), _dtype(dtype),
-                                                    heads, window)
+    n = load().gphq_paged_attention_workspace_bytes(kv.ref, batch.ref, _dtype(dtype), heads, window)
     return n if n >= 0 else check(n)
 
 
@@ -1163,6 +1161,7 @@ def paged_attention(kv, batch, q, out, heads, scale, window=0, work=None, stream
     """gphq_paged_attention: out [rows][heads head_dim] = causal attention of
     the rows q over their sequences' pages. work: a uint8 device tensor of
     paged_attention_workspace_bytes, or None for one of this call's own."""
+    lib = load()
     _here(kv.k, batch.lens, q, out, work)
     if q.dtype != out.dtype:
         check(ERR_PAGED_SHAPE)
@@ -1170,9 +1169,8 @@ def paged_attention(kv, batch, q, out, heads, scale, window=0, work=None, stream
     os_ = _rows2(out, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
     if work is None:
         work = _work(paged_attention_workspace_bytes(kv, batch, q.dtype, heads, window), q.device)
-    return check(load().gphq_paged_attention(ctypes.byref(kv.desc), ctypes.byref(batch.desc), _dtype(q.dtype), ptr(q),
-                                             qs, heads, scale, window, ptr(out), os_, ptr(work),
-                                             work.numel() * work.element_size(), stream_handle(stream)))
+    return check(lib.gphq_paged_attention(kv.ref, batch.ref, _dtype(q.dtype), ptr(q), qs, heads, scale, window, ptr(out),
+                                          os_, ptr(work), work.numel() * work.element_size(), stream_handle(stream)))
 
 
 class _PoolMemory:
@@ -1226,23 +1224,22 @@ def lora_add(a, b, x, y, row_slots, ranks=None, scales=None, work=None, stream=N
     for the rows with a slot in 0 .. slots - 1. a [slots][max_rank][k] and
     b [slots][n][max_rank]; x [rows][k] and y [rows][n] float32; row_slots and
     ranks int32, scales float32."""
-    import torch
-
+    lib = load()
     _here(a, b, x, y, row_slots, ranks, scales, work)
     if a.dim() != 3 or b.dim() != 3 or a.dtype != b.dtype or not a.is_contiguous() or not b.is_contiguous():
         check(ERR_DIMENSIONS)
     slots, max_rank, k = a.shape
     n, rows = b.shape[1], x.shape[0] if x.dim() == 2 else -1
-    if b.shape != (slots, n, max_rank) or x.dtype != torch.float32 or y.dtype != torch.float32 or rows < 0:
+    if b.shape != (slots, n, max_rank) or x.dtype != _torch.float32 or y.dtype != _torch.float32 or rows < 0:
         check(ERR_DIMENSIONS)
-    for t, count, dt in ((row_slots, rows, torch.int32), (ranks, slots, torch.int32), (scales, slots, torch.float32)):
+    for t, count, dt in ((row_slots, rows, _torch.int32), (ranks, slots, _torch.int32), (scales, slots, _torch.float32)):
         _values(t, dt, count, ERR_DIMENSIONS)
     xs, ys = _rows2(x, rows, k, ERR_DIMENSIONS), _rows2(y, rows, n, ERR_DIMENSIONS)
     if work is None:
         work = _work(lora_workspace_bytes(rows, k, max_rank), x.device)
-    return check(load().gphq_lora_add(_dtype(a.dtype), ptr(a), ptr(b), ptr(ranks), ptr(scales), slots, max_rank,
-                                      ptr(row_slots), ptr(x), xs, ptr(y), ys, rows, k, n, ptr(work),
-                                      work.numel() * work.element_size(), stream_handle(stream)))
+    return check(lib.gphq_lora_add(_dtype(a.dtype), ptr(a), ptr(b), ptr(ranks), ptr(scales), slots, max_rank,
+                                   ptr(row_slots), ptr(x), xs, ptr(y), ys, rows, k, n, ptr(work),
+                                   work.numel() * work.element_size(), stream_handle(stream)))
 
 
 # ---- weight preparation (gphq_prepare_projection) ----------------------------
