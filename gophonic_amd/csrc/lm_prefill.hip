@@ -26,6 +26,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <new>
 #include <type_traits>
 #include <utility>
 #include <vector>
@@ -1144,7 +1145,7 @@ int gphq_prefill_batch(gphq_prefill *ws, const gphq_prefix *shared, int64_t past
 
 int gphq_prefill_paged(gphq_prefill *ws, gphq_paged_pool *pool, const int32_t *tokens, const int64_t *lens,
                        const int64_t *past, int64_t count, const int32_t *table, int64_t table_stride,
-                       float *hidden_dev, int64_t hidden_len, void *stream) {
+                       float *hidden_dev, int64_t hidden_len, void *stream) try {
     if (!ws || !ws->lm) return GPHQ_ERR_WORKSPACE;
     const gphq_lm *lm = ws->lm;
     const gphq_lm_config &c = lm->cfg;
@@ -1164,18 +1165,18 @@ int gphq_prefill_paged(gphq_prefill *ws, gphq_paged_pool *pool, const int32_t *t
         total += n;
     }
     if (!table || table_stride < 1) return GPHQ_ERR_PAGED_SHAPE;
-    std::vector<char> written((size_t)pool->pages, 0);
+    std::vector<int32_t> written;  // the pages that receive tokens, each through one entry only
     for (int64_t q = 0; q < count; ++q) {
         const int64_t last = past[q] + lens[q] - 1;
         if (last / page >= table_stride) return GPHQ_ERR_PAGED_SHAPE;
         for (int64_t e = 0; e <= last / page; ++e) {
             const int32_t p = table[q * table_stride + e];
             if (p < 0 || p >= pool->pages) return GPHQ_ERR_PAGED_BATCH;
-            if (e < past[q] / page) continue;
-            if (written[p]) return GPHQ_ERR_PAGED_BATCH;
-            written[p] = 1;
+            if (e >= past[q] / page) written.push_back(p);
         }
     }
+    std::sort(written.begin(), written.end());
+    if (std::adjacent_find(written.begin(), written.end()) != written.end()) return GPHQ_ERR_PAGED_BATCH;
     hipStream_t st = (hipStream_t)stream;
     // Consecutive passes of up to the workspace's rows; a sequence may continue in the next.
     std::vector<int32_t> ints;
@@ -1235,6 +1236,8 @@ int gphq_prefill_paged(gphq_prefill *ws, gphq_paged_pool *pool, const int32_t *t
         done = off;
     }
     return GPHQ_OK;
+} catch (const std::bad_alloc &) {
+    return GPHQ_ERR_SCRATCH_LIMIT;  // host memory for the pass's tables
 }
 
 int gphq_prefill_check(gphq_prefill *ws, void *stream) {

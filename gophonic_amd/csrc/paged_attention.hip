@@ -2,6 +2,8 @@
 // join of split results. Kernels: paged_rows.hip and paged_chunk.hip.
 #include <math.h>
 
+#include <new>
+
 #include "lm_model.h"
 #include "paged_attention.h"
 
@@ -285,7 +287,8 @@ int gphq_paged_pool_new(const gphq_lm *lm, int64_t pages, int64_t page_tokens, i
     const gphq_lm_config &c = lm->cfg;
     const int64_t token = lm->kvd * (dtype == GPHQ_DTYPE_F32 ? 4 : 2);
     if (pages > INT64_MAX / (token * page_tokens * c.layers)) return GPHQ_ERR_PAGED_SHAPE;
-    gphq_paged_pool *p = new gphq_paged_pool();
+    gphq_paged_pool *p = new (std::nothrow) gphq_paged_pool();
+    if (!p) return GPHQ_ERR_SCRATCH_LIMIT;
     p->lm = lm;
     p->pages = pages;
     p->page_tokens = page_tokens;

@@ -1151,10 +1151,10 @@ def paged_attention_workspace_bytes(kv, batch, dtype, heads, window=0):
     return n if n >= 0 else check(n)
 
 
-def _work(need, device):
-    import torch
-
-    return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+def _work(need, device, stream):
+    """Scratch of one call, taken from the memory of the stream that the call runs on: there alone it is used again."""
+    with _torch.cuda.stream(stream):
+        return _torch.empty(max(need, 16), dtype=_torch.uint8, device=device)
 
 
 def paged_attention(kv, batch, q, out, heads, scale, window=0, work=None, stream=None):
@@ -1168,7 +1168,7 @@ def paged_attention(kv, batch, q, out, heads, scale, window=0, work=None, stream
     qs = _rows2(q, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
     os_ = _rows2(out, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
     if work is None:
-        work = _work(paged_attention_workspace_bytes(kv, batch, q.dtype, heads, window), q.device)
+        work = _work(paged_attention_workspace_bytes(kv, batch, q.dtype, heads, window), q.device, stream)
     return check(lib.gphq_paged_attention(kv.ref, batch.ref, _dtype(q.dtype), ptr(q), qs, heads, scale, window, ptr(out),
                                           os_, ptr(work), work.numel() * work.element_size(), stream_handle(stream)))
 
@@ -1236,7 +1236,7 @@ def lora_add(a, b, x, y, row_slots, ranks=None, scales=None, work=None, stream=N
         _values(t, dt, count, ERR_DIMENSIONS)
     xs, ys = _rows2(x, rows, k, ERR_DIMENSIONS), _rows2(y, rows, n, ERR_DIMENSIONS)
     if work is None:
-        work = _work(lora_workspace_bytes(rows, k, max_rank), x.device)
+        work = _work(lora_workspace_bytes(rows, k, max_rank), x.device, stream)
     return check(lib.gphq_lora_add(_dtype(a.dtype), ptr(a), ptr(b), ptr(ranks), ptr(scales), slots, max_rank,
                                    ptr(row_slots), ptr(x), xs, ptr(y), ys, rows, k, n, ptr(work),
                                    work.numel() * work.element_size(), stream_handle(stream)))

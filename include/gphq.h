@@ -603,10 +603,11 @@ int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, in
  * over the tokens j of row i's sequence up to its position p, and with
  * window > 0 only those past p - window. A row before token 0 sees none and
  * becomes 0. What a row does not see, whatever it holds (NaN included), does
- * not reach it. Any number of rows per sequence: prompt chunks and single
+ * not reach it; a row that sees a value that is not finite becomes not finite.
+ * scale may have either sign. Any number of rows per sequence: prompt chunks and single
  * tokens may stand in one call. fp32 rows are multiplied to fp32 accuracy
  * whatever the pool's type; 16-bit rows (the pool's type) round probabilities
- * to that type before the product with the values. out may not overlap q. work
+ * to that type before the product with the values. out may not overlap q (nor the pool). work
  * (16-byte aligned) of at least gphq_paged_attention_workspace_bytes for the
  * same pool, batch, row type, heads and window; its contents need not be kept
  * between calls, and calls that may run at the same time need one each. Sums
@@ -641,7 +642,8 @@ int gphq_paged_pool_layer(const gphq_paged_pool *pool, int64_t layer, gphq_paged
  * row_slots: device int32[rows]; a row whose slot is outside 0 .. slots - 1 has
  * no adapter and is left as it is. Rows may come in any order; neighbouring rows
  * of one adapter are fastest. fp32 products and sums in a fixed order.
- * k % 32 == 0, max_rank % 8 == 0 up to GPHQ_LORA_MAX_RANK, x_stride % 4 == 0;
+ * k % 32 == 0, max_rank % 8 == 0 up to GPHQ_LORA_MAX_RANK, x_stride % 4 == 0,
+ * rows x n below about 2^41;
  * A, B, x and work 16-byte aligned; y_stride and y are best multiples of 16
  * bytes. y must not overlap x. work: gphq_lora_workspace_bytes, one per call
  * that may run at the same time. */

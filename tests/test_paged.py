@@ -88,6 +88,7 @@ def test_append_refuses_queries_laid_over_other_rows():
 
 @pytest.mark.parametrize("over,want", [
     (dict(dtype=gphq.DTYPE_BF16), gphq.ERR_UNSUPPORTED), (dict(heads=0), gphq.ERR_PAGED_SHAPE),
+    (dict(scale=float("nan")), gphq.ERR_PAGED_SHAPE), (dict(scale=float("-inf")), gphq.ERR_PAGED_SHAPE),
     (dict(window=-1), gphq.ERR_PAGED_SHAPE), (dict(q_stride=252), gphq.ERR_PAGED_SHAPE),
     (dict(out_stride=258), gphq.ERR_PAGED_SHAPE), (dict(q=None), gphq.ERR_PAGED_SHAPE),
     (dict(out=P + (1 << 20) + 8), gphq.ERR_PAGED_SHAPE), (dict(out=P), gphq.ERR_OVERLAP),
@@ -141,6 +142,7 @@ def lora(**over):
     (dict(row_slots=None), gphq.ERR_DIMENSIONS), (dict(x=P + 8), gphq.ERR_DIMENSIONS), (dict(b=P + 8), gphq.ERR_DIMENSIONS),
     (dict(work=None), gphq.ERR_DIMENSIONS), (dict(bytes=191), gphq.ERR_DIMENSIONS), (dict(y=P + 2), gphq.ERR_DIMENSIONS),
     (dict(y=P), gphq.ERR_OVERLAP),
+    (dict(rows=1 << 20, n=1 << 30, y_stride=1 << 30, x=1 << 60, bytes=1 << 60), gphq.ERR_DIMENSIONS),
 ], ids=lambda v: str(v))
 def test_lora_refuses(over, want):
     assert lora(**over) == want

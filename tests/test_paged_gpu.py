@@ -311,6 +311,53 @@ def test_a_call_of_loose_bounds_gives_the_same_rows():
         assert (out[n:] == 7).all()
 
 
+@pytest.mark.parametrize("new", [1, 3, 9, 60])
+def test_one_sequence_of_fewer_rows_than_its_bound(new):
+    b = Batch([(new, 333)], 2, 128, 16, F16, seed=20, spare_rows=4)
+    q = b.randn(b.rows, 8 * 128)
+    out = attend(b, q, 8, 0.1, max_rows=64, max_len=16 * b.entries)
+    want, tol = attention64(b, q, 8, 0.1)
+    assert ((out[:new].cpu().double() - want[:new]).abs() <= tol[:new]).all()
+    assert (out[new:] == 7).all()
+
+
+@pytest.mark.parametrize("scale", [-0.15, 0.0, 1e-32, -1e-32])
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+def test_scales_of_every_kind(rt, ct, scale):
+    check_attention(Batch([(1, 200), (40, 70), (1, 0)], 2, 64, 16, ct, seed=21), 4, rt, scale=scale)
+
+
+def test_without_a_word_for_bad_values():
+    b = Batch([(1, 40), (2, 50)], 1, 64, 16, F32, seed=22)
+    kv, dev = b.device(gphq)
+    dev.desc.bad_dev = None
+    dev.lens.copy_(torch.tensor([40, 51], dtype=torch.int32))
+    out = torch.full((3, 128), 7.0, device="cuda")
+    q = b.randn(3, 128)
+    gphq.paged_attention(kv, dev, q.cuda(), out, 2, 0.1)
+    torch.cuda.synchronize()
+    want, tol = attention64(b, q, 2, 0.1)
+    assert ((out[0].cpu().double() - want[0]).abs() <= tol[0]).all() and (out[1:] == 7).all()
+
+
+def test_scratch_of_a_call_on_another_stream():
+    """Calls without a workspace on a side stream, with work on the current stream taking and giving back memory."""
+    b = Batch([(1, 3000), (1, 2500)], 1, 128, 16, BF16, seed=23)
+    q = b.randn(2, 4 * 128)
+    kv, dev = b.device(gphq)
+    dq, side = q.cuda(), torch.cuda.Stream()
+    want, tol = attention64(b, q, 4, 0.1)
+    torch.cuda.synchronize()
+    outs = [torch.empty(2, 512, device="cuda") for _ in range(8)]
+    torch.cuda.synchronize()
+    for o in outs:
+        gphq.paged_attention(kv, dev, dq, o, 4, 0.1, stream=side)
+        torch.full((1 << 16,), float("nan"), device="cuda")
+    torch.cuda.synchronize()
+    for o in outs:
+        assert ((o.cpu().double() - want).abs() <= tol).all()
+
+
 def test_strided_rows_another_stream_and_repeats():
     b = Batch([(1, 900), (1, 40), (20, 500)], 2, 128, 32, F16, seed=14)
     heads, D = 8, 128
