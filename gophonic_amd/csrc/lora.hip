@@ -140,7 +140,9 @@ __device__ __forceinline__ f32x4 product(const Frag<float>::weight &a, const Fra
 
 // t[split][r][0 .. max_rank) of a tile's rows, over k of one split: D (16 ranks x 16 rows)
 // = A . X^T per 16 ranks and 16 rows. The four wavefronts take every fourth 32 k and are
-// added in order.
+// added in order. Bound by reading x and A in long calls (4814 rows of 4096 and rank 64: 25 us,
+// 79 MB of x), by one wavefront's chain of loads in short ones, where k is cut into as many
+// ranges as leave a block two steps (32 rows of eight adapters: 7 us).
 template <typename W, int RT>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraArgs a) {
     typedef Frag<W> F;
@@ -215,7 +217,9 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraArgs a) {
 
 // y[r][n0 .. n0 + n_block) += scale * B t[r] of the tile's 16 RH rows: D (16 rows x 16
 // columns) = T . B^T, four column tiles at once, tile j holding columns 4 i + j, so that a
-// lane has four neighbouring columns of y. EARLY: y is read before the products, so that the
+// lane has four neighbouring columns of y. Bound by reading and writing y in long calls (4814
+// rows of 6144: 56 us, 237 MB), by the chain t, B, y in short ones (32 rows of eight adapters
+// beside 24576 columns: 13 us). EARLY: y is read before the products, so that the
 // two reads are on their way together, at the price of registers and so of wavefronts at once
 // (4814 rows beside 6144 columns: 106 us, 125 without; 32 rows of eight adapters beside 24576
 // columns, whose blocks have one adapter each and are many: 25 us, 21 without).
