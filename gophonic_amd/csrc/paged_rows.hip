@@ -335,13 +335,13 @@ __global__ __launch_bounds__(256, 2) void attn_rows16_kernel(const AttnArgs a, i
     rows_finish<RT, HD>(a, t, m, l, o);
 }
 
+// fp32 pages, the same walk on v_mfma_f32_16x16x4_f32: its operands are one fp32 value a
+// lane, so V needs no exchange between registers, and a lane's 16-byte pieces of K and Q
+// hold the same dims (16 i + 4 g4 ..), in whatever order they are multiplied.
 // 16 rows of 2000 to 4095 tokens, eight KV heads: 72 us with the join (364 MB, 5.1 TB/s). A
 // 32-key step's 128 instructions take 4096 cycles for 32 KB, so the memory stays the bound;
 // one block a CU with all the registers it asks for measured faster than two with 256 a lane
 // (kernel alone 72.7 and 78.7 us).
-// fp32 pages, the same walk on v_mfma_f32_16x16x4_f32: its operands are one fp32 value a
-// lane, so V needs no exchange between registers, and a lane's 16-byte pieces of K and Q
-// hold the same dims (16 i + 4 g4 ..), in whatever order they are multiplied.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int tiles, int splits) {
     constexpr int KC = HD / 16, VD = HD / 16;
