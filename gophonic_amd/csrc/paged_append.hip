@@ -53,8 +53,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const AppendArgs a) {
 
     const SeqRow s = find_seq(a.b, row);
     if (row < s.start || row >= s.end) {
-        // Behind the last sequence: left alone. Inside it by no valid starts: bad.
-        if (row < a.b.starts[a.b.seqs] && lane == 0) paged_flag(a.b, PAGED_BAD_SEQ);
+        // Before the first sequence or behind the last: left alone. Else in none by bad starts.
+        if (row >= a.b.starts[0] && row < a.b.starts[a.b.seqs] && lane == 0) paged_flag(a.b, PAGED_BAD_SEQ);
         return;
     }
     const int pos = s.len - (s.end - row);

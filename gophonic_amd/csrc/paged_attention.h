@@ -24,11 +24,12 @@ struct AttnArgs {
     PagedPool pool;
     const void *q;
     void *out;
-    float *part_o;   // [row][head][parts][hd]
-    float *part_ml;  // [row][head][parts][2]: reference, sum
+    // Split results, output and (reference, sum): the chunk kernel's by [row][head][parts], the
+    // row kernel's, whose splits may be many, by [sequence][small_rows][head][small_parts].
+    float *part_o, *part_ml, *small_o, *small_ml;
     int64_t q_stride, out_stride;
     int heads, group, window;
-    int parts;             // split slots per (row, head) in the workspace
+    int parts, small_parts, small_rows;
     int small_cols;        // sequences of at most this many columns are the row kernel's
     int big_tile;          // columns of the chunk kernel's tiles
     float q_sign;          // the sign of scale (0 if scale is 0), applied to the queries

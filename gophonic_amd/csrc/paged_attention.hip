@@ -50,7 +50,7 @@ namespace {
 struct AttnPlan {
     int small_cols, small_tiles, small_splits, small_len;  // small_tiles per sequence; 0: the row kernel is not run
     int big_tiles, big_splits, big_len;                    // big_tiles in all; 0: the chunk kernel is not run
-    int parts;
+    int small_rows;  // rows that a sequence of the row kernel may have
 };
 
 // Keys per split of `span` keys and how many splits that makes, for about `want` of them.
@@ -72,7 +72,8 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
     auto span = [&](int64_t tile) {  // keys a tile of that many columns may see, from a multiple of 64
         return window > 0 ? std::min<int64_t>(b.max_len, (int64_t)window + tile / group + 65) : (int64_t)b.max_len;
     };
-    if (p.small_cols) {
+    if (p.small_cols && group <= p.small_cols) {
+        p.small_rows = std::min(p.small_cols / group, b.max_rows);
         p.small_tiles = (int)((std::min<int64_t>(cols, p.small_cols) + kSmallTile - 1) / kSmallTile);
         const int64_t units = std::min<int64_t>(b.seqs, rows) * p.small_tiles * kv_heads;
         // As many splits as leave one block on a CU: its four wavefronts keep enough loads in
@@ -96,20 +97,24 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         p.big_tiles = (int)((all + s * (big_tile - 1)) / big_tile);
         const int64_t units = (int64_t)p.big_tiles * kv_heads;
         const int64_t slots = big_tile == 256 ? cus : 2 * cus;  // blocks that run at once
-        // Tiles enough for the chip are not split (three chunks of 300 to 1300 fp32 rows over FP16 pages: 106 us, split in
-        // three 133). Fewer tiles of one sequence take as many splits as fill it (512 FP16 rows
-        // over 7512 tokens: 84 us, twice as many 100); of several, whose lengths differ, three times
-        // as many, so that the long ones do not come last alone (twelve chunks of 1 to 300 fp32
-        // rows over up to 4000 bfloat16 tokens: 240 us, 293 with one round, 261 with four times).
+        // Tiles enough for the chip are not split (three chunks of 300 to 1300 fp32 rows over
+        // FP16 pages: 106 us, split in three 133). Fewer tiles of one sequence take as many splits
+        // as fill it (512 FP16 rows over 7512 tokens: 84 us, twice as many 100); of several, whose
+        // lengths differ, three times as many, so that the long ones do not come last alone (twelve
+        // chunks of 1 to 300 fp32 rows over up to 4000 bfloat16 tokens: 240 us, 293 with one round,
+        // 261 with four times).
         const int64_t want = units >= slots ? 1 : (b.seqs == 1 ? 1 : 3) * slots / units;
         cut(span(big_tile), want, p.big_len, p.big_splits);
     }
-    p.parts = std::max(p.small_tiles ? p.small_splits : 1, p.big_tiles ? p.big_splits : 1);
     return p;
 }
 
-int64_t work_bytes_of(const AttnPlan &p, int64_t rows, int64_t heads, int64_t hd) {
-    return p.parts > 1 ? rows * heads * p.parts * (hd + 2) * 4 : 0;
+// Split results that the workspace holds for each kernel.
+int64_t small_count(const AttnPlan &p, const PagedBatch &b, int64_t heads) {
+    return p.small_tiles && p.small_splits > 1 ? (int64_t)b.seqs * p.small_rows * heads * p.small_splits : 0;
+}
+int64_t big_count(const AttnPlan &p, const PagedBatch &b, int64_t heads) {
+    return p.big_tiles && p.big_splits > 1 ? b.rows * heads * p.big_splits : 0;
 }
 
 // Adds the split results of every (row, head): with M = max m_i,
@@ -135,7 +140,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
     const TileKeys k = tile_keys(n, s.len, c0 / a.group, min((c0 + tm - 1) / a.group, n - 1), a.window);
     const int all = head < a.heads ? tile_splits(k, small ? a.split_small : a.split_big) : 1;
     const int splits = all > 1 ? all : 0;  // (heads of a row may lie in different tiles)
-    const int64_t at = ((int64_t)row * a.heads + min(head, a.heads - 1)) * a.parts;
+    const int hc = min(head, a.heads - 1);
+    const int64_t at = small ? (((int64_t)s.seq * a.small_rows + i) * a.heads + hc) * a.small_parts
+                             : ((int64_t)row * a.heads + hc) * a.parts;
+    const float *part_o = small ? a.small_o : a.part_o, *part_ml = small ? a.small_ml : a.part_ml;
     const int d = 4 * (lane % LH);
     float M = -INFINITY, L = 0.0f;
     f32x4 o{};
@@ -146,8 +154,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int64_t e = at + min(j0 + u, splits - 1);
-            ml[u] = *(const f32x2 *)(a.part_ml + 2 * e);
-            v[u] = *(const f32x4 *)(a.part_o + e * HD + d);
+            ml[u] = *(const f32x2 *)(part_ml + 2 * e);
+            v[u] = *(const f32x4 *)(part_o + e * HD + d);
         }
         float mx = M;
 #pragma unroll
@@ -197,7 +205,7 @@ template <typename RT, int HD>
 int join_launch(const AttnArgs &a, hipStream_t st) {
     constexpr int HW = 256 / HD;
     const int64_t units = (int64_t)a.b.rows * ((a.heads + HW - 1) / HW);
-    if (a.parts > 8)
+    if (std::max(a.parts, a.small_parts) > 8)
         hipLaunchKernelGGL((paged_join_kernel<RT, HD, 4>), dim3((unsigned)units), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((paged_join_kernel<RT, HD, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
@@ -208,8 +216,12 @@ template <typename RT, typename CT>
 int attend(const AttnArgs &a, const AttnPlan &p, int hd, hipStream_t st) {
     if (p.big_tiles) GPHQ_TRY((attn_chunk_launch<RT, CT>(a, hd, p.big_splits, p.big_tiles, st)));
     if (p.small_tiles) GPHQ_TRY((attn_rows_launch<RT, CT>(a, hd, p.small_splits, p.small_tiles, st)));
-    if (p.parts == 1) return GPHQ_OK;
+    if (!small_count(p, a.b, a.heads) && !big_count(p, a.b, a.heads)) return GPHQ_OK;
     return hd == 128 ? join_launch<RT, 128>(a, st) : join_launch<RT, 64>(a, st);
+}
+
+AttnPlan plan_of(const AttnArgs &a, const gphq_paged_kv *kv) {
+    return attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile, kv->dtype == GPHQ_DTYPE_F32);
 }
 
 // The checks that the attention and its workspace size share.
@@ -240,7 +252,8 @@ int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq
     AttnArgs a{};
     GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
     if (a.b.rows == 0) return 0;
-    return work_bytes_of(attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile, kv->dtype == GPHQ_DTYPE_F32), a.b.rows, heads, kv->head_dim);
+    const AttnPlan p = plan_of(a, kv);
+    return (small_count(p, a.b, heads) + big_count(p, a.b, heads)) * (kv->head_dim + 2) * 4;
 }
 
 int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
@@ -256,16 +269,21 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     if (spans_overlap(q, span_bytes(a.b.rows, q_stride, heads * hd, size), out,
                       span_bytes(a.b.rows, out_stride, heads * hd, size)))
         return GPHQ_ERR_OVERLAP;
-    const AttnPlan p = attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile, kv->dtype == GPHQ_DTYPE_F32);
-    if (p.parts > 1 && (!work || (uintptr_t)work % 16 || work_bytes < work_bytes_of(p, a.b.rows, heads, hd)))
+    const AttnPlan p = plan_of(a, kv);
+    const int64_t big = big_count(p, a.b, heads), small = small_count(p, a.b, heads);
+    if (big + small && (!work || (uintptr_t)work % 16 || work_bytes < (big + small) * (hd + 2) * 4))
         return GPHQ_ERR_PAGED_SHAPE;
     a.q = q;
     a.out = out;
     a.q_stride = q_stride;
     a.out_stride = out_stride;
-    a.parts = p.parts;
+    a.parts = big ? p.big_splits : 1;
+    a.small_parts = small ? p.small_splits : 1;
+    a.small_rows = p.small_rows;
     a.part_o = (float *)work;
-    a.part_ml = (float *)work + (int64_t)a.b.rows * heads * p.parts * hd;
+    a.small_o = a.part_o + big * hd;
+    a.part_ml = a.small_o + small * hd;
+    a.small_ml = a.part_ml + 2 * big;
     a.small_cols = p.small_cols;
     a.split_small = p.small_len;
     a.split_big = p.big_len;

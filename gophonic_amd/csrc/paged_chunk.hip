@@ -302,6 +302,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
     int buf = 0;
     for (int kt = t.k0; kt < t.k1; kt += KB, buf ^= 1) {
         wait_vm_lgkm0<0>();
+        asm volatile("" ::: "memory");  // the wait is no memory operation: mend's reads stay behind it
         const unsigned okc = ok;
         const bool edge = chunk_edge(a, t, kt, KB) || okc != 15;
         if (edge) mend(kt, okc, buf);

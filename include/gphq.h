@@ -560,8 +560,8 @@ typedef struct gphq_paged_kv {
  * lens[s] - n + i), and token p of it lies in slot p % page_tokens of page
  * table[s * table_stride + p / page_tokens]. All three are device arrays of
  * int32, read when the work runs: a captured call may be replayed with other
- * values. rows is what the row buffers hold; rows behind starts[seqs] are left
- * as they are. max_rows and max_len bound the rows of one sequence and lens;
+ * values. rows is what the row buffers hold; rows before starts[0] and behind
+ * starts[seqs] are left as they are. max_rows and max_len bound the rows of one sequence and lens;
  * the work is cut by these bounds, so tight ones are faster. Table entries
  * that no token of the call needs may hold anything.
  * The device checks what it reads. A sequence whose starts descend or leave

@@ -112,6 +112,17 @@ def test_attention_refuses_a_short_workspace():
         assert lib.gphq_paged_attention_workspace_bytes(ctypes.byref(k), ctypes.byref(b), *d.values()) < 0
 
 
+@pytest.mark.parametrize("seqs,rows,max_rows,max_len", [(2, 8192, 8192, 40960), (16, 1 << 20, 1 << 20, 40960),
+                                                        (1, 2048, 2048, 1 << 20), (300, 4096, 2048, 40960)])
+def test_the_workspace_stays_small(seqs, rows, max_rows, max_len):
+    """Splits are cut so that the blocks in flight hold them, at most a few rounds of the chip's: under 256 MiB."""
+    k = kv(kv_heads=8, pages=1 << 20, head_stride=2048, page_stride=16384)
+    b = batch(seqs=seqs, rows=rows, max_rows=max_rows, max_len=max_len, table_stride=max_len // 16)
+    for heads in (8, 32, 64):
+        n = gphq.load().gphq_paged_attention_workspace_bytes(ctypes.byref(k), ctypes.byref(b), gphq.DTYPE_F32, heads, 0)
+        assert 0 <= n < 256 << 20
+
+
 def test_null_descriptions_are_refused():
     lib = gphq.load()
     assert lib.gphq_paged_attention_workspace_bytes(None, ctypes.byref(batch()), 3, 2, 0) == gphq.ERR_PAGED_SHAPE

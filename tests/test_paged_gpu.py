@@ -327,6 +327,24 @@ def test_scales_of_every_kind(rt, ct, scale):
     check_attention(Batch([(1, 200), (40, 70), (1, 0)], 2, 64, 16, ct, seed=21), 4, rt, scale=scale)
 
 
+def test_a_slice_of_a_batch():
+    """Sequences 1 and 2 of three, by views of the tables: rows of the others stay as they are, and none is bad."""
+    b = Batch([(3, 40), (1, 700), (50, 90), (2, 30)], 2, 64, 16, F16, seed=24)
+    q = b.randn(b.rows, 4 * 64)
+    kv, dev = b.device(gphq)
+    part = gphq.PagedBatch(dev.starts[1:4], dev.lens[1:3], dev.table[1:3], b.rows, 50, 700)
+    out = torch.full((b.rows, 4 * 64), 7.0, device="cuda")
+    gphq.paged_attention(kv, part, q.cuda(), out, 4, 0.1)
+    part.check()
+    want, tol = attention64(b, q, 4, 0.1)
+    assert ((out[3:54].cpu().double() - want[3:54]).abs() <= tol[3:54]).all()
+    assert (out[:3] == 7).all() and (out[54:] == 7).all()
+    out.fill_(7.0)
+    gphq.paged_append(kv, part, b.randn(b.rows, 8 * 64).cuda(), out, 4)
+    part.check()
+    assert (out[:3] == 7).all() and (out[54:] == 7).all() and (out[3:54] != 7).all()
+
+
 def test_without_a_word_for_bad_values():
     b = Batch([(1, 40), (2, 50)], 1, 64, 16, F32, seed=22)
     kv, dev = b.device(gphq)
