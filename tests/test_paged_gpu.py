@@ -327,6 +327,17 @@ def test_scales_of_every_kind(rt, ct, scale):
     check_attention(Batch([(1, 200), (40, 70), (1, 0)], 2, 64, 16, ct, seed=21), 4, rt, scale=scale)
 
 
+@pytest.mark.parametrize("heads,kv_heads,rows", [(2, 2, (63, 64, 65)), (8, 2, (15, 16, 17)), (14, 2, (9, 10, 1)),
+                                                 (64, 1, (1, 2, 1)), (65, 1, (1, 1, 2))])
+@pytest.mark.parametrize("rt,ct", [(F32, F32), (F32, F16), (torch.bfloat16, torch.bfloat16)])
+def test_columns_on_both_sides_of_the_two_kernels(heads, kv_heads, rows, rt, ct):
+    """Rows times group about 64: each sequence in one kernel or the other, alone and with the rest."""
+    shape = [(n, n + 150 + 700 * i) for i, n in enumerate(rows)]
+    check_attention(Batch(shape, kv_heads, 64, 16, ct, seed=25), heads, rt)
+    for one in shape:
+        check_attention(Batch([one], kv_heads, 64, 16, ct, seed=26), heads, rt)
+
+
 def test_a_slice_of_a_batch():
     """Sequences 1 and 2 of three, by views of the tables: rows of the others stay as they are, and none is bad."""
     b = Batch([(3, 40), (1, 700), (50, 90), (2, 30)], 2, 64, 16, F16, seed=24)
