@@ -393,7 +393,7 @@ using namespace gphq;
 extern "C" {
 
 int64_t gphq_lora_workspace_bytes(int64_t rows, int64_t k, int64_t max_rank) {
-    if (rows < 0 || rows > GPHQ_PAGED_MAX_ROWS || k < 0 || k > INT32_MAX || k % 32 || max_rank < 0 ||
+    if (rows < 0 || rows > GPHQ_PAGED_MAX_ROWS || k < 0 || k > 1 << 30 || k % 32 || max_rank < 0 ||
         max_rank > GPHQ_LORA_MAX_RANK || max_rank % 8)
         return GPHQ_ERR_DIMENSIONS;
     if (rows == 0 || k == 0) return 0;
