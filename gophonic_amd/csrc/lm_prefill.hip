@@ -1165,18 +1165,21 @@ int gphq_prefill_paged(gphq_prefill *ws, gphq_paged_pool *pool, const int32_t *t
         total += n;
     }
     if (!table || table_stride < 1) return GPHQ_ERR_PAGED_SHAPE;
-    std::vector<int32_t> written;  // the pages that receive tokens, each through one entry only
+    std::vector<bool> written((size_t)pool->pages);  // the pages that receive tokens, each through one entry only
     for (int64_t q = 0; q < count; ++q) {
         const int64_t last = past[q] + lens[q] - 1;
         if (last / page >= table_stride) return GPHQ_ERR_PAGED_SHAPE;
         for (int64_t e = 0; e <= last / page; ++e) {
             const int32_t p = table[q * table_stride + e];
             if (p < 0 || p >= pool->pages) return GPHQ_ERR_PAGED_BATCH;
-            if (e >= past[q] / page) written.push_back(p);
+            if (e < past[q] / page) continue;
+            if (written[p]) return GPHQ_ERR_PAGED_BATCH;
+            written[p] = true;
         }
     }
-    std::sort(written.begin(), written.end());
-    if (std::adjacent_find(written.begin(), written.end()) != written.end()) return GPHQ_ERR_PAGED_BATCH;
+    for (int64_t q = 0; q < count; ++q)
+        for (int64_t e = 0; e < past[q] / page; ++e)
+            if (written[table[q * table_stride + e]]) return GPHQ_ERR_PAGED_BATCH;
     hipStream_t st = (hipStream_t)stream;
     // Consecutive passes of up to the workspace's rows; a sequence may continue in the next.
     std::vector<int32_t> ints;

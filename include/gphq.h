@@ -561,14 +561,15 @@ typedef struct gphq_paged_kv {
  * table[s * table_stride + p / page_tokens]. All three are device arrays of
  * int32, read when the work runs: a captured call may be replayed with other
  * values. rows is what the row buffers hold; rows before starts[0] and behind
- * starts[seqs] are left as they are. max_rows and max_len bound the rows of one sequence and lens;
- * the work is cut by these bounds, so tight ones are faster. Table entries
- * that no token of the call needs may hold anything.
+ * starts[seqs] are left as they are. max_rows and max_len bound the rows of one
+ * sequence and lens; the work is cut by these bounds, so tight ones are faster.
+ * Table entries that no token of the call needs may hold anything.
  * The device checks what it reads. A sequence whose starts descend or leave
  * the rows, with more than max_rows rows, or with lens outside 0 .. max_len is
- * skipped whole (and where starts descend, others may be with it); a needed page number outside the pool stores nothing and
- * reads as masked keys; each also sets a bit of *bad_dev (may be NULL), which
- * gphq_paged_check waits for, reports as GPHQ_ERR_PAGED_BATCH and clears. */
+ * skipped whole (and where starts descend, others may be with it); a needed
+ * page number outside the pool stores nothing and reads as masked keys; each
+ * also sets a bit of *bad_dev (may be NULL), which gphq_paged_check waits for,
+ * reports as GPHQ_ERR_PAGED_BATCH and clears. */
 typedef struct gphq_paged_batch {
     const int32_t *starts_dev; /* [seqs + 1], ascending */
     const int32_t *lens_dev;   /* [seqs] */
@@ -809,10 +810,10 @@ int gphq_prefill_batch(gphq_prefill *ws, const gphq_prefix *shared, int64_t past
  * [count][hidden] receives the post-final-norm state of sequence s's last
  * token. Tokens beyond the workspace's rows run as consecutive passes, in
  * order. Validation as gphq_prefill_batch's per sequence, then the table: a
- * needed entry outside the pool, or a page that would be written through two
- * entries, is GPHQ_ERR_PAGED_BATCH; before any device work. Sequences may share
- * pages of earlier tokens, which are only read. Waits for each pass's host
- * arrays to be consumed. gphq_prefill_check reports a non-finite state. */
+ * needed entry outside the pool, or a page that receives tokens and stands in
+ * another needed entry too, is GPHQ_ERR_PAGED_BATCH; before any device work.
+ * Sequences may share full pages of earlier tokens, which are only read. Waits
+ * for each pass's host arrays to be consumed. gphq_prefill_check reports a non-finite state. */
 int gphq_prefill_paged(gphq_prefill *ws, gphq_paged_pool *pool, const int32_t *tokens, const int64_t *lens,
                        const int64_t *past, int64_t count, const int32_t *table, int64_t table_stride,
                        float *hidden_dev, int64_t hidden_len, void *stream);

@@ -146,6 +146,17 @@ def test_paged_pass_refuses(lm, seqs, past, table, status):
     assert (h == 7).all()
 
 
+@pytest.mark.parametrize("seqs,past,table", [
+    ([[1]], [16], [[3, 3]]), ([[1], [2]], [16, 0], [[3, 4], [3, 5]]), ([[1], [2]], [5, 40], [[3, 0, 0], [4, 3, 5]]),
+])
+def test_paged_pass_refuses_to_write_a_page_that_is_read(lm, seqs, past, table):
+    """A page of earlier tokens, of the same sequence or another's, that this step would write over."""
+    pool, pf = gphq.PagedPool(lm, 12, 16, F16), gphq.Prefill(lm, 128)
+    with pytest.raises(gphq.GphqError) as e:
+        pf.paged(pool, seqs, past, np.asarray(table), torch.empty(len(seqs), GEOM["hidden"], device="cuda"))
+    assert e.value.status == gphq.ERR_PAGED_BATCH
+
+
 def test_paged_pass_refuses_another_model_s_pool(lm):
     other = gphq.lm_random(dict(GEOM, layers=1), gphq.FMT_Q8B, 7)[0]
     pool, pf = gphq.PagedPool(other, 4, 16, F16), gphq.Prefill(lm, 16)
