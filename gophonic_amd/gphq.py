@@ -1091,6 +1091,8 @@ class PagedKv:
     def __init__(self, k, v):
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
             check(ERR_PAGED_SHAPE)
+        if k.device != v.device:
+            check(ERR_PAGED_SHAPE)
         self.k, self.v, self.dtype = k, v, k.dtype
         pages, tokens, heads, hd = k.shape
         # The stride of a dimension of one is never taken: one that the checks allow.
@@ -1115,6 +1117,8 @@ class PagedBatch:
             check(ERR_PAGED_SHAPE)
         for v, n in ((starts, seqs + 1), (lens, seqs), (table, 0)):
             _values(v, torch.int32, n, ERR_PAGED_SHAPE)
+            if v.device != lens.device:
+                check(ERR_PAGED_SHAPE)
         self.starts, self.lens, self.table = starts, lens, table
         self.bad = torch.zeros(1, dtype=torch.int32, device=lens.device)
         self.rows = rows

@@ -175,3 +175,20 @@ def test_pool_and_paged_pass_refuse_null_handles():
     assert lib.gphq_paged_pool_layer(None, 0, ctypes.byref(kv())) == gphq.ERR_PAGED_SHAPE
     assert lib.gphq_prefill_paged(None, None, None, None, None, 1, None, 1, None, 0, None) == gphq.ERR_WORKSPACE
     lib.gphq_paged_pool_free(None)
+
+
+def test_descriptions_over_two_devices_are_refused():
+    import torch
+
+    def ints(n, device="cpu"):
+        return torch.zeros(n, dtype=torch.int32, device=device)
+
+    pages = torch.zeros(2, 16, 1, 64)
+    cases = [lambda: gphq.PagedKv(pages, torch.empty_like(pages, device="meta")),
+             lambda: gphq.PagedBatch(ints(3, "meta"), ints(2), ints((2, 1)), 2, 1, 16),
+             lambda: gphq.PagedBatch(ints(3), ints(2), ints((2, 1), "meta"), 2, 1, 16),
+             lambda: gphq.PagedBatch(ints(3, "meta"), ints(2, "meta"), ints((2, 1)), 2, 1, 16)]
+    for make in cases:
+        with pytest.raises(gphq.GphqError) as e:
+            make()
+        assert e.value.status == gphq.ERR_PAGED_SHAPE
