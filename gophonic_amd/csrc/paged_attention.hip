@@ -205,11 +205,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
     store_vec((RT *)a.out + (int64_t)row * a.out_stride + head * HD + d, r);
 }
 
+constexpr int64_t kMaxBlocks = (1 << 23) - 1;  // of a launch: 2^32 threads at 512 a block are one too many
+
+int64_t join_units(const PagedBatch &b, int64_t heads, int hd) { return b.rows * ((heads * hd + 255) / 256); }
+
 template <typename RT, int HD>
 int join_launch(const AttnArgs &a, hipStream_t st) {
-    constexpr int HW = 256 / HD;
-    const int64_t units = (int64_t)a.b.rows * ((a.heads + HW - 1) / HW);
-    if (std::max(a.parts, a.small_parts) > 8)
+    const int64_t units = join_units(a.b, a.heads, HD);
+    if (std::max(a.parts, a.small_parts) > 8 && units <= kMaxBlocks)
         hipLaunchKernelGGL((paged_join_kernel<RT, HD, 4>), dim3((unsigned)units), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((paged_join_kernel<RT, HD, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
@@ -224,8 +227,16 @@ int attend(const AttnArgs &a, const AttnPlan &p, int hd, hipStream_t st) {
     return hd == 128 ? join_launch<RT, 128>(a, st) : join_launch<RT, 64>(a, st);
 }
 
-AttnPlan plan_of(const AttnArgs &a, const gphq_paged_kv *kv) {
-    return attn_plan(a.b, a.pool.kv_heads, a.group, a.window, a.big_tile, kv->dtype == GPHQ_DTYPE_F32);
+// The call's cut, refused where a launch would have too many blocks.
+int plan_of(const AttnArgs &a, const gphq_paged_kv *kv, AttnPlan &p) {
+    const int64_t kvh = a.pool.kv_heads;
+    p = attn_plan(a.b, (int)kvh, a.group, a.window, a.big_tile, kv->dtype == GPHQ_DTYPE_F32);
+    if ((int64_t)a.b.seqs * p.small_tiles * p.small_splits * kvh > kMaxBlocks ||
+        (int64_t)p.big_tiles * p.big_splits * kvh > kMaxBlocks)
+        return GPHQ_ERR_PAGED_SHAPE;
+    const bool join = small_count(p, a.b, a.heads) || big_count(p, a.b, a.heads);
+    // (The join's blocks take 256 threads, and four units where there are many.)
+    return join && join_units(a.b, a.heads, (int)kv->head_dim) / 8 > kMaxBlocks ? GPHQ_ERR_PAGED_SHAPE : GPHQ_OK;
 }
 
 // The checks that the attention and its workspace size share.
@@ -256,7 +267,8 @@ int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq
     AttnArgs a{};
     GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
     if (a.b.rows == 0) return 0;
-    const AttnPlan p = plan_of(a, kv);
+    AttnPlan p;
+    GPHQ_TRY(plan_of(a, kv, p));
     return (small_count(p, a.b, heads) + big_count(p, a.b, heads)) * (kv->head_dim + 2) * 4;
 }
 
@@ -273,7 +285,8 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     if (spans_overlap(q, span_bytes(a.b.rows, q_stride, heads * hd, size), out,
                       span_bytes(a.b.rows, out_stride, heads * hd, size)))
         return GPHQ_ERR_OVERLAP;
-    const AttnPlan p = plan_of(a, kv);
+    AttnPlan p;
+    GPHQ_TRY(plan_of(a, kv, p));
     const int64_t big = big_count(p, a.b, heads), small = small_count(p, a.b, heads);
     if (big + small && (!work || (uintptr_t)work % 16 || work_bytes < (big + small) * (hd + 2) * 4))
         return GPHQ_ERR_PAGED_SHAPE;

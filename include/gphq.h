@@ -608,7 +608,9 @@ int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, in
  * scale may have either sign. Any number of rows per sequence: prompt chunks and single
  * tokens may stand in one call. fp32 rows are multiplied to fp32 accuracy
  * whatever the pool's type; 16-bit rows (the pool's type) round probabilities
- * to that type before the product with the values. out may not overlap q (nor the pool). work
+ * to that type before the product with the values. out may not overlap q (nor
+ * the pool). A batch of about 2^23 tiles (16 columns of a KV head in sequences
+ * of up to 64 columns, 128 in others) or more is GPHQ_ERR_PAGED_SHAPE. work
  * (16-byte aligned) of at least gphq_paged_attention_workspace_bytes for the
  * same pool, batch, row type, heads and window; its contents need not be kept
  * between calls, and calls that may run at the same time need one each. Sums

@@ -123,6 +123,19 @@ def test_the_workspace_stays_small(seqs, rows, max_rows, max_len):
         assert 0 <= n < 256 << 20
 
 
+@pytest.mark.parametrize("over,heads,kv_heads,fits", [
+    (dict(seqs=65536, rows=65536, max_rows=1), 127, 127, True), (dict(seqs=65536, rows=65536, max_rows=1), 128, 128, False),
+    (dict(seqs=65536, rows=1 << 20, max_rows=16), 128, 32, False),
+    (dict(seqs=1, rows=1 << 20, max_rows=1 << 20), 512, 8, True), (dict(seqs=1, rows=1 << 20, max_rows=1 << 20), 1024, 8, False),
+    (dict(seqs=2, rows=1 << 20, max_rows=1 << 20), 128, 2, False),
+])
+def test_attention_refuses_more_blocks_than_a_launch_takes(over, heads, kv_heads, fits):
+    k = kv(kv_heads=kv_heads, head_stride=2048, page_stride=2048 * kv_heads)
+    b = batch(max_len=4096, table_stride=256, **over)
+    n = gphq.load().gphq_paged_attention_workspace_bytes(ctypes.byref(k), ctypes.byref(b), gphq.DTYPE_F16, heads, 0)
+    assert (n >= 0) == fits and (fits or n == gphq.ERR_PAGED_SHAPE)
+
+
 def test_null_descriptions_are_refused():
     lib = gphq.load()
     assert lib.gphq_paged_attention_workspace_bytes(None, ctypes.byref(batch()), 3, 2, 0) == gphq.ERR_PAGED_SHAPE
