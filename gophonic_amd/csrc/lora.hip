@@ -436,10 +436,11 @@ int gphq_lora_add(int dtype, const void *a_dev, const void *b_dev, const int32_t
     p.n = (int)n;
     p.vec = y_stride % 4 == 0 && (uintptr_t)y % 16 == 0;
     lora_plan(rows, k, n, p);
-    const int64_t tiles = (rows + 15) / 16, per = (n + p.n_block - 1) / p.n_block;
-    if (tiles * std::max<int64_t>(per, p.splits) > INT32_MAX / 16) return GPHQ_ERR_DIMENSIONS;  // the grid's blocks
     // Few tiles: the adapters of a tile go to blocks of their own.
     p.passes = rows <= kFewRows ? (int)std::min<int64_t>(std::min<int64_t>(slots, rows), 16) : 1;
+    const int64_t tiles = (rows + 15) / 16, per = (n + p.n_block - 1) / p.n_block;
+    if (tiles * std::max<int64_t>(per, p.splits) * p.passes > (1 << 24) - 1)  // blocks of 256, under 2^32 threads
+        return GPHQ_ERR_DIMENSIONS;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == GPHQ_DTYPE_F32) return lora_run<float>(p, st);
     if (dtype == GPHQ_DTYPE_F16) return lora_run<f16>(p, st);

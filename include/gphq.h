@@ -646,7 +646,7 @@ int gphq_paged_pool_layer(const gphq_paged_pool *pool, int64_t layer, gphq_paged
  * no adapter and is left as it is. Rows may come in any order; neighbouring rows
  * of one adapter are fastest. fp32 products and sums in a fixed order.
  * k % 32 == 0, max_rank % 8 == 0 up to GPHQ_LORA_MAX_RANK, x_stride % 4 == 0,
- * k up to 2^30, rows x n below about 2^41;
+ * k up to 2^30, rows x n up to 2^33;
  * A, B, x and work 16-byte aligned; y_stride and y are best multiples of 16
  * bytes. y must not overlap x. work: gphq_lora_workspace_bytes, one per call
  * that may run at the same time. */

@@ -167,6 +167,7 @@ def lora(**over):
     (dict(work=None), gphq.ERR_DIMENSIONS), (dict(bytes=191), gphq.ERR_DIMENSIONS), (dict(y=P + 2), gphq.ERR_DIMENSIONS),
     (dict(y=P), gphq.ERR_OVERLAP),
     (dict(k=(1 << 31) - 32, x_stride=1 << 31, y=1 << 60, bytes=1 << 60), gphq.ERR_DIMENSIONS),
+    (dict(rows=256, n=1 << 27, y_stride=1 << 27, x=1 << 60, slots=16, bytes=1 << 60), gphq.ERR_DIMENSIONS),
     (dict(rows=1 << 20, n=1 << 30, y_stride=1 << 30, x=1 << 60, bytes=1 << 60), gphq.ERR_DIMENSIONS),
 ], ids=lambda v: str(v))
 def test_lora_refuses(over, want):
