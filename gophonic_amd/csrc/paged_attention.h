@@ -94,6 +94,18 @@ __device__ __forceinline__ void pages_start(const AttnArgs &a, PageWalk &w, int 
     pages_fill<CT>(a, w, seq, g, kt >> a.pool.shift);
 }
 
+// Whether a row at position pos that sees the keys from `first` on has one in a page of the pool.
+// Asked only where no score was above -inf: a row without such a key sees nothing and is 0, one
+// whose scores are all -inf or NaN is not finite.
+__device__ __forceinline__ bool sees_any(const AttnArgs &a, int seq, int first, int pos) {
+    if (pos < 0) return false;
+    for (int e = max(first, 0) >> a.pool.shift; e <= pos >> a.pool.shift; ++e) {
+        const int page = a.b.table[seq * a.b.table_stride + e];
+        if (page >= 0 && page < a.pool.pages) return true;
+    }
+    return false;
+}
+
 // Byte offsets of the 16-key groups kt, kt + 16, ... of a step; a bit per group that is not bad.
 template <typename CT, int N>
 __device__ __forceinline__ unsigned pages_step(const AttnArgs &a, PageWalk &w, int seq, int g, int kt,

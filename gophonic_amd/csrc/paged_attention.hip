@@ -198,7 +198,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
         }
     }
     if (!splits) return;
-    const bool empty = s.len - n + i < 0;
+    const int pos = s.len - n + i;
+    const bool empty = M == -INFINITY && !sees_any(a, s.seq, a.window > 0 ? pos - a.window + 1 : 0, pos);
     float r[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) r[e] = empty ? 0.0f : o[e] / L;

@@ -138,12 +138,13 @@ __device__ __forceinline__ void chunk_finish(const AttnArgs &a, const ChunkTile 
     if (!t.live) return;
     if (t.splits == 1) {
         const float inv = 1.0f / l;
+        const bool empty = m == -INFINITY && !sees_any(a, t.seq, t.first, t.pos);
         RT *out = (RT *)a.out + (int64_t)(t.start + t.row) * a.out_stride + t.head * HD;
 #pragma unroll
         for (int d = 0; d < HD; d += 8) {
             const f32x4 v = o(d / 8);
-            const float w[4] = {t.pos < 0 ? 0.0f : v[0] * inv, t.pos < 0 ? 0.0f : v[1] * inv,
-                                t.pos < 0 ? 0.0f : v[2] * inv, t.pos < 0 ? 0.0f : v[3] * inv};
+            const float w[4] = {empty ? 0.0f : v[0] * inv, empty ? 0.0f : v[1] * inv,
+                                empty ? 0.0f : v[2] * inv, empty ? 0.0f : v[3] * inv};
             store_vec(out + d + 4 * hi, w);
         }
         return;
@@ -489,6 +490,7 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
     l += __shfl_xor(l, 32);
     if (!t.live) return;
     const float inv = 1.0f / l;
+    const bool empty = t.splits == 1 && m == -INFINITY && !sees_any(a, t.seq, t.first, t.pos);
     float *out = (float *)a.out + (int64_t)(t.start + t.row) * a.out_stride + t.head * HD;
     const int64_t at = ((int64_t)(t.start + t.row) * a.heads + t.head) * a.parts + t.split;
 #pragma unroll
@@ -496,7 +498,7 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
         const int d0 = DT * (8 * (r >> 2) + 4 * hi + (r & 3));
         vdim v;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) v[d] = t.splits > 1 ? o[d][r] : t.pos < 0 ? 0.0f : o[d][r] * inv;
+        for (int d = 0; d < DT; ++d) v[d] = t.splits > 1 ? o[d][r] : empty ? 0.0f : o[d][r] * inv;
         *(vdim *)((t.splits > 1 ? a.part_o + at * HD : out) + d0) = v;
     }
     if (t.splits > 1 && hi == 0) {

@@ -160,12 +160,13 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t,
     }
     if (t.splits == 1) {
         const float inv = 1.0f / L;
+        const bool empty = M == -INFINITY && !sees_any(a, t.seq, a.window > 0 ? pos - a.window + 1 : 0, pos);
         RT *out = (RT *)a.out + (int64_t)(t.start + row) * a.out_stride + head * HD + d;
 #pragma unroll
         for (int i = 0; i < VD; i += 4) {
             float w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = pos < 0 ? 0.0f : v[i + k] * inv;
+            for (int k = 0; k < 4; ++k) w[k] = empty ? 0.0f : v[i + k] * inv;
             store_vec(out + i, w);
         }
         return;

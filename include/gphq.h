@@ -602,11 +602,12 @@ int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, in
  * among them (append them first):
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j][h / (heads / kv_heads)]) v[j][...]
  * over the tokens j of row i's sequence up to its position p, and with
- * window > 0 only those past p - window. A row before token 0 sees none and
- * becomes 0. What a row does not see, whatever it holds (NaN included), does
- * not reach it; a row that sees a value that is not finite becomes not finite.
- * scale may have either sign. Any number of rows per sequence: prompt chunks and single
- * tokens may stand in one call. fp32 rows are multiplied to fp32 accuracy
+ * window > 0 only those past p - window. A row that sees no key, being before
+ * token 0 or with none of its keys in a page of the pool, becomes 0. What a row
+ * does not see, whatever it holds (NaN included), does not reach it; a row that
+ * sees a value of V that is not finite, or whose scores are NaN or all -inf,
+ * becomes not finite. scale may have either sign. Any number of rows per
+ * sequence: prompt chunks and single tokens may stand in one call. fp32 rows are multiplied to fp32 accuracy
  * whatever the pool's type; 16-bit rows (the pool's type) round probabilities
  * to that type before the product with the values. out may not overlap q (nor
  * the pool). A batch of about 2^23 tiles (16 columns of a KV head in sequences

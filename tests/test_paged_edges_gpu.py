@@ -1,0 +1,96 @@
+"""Paged attention where a batch is unusual: rows whose pages are bad, values at the ends of a type's range, batches of
+mostly idle sequences, walks over many pages. Against the definition in float64, on sampled rows."""
+import math
+
+import pytest
+import torch
+
+from gophonic_amd import gphq
+from tests.paged_common import BF16, F16, F32, NAN, Batch, half_step
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)]
+TYPE_IDS = ["f32-f32", "f32-f16", "f32-bf16", "f16-f16", "bf16-bf16"]
+
+
+def run(b, q, heads, scale, window=0, bad=False, **over):
+    kv, dev = b.device(gphq, **over)
+    out = torch.full((b.rows, heads * b.hd), 7.0, dtype=q.dtype, device="cuda")
+    gphq.paged_attention(kv, dev, q.cuda(), out, heads, scale, window)
+    if bad:
+        with pytest.raises(gphq.GphqError) as e:
+            dev.check()
+        assert e.value.status == gphq.ERR_PAGED_BATCH
+    dev.check()
+    return out.cpu()
+
+
+def row64(b, q, heads, scale, r, window=0):
+    """The definition of one row in float64 and a bound of fp32 arithmetic's error, as paged_common.attention64 derives
+    it, over the keys that lie in pages of the pool."""
+    s = max(i for i in range(len(b.new)) if b.starts[i] <= r)
+    p = b.lens[s] - b.new[s] + r - b.starts[s]
+    keys = torch.arange(max(0, p - window + 1) if window else 0, p + 1)
+    page = torch.from_numpy(b.table[s]).long()[keys // b.page]
+    good = (page >= 0) & (page < b.pages)
+    keys, page = keys[good], page[good]
+    m, group, u, half = len(keys), heads // b.kv_heads, 2.0 ** -24, half_step(q.dtype)
+    if m == 0:
+        zero = torch.zeros(heads * b.hd, dtype=torch.float64)
+        return zero, zero
+    k = b.k[page, keys % b.page].double().transpose(0, 1)  # [KV heads][keys][hd]
+    v = b.v[page, keys % b.page].double().transpose(0, 1)
+    x = q[r].double().view(b.kv_heads, group, b.hd)
+    w = torch.softmax(x @ k.transpose(1, 2) * scale, -1)
+    out, a = w @ v, w @ v.abs()
+    e = abs(scale) * ((b.hd + 4) * u * (x.abs() @ k.abs().transpose(1, 2)).amax(-1)
+                      + 2.0 ** -22 * x.abs().amax(-1) * k.abs().sum(-1).amax(-1)[:, None])
+    tol = (torch.expm1(2 * e)[..., None] + (2 * m + 64) * u) * a + m * 2.0 ** -32 * v.abs().amax((1, 2))[:, None, None]
+    if half > u:
+        tol = tol + half * a
+    return out.reshape(-1), (tol + half * out.abs() + 2.0 ** -25).reshape(-1)
+
+
+def check_rows(b, q, heads, scale, got, rows, window=0):
+    for r in rows:
+        want, tol = row64(b, q, heads, scale, r, window)
+        err = (got[r].double() - want).abs()
+        assert (err <= tol).all(), f"row {r}: {float((err / tol.clamp(min=1e-30)).max())} of the bound"
+
+
+# ---- rows that see no key because their pages are bad ------------------------------
+
+
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("seqs,bad,window", [
+    ([(1, 9)], [(0, 0)], 0),                                    # the only page
+    ([(1, 9), (1, 2000)], [(0, 0)], 0),                         # beside one that is split
+    ([(1, 2000)], [(0, e) for e in range(125)], 0),             # every split's pages
+    ([(1, 2000), (3, 700)], [(0, 124), (1, 43), (1, 42)], 16),  # a window inside bad pages, or partly
+    ([(70, 70)], [(0, 0)], 0),                                  # a chunk whose first rows have no other page
+    ([(70, 70), (80, 3000)], [(0, 0), (0, 1)], 0),              # the same, beside one that is split
+    ([(90, 600)], [(0, e) for e in range(32, 38)], 20),         # a chunk's windows
+    ([(80, 3000)], [(0, e) for e in range(188)], 0),            # a split chunk without a page
+], ids=range(8))
+def test_rows_without_a_good_page_are_zero(seqs, bad, window, rt, ct):
+    heads = 4
+    b = Batch(seqs, 2, 64, 16, ct, seed=40)
+    for i, (s, e) in enumerate(bad):
+        b.table[s, e] = (b.pages, -1, 2 ** 31 - 1)[i % 3]
+    q = b.randn(b.rows, heads * 64).to(rt)
+    got = run(b, q, heads, 0.1, window, bad=True)
+    check_rows(b, q, heads, 0.1, got, range(b.rows), window)
+    empty = [r for r in range(b.rows) if not row64(b, q, heads, 0.1, r, window)[0].any()]
+    assert empty and (got[empty] == 0).all()
+
+
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("seqs", [[(1, 9)], [(1, 2000)], [(70, 70)], [(80, 3000)]], ids=str)
+def test_rows_whose_scores_are_all_minus_infinity_are_not_finite(seqs, rt, ct):
+    """They do see keys, so they are not the rows above: the quotient is 0 / 0."""
+    b = Batch(seqs, 2, 64, 16, ct, seed=41)
+    b.k.fill_(-math.inf)
+    q = (b.randn(b.rows, 4 * 64).abs() + 0.1).to(rt)
+    got = run(b, q, 4, 0.1)
+    assert not got.isfinite().any()
