@@ -25,7 +25,8 @@ struct AttnArgs {
     const void *q;
     void *out;
     // Split results, output and (reference, sum): the chunk kernel's by [row][head][parts], the
-    // row kernel's, whose splits may be many, by [sequence][small_rows][head][small_parts].
+    // row kernel's, whose splits may be many, by [sequence][small_rows][head][small_parts], or by
+    // [row][head][small_parts] (small_rows 0) where the batch has fewer rows than that has places.
     float *part_o, *part_ml, *small_o, *small_ml;
     int64_t q_stride, out_stride;
     int heads, group, window;
@@ -57,6 +58,11 @@ __device__ __forceinline__ TileKeys tile_keys(int n, int len, int r0, int r1, in
 }
 __device__ __forceinline__ int tile_splits(const TileKeys &t, int split_len) {
     return t.hi > t.lo ? (t.hi - t.from + split_len - 1) / split_len : 1;
+}
+
+// The place of row i of a sequence that starts at row `start` among the row kernel's split results.
+__device__ __forceinline__ int64_t small_place(const AttnArgs &a, int seq, int start, int i) {
+    return a.small_rows ? (int64_t)seq * a.small_rows + i : start + i;
 }
 
 // The pages of a tile's keys [lo, hi): lane i of a wavefront holds where entry first + i of

@@ -46,11 +46,13 @@ int paged_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, PagedPool &po
 
 namespace {
 
+constexpr int64_t kMaxBlocks = (1 << 23) - 1;  // of a launch: 2^32 threads at 512 a block are one too many
+
 // How a call is cut: which kernels run, over how many tiles and splits.
 struct AttnPlan {
     int small_cols, small_tiles, small_splits, small_len;  // small_tiles per sequence; 0: the row kernel is not run
     int big_tiles, big_splits, big_len;                    // big_tiles in all; 0: the chunk kernel is not run
-    int small_rows;  // rows that a sequence of the row kernel may have
+    int small_rows;  // rows that a sequence of the row kernel may have; 0: split results kept by row
 };
 
 // Keys per split of `span` keys and how many splits that makes, for about `want` of them.
@@ -92,7 +94,10 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         // twelve sequences over up to 4000 bfloat16 tokens: 15 us, 20 before).
         const bool mixed = cols > p.small_cols;
         const int64_t want = mixed ? 2 * cus / (units / p.small_tiles) : cus / units;
-        cut(span(kSmallTile), brief ? 1 : want, p.small_len, p.small_splits);
+        // The grid has a place for every sequence, with rows or without: no more splits than a launch takes.
+        const int64_t most = kMaxBlocks / (b.seqs * (int64_t)p.small_tiles * kv_heads);
+        cut(span(kSmallTile), brief ? 1 : std::min(want, most), p.small_len, p.small_splits);
+        if ((int64_t)b.seqs * p.small_rows > rows) p.small_rows = 0;  // at most `rows` sequences have any
     }
     if (cols > p.small_cols) {
         const int64_t all = rows * group;
@@ -115,7 +120,8 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
 
 // Split results that the workspace holds for each kernel.
 int64_t small_count(const AttnPlan &p, const PagedBatch &b, int64_t heads) {
-    return p.small_tiles && p.small_splits > 1 ? (int64_t)b.seqs * p.small_rows * heads * p.small_splits : 0;
+    const int64_t places = p.small_rows ? (int64_t)b.seqs * p.small_rows : b.rows;
+    return p.small_tiles && p.small_splits > 1 ? places * heads * p.small_splits : 0;
 }
 int64_t big_count(const AttnPlan &p, const PagedBatch &b, int64_t heads) {
     return p.big_tiles && p.big_splits > 1 ? b.rows * heads * p.big_splits : 0;
@@ -145,7 +151,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
     const int all = head < a.heads ? tile_splits(k, small ? a.split_small : a.split_big) : 1;
     const int splits = all > 1 ? all : 0;  // (heads of a row may lie in different tiles)
     const int hc = min(head, a.heads - 1);
-    const int64_t at = small ? (((int64_t)s.seq * a.small_rows + i) * a.heads + hc) * a.small_parts
+    const int64_t at = small ? (small_place(a, s.seq, s.start, i) * a.heads + hc) * a.small_parts
                              : ((int64_t)row * a.heads + hc) * a.parts;
     const float *part_o = small ? a.small_o : a.part_o, *part_ml = small ? a.small_ml : a.part_ml;
     const int d = 4 * (lane % LH);
@@ -205,8 +211,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
     for (int e = 0; e < 4; ++e) r[e] = empty ? 0.0f : o[e] / L;
     store_vec((RT *)a.out + (int64_t)row * a.out_stride + head * HD + d, r);
 }
-
-constexpr int64_t kMaxBlocks = (1 << 23) - 1;  // of a launch: 2^32 threads at 512 a block are one too many
 
 int64_t join_units(const PagedBatch &b, int64_t heads, int hd) { return b.rows * ((heads * hd + 255) / 256); }
 

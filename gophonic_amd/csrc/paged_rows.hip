@@ -171,7 +171,7 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t,
         }
         return;
     }
-    const int64_t at = (((int64_t)t.seq * a.small_rows + row) * a.heads + head) * a.small_parts + t.split;
+    const int64_t at = (small_place(a, t.seq, t.start, row) * a.heads + head) * a.small_parts + t.split;
 #pragma unroll
     for (int i = 0; i < VD; i += 4) *(f32x4 *)(a.small_o + at * HD + d + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
     if (d == 0) {

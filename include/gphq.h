@@ -607,15 +607,19 @@ int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, in
  * does not see, whatever it holds (NaN included), does not reach it; a row that
  * sees a value of V that is not finite, or whose scores are NaN or all -inf,
  * becomes not finite. scale may have either sign. Any number of rows per
- * sequence: prompt chunks and single tokens may stand in one call. fp32 rows are multiplied to fp32 accuracy
- * whatever the pool's type; 16-bit rows (the pool's type) round probabilities
- * to that type before the product with the values. out may not overlap q (nor
- * the pool). A batch of about 2^23 tiles (16 columns of a KV head in sequences
- * of up to 64 columns, 128 in others) or more is GPHQ_ERR_PAGED_SHAPE. work
- * (16-byte aligned) of at least gphq_paged_attention_workspace_bytes for the
- * same pool, batch, row type, heads and window; its contents need not be kept
- * between calls, and calls that may run at the same time need one each. Sums
- * are taken in a fixed order: the same call gives the same bits. */
+ * sequence: prompt chunks and single tokens may stand in one call. fp32 rows
+ * are multiplied to fp32 accuracy whatever the pool's type; 16-bit rows (the
+ * pool's type) round probabilities to that type before the product with the
+ * values. out may not overlap q (nor the pool).
+ * A batch of more blocks than a launch takes is GPHQ_ERR_PAGED_SHAPE: with
+ * g = heads / kv_heads, where kv_heads seqs ceil(min(max_rows g, 64) / 16)
+ * (g <= 64), or kv_heads times about rows g / 128 (256 for fp32 rows; where
+ * max_rows g > 64), passes 2^23 - 1, or rows ceil(heads head_dim / 256) passes
+ * 2^26 - 1 in a batch whose keys are split.
+ * work (16-byte aligned) of at least gphq_paged_attention_workspace_bytes for
+ * the same pool, batch, row type, heads and window; its contents need not be
+ * kept between calls, and calls that may run at the same time need one each.
+ * Sums are taken in a fixed order: the same call gives the same bits. */
 int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype,
                                              int64_t heads, int64_t window);
 int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q_dev,

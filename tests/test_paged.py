@@ -123,6 +123,19 @@ def test_the_workspace_stays_small(seqs, rows, max_rows, max_len):
         assert 0 <= n < 256 << 20
 
 
+@pytest.mark.parametrize("seqs,rows", [(2048, 1), (16384, 1), (65536, 1), (65536, 40), (4096, 4096), (65536, 1 << 16)])
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (8, 1), (64, 64)])
+@pytest.mark.parametrize("max_rows", [1, 16])
+def test_idle_sequences_cost_no_workspace(seqs, rows, heads, kv_heads, max_rows):
+    """A batch made for many sequences of which few bring rows: at most `rows` of them hold split results, and it is
+    not refused while its tiles, kv_heads seqs ceil(min(max_rows g, 64) / 16), are under 2^23."""
+    k = kv(kv_heads=kv_heads, pages=1 << 20, head_stride=2048, page_stride=2048 * kv_heads)
+    b = batch(seqs=seqs, rows=rows, max_rows=max_rows, max_len=40960, table_stride=2560)
+    for dtype in (gphq.DTYPE_F16, gphq.DTYPE_F32):
+        n = gphq.load().gphq_paged_attention_workspace_bytes(ctypes.byref(k), ctypes.byref(b), dtype, heads, 0)
+        assert 0 <= n < 256 << 20
+
+
 @pytest.mark.parametrize("over,heads,kv_heads,fits", [
     (dict(seqs=65536, rows=65536, max_rows=1), 127, 127, True), (dict(seqs=65536, rows=65536, max_rows=1), 128, 128, False),
     (dict(seqs=65536, rows=1 << 20, max_rows=16), 128, 32, False),

@@ -94,3 +94,47 @@ def test_rows_whose_scores_are_all_minus_infinity_are_not_finite(seqs, rt, ct):
     q = (b.randn(b.rows, 4 * 64).abs() + 0.1).to(rt)
     got = run(b, q, 4, 0.1)
     assert not got.isfinite().any()
+
+
+# ---- batches of mostly idle sequences ----------------------------------------------
+
+
+def idle(seqs, live):
+    """`seqs` sequences of which those in `live`, {number: (new, tokens)}, bring rows; the others hold tokens or none."""
+    return [live.get(s, (0, 5 * (s % 3))) for s in range(seqs)]
+
+
+@pytest.mark.parametrize("rt,ct", [(F32, F32), (F32, F16), (BF16, BF16)], ids=["f32-f32", "f32-f16", "bf16-bf16"])
+@pytest.mark.parametrize("seqs,live,spare", [
+    (300, {17: (1, 3000)}, 0), (300, {0: (1, 2500), 64: (3, 2900), 299: (2, 700)}, 0),
+    (300, {0: (1, 2500), 64: (3, 2900), 299: (2, 700)}, 5), (150, {3: (1, 2600), 70: (40, 2100), 128: (5, 2200)}, 0),
+], ids=range(4))
+def test_few_rows_in_a_batch_of_many_sequences(seqs, live, spare, rt, ct):
+    b = Batch(idle(seqs, live), 2, 64, 16, ct, seed=50, spare_rows=spare)
+    q = (b.randn(b.rows, 8 * 64) * 1.5).to(rt)
+    got = run(b, q, 8, 0.125)
+    check_rows(b, q, 8, 0.125, got, range(b.starts[-1]))
+    assert (got[b.starts[-1]:] == 7).all()
+
+
+def test_a_batch_of_all_the_sequences_that_fit():
+    """65536 sequences over one KV head, three of them with a row: the most that a batch may hold."""
+    n, page, heads = 65536, 16, 4
+    lens = {5: 40, 40000: 3000, 65535: 700}
+    need = 188
+    b = Batch([(1, t) for t in lens.values()], 1, 64, page, F16, seed=51)
+    starts = torch.zeros(n + 1, dtype=torch.int32)
+    for s in lens:
+        starts[s + 1:] += 1
+    table = torch.full((n, need), -1, dtype=torch.int32)
+    length = torch.zeros(n, dtype=torch.int32)
+    for i, (s, t) in enumerate(lens.items()):
+        length[s] = t
+        table[s, :b.entries] = torch.from_numpy(b.table[i])[:need]
+    kv, _ = b.device(gphq)
+    dev = gphq.PagedBatch(starts.cuda(), length.cuda(), table.cuda(), 3, 1, 3000)
+    q = b.randn(3, heads * 64)
+    out = torch.full((3, heads * 64), 7.0, device="cuda")
+    gphq.paged_attention(kv, dev, q.cuda(), out, heads, 0.125)
+    dev.check()
+    check_rows(b, q, heads, 0.125, out.cpu(), range(3))
