@@ -212,6 +212,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
     store_vec((RT *)a.out + (int64_t)row * a.out_stride + head * HD + d, r);
 }
 
+// Takes the bits that were reported out of a batch's word; one that another stream has set since stays.
+__global__ void paged_clear_kernel(int32_t *bad, int32_t reported) { atomicAnd(bad, ~reported); }
+
 int64_t join_units(const PagedBatch &b, int64_t heads, int hd) { return b.rows * ((heads * hd + 255) / 256); }
 
 template <typename RT, int HD>
@@ -376,11 +379,14 @@ int gphq_paged_pool_layer(const gphq_paged_pool *p, int64_t layer, gphq_paged_kv
 
 int gphq_paged_check(int32_t *bad_dev, void *stream) {
     if (!bad_dev) return GPHQ_ERR_PAGED_SHAPE;
-    GPHQ_TRY(hip_status(hipStreamSynchronize((hipStream_t)stream)));
+    // All on the caller's stream: a call that follows on it finds the word cleared, not about to be.
+    hipStream_t st = (hipStream_t)stream;
     int32_t bad = 0;
-    GPHQ_TRY(hip_status(hipMemcpy(&bad, bad_dev, 4, hipMemcpyDeviceToHost)));
+    GPHQ_TRY(hip_status(hipMemcpyAsync(&bad, bad_dev, 4, hipMemcpyDeviceToHost, st)));
+    GPHQ_TRY(hip_status(hipStreamSynchronize(st)));
     if (!bad) return GPHQ_OK;
-    GPHQ_TRY(hip_status(hipMemset(bad_dev, 0, 4)));
+    hipLaunchKernelGGL(paged_clear_kernel, dim3(1), dim3(1), 0, st, bad_dev, bad);
+    GPHQ_TRY(launch_status());
     return GPHQ_ERR_PAGED_BATCH;
 }
 

@@ -1107,7 +1107,9 @@ class PagedBatch:
     lens int32 [seqs] and table int32 [seqs][entries] are device tensors, read
     when the work runs (their values may change between calls); rows is what
     the row buffers hold, max_rows and max_len bound one sequence's rows and
-    lens. check() waits and raises for values out of bounds that a call met."""
+    lens. check() waits and raises for values out of bounds that a call met.
+    Like its tensors it is made on the current stream: a call on another stream
+    has to come after that one's work."""
 
     def __init__(self, starts, lens, table, rows, max_rows, max_len):
         import torch

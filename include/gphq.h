@@ -625,8 +625,8 @@ int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq
 int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q_dev,
                          int64_t q_stride, int64_t heads, double scale, int64_t window, void *out_dev,
                          int64_t out_stride, void *work_dev, int64_t work_bytes, void *stream);
-/* Waits for the stream; GPHQ_ERR_PAGED_BATCH if *bad_dev was set, which is then
- * cleared. */
+/* Waits for the stream, and for no other; GPHQ_ERR_PAGED_BATCH if *bad_dev was
+ * set, which is then cleared, on the stream. */
 int gphq_paged_check(int32_t *bad_dev, void *stream);
 
 /* A pool of one model's layers: `pages` pages of page_tokens tokens of every

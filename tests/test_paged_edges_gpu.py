@@ -138,3 +138,28 @@ def test_a_batch_of_all_the_sequences_that_fit():
     gphq.paged_attention(kv, dev, q.cuda(), out, heads, 0.125)
     dev.check()
     check_rows(b, q, heads, 0.125, out.cpu(), range(3))
+
+
+# ---- what a call found out of bounds ------------------------------------------------
+
+
+def test_check_keeps_to_its_stream():
+    """The check reads and clears the batch's word on the stream that it is given: it does not wait for the default
+    stream's work, and what the next call on its own stream finds is not lost."""
+    b = Batch([(1, 40)], 1, 64, 16, F16, seed=60)
+    b.table[0, 1] = -5
+    kv, dev = b.device(gphq)
+    q, out = b.randn(1, 128).half().cuda(), torch.empty(1, 128, dtype=F16, device="cuda")
+    x, side, done = torch.randn(8192, 8192, device="cuda"), torch.cuda.Stream(), torch.cuda.Event()
+    y = x @ x
+    torch.cuda.synchronize()
+    for _ in range(60):  # some hundreds of milliseconds
+        torch.matmul(x, x, out=y)
+    done.record()
+    for _ in range(3):
+        gphq.paged_attention(kv, dev, q, out, 2, 0.1, stream=side)
+        with pytest.raises(gphq.GphqError):
+            dev.check(side)
+    dev.check(side)
+    assert not done.query()
+    torch.cuda.synchronize()
