@@ -40,8 +40,12 @@ struct AttnArgs {
 
 constexpr int kSmallTile = 16;
 constexpr float kLag = 8.0f;    // the reference maximum may be passed by this much (in log2)
-constexpr float kLift = 7.0f;   // exponentials are 2^(x - m + 7): at most 2^15, so that FP16
-                                // probabilities keep 2^-24 of a 2^7 .. 2^15 maximum, not of 1
+// Exponentials are 2^(x - m + lift). FP16 probabilities reach 2^15, so that they keep 2^-24 of a
+// 2^7 .. 2^15 maximum, not of 1 (and FP16 values, up to 2^16, stay far inside fp32). Elsewhere none
+// passes 1: a sum over finite values leaves fp32's range only where that of their magnitudes,
+// each times a probability of at most 1, does.
+template <typename CT>
+constexpr float kLift = std::is_same<CT, f16>::value ? 7.0f : -kLag;
 
 // The keys [lo, hi) that rows r0 .. r1 of a sequence of n rows and len keys see, and the
 // key, a multiple of 64, that its splits count from.

@@ -92,7 +92,7 @@ __device__ __forceinline__ bool chunk_edge(const AttnArgs &a, const ChunkTile &t
 
 // One step's exponentials over N 32-key score tiles: s[h][r] is key kt + 32 h + 8 (r / 4) +
 // 4 hi + r % 4; as the row kernel's softmax_step. ok: a bit per 16 keys.
-template <int N>
+template <typename CT, int N>
 __device__ __forceinline__ float chunk_softmax(const ChunkTile &t, f32x16 (&s)[N], float fac, bool masked, int kt,
                                                unsigned ok, float &m, float &l, bool &moved) {
     const int hi = (threadIdx.x & 63) >> 5;
@@ -113,8 +113,8 @@ __device__ __forceinline__ float chunk_softmax(const ChunkTile &t, f32x16 (&s)[N
     mx = fmaxf(mx, __shfl_xor(mx, 32)) * fac;
     const bool grew = mx > m + kLag;
     const float mn = grew ? mx : m;
-    const float ref = mn == -INFINITY ? 0.0f : mn - kLift;
-    const float corr = __builtin_amdgcn_exp2f((m == -INFINITY ? m : m - kLift) - ref);
+    const float ref = mn == -INFINITY ? 0.0f : mn - kLift<CT>;
+    const float corr = __builtin_amdgcn_exp2f((m == -INFINITY ? m : m - kLift<CT>) - ref);
     m = mn;
     float sum = 0.0f;
 #pragma unroll
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_chunk16_kernel(const AttnArgs
         const bool masked =
             kt + KB - 1 > t.p0 || kt < t.w_lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 15;
         bool moved;
-        const float corr = chunk_softmax(t, s, fac, masked, kt, okc, m, l, moved);
+        const float corr = chunk_softmax<CT>(t, s, fac, masked, kt, okc, m, l, moved);
         if (moved) {
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] *= corr;
@@ -458,7 +458,7 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
         const bool masked =
             kt + KB - 1 > t.p0 || kt < t.w_lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 3;
         bool moved;
-        const float corr = chunk_softmax(t, s, score_factor(a.scale_log2), masked, kt, okc, m, l, moved);
+        const float corr = chunk_softmax<float>(t, s, score_factor(a.scale_log2), masked, kt, okc, m, l, moved);
         if (moved) {
 #pragma unroll
             for (int i = 0; i < DT; ++i) o[i] *= corr;

@@ -56,8 +56,9 @@ __device__ __forceinline__ bool row_tile(const AttnArgs &a, int tiles, int split
 
 // One 32-key step's exponentials: s[0], s[1] are the scores (fac times them in log2) of keys
 // kt + 4 g4 + r and kt + 16 + 4 g4 + r; those that the lane's column does not see are left
-// out. p[8] are 2^(x - m + 7), m and l the running reference and this lane's running sum;
+// out. p[8] are 2^(x - m + lift), m and l the running reference and this lane's running sum;
 // returns what o is to be multiplied by, and whether any lane's reference moved.
+template <typename CT>
 __device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)[2], float fac, bool masked, int kt,
                                               unsigned ok, float (&p)[8], float &m, float &l, bool &moved) {
     const int g4 = (threadIdx.x & 63) >> 4;
@@ -78,8 +79,8 @@ __device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)
     mx = fmaxf(mx, __shfl_xor(mx, 32)) * fac;
     const bool grew = mx > m + kLag;
     const float mn = grew ? mx : m;
-    const float ref = mn == -INFINITY ? 0.0f : mn - kLift;
-    const float corr = __builtin_amdgcn_exp2f((m == -INFINITY ? m : m - kLift) - ref);
+    const float ref = mn == -INFINITY ? 0.0f : mn - kLift<CT>;
+    const float corr = __builtin_amdgcn_exp2f((m == -INFINITY ? m : m - kLift<CT>) - ref);
     m = mn;
     float sum = 0.0f;
 #pragma unroll
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows16_kernel(const AttnArgs a, i
         const bool masked = kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 3;
         float p[8];
         bool moved;
-        const float corr = softmax_step(t, s, fac, masked, kt, okc, p, m, l, moved);
+        const float corr = softmax_step<CT>(t, s, fac, masked, kt, okc, p, m, l, moved);
         unsigned odd = 0;  // of this lane's eight keys, those with a value that is not finite
         if (masked) {
 #pragma unroll
@@ -396,7 +397,7 @@ __global__ __launch_bounds__(256) void attn_rows32_kernel(const AttnArgs a, int 
         const bool masked = kt + 31 > t.p0 || kt < t.lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 3;
         float p[8];
         bool moved;
-        const float corr = softmax_step(t, s, score_factor(a.scale_log2), masked, kt, okc, p, m, l, moved);
+        const float corr = softmax_step<float>(t, s, score_factor(a.scale_log2), masked, kt, okc, p, m, l, moved);
         unsigned odd = 0;  // of this lane's eight keys, those with a value that is not finite
         if (masked) {
 #pragma unroll

@@ -606,9 +606,11 @@ int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, in
  * token 0 or with none of its keys in a page of the pool, becomes 0. What a row
  * does not see, whatever it holds (NaN included), does not reach it; a row that
  * sees a value of V that is not finite, or whose scores are NaN or all -inf,
- * becomes not finite. scale may have either sign. Any number of rows per
- * sequence: prompt chunks and single tokens may stand in one call. fp32 rows
- * are multiplied to fp32 accuracy whatever the pool's type; 16-bit rows (the
+ * becomes not finite. Sums are fp32, over probabilities of at most 1 before the
+ * division: finite values whose sum of magnitudes stays in range give finite
+ * rows. scale may have either sign. Any number of rows per sequence: prompt
+ * chunks and single tokens may stand in one call. fp32 rows are multiplied to
+ * fp32 accuracy whatever the pool's type; 16-bit rows (the
  * pool's type) round probabilities to that type before the product with the
  * values. out may not overlap q (nor the pool).
  * A batch of more blocks than a launch takes is GPHQ_ERR_PAGED_SHAPE: with

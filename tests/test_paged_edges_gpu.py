@@ -163,3 +163,27 @@ def test_check_keeps_to_its_stream():
     dev.check(side)
     assert not done.query()
     torch.cuda.synchronize()
+
+
+# ---- values at the end of their type's range -----------------------------------------
+
+
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("ahead", [0.0, 7.5], ids=["level", "ahead"])
+@pytest.mark.parametrize("seqs", [[(1, 1)], [(1, 300), (3, 40)], [(1, 3000)], [(70, 200)], [(80, 3000)]], ids=str)
+def test_values_at_the_end_of_the_range(seqs, ahead, rt, ct):
+    """One finite value of nearly the type's largest magnitude among small ones: a weighted mean of them is finite, also
+    where its key's score is `ahead` (in log2) of all before it."""
+    b = Batch(seqs, 2, 64, 16, ct, seed=70)
+    big = 0.99 * torch.finfo(ct).max
+    for s, (n, t) in enumerate(seqs):
+        for p in range(t):
+            b.k[b.token(s, p)] = 0.0
+        at = b.token(s, t - n)  # the first new token, which every row sees
+        b.k[at] = ahead * math.log(2) / 64
+        b.v[at] = big
+        b.v[at][:, ::2] = -big
+    q = torch.ones(b.rows, 4 * 64, dtype=rt)
+    got = run(b, q, 4, 1.0)
+    assert got.isfinite().all()
+    check_rows(b, q, 4, 1.0, got, range(b.rows))
