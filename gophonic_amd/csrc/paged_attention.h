@@ -190,7 +190,7 @@ struct Half<bf16> {
 // instructions: one where they are the same type; an fp32 value as two FP16 pieces
 // (22 bits, the value scaled into FP16's range) or three bfloat16 ones (24 bits). Products
 // of pieces with the cache's values are exact in fp32, so an fp32 row loses at most 2^-22
-// of its largest value.
+// of its largest value. Probabilities of fp32 rows are split alike.
 template <typename RT, typename CT>
 constexpr int kPieces = sizeof(RT) == 2 ? 1 : (std::is_same<CT, f16>::value ? 2 : 3);
 

@@ -193,7 +193,9 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t,
 // brings 16 KB, at any rate of the memory less than half of a SIMD's time. K of the next step
 // is loaded as soon as this one's scores are made, V as soon as it is multiplied, so a block's
 // four wavefronts keep 64 KB on their way; 16 columns, not more, because one row of a group of
-// up to 16 heads needs no more and every column costs registers. Two rows over 36286 and 39946
+// up to 16 heads needs no more and every column costs registers. Probabilities of 16-bit rows
+// take two pieces, 2^-16 (bfloat16) or 2^-22 of one lost: the matrix cores have the time (59.7 us
+// either way in the case that follows). Two rows over 36286 and 39946
 // tokens, eight KV heads, bfloat16: 59.5 us with the join (312 MB, 5.25 TB/s; a kernel that
 // only reads makes 6.2).
 template <typename RT, typename CT, int HD>
@@ -201,6 +203,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows16_kernel(const AttnArgs a, i
     typedef Half<CT> H;
     typedef typename H::vec8 vec8;
     constexpr int NP = kPieces<RT, CT>, KC = HD / 32, VD = HD / 16, VW = VD / 2;  // VW: dwords of V per key
+    constexpr int PP = NP == 1 ? 2 : NP;  // pieces of a probability
     RowTile t;
     if (!row_tile(a, tiles, splits, t)) return;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
@@ -301,13 +304,13 @@ __global__ __launch_bounds__(256, 2) void attn_rows16_kernel(const AttnArgs a, i
                 odd |= any ? 1u << i : 0u;
             }
         }
-        vec8 pf[NP];
+        vec8 pf[PP];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            CT pc[NP];
+            CT pc[PP];
             split_pieces(p[i], pc);
 #pragma unroll
-            for (int k = 0; k < NP; ++k) pf[k][i] = pc[k];
+            for (int k = 0; k < PP; ++k) pf[k][i] = pc[k];
         }
         if (moved) {
 #pragma unroll
@@ -320,7 +323,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows16_kernel(const AttnArgs a, i
             for (int j = 0; j < 4; ++j)
                 f[j] = __builtin_amdgcn_perm(v[2 * j + 1][d / 2], v[2 * j][d / 2], d % 2 ? 0x07060302 : 0x05040100);
 #pragma unroll
-            for (int k = 0; k < NP; ++k) o[d] = H::mfma16(__builtin_bit_cast(vec8, f), pf[k], o[d]);
+            for (int k = 0; k < PP; ++k) o[d] = H::mfma16(__builtin_bit_cast(vec8, f), pf[k], o[d]);
         }
         if (more) load_v();
         if (__any(odd)) add_not_finite<CT, HD>(t, vp, now, ts, kt, odd, o);

@@ -610,9 +610,11 @@ int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, in
  * division: finite values whose sum of magnitudes stays in range give finite
  * rows. scale may have either sign. Any number of rows per sequence: prompt
  * chunks and single tokens may stand in one call. fp32 rows are multiplied to
- * fp32 accuracy whatever the pool's type; 16-bit rows (the
- * pool's type) round probabilities to that type before the product with the
- * values. out may not overlap q (nor the pool).
+ * fp32 accuracy whatever the pool's type. So are 16-bit rows (of the pool's
+ * type) in sequences whose rows times heads / kv_heads are at most 64, single
+ * tokens among them; longer ones round each probability to that type before the
+ * product with the values, an error of at most half a step of sum p |v|. out
+ * may not overlap q (nor the pool).
  * A batch of more blocks than a launch takes is GPHQ_ERR_PAGED_SHAPE: with
  * g = heads / kv_heads, where kv_heads seqs ceil(min(max_rows g, 64) / 16)
  * (g <= 64), or kv_heads times about rows g / 128 (256 for fp32 rows; where

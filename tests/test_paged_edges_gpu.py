@@ -26,9 +26,10 @@ def run(b, q, heads, scale, window=0, bad=False, **over):
     return out.cpu()
 
 
-def row64(b, q, heads, scale, r, window=0):
+def row64(b, q, heads, scale, r, window=0, pieces=1):
     """The definition of one row in float64 and a bound of fp32 arithmetic's error, as paged_common.attention64 derives
-    it, over the keys that lie in pages of the pool."""
+    it, over the keys that lie in pages of the pool. Probabilities of 16-bit rows in `pieces` pieces of the type, each
+    off by at most half a step of what is left of them."""
     s = max(i for i in range(len(b.new)) if b.starts[i] <= r)
     p = b.lens[s] - b.new[s] + r - b.starts[s]
     keys = torch.arange(max(0, p - window + 1) if window else 0, p + 1)
@@ -48,13 +49,13 @@ def row64(b, q, heads, scale, r, window=0):
                       + 2.0 ** -22 * x.abs().amax(-1) * k.abs().sum(-1).amax(-1)[:, None])
     tol = (torch.expm1(2 * e)[..., None] + (2 * m + 64) * u) * a + m * 2.0 ** -32 * v.abs().amax((1, 2))[:, None, None]
     if half > u:
-        tol = tol + half * a
+        tol = tol + half ** pieces * a
     return out.reshape(-1), (tol + half * out.abs() + 2.0 ** -25).reshape(-1)
 
 
-def check_rows(b, q, heads, scale, got, rows, window=0):
+def check_rows(b, q, heads, scale, got, rows, window=0, pieces=1):
     for r in rows:
-        want, tol = row64(b, q, heads, scale, r, window)
+        want, tol = row64(b, q, heads, scale, r, window, pieces)
         err = (got[r].double() - want).abs()
         assert (err <= tol).all(), f"row {r}: {float((err / tol.clamp(min=1e-30)).max())} of the bound"
 
@@ -187,3 +188,16 @@ def test_values_at_the_end_of_the_range(seqs, ahead, rt, ct):
     got = run(b, q, 4, 1.0)
     assert got.isfinite().all()
     check_rows(b, q, 4, 1.0, got, range(b.rows))
+
+
+# ---- 16-bit rows of single tokens -----------------------------------------------------
+
+
+@pytest.mark.parametrize("ct", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_single_16_bit_rows_are_rounded_once(ct, hd):
+    """Sequences of up to 64 columns: only the result is rounded to 16 bits, not the probabilities."""
+    b = Batch([(1, 40), (1, 100), (1, 700), (1, 3000), (5, 300), (16, 90)], 2, hd, 16, ct, seed=80)
+    q = (b.randn(b.rows, 8 * hd) * 1.5).to(ct)
+    got = run(b, q, 8, hd ** -0.5)
+    check_rows(b, q, 8, hd ** -0.5, got, range(b.rows), pieces=2)
