@@ -17,6 +17,7 @@ void set_hip_error(hipError_t e);
 // Converts a HIP status into a gphq status, remembering the HIP code.
 inline int hip_status(hipError_t e) {
     if (e == hipSuccess) return GPHQ_OK;
+    (void)hipGetLastError();  // reported here: the next launch, the library's or the caller's, must not report it again
     set_hip_error(e);
     return GPHQ_ERR_HIP;
 }

@@ -250,3 +250,18 @@ def test_one_layer_by_hand_with_adapters(lm):
     # The O projection of both: its activations are rounded to FP16 per row (2^-11 of the row's largest).
     assert cos(out, ref) >= 0.99999
     assert math.isfinite(float(out.sum()))
+
+
+def test_memory_that_is_not_there_leaves_no_error(lm):
+    """A pool too large for the device is refused; neither the next call nor torch's next kernel reports it again."""
+    for _ in range(2):
+        with pytest.raises(gphq.GphqError):
+            gphq.PagedPool(lm, 2 ** 31 - 1, 4096, F32)
+        x = torch.zeros(64, device="cuda") + 1
+        pool, pf = gphq.PagedPool(lm, 4, 16, F16), gphq.Prefill(lm, 16)
+        h = torch.empty(1, GEOM["hidden"], device="cuda")
+        with pytest.raises(gphq.GphqError):
+            gphq.PagedPool(lm, 2 ** 31 - 1, 4096, F32)
+        pf.paged(pool, [[1, 2, 3]], [0], [[2]], h)
+        pf.check()
+        assert h.isfinite().all() and float(x.sum()) == 64
