@@ -1157,6 +1157,13 @@ def paged_attention_workspace_bytes(kv, batch, dtype, heads, window=0):
     return n if n >= 0 else check(n)
 
 
+def _scratch_bytes(work, err):
+    """A caller's workspace's bytes; refuses a view whose values do not lie side by side (an expanded one has fewer)."""
+    if not work.is_contiguous():
+        check(err)
+    return work.numel() * work.element_size()
+
+
 def _work(need, device, stream):
     """Scratch of one call, taken from the memory of the stream that the call runs on: there alone it is used again."""
     with _torch.cuda.stream(stream):
@@ -1176,7 +1183,7 @@ def paged_attention(kv, batch, q, out, heads, scale, window=0, work=None, stream
     if work is None:
         work = _work(paged_attention_workspace_bytes(kv, batch, q.dtype, heads, window), q.device, stream)
     return check(lib.gphq_paged_attention(kv.ref, batch.ref, _dtype(q.dtype), ptr(q), qs, heads, scale, window, ptr(out),
-                                          os_, ptr(work), work.numel() * work.element_size(), stream_handle(stream)))
+                                          os_, ptr(work), _scratch_bytes(work, ERR_PAGED_SHAPE), stream_handle(stream)))
 
 
 class _PoolMemory:
@@ -1245,7 +1252,7 @@ def lora_add(a, b, x, y, row_slots, ranks=None, scales=None, work=None, stream=N
         work = _work(lora_workspace_bytes(rows, k, max_rank), x.device, stream)
     return check(lib.gphq_lora_add(_dtype(a.dtype), ptr(a), ptr(b), ptr(ranks), ptr(scales), slots, max_rank,
                                    ptr(row_slots), ptr(x), xs, ptr(y), ys, rows, k, n, ptr(work),
-                                   work.numel() * work.element_size(), stream_handle(stream)))
+                                   _scratch_bytes(work, ERR_DIMENSIONS), stream_handle(stream)))
 
 
 # ---- weight preparation (gphq_prepare_projection) ----------------------------

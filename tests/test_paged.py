@@ -219,3 +219,32 @@ def test_descriptions_over_two_devices_are_refused():
         with pytest.raises(gphq.GphqError) as e:
             make()
         assert e.value.status == gphq.ERR_PAGED_SHAPE
+
+
+@pytest.fixture
+def on_the_cpu(monkeypatch):
+    """The binding's checks on tensors in host memory; what they let through finds no device here."""
+    import torch
+
+    gphq.load()
+    monkeypatch.setattr(gphq, "_here", lambda *tensors: None)
+    monkeypatch.setattr(gphq, "stream_handle", lambda stream=None: None)
+    return torch
+
+
+@pytest.mark.parametrize("view", [lambda w: w[:1].expand(1 << 24), lambda w: w[::2], lambda w: w[:64].view(8, 8).t()],
+                         ids=["expanded", "every other", "transposed"])
+def test_a_workspace_that_is_not_one_piece_is_refused(on_the_cpu, view):
+    """Its numbers of values would pass for more bytes than lie behind its address."""
+    torch = on_the_cpu
+    work = view(torch.zeros(1 << 20, dtype=torch.uint8))
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32)
+    pages, row = torch.zeros(2, 16, 1, 64), torch.zeros(1, 64)
+    kv, b = gphq.PagedKv(pages, pages.clone()), gphq.PagedBatch(ints(0, 1), ints(5), ints(0).view(1, 1), 1, 1, 5)
+    with pytest.raises(gphq.GphqError) as e:
+        gphq.paged_attention(kv, b, row, row.clone(), 1, 1.0, work=work)
+    assert e.value.status == gphq.ERR_PAGED_SHAPE
+    a, x = torch.zeros(1, 8, 32), torch.zeros(1, 32)
+    with pytest.raises(gphq.GphqError) as e:
+        gphq.lora_add(a, torch.zeros(1, 16, 8), x, torch.zeros(1, 16), ints(0), work=work)
+    assert e.value.status == gphq.ERR_DIMENSIONS
