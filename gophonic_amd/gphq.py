@@ -885,13 +885,15 @@ class Prefill:
         device tensor receives each sequence's last-token state."""
         import numpy as np
 
+        def int32(a):  # numbers past 32 bits become the nearest, which the call refuses, not their low halves
+            return np.clip(np.asarray(a, np.int64), -2 ** 31, 2 ** 31 - 1)
+
         lens, lp = _host([len(q) for q in seqs], np.int64)
         old, op = _host(past, np.int64)
-        tab, tp = _host(table, np.int32)
+        tab, tp = _host(int32(table), np.int32)
         if tab.ndim != 2 or tab.shape[0] != len(seqs) or old.size != len(seqs):
             check(ERR_PAGED_SHAPE)
-        flat = np.ascontiguousarray(np.concatenate([np.asarray(q, np.int64) for q in seqs]) if len(seqs) else
-                                    np.zeros(0), dtype=np.int32)
+        flat, _ = _host(np.concatenate([int32(q) for q in seqs]) if len(seqs) else [], np.int32)
         check(load().gphq_prefill_paged(self.h, pool.h if pool is not None else None,
                                         flat.ctypes.data if flat.size else None, lp, op, len(seqs), tp, tab.shape[1],
                                         ptr(hidden), 0 if hidden is None else hidden.numel(), stream_handle(stream)))

@@ -157,6 +157,18 @@ def test_paged_pass_refuses_to_write_a_page_that_is_read(lm, seqs, past, table):
     assert e.value.status == gphq.ERR_PAGED_BATCH
 
 
+@pytest.mark.parametrize("ids,table,status", [
+    ([2 ** 32 + 5], [[3]], gphq.ERR_TOKEN_VOCAB), ([-2 ** 32 + 5], [[3]], gphq.ERR_TOKEN_VOCAB),
+    ([5], [[2 ** 32 + 3]], gphq.ERR_PAGED_BATCH), ([5], [[-2 ** 32 + 3]], gphq.ERR_PAGED_BATCH),
+])
+def test_paged_pass_refuses_numbers_past_32_bits(lm, ids, table, status):
+    """They are not taken for their low halves, which name a token and a page."""
+    pool, pf = gphq.PagedPool(lm, 12, 16, F16), gphq.Prefill(lm, 128)
+    with pytest.raises(gphq.GphqError) as e:
+        pf.paged(pool, [np.array(ids)], [0], np.array(table), torch.empty(1, GEOM["hidden"], device="cuda"))
+    assert e.value.status == status
+
+
 def test_paged_pass_refuses_another_model_s_pool(lm):
     other = gphq.lm_random(dict(GEOM, layers=1), gphq.FMT_Q8B, 7)[0]
     pool, pf = gphq.PagedPool(other, 4, 16, F16), gphq.Prefill(lm, 16)
