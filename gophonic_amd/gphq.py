@@ -894,6 +894,9 @@ class Prefill:
         if tab.ndim != 2 or tab.shape[0] != len(seqs) or old.size != len(seqs):
             check(ERR_PAGED_SHAPE)
         flat, _ = _host(np.concatenate([int32(q) for q in seqs]) if len(seqs) else [], np.int32)
+        load()
+        _values(hidden, _torch.float32, 0, ERR_DEST_WIDTH)
+        _here(hidden)
         check(load().gphq_prefill_paged(self.h, pool.h if pool is not None else None,
                                         flat.ctypes.data if flat.size else None, lp, op, len(seqs), tp, tab.shape[1],
                                         ptr(hidden), 0 if hidden is None else hidden.numel(), stream_handle(stream)))

@@ -169,6 +169,15 @@ def test_paged_pass_refuses_numbers_past_32_bits(lm, ids, table, status):
     assert e.value.status == status
 
 
+@pytest.mark.parametrize("make", [lambda h: h.half(), lambda h: h.cpu(), lambda h: h.t().contiguous().t(),
+                                  lambda h: h.repeat(1, 2)[:, :h.shape[1]], lambda h: h[:, :1].expand(*h.shape)],
+                         ids=["half", "host", "transposed", "wider", "expanded"])
+def test_paged_pass_refuses_a_result_that_is_not_rows_of_float32(lm, make):
+    pool, pf = gphq.PagedPool(lm, 12, 16, F16), gphq.Prefill(lm, 128)
+    with pytest.raises(gphq.GphqError):
+        pf.paged(pool, [[1], [2, 3]], [0, 0], [[3], [4]], make(torch.empty(2, GEOM["hidden"], device="cuda")))
+
+
 def test_paged_pass_refuses_another_model_s_pool(lm):
     other = gphq.lm_random(dict(GEOM, layers=1), gphq.FMT_Q8B, 7)[0]
     pool, pf = gphq.PagedPool(other, 4, 16, F16), gphq.Prefill(lm, 16)
