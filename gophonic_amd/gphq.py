@@ -1201,12 +1201,14 @@ class _PoolMemory:
 
 class PagedPool:
     """gphq_paged_pool: a model's layers' pages, for Prefill.paged and, layer
-    by layer, for paged_append and paged_attention."""
+    by layer, for paged_append and paged_attention. In the memory of the
+    device that is current when it is made; close() ends its layers' tensors
+    with it."""
 
     def __init__(self, lm, pages, page_tokens, dtype):
         h = ctypes.c_void_p()
         check(load().gphq_paged_pool_new(lm.h, pages, page_tokens, _dtype(dtype), ctypes.byref(h)))
-        self.h, self.lm, self.dtype = h, lm, dtype
+        self.h, self.lm, self.dtype, self.device = h, lm, dtype, _torch.cuda.current_device()
 
     def close(self):
         if self.h:
@@ -1227,8 +1229,9 @@ class PagedPool:
         check(load().gphq_paged_pool_layer(self.h, i, ctypes.byref(d)))
         shape = (d.pages, d.kv_heads, d.page_tokens, d.head_dim)
         name = {DTYPE_F32: "<f4"}.get(d.dtype, "<i2")
-        k, v = (torch.as_tensor(_PoolMemory(self, a, shape, name), device="cuda").view(self.dtype).transpose(1, 2)
-                for a in (d.k_dev, d.v_dev))
+        # Asked for on another device than their memory's, the tensors would be copies.
+        k, v = (torch.as_tensor(_PoolMemory(self, a, shape, name), device=torch.device("cuda", self.device))
+                .view(self.dtype).transpose(1, 2) for a in (d.k_dev, d.v_dev))
         return PagedKv(k, v)
 
 

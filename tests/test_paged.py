@@ -248,3 +248,39 @@ def test_a_workspace_that_is_not_one_piece_is_refused(on_the_cpu, view):
     with pytest.raises(gphq.GphqError) as e:
         gphq.lora_add(a, torch.zeros(1, 16, 8), x, torch.zeros(1, 16), ints(0), work=work)
     assert e.value.status == gphq.ERR_DIMENSIONS
+
+
+def test_a_pool_s_layers_lie_on_its_own_device(monkeypatch):
+    """Made while device 1 is current and described while device 0 is: views of device 1's memory, not copies."""
+    import torch
+
+    gphq.load()
+    asked = []
+
+    class Lib:
+        def gphq_paged_pool_new(self, lm, pages, page_tokens, dtype, out):
+            out._obj.value = P
+            return gphq.OK
+
+        def gphq_paged_pool_layer(self, pool, layer, out):
+            for name, value in dict(k_dev=P, v_dev=2 * P, pages=3, page_tokens=16, kv_heads=2, head_dim=64,
+                                    dtype=gphq.DTYPE_F32).items():
+                setattr(out._obj, name, value)
+            return gphq.OK
+
+        def gphq_paged_pool_free(self, pool):
+            pass
+
+    def as_tensor(memory, device):
+        asked.append((memory.__cuda_array_interface__["data"][0], torch.device(device)))
+        return torch.zeros(memory.__cuda_array_interface__["shape"])
+
+    monkeypatch.setattr(gphq, "load", Lib)
+    monkeypatch.setattr(torch, "as_tensor", as_tensor)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    pool = gphq.PagedPool(type("Lm", (), dict(h=None)), 3, 16, torch.float32)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    kv = pool.layer(0)
+    assert asked == [(P, torch.device("cuda", 1)), (2 * P, torch.device("cuda", 1))]
+    assert kv.k.shape == (3, 16, 2, 64)
+    pool.close()
