@@ -242,11 +242,12 @@ class GphqError(RuntimeError):
 
 _lib = None
 _torch = None  # set by load(): an import statement in a call costs it about 0.3 us
+_raw_stream = None  # torch's private way to the current stream's handle, where this torch has it
 
 
 def load():
     """Loads libgphq.so (raises if it has not been built)."""
-    global _lib, _torch
+    global _lib, _torch, _raw_stream
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(f"{LIB_PATH} is missing: run `python -m gophonic_amd.build` first")
@@ -257,6 +258,7 @@ def load():
         import torch
 
         _torch = torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         lib = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(lib, name)
@@ -285,9 +287,11 @@ def ptr(t):
 
 
 def stream_handle(stream=None):
-    if stream is None:  # the current stream's handle, without a Stream object (2.7 us less a call)
+    if stream is None:
         load()
-        return _torch._C._cuda_getCurrentRawStream(_torch.cuda.current_device())
+        if _raw_stream is not None:  # without a Stream object: 2.7 us less a call
+            return _raw_stream(_torch.cuda.current_device())
+        stream = _torch.cuda.current_stream()
     return stream.cuda_stream
 
 

@@ -284,3 +284,15 @@ def test_a_pool_s_layers_lie_on_its_own_device(monkeypatch):
     assert asked == [(P, torch.device("cuda", 1)), (2 * P, torch.device("cuda", 1))]
     assert kv.k.shape == (3, 16, 2, 64)
     pool.close()
+
+
+def test_the_current_stream_s_handle_without_torch_s_private_call(monkeypatch):
+    """A torch that has no such call is asked for the stream in the public way."""
+    import torch
+
+    gphq.load()
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    monkeypatch.setattr(gphq, "_raw_stream", None, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: type("Stream", (), dict(cuda_stream=1234)))
+    assert gphq.stream_handle() == 1234

@@ -166,6 +166,13 @@ def test_check_keeps_to_its_stream():
     torch.cuda.synchronize()
 
 
+def test_the_current_stream_s_handle():
+    side = torch.cuda.Stream()
+    for s in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(s):
+            assert gphq.stream_handle() == s.cuda_stream == gphq.stream_handle(s)
+
+
 # ---- values at the end of their type's range -----------------------------------------
 
 
