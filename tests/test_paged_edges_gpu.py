@@ -208,3 +208,125 @@ def test_single_16_bit_rows_are_rounded_once(ct, hd):
     q = (b.randn(b.rows, 8 * hd) * 1.5).to(ct)
     got = run(b, q, 8, hd ** -0.5)
     check_rows(b, q, 8, hd ** -0.5, got, range(b.rows), pieces=2)
+
+
+# ---- long walks ------------------------------------------------------------------------
+
+
+def filled(seqs, kv_heads, hd, page, dtype, seed, **over):
+    """A Batch whose tokens are drawn all at once, unused slots NaN."""
+    b = Batch(seqs, kv_heads, hd, page, dtype, seed=seed, tokens=False, **over)
+    used = torch.zeros(b.pages, page, dtype=torch.bool)
+    for s, t in enumerate(b.lens):
+        p = torch.arange(t)
+        used[torch.from_numpy(b.table[s]).long()[p // page], p % page] = True
+    n = int(used.sum())
+    b.k[used] = b.randn(n, kv_heads, hd).to(dtype)
+    b.v[used] = (b.randn(n, kv_heads, hd) + 0.25).to(dtype)
+    return b
+
+
+def splits(b, rt, heads, rows, window=0):
+    """How many splits of `rows` rows the call's workspace holds."""
+    kv, dev = b.device(gphq)
+    n = gphq.paged_attention_workspace_bytes(kv, dev, rt, heads, window)
+    assert n % (rows * heads * (b.hd + 2) * 4) == 0
+    return n // (rows * heads * (b.hd + 2) * 4)
+
+
+def spread(rows, count=24):
+    return sorted({round(i * (rows - 1) / (count - 1)) for i in range(count)})
+
+
+def in_blocks(rt, blocks):
+    """Rows of group 8 and eight KV heads that make as many blocks of the chunk kernel as `blocks` times what runs at
+    once: 128 columns and two blocks a CU, 256 and one for fp32 rows."""
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    return int(blocks * (2 * cus * 128 if rt != F32 else cus * 256) / 64)
+
+
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 16), (128, 256)])
+def test_chunks_that_are_not_split(hd, page, rt, ct):
+    """A block walks all of a chunk's keys: some forty steps, more table entries than a wavefront holds at once."""
+    rows = in_blocks(rt, 1)
+    b = filled([(rows, rows + 1537)], 8, hd, page, ct, seed=90)
+    q = b.randn(rows, 64 * hd).to(rt)
+    assert splits(b, rt, 64, rows) == 0
+    got = run(b, q, 64, 0.1)
+    check_rows(b, q, 64, 0.1, got, spread(rows))
+
+
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_chunks_of_two_long_splits(hd, rt, ct):
+    rows = in_blocks(rt, 0.5)
+    b = filled([(rows, 6033)], 8, hd, 16, ct, seed=91)
+    q = b.randn(rows, 64 * hd).to(rt)
+    assert splits(b, rt, 64, rows) == 2
+    got = run(b, q, 64, 0.1)
+    check_rows(b, q, 64, 0.1, got, spread(rows))
+
+
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_single_tokens_of_long_splits(hd, rt, ct):
+    """Sixteen single tokens over ragged caches of small pages, two splits of some 2000 keys each."""
+    b = filled([(1, 4000 - 177 * i) for i in range(16)], 8, hd, 16, ct, seed=92)
+    q = (b.randn(16, 32 * hd) * 1.5).to(rt)
+    assert splits(b, rt, 32, 16) == 2
+    got = run(b, q, 32, hd ** -0.5)
+    check_rows(b, q, 32, hd ** -0.5, got, range(16))
+
+
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+def test_many_sequences_of_every_kind(rt, ct):
+    """170 sequences, chunks, a few rows, single tokens and none, both kernels split: more than the 64 that a wavefront
+    looks at together."""
+    kinds = [(0, 0), (1, 1400), (1, 33), (0, 50), (5, 900), (1, 17), (70, 1300), (1, 1), (3, 2), (40, 40)]
+    seqs = [(n, t + 3 * i if t > 2 else t) for i in range(17) for n, t in kinds]
+    b = filled(seqs, 1, 64, 16, ct, seed=93, spare_rows=3)
+    q = (b.randn(b.rows, 4 * 64) * 1.5).to(rt)
+    small = 170 * (64 // 4)  # places of the row kernel's split results: up to 16 rows a sequence
+    kv, dev = b.device(gphq)
+    n = gphq.paged_attention_workspace_bytes(kv, dev, rt, 4)
+    places, rest = n // (4 * (64 + 2) * 4), min(small, b.rows)
+    assert any((places - i * b.rows) > 0 and (places - i * b.rows) % rest == 0 for i in range(2, 40))
+    got = run(b, q, 4, 0.125)
+    last = b.starts[-1]
+    check_rows(b, q, 4, 0.125, got, sorted(set(spread(last, 150)) | {r for r in b.starts[:-1] if r < last}))
+    assert (got[last:] == 7).all()
+
+
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("window", [0, 300])
+def test_infinite_values_on_many_steps(window, rt, ct):
+    """Infinities in some dims of many values of a chunk, on every step of the tiles' edges, LDS buffers used many times
+    over: exactly the rows that see one are not finite in that dim (NaN where a probability has several pieces, of
+    which one may be 0 or negative), every other value keeps to the definition."""
+    heads, hd = 8, 64  # group 1: a tile is 128 or 256 rows, its edges several steps
+    rows = in_blocks(rt, 1) * 8
+    b = filled([(rows, rows + 200)], 8, hd, 16, ct, seed=94)
+    q = b.randn(rows, heads * hd).to(rt)
+    assert splits(b, rt, heads, rows, window) == 0
+    # Token p holds an infinity in KV head p % 8, dim p % 64 or the next: three of 64 neighbouring tokens, from half
+    # of the rows on (without a window, all rows behind it see the early ones).
+    bad = [p for p in range(200 + rows // 2, 200 + rows) if p % 64 in (0, 17, 50)]
+    held = torch.zeros(rows + 200, 8, hd, dtype=torch.bool)
+    clean = b.v.clone()
+    for p in bad:
+        at, d = b.token(0, p), (p + p // 64) % hd
+        b.v[at][p // 64 % 8, d] = math.inf
+        clean[at][p // 64 % 8, d] = 0.0
+        held[p, p // 64 % 8, d] = True
+    got = run(b, q, heads, 0.1, window)
+    b.v = clean
+    for r in sorted(set(spread(rows, 16)) | set(range(rows // 2 - 2, rows, rows // 29)) | {rows // 2 + i for i in range(5)}):
+        p = 200 + r
+        lo = max(0, p - window + 1) if window else 0
+        inf = held[lo:p + 1].any(0).reshape(-1)
+        assert torch.equal(~got[r].isfinite(), inf), f"row {r}"
+        want, tol = row64(b, q, heads, 0.1, r, window)
+        # Where a token's own value is infinite the definition is too; the other dims have the values as they are.
+        err = (got[r].double() - want).abs()[~inf]
+        assert (err <= tol[~inf]).all(), f"row {r}"
