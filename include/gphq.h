@@ -602,26 +602,26 @@ int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, in
  * among them (append them first):
  *   out[i][h] = sum_j softmax_j(scale * q[i][h] . k[j][h / (heads / kv_heads)]) v[j][...]
  * over the tokens j of row i's sequence up to its position p, and with
- * window > 0 only those past p - window. A row that sees no key, being before
- * token 0 or with none of its keys in a page of the pool, becomes 0. What a row
- * does not see, whatever it holds (NaN included), does not reach it; a row that
- * sees a value of V that is not finite, or whose scores are NaN or all -inf,
- * becomes not finite. Sums are fp32, over probabilities of at most 1 before the
- * division: finite values whose sum of magnitudes stays in range give finite
- * rows. scale may have either sign. Any number of rows per sequence: prompt
- * chunks and single tokens may stand in one call. fp32 rows are multiplied to
- * fp32 accuracy whatever the pool's type. So are 16-bit rows (of the pool's
- * type) in sequences whose rows times heads / kv_heads are at most 64, single
- * tokens among them; longer ones round each probability to that type before the
- * product with the values, an error of at most half a step of sum p |v|. out
- * may not overlap q (nor the pool).
- * A batch of more blocks than a launch takes is GPHQ_ERR_PAGED_SHAPE: with
- * g = heads / kv_heads, where kv_heads seqs ceil(min(max_rows g, 64) / 16)
- * (g <= 64), or kv_heads times about rows g / 128 (256 for fp32 rows; where
- * max_rows g > 64), passes 2^23 - 1, or rows ceil(heads head_dim / 256) passes
- * 2^26 - 1 in a batch whose keys are split.
- * work (16-byte aligned) of at least gphq_paged_attention_workspace_bytes for
- * the same pool, batch, row type, heads and window; its contents need not be
+ * window > 0 only those past p - window. Any number of rows per sequence: prompt
+ * chunks and single tokens may stand in one call. scale may have either sign.
+ * A row that sees no key, being before token 0 or with none of its keys in a
+ * page of the pool, becomes 0. What a row does not see, whatever it holds (NaN
+ * included), does not reach it; a row that sees a value of V that is not finite,
+ * or whose scores are NaN or all -inf, becomes not finite. Sums are fp32, over
+ * probabilities of at most 1 before the division: finite values whose sum of
+ * magnitudes stays in range give finite rows.
+ * fp32 rows are multiplied to fp32 accuracy whatever the pool's type. So are
+ * 16-bit rows (of the pool's type) in sequences whose rows times
+ * heads / kv_heads are at most 64, single tokens among them; longer ones round
+ * each probability to that type before the product with the values, an error of
+ * at most half a step of sum p |v|.
+ * out may not overlap q (nor the pool). A batch of more blocks than a launch
+ * takes is GPHQ_ERR_PAGED_SHAPE: with g = heads / kv_heads, where
+ * kv_heads seqs ceil(min(max_rows g, 64) / 16) (g <= 64), or kv_heads times
+ * about rows g / 128 (256 for fp32 rows; where max_rows g > 64), passes 2^23 - 1,
+ * or rows ceil(heads head_dim / 256) passes 2^26 - 1 in a batch whose keys are
+ * split. work (16-byte aligned) of at least gphq_paged_attention_workspace_bytes
+ * for the same pool, batch, row type, heads and window; its contents need not be
  * kept between calls, and calls that may run at the same time need one each.
  * Sums are taken in a fixed order: the same call gives the same bits. */
 int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype,
@@ -647,6 +647,11 @@ int gphq_paged_pool_layer(const gphq_paged_pool *pool, int64_t layer, gphq_paged
  * (gphq_gemv_vec, gphq_mm, gphq_prefill_project) the adapters that some of them
  * carry:
  *   y[r] += scales[s] * B[s] (A[s] x[r]),  s = row_slots[r]
+ * x are the rows that the projection multiplies and y its output, in their basis:
+ * gphq_prefill_project 0 normalizes its input first, 2 applies SwiGLU to its
+ * output (no adapter fits behind that), 3 rotates its input in Q8 / Q4 layers,
+ * and a model's rows are rotated and its norms' weights folded as
+ * gphq_prepare_layer_jobs says, so a checkpoint's A and B are to be too.
  * x fp32 [rows][x_stride], y fp32 [rows][y_stride]; A [slots][max_rank][k] and
  * B [slots][n][max_rank] of dtype (GPHQ_DTYPE_*), adapter s using its first
  * ranks[s] of max_rank (device int32[slots], taken into 0 .. max_rank; NULL: all;

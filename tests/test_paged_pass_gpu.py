@@ -286,3 +286,30 @@ def test_memory_that_is_not_there_leaves_no_error(lm):
         pf.paged(pool, [[1, 2, 3]], [0], [[2]], h)
         pf.check()
         assert h.isfinite().all() and float(x.sum()) == 64
+
+
+def test_adapters_beside_a_layer_s_projections(lm):
+    """The adapters of QKV on the rows that the projection multiplies (normalized by the caller), those of O on the
+    context: what they add is B (A x) of those rows, on top of what the projections give alone."""
+    H, heads, G, D, rank, rows = GEOM["hidden"], GEOM["heads"], GEOM["kv_heads"], 128, 16, 45
+    g = torch.Generator().manual_seed(21)
+    x, ctx = torch.randn(rows, H, generator=g).cuda() * 2, torch.randn(rows, heads * D, generator=g).cuda()
+    slots = torch.arange(rows, dtype=torch.int32).cuda() % 4 - 1
+    pf = gphq.Prefill(lm, 64)
+    xn = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + GEOM["eps"])
+    for proj, rows_in, width, y in ((0, xn, (heads + 2 * G) * D, torch.empty(rows, (heads + 2 * G) * D, device="cuda")),
+                                    (1, ctx, H, x.clone())):
+        a = (torch.randn(3, rank, rows_in.shape[1], generator=g) * 0.05).bfloat16().cuda()
+        b = (torch.randn(3, width, rank, generator=g) * 0.05).bfloat16().cuda()
+        pf.project(0, proj, x if proj == 0 else ctx, rows, y)
+        alone = y.double()
+        gphq.lora_add(a, b, rows_in, y, slots)
+        A, B, v = a.double()[slots.clamp(min=0).long()], b.double()[slots.clamp(min=0).long()], rows_in.double()
+        on = (slots >= 0).double()[:, None]
+        low = (A * v[:, None]).sum(-1)
+        want = alone + on * (B * low[:, None]).sum(-1)
+        # (k + rank + 8) u of the products' magnitudes, and one u of the sum with what was there.
+        size = (B.abs() * (A.abs() * v.abs()[:, None]).sum(-1)[:, None]).sum(-1)
+        tol = (rows_in.shape[1] + rank + 8) * 2.0 ** -24 * size + 2.0 ** -24 * (alone.abs() + want.abs())
+        assert ((y.double() - want).abs() <= tol).all()
+        assert torch.equal(y[0].double(), alone[0])  # no adapter
