@@ -4,7 +4,7 @@
 //
 // Two launches. The shrink makes t[r] = A[s] x[r] (rank values a row) over ranges of k, one
 // partial sum each; the expand adds the partial sums in order, scales them and adds B[s] t[r]
-// into y. Both work on tiles of rows (32 and up to 64) and pass over a tile once for every
+// into y. Both work on tiles of rows (32; 16 in the expand of a call of up to 16) and pass over a tile once for every
 // distinct adapter among its rows: rows of one request stand side by side, so a tile of a
 // prompt mostly has one, a tile of decode lanes many.
 //
@@ -140,7 +140,7 @@ __device__ __forceinline__ f32x4 product(const Frag<float>::weight &a, const Fra
 
 // t[split][r][0 .. max_rank) of a tile's rows, over k of one split: D (16 ranks x 16 rows)
 // = A . X^T per 16 ranks and 16 rows. The four wavefronts take every fourth 32 k and are
-// added in order. Bound by reading x and A in long calls (4814 rows of 4096 and rank 64: 25 us,
+// added in order. Bound by reading x and A in long calls (4814 rows of 4096 and one adapter of rank 64: 25 us,
 // 79 MB of x), by one wavefront's chain of loads in short ones, where k is cut into as many
 // ranges as leave a block two steps (32 rows of eight adapters: 7 us).
 template <typename W, int RT>
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(const LoraArgs a) {
     }
 }
 
-// Row tiles of 16 in a block of the expand.
+// Rows of a block of the expand.
 int expand_rows(int64_t rows) { return rows <= 16 ? 16 : 32; }
 
 // How a call of `rows` rows is cut.

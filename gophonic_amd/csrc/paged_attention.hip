@@ -90,8 +90,10 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         // split 9.4; 768 keys: 10.3 and 9.3) and 256 of 32 (10.6 and 11.0; 384: 13.4 and 11.1).
         const bool brief = span(kSmallTile) <= (wide ? 256 : 512);
         // Beside longer sequences, which are the chunk kernel's, only some of the sequences are
-        // this kernel's, in one tile mostly: twice as many splits of one tile each (three rows of
-        // twelve sequences over up to 4000 bfloat16 tokens: 15 us, 20 before).
+        // this kernel's, in one tile mostly: twice as many splits of one tile each. Whole calls,
+        // so and with the rule above: twelve sequences (three single rows) over up to 4000
+        // bfloat16 tokens 233 and 241 us, twenty (ten) up to 8000 274 and 355, six (five), FP16,
+        // up to 6000 106 and 149, thirty (fifteen) up to 3000 FP16 tokens 123 and 136.
         const bool mixed = cols > p.small_cols;
         const int64_t want = mixed ? 2 * cus / (units / p.small_tiles) : cus / units;
         // The grid has a place for every sequence, with rows or without: no more splits than a launch takes.
@@ -109,9 +111,11 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         // Tiles enough for the chip are not split (three chunks of 300 to 1300 fp32 rows over
         // FP16 pages: 106 us, split in three 133). Fewer tiles of one sequence take as many splits
         // as fill it (512 FP16 rows over 7512 tokens: 84 us, twice as many 100); of several, whose
-        // lengths differ, three times as many, so that the long ones do not come last alone (twelve
-        // chunks of 1 to 300 fp32 rows over up to 4000 bfloat16 tokens: 240 us, 293 with one round,
-        // 261 with four times).
+        // lengths differ, three times as many, so that the long ones do not come last alone: the
+        // twelve sequences above 233 us, 302 with one round (261 with four times, 240 with three, at
+        // that time), the twenty 274 and 535, the thirty 123 and 154. That loses where the chunks are
+        // alike or one alone: three of 83 to 234 FP16 rows over 6000 tokens 106 us, 94 with one
+        // round, the six (one chunk) 106 and 88.
         const int64_t want = units >= slots ? 1 : (b.seqs == 1 ? 1 : 3) * slots / units;
         cut(span(big_tile), want, p.big_len, p.big_splits);
     }
