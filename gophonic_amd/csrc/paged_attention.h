@@ -106,14 +106,20 @@ __device__ __forceinline__ void pages_start(const AttnArgs &a, PageWalk &w, int 
 
 // Whether a row at position pos that sees the keys from `first` on has one in a page of the pool.
 // Asked only where no score was above -inf: a row without such a key sees nothing and is 0, one
-// whose scores are all -inf or NaN is not finite.
-__device__ __forceinline__ bool sees_any(const AttnArgs &a, int seq, int first, int pos) {
-    if (pos < 0) return false;
-    for (int e = max(first, 0) >> a.pool.shift; e <= pos >> a.pool.shift; ++e) {
-        const int page = a.b.table[seq * a.b.table_stride + e];
-        if (page >= 0 && page < a.pool.pages) return true;
+// whose scores are all -inf or NaN is not finite. The G lanes of `group`, numbered by `lane`, ask
+// together, each about every G-th entry, eight at a time.
+template <int G>
+__device__ __forceinline__ bool sees_any(const AttnArgs &a, int seq, int first, int pos, int lane, uint64_t group) {
+    bool any = false;
+    const int last = pos < 0 ? -1 : pos >> a.pool.shift;
+    for (int e = max(first, 0) >> a.pool.shift; e <= last && !any; e += 8 * G) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int page = a.b.table[seq * a.b.table_stride + min(e + u * G + lane, last)];
+            any |= page >= 0 && page < a.pool.pages;
+        }
     }
-    return false;
+    return (__ballot(any) & group) != 0;
 }
 
 // Byte offsets of the 16-key groups kt, kt + 16, ... of a step; a bit per group that is not bad.

@@ -138,7 +138,8 @@ __device__ __forceinline__ void chunk_finish(const AttnArgs &a, const ChunkTile 
     if (!t.live) return;
     if (t.splits == 1) {
         const float inv = 1.0f / l;
-        const bool empty = m == -INFINITY && !sees_any(a, t.seq, t.first, t.pos);
+        const int q = threadIdx.x & 31;
+        const bool empty = m == -INFINITY && !sees_any<2>(a, t.seq, t.first, t.pos, hi, 0x100000001ull << q);
         RT *out = (RT *)a.out + (int64_t)(t.start + t.row) * a.out_stride + t.head * HD;
 #pragma unroll
         for (int d = 0; d < HD; d += 8) {
@@ -491,7 +492,8 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
     l += __shfl_xor(l, 32);
     if (!t.live) return;
     const float inv = 1.0f / l;
-    const bool empty = t.splits == 1 && m == -INFINITY && !sees_any(a, t.seq, t.first, t.pos);
+    const bool empty =
+        t.splits == 1 && m == -INFINITY && !sees_any<2>(a, t.seq, t.first, t.pos, hi, 0x100000001ull << q);
     float *out = (float *)a.out + (int64_t)(t.start + t.row) * a.out_stride + t.head * HD;
     const int64_t at = ((int64_t)(t.start + t.row) * a.heads + t.head) * a.parts + t.split;
 #pragma unroll

@@ -161,7 +161,8 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t,
     }
     if (t.splits == 1) {
         const float inv = 1.0f / L;
-        const bool empty = M == -INFINITY && !sees_any(a, t.seq, a.window > 0 ? pos - a.window + 1 : 0, pos);
+        const bool empty = M == -INFINITY && !sees_any<16>(a, t.seq, a.window > 0 ? pos - a.window + 1 : 0, pos, c,
+                                                           0xFFFFull << (lane & 48));
         RT *out = (RT *)a.out + (int64_t)(t.start + row) * a.out_stride + head * HD + d;
 #pragma unroll
         for (int i = 0; i < VD; i += 4) {

@@ -151,6 +151,7 @@ def test_check_keeps_to_its_stream():
     b.table[0, 1] = -5
     kv, dev = b.device(gphq)
     q, out = b.randn(1, 128).half().cuda(), torch.empty(1, 128, dtype=F16, device="cuda")
+    work = torch.empty(16, dtype=torch.uint8, device="cuda")
     x, side, done = torch.randn(8192, 8192, device="cuda"), torch.cuda.Stream(), torch.cuda.Event()
     y = x @ x
     torch.cuda.synchronize()
@@ -158,7 +159,7 @@ def test_check_keeps_to_its_stream():
         torch.matmul(x, x, out=y)
     done.record()
     for _ in range(3):
-        gphq.paged_attention(kv, dev, q, out, 2, 0.1, stream=side)
+        gphq.paged_attention(kv, dev, q, out, 2, 0.1, work=work, stream=side)
         with pytest.raises(gphq.GphqError):
             dev.check(side)
     dev.check(side)
@@ -330,3 +331,31 @@ def test_infinite_values_on_many_steps(window, rt, ct):
         # Where a token's own value is infinite the definition is too; the other dims have the values as they are.
         err = (got[r].double() - want).abs()[~inf]
         assert (err <= tol[~inf]).all(), f"row {r}"
+
+
+@pytest.mark.parametrize("rt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("seqs,split", [([(1, 9000)], True), ([(1, 9000)] * 2 + [(1, 2500)] * 130, False),
+                                        ([(80, 9000)], True), ("chunk", False)], ids=["rows", "rows whole", "chunk", "chunk whole"])
+def test_long_runs_of_bad_pages(seqs, split, rt, ct):
+    """Hundreds of bad table entries before the only good one, whose keys give scores of -inf to some KV heads: those
+    are not finite, the others are that page's mean, and without a good entry the row is 0."""
+    rows = in_blocks(rt, 1)
+    heads, G = (64, 8) if seqs == "chunk" else (8, 2)
+    b = filled([(rows, rows + 5000)] if seqs == "chunk" else seqs, G, 64, 16, ct, seed=95)
+    q = (b.randn(b.rows, heads * 64).abs() + 0.1).to(rt)
+    assert (splits(b, rt, heads, b.rows) == 0) != split
+    first = b.lens[0] - b.new[0]  # the first row's position
+    for s in range(min(2, len(b.new))):
+        b.table[s, :first // 16] = -1
+    at, before = int(b.table[0, first // 16]), first % 16
+    b.k[at][:before + 1, 0] = -math.inf  # what the first row sees, in the KV head 0
+    if len(b.new) > 1:
+        b.table[1] = b.pages
+    got = run(b, q, heads, 0.1, bad=True)
+    group = heads // G * 64
+    assert not got[0, :group].isfinite().any()
+    want, tol = row64(b, q, heads, 0.1, 0)
+    assert ((got[0].double() - want).abs() <= tol)[group:].all()
+    if len(b.new) > 1:
+        assert (got[1] == 0).all()
+        check_rows(b, q, heads, 0.1, got, range(2, b.rows, 9))
