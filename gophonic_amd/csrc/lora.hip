@@ -140,7 +140,7 @@ __device__ __forceinline__ f32x4 product(const Frag<float>::weight &a, const Fra
 
 // t[split][r][0 .. max_rank) of a tile's rows, over k of one split: D (16 ranks x 16 rows)
 // = A . X^T per 16 ranks and 16 rows. The four wavefronts take every fourth 32 k and are
-// added in order. Bound by reading x and A in long calls (4814 rows of 4096 and one adapter of rank 64: 25 us,
+// added in order. Bound by reading x and A in long calls (4814 rows of 4096, one adapter of rank 64: 25 us,
 // 79 MB of x), by one wavefront's chain of loads in short ones, where k is cut into as many
 // ranges as leave a block two steps (32 rows of eight adapters: 7 us).
 template <typename W, int RT>

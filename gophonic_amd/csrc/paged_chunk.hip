@@ -177,7 +177,8 @@ __device__ __forceinline__ void chunk_finish(const AttnArgs &a, const ChunkTile 
 // 32 heads over 7512 tokens: 84 us with the join, 0.73 PFLOP/s; 4096 fp32 rows, FP16 pages: 258
 // us, 0.53 PFLOP/s and twice that in pieces, the rate at which a large FP16 library product
 // runs on this card (1.1). 16-bit rows take their probabilities in one piece, rounded to the
-// rows' type: a second one, as the row kernel has, makes the 84 us 108. Half-step offsets between the wavefronts of a SIMD, to set one's
+// rows' type: a second one, as the row kernel has, makes the 84 us 108. Half-step offsets
+// between the wavefronts of a SIMD, to set one's
 // exponentials beside the other's products, measured the same or slower (268 us before, 273
 // to 275 with them).
 template <typename RT, typename CT, int HD, int NW>

@@ -610,11 +610,11 @@ int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, in
  * or whose scores are NaN or all -inf, becomes not finite. Sums are fp32, over
  * probabilities of at most 1 before the division: finite values whose sum of
  * magnitudes stays in range give finite rows.
- * fp32 rows are multiplied to fp32 accuracy whatever the pool's type. So are
- * 16-bit rows (of the pool's type) in sequences whose rows times
- * heads / kv_heads are at most 64, single tokens among them; longer ones round
- * each probability to that type before the product with the values, an error of
- * at most half a step of sum p |v|.
+ * fp32 rows are multiplied to fp32 accuracy whatever the pool's type. 16-bit
+ * rows (of the pool's type) keep 16 bits (bfloat16) or 22 (FP16) of each
+ * probability in sequences whose rows times heads / kv_heads are at most 64,
+ * single tokens among them; longer ones round it to the type before the product
+ * with the values, an error of at most half a step of sum p |v|.
  * out may not overlap q (nor the pool). A batch of more blocks than a launch
  * takes is GPHQ_ERR_PAGED_SHAPE: with g = heads / kv_heads, where
  * kv_heads seqs ceil(min(max_rows g, 64) / 16) (g <= 64), or kv_heads times
