@@ -6,7 +6,9 @@
 //   o = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),  x_j = scale log2(e) q.k_j,
 // one pass over the keys with a running reference m: x is exponentiated against
 // m, and m moves to a larger x only when that passes it by more than 8, so most
-// steps rescale nothing. Scores, sums and outputs are fp32.
+// steps rescale nothing. Scores, sums and outputs are fp32. m is -inf until the row sees a key,
+// then kLeast or more, whatever that key's score: a row whose m is -inf at the end has seen none
+// and is 0, one that saw scores of -inf or NaN alone is 0 / 0 or NaN.
 //
 // A query tile is TM columns of one sequence and one KV head: column c is query
 // row c / group, query head KV head * group + c % group, so all heads that share
@@ -15,6 +17,8 @@
 // where that gives more than one piece, each writes its unnormalized output, its
 // reference and its sum, and paged_join_kernel adds them in order.
 #pragma once
+#include <float.h>
+
 #include "paged.h"
 
 namespace gphq {
@@ -39,7 +43,9 @@ struct AttnArgs {
 };
 
 constexpr int kSmallTile = 16;
-constexpr float kLag = 8.0f;    // the reference maximum may be passed by this much (in log2)
+constexpr float kLag = 8.0f;  // the reference maximum may be passed by this much (in log2)
+constexpr float kLeast = -FLT_MAX;  // the least reference of a row that has seen a key
+
 // Exponentials are 2^(x - m + lift). FP16 probabilities reach 2^15, so that they keep 2^-24 of a
 // 2^7 .. 2^15 maximum, not of 1 (and FP16 values, up to 2^16, stay far inside fp32). Elsewhere none
 // passes 1: a sum over finite values leaves fp32's range only where that of their magnitudes,
@@ -102,24 +108,6 @@ __device__ __forceinline__ void pages_start(const AttnArgs &a, PageWalk &w, int 
     w.lo_entry = lo >> a.pool.shift;
     w.hi_entry = (hi - 1) >> a.pool.shift;
     pages_fill<CT>(a, w, seq, g, kt >> a.pool.shift);
-}
-
-// Whether a row at position pos that sees the keys from `first` on has one in a page of the pool.
-// Asked only where no score was above -inf: a row without such a key sees nothing and is 0, one
-// whose scores are all -inf or NaN is not finite. The G lanes of `group`, numbered by `lane`, ask
-// together, each about every G-th entry, eight at a time.
-template <int G>
-__device__ __forceinline__ bool sees_any(const AttnArgs &a, int seq, int first, int pos, int lane, uint64_t group) {
-    bool any = false;
-    const int last = pos < 0 ? -1 : pos >> a.pool.shift;
-    for (int e = max(first, 0) >> a.pool.shift; e <= last && !any; e += 8 * G) {
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int page = a.b.table[seq * a.b.table_stride + min(e + u * G + lane, last)];
-            any |= page >= 0 && page < a.pool.pages;
-        }
-    }
-    return (__ballot(any) & group) != 0;
 }
 
 // Byte offsets of the 16-key groups kt, kt + 16, ... of a step; a bit per group that is not bad.

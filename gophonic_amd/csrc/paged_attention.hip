@@ -208,13 +208,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
         }
     }
     if (!splits) return;
-    const int pos = s.len - n + i;
-    const uint64_t group = (1ull << LH) - 1 << (lane & ~(LH - 1));
-    const bool empty = M == -INFINITY &&
-                       !sees_any<LH>(a, s.seq, a.window > 0 ? pos - a.window + 1 : 0, pos, lane % LH, group);
     float r[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = empty ? 0.0f : o[e] / L;
+    for (int e = 0; e < 4; ++e) r[e] = M == -INFINITY ? 0.0f : o[e] / L;
     store_vec((RT *)a.out + (int64_t)row * a.out_stride + head * HD + d, r);
 }
 

@@ -96,21 +96,26 @@ template <typename CT, int N>
 __device__ __forceinline__ float chunk_softmax(const ChunkTile &t, f32x16 (&s)[N], float fac, bool masked, int kt,
                                                unsigned ok, float &m, float &l, bool &moved) {
     const int hi = (threadIdx.x & 63) >> 5;
-    float mx = -INFINITY;
+    float mx = kLeast;
     if (masked) {
+        bool any = false;
 #pragma unroll
         for (int h = 0; h < N; ++h)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int key = kt + 32 * h + 8 * (r >> 2) + 4 * hi + (r & 3);
-                if (key > t.pos || key < t.first || !(ok >> (2 * h + (r >> 3)) & 1)) s[h][r] = -INFINITY;
+                const bool sees = key <= t.pos && key >= t.first && (ok >> (2 * h + (r >> 3)) & 1);
+                if (!sees) s[h][r] = -INFINITY;
+                any |= sees;
             }
+        mx = any ? kLeast : -INFINITY;
     }
 #pragma unroll
     for (int h = 0; h < N; ++h)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[h][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32)) * fac;
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mx = mx == -INFINITY ? mx : fmaxf(mx * fac, kLeast);
     const bool grew = mx > m + kLag;
     const float mn = grew ? mx : m;
     const float ref = mn == -INFINITY ? 0.0f : mn - kLift<CT>;
@@ -138,8 +143,7 @@ __device__ __forceinline__ void chunk_finish(const AttnArgs &a, const ChunkTile 
     if (!t.live) return;
     if (t.splits == 1) {
         const float inv = 1.0f / l;
-        const int q = threadIdx.x & 31;
-        const bool empty = m == -INFINITY && !sees_any<2>(a, t.seq, t.first, t.pos, hi, 0x100000001ull << q);
+        const bool empty = m == -INFINITY;
         RT *out = (RT *)a.out + (int64_t)(t.start + t.row) * a.out_stride + t.head * HD;
 #pragma unroll
         for (int d = 0; d < HD; d += 8) {
@@ -493,8 +497,6 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
     l += __shfl_xor(l, 32);
     if (!t.live) return;
     const float inv = 1.0f / l;
-    const bool empty =
-        t.splits == 1 && m == -INFINITY && !sees_any<2>(a, t.seq, t.first, t.pos, hi, 0x100000001ull << q);
     float *out = (float *)a.out + (int64_t)(t.start + t.row) * a.out_stride + t.head * HD;
     const int64_t at = ((int64_t)(t.start + t.row) * a.heads + t.head) * a.parts + t.split;
 #pragma unroll
@@ -502,7 +504,7 @@ __global__ __launch_bounds__(64 * NW) void attn_chunk32_kernel(const AttnArgs a,
         const int d0 = DT * (8 * (r >> 2) + 4 * hi + (r & 3));
         vdim v;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) v[d] = t.splits > 1 ? o[d][r] : empty ? 0.0f : o[d][r] * inv;
+        for (int d = 0; d < DT; ++d) v[d] = t.splits > 1 ? o[d][r] : m == -INFINITY ? 0.0f : o[d][r] * inv;
         *(vdim *)((t.splits > 1 ? a.part_o + at * HD : out) + d0) = v;
     }
     if (t.splits > 1 && hi == 0) {

@@ -65,18 +65,23 @@ __device__ __forceinline__ float softmax_step(const RowTile &t, const f32x4 (&s)
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3];
+    float mx = kLeast;
     if (masked) {
+        bool any = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int key = kt + 16 * (i >> 2) + 4 * g4 + (i & 3);
-            if (key > t.pos || key < t.first || !(ok >> (i >> 2) & 1)) x[i] = -INFINITY;
+            const bool sees = key <= t.pos && key >= t.first && (ok >> (i >> 2) & 1);
+            if (!sees) x[i] = -INFINITY;
+            any |= sees;
         }
+        mx = any ? kLeast : -INFINITY;
     }
-    float mx = x[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, x[i]);
+    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
     mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = fmaxf(mx, __shfl_xor(mx, 32)) * fac;
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mx = mx == -INFINITY ? mx : fmaxf(mx * fac, kLeast);
     const bool grew = mx > m + kLag;
     const float mn = grew ? mx : m;
     const float ref = mn == -INFINITY ? 0.0f : mn - kLift<CT>;
@@ -141,7 +146,7 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t,
     // The column of thread i is i / 16: this lane's own numbers come from the lane holding it.
     const int col = threadIdx.x >> 4, d = (threadIdx.x & 15) * VD;
     const int from = col;  // lanes 0..15 of any wavefront hold columns 0..15
-    const int row = __shfl(t.row, from), head = __shfl(t.head, from), pos = __shfl(t.pos, from);
+    const int row = __shfl(t.row, from), head = __shfl(t.head, from);
     const bool live = __shfl((int)t.live, from) != 0;
     __syncthreads();
     if (!live) return;
@@ -161,14 +166,12 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t,
     }
     if (t.splits == 1) {
         const float inv = 1.0f / L;
-        const bool empty = M == -INFINITY && !sees_any<16>(a, t.seq, a.window > 0 ? pos - a.window + 1 : 0, pos, c,
-                                                           0xFFFFull << (lane & 48));
         RT *out = (RT *)a.out + (int64_t)(t.start + row) * a.out_stride + head * HD + d;
 #pragma unroll
         for (int i = 0; i < VD; i += 4) {
             float w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = empty ? 0.0f : v[i + k] * inv;
+            for (int k = 0; k < 4; ++k) w[k] = M == -INFINITY ? 0.0f : v[i + k] * inv;
             store_vec(out + i, w);
         }
         return;
