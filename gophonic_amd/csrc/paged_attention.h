@@ -35,6 +35,7 @@ struct AttnArgs {
     int64_t q_stride, out_stride;
     int heads, group, window;
     int parts, small_parts, small_rows;
+    int row_tiles;         // the row kernel's grid has this many tiles for every row; 0: all tiles for every sequence
     int small_cols;        // sequences of at most this many columns are the row kernel's
     int big_tile;          // columns of the chunk kernel's tiles
     float q_sign;          // the sign of scale (0 if scale is 0), applied to the queries

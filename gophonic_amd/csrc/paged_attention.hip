@@ -53,6 +53,8 @@ struct AttnPlan {
     int small_cols, small_tiles, small_splits, small_len;  // small_tiles per sequence; 0: the row kernel is not run
     int big_tiles, big_splits, big_len;                    // big_tiles in all; 0: the chunk kernel is not run
     int small_rows;  // rows that a sequence of the row kernel may have; 0: split results kept by row
+    int row_tiles;   // tiles of a row; 0: the row kernel's grid is by sequence, small_tiles each
+    int64_t small_units;  // tiles of the row kernel's grid
 };
 
 // Keys per split of `span` keys and how many splits that makes, for about `want` of them.
@@ -96,8 +98,16 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         // up to 6000 106 and 149, thirty (fifteen) up to 3000 FP16 tokens 123 and 136.
         const bool mixed = cols > p.small_cols;
         const int64_t want = mixed ? 2 * cus / (units / p.small_tiles) : cus / units;
-        // The grid has a place for every sequence, with rows or without: no more splits than a launch takes.
-        const int64_t most = kMaxBlocks / (b.seqs * (int64_t)p.small_tiles * kv_heads);
+        // The grid is by sequence, or by row where a batch has more room for sequences than rows (one
+        // row of 40000 bfloat16 tokens, alone 26 us, among 2047 idle sequences 26 by row and 544 by
+        // sequence). No more splits than a launch takes.
+        const int64_t row_tiles = (group + kSmallTile - 1) / kSmallTile;
+        p.small_units = (int64_t)b.seqs * p.small_tiles;
+        if (rows * row_tiles < p.small_units) {
+            p.small_units = rows * row_tiles;
+            p.row_tiles = (int)row_tiles;
+        }
+        const int64_t most = kMaxBlocks / (p.small_units * kv_heads);
         cut(span(kSmallTile), brief ? 1 : std::min(want, most), p.small_len, p.small_splits);
         if ((int64_t)b.seqs * p.small_rows > rows) p.small_rows = 0;  // at most `rows` sequences have any
     }
@@ -241,7 +251,7 @@ int attend(const AttnArgs &a, const AttnPlan &p, int hd, hipStream_t st) {
 int plan_of(const AttnArgs &a, const gphq_paged_kv *kv, AttnPlan &p) {
     const int64_t kvh = a.pool.kv_heads;
     p = attn_plan(a.b, (int)kvh, a.group, a.window, a.big_tile, kv->dtype == GPHQ_DTYPE_F32);
-    if ((int64_t)a.b.seqs * p.small_tiles * p.small_splits * kvh > kMaxBlocks ||
+    if (p.small_units * p.small_splits * kvh > kMaxBlocks ||
         (int64_t)p.big_tiles * p.big_splits * kvh > kMaxBlocks)
         return GPHQ_ERR_PAGED_SHAPE;
     const bool join = small_count(p, a.b, a.heads) || big_count(p, a.b, a.heads);
@@ -307,6 +317,7 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     a.parts = big ? p.big_splits : 1;
     a.small_parts = small ? p.small_splits : 1;
     a.small_rows = p.small_rows;
+    a.row_tiles = p.row_tiles;
     a.part_o = (float *)work;
     a.small_o = a.part_o + big * hd;
     a.part_ml = a.small_o + small * hd;

@@ -617,8 +617,9 @@ int gphq_paged_append(const gphq_paged_kv *kv, const gphq_paged_batch *batch, in
  * with the values, an error of at most half a step of sum p |v|.
  * out may not overlap q (nor the pool). A batch of more blocks than a launch
  * takes is GPHQ_ERR_PAGED_SHAPE: with g = heads / kv_heads, where
- * kv_heads seqs ceil(min(max_rows g, 64) / 16) (g <= 64), or kv_heads times
- * about rows g / 128 (256 for fp32 rows; where max_rows g > 64), passes 2^23 - 1,
+ * kv_heads seqs ceil(min(max_rows g, 64) / 16) and kv_heads rows ceil(g / 16)
+ * (where g <= 64), or kv_heads times about rows g / 128 (256 for fp32 rows;
+ * where max_rows g > 64), pass 2^23 - 1,
  * or rows ceil(heads head_dim / 256) passes 2^26 - 1 in a batch whose keys are
  * split. work (16-byte aligned) of at least gphq_paged_attention_workspace_bytes
  * for the same pool, batch, row type, heads and window; its contents need not be

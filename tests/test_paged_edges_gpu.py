@@ -118,6 +118,45 @@ def test_few_rows_in_a_batch_of_many_sequences(seqs, live, spare, rt, ct):
     assert (got[b.starts[-1]:] == 7).all()
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(40, 1), (16, 1), (17, 1), (2, 2), (64, 1), (65, 1)])
+@pytest.mark.parametrize("rt,ct", [(F32, F16), (F32, F32)], ids=["f32-f16", "f32-f32"])
+def test_few_rows_of_every_group_size_among_idle_sequences(heads, kv_heads, rt, ct):
+    """Rows of one to five tiles each, of sequences of one to three rows."""
+    b = filled(idle(400, {3: (3, 700), 200: (1, 90), 399: (2, 1300)}), kv_heads, 64, 16, ct, seed=52)
+    q = (b.randn(b.rows, heads * 64) * 1.5).to(rt)
+    got = run(b, q, heads, 0.125)
+    check_rows(b, q, heads, 0.125, got, range(b.rows))
+
+
+@pytest.mark.parametrize("what", ["idle length", "live length", "descending starts", "rows past the end"])
+def test_bad_sequences_among_idle_ones_are_reported(what):
+    """As in a batch without idle sequences: the bad one is skipped and reported, rows of good ones are as they were."""
+    b = filled(idle(400, {3: (1, 700), 200: (1, 90), 399: (1, 1300)}), 2, 64, 16, F16, seed=53)
+    q = b.randn(b.rows, 8 * 64)
+    kv, dev = b.device(gphq)
+    if what == "idle length":
+        dev.lens[77] = 5000
+        good = [0, 1, 2]
+    elif what == "live length":
+        dev.lens[200] = -1
+        good = [0, 2]
+    elif what == "descending starts":
+        dev.starts[201] = 0  # sequence 200 ends before it starts, sequence 201 has two rows where one may be
+        good = [0, 2]
+    else:
+        dev.starts[400] = 9
+        good = [0, 1]
+    out = torch.full((b.rows, 8 * 64), 7.0, device="cuda")
+    gphq.paged_attention(kv, dev, q.cuda(), out, 8, 0.125)
+    with pytest.raises(gphq.GphqError) as e:
+        dev.check()
+    assert e.value.status == gphq.ERR_PAGED_BATCH
+    dev.check()
+    out = out.cpu()
+    check_rows(b, q, 8, 0.125, out, good)
+    assert (out[[r for r in range(3) if r not in good]] == 7).all()
+
+
 def test_a_batch_of_all_the_sequences_that_fit():
     """65536 sequences over one KV head, three of them with a row: the most that a batch may hold."""
     n, page, heads = 65536, 16, 4
