@@ -565,7 +565,7 @@ def _exact_plan(c, s):
         stack += table[i][left:t]
         taken[i] = left
     free[:len(stack)] = stack
-    starts, lens, short = [0], [], False
+    starts, lens, short, asked = [0], [], False, 0
     for i, n in enumerate(new):
         want = max(0, need[i] - taken[i])
         short |= want > len(stack)
@@ -575,7 +575,8 @@ def _exact_plan(c, s):
             for e in range(want):
                 table[i][taken[i] + e] = stack.pop()
             taken[i] += want
-        if starts[-1] + n > s["rows"]:
+        asked += n
+        if asked > s["rows"]:
             n = 0
         lens.append(held[i] + n)
         starts.append(starts[-1] + n)
