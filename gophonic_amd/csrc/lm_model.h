@@ -34,11 +34,13 @@ struct gphq_prefix {
     uint64_t gen = 0;
 };
 
-// gphq_paged_pool: one allocation each for keys and values, [layers][pages][kv_heads][page_tokens][head_dim].
+// gphq_paged_pool: one allocation each for keys and values, [layers][pages][kv_heads][page_tokens][head_dim], and
+// where those are 8-bit codes one for each's scales, [layers][pages][kv_heads][page_tokens / 16].
 struct gphq_paged_pool {
     const gphq_lm *lm;
     char *k = nullptr, *v = nullptr;
-    int64_t pages = 0, page_tokens = 0, layer_bytes = 0;
+    float *k_scales = nullptr, *v_scales = nullptr;
+    int64_t pages = 0, page_tokens = 0, layer_bytes = 0, layer_scales = 0;
     int dtype = 0;
 };
 

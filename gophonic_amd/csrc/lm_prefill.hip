@@ -767,9 +767,18 @@ struct PassKV {
 int paged_layer(gphq_prefill *ws, const PassPaged &p, int layer, hipStream_t st) {
     const gphq_lm *lm = ws->lm;
     const int64_t qkvw = lm->qd + 2 * lm->kvd;
+    const float *norms = lm->norms + (size_t)layer * 2 * kHeadDim;
+    if (p.pool->k_scales) {
+        gphq_paged8_kv kv;
+        GPHQ_TRY(gphq_paged_pool_layer8(p.pool, layer, &kv));
+        GPHQ_TRY(gphq_paged8_append(&kv, &p.batch, GPHQ_DTYPE_F32, ws->qkv, qkvw, lm->cfg.heads, norms,
+                                    norms + kHeadDim, lm->cfg.eps, lm->rope, lm->rope + lm->positions * 64,
+                                    lm->positions, (float)(1.0 / sqrt((double)lm->cfg.head_dim)), ws->qkv, qkvw, st));
+        return gphq_paged8_attention(&kv, &p.batch, GPHQ_DTYPE_F32, ws->qkv, qkvw, lm->cfg.heads, 1.0, 0, ws->ctx,
+                                     lm->qd, ws->attn, (int64_t)ws->attn_bytes, st);
+    }
     gphq_paged_kv kv;
     GPHQ_TRY(gphq_paged_pool_layer(p.pool, layer, &kv));
-    const float *norms = lm->norms + (size_t)layer * 2 * kHeadDim;
     GPHQ_TRY(gphq_paged_append(&kv, &p.batch, GPHQ_DTYPE_F32, ws->qkv, qkvw, lm->cfg.heads, norms, norms + kHeadDim,
                                lm->cfg.eps, lm->rope, lm->rope + lm->positions * 64, lm->positions,
                                (float)(1.0 / sqrt((double)lm->cfg.head_dim)), ws->qkv, qkvw, st));
@@ -1221,9 +1230,13 @@ int gphq_prefill_paged(gphq_prefill *ws, gphq_paged_pool *pool, const int32_t *t
         paged.batch.rows = R;
         paged.batch.max_rows = max_rows;
         paged.batch.max_len = max_len;
+        gphq_paged8_kv kv8;
         gphq_paged_kv kv;
-        GPHQ_TRY(gphq_paged_pool_layer(pool, 0, &kv));
-        const int64_t need = gphq_paged_attention_workspace_bytes(&kv, &paged.batch, GPHQ_DTYPE_F32, c.heads, 0);
+        GPHQ_TRY(pool->k_scales ? gphq_paged_pool_layer8(pool, 0, &kv8) : gphq_paged_pool_layer(pool, 0, &kv));
+        const int64_t need =
+            pool->k_scales
+                ? gphq_paged8_attention_workspace_bytes(&kv8, &paged.batch, GPHQ_DTYPE_F32, c.heads, 0)
+                : gphq_paged_attention_workspace_bytes(&kv, &paged.batch, GPHQ_DTYPE_F32, c.heads, 0);
         if (need < 0) return (int)need;
         GPHQ_TRY(grow(ws->attn, ws->attn_bytes, (size_t)need));
         GPHQ_TRY(hip_status(hipMemcpyAsync(ws->seqs, ints.data(), ints.size() * 4, hipMemcpyHostToDevice, st)));

@@ -6,7 +6,7 @@
 namespace gphq {
 
 // Bits a kernel sets in a batch's bad word.
-enum { PAGED_BAD_SEQ = 1, PAGED_BAD_PAGE = 2, PAGED_BAD_POSITION = 4 };
+enum { PAGED_BAD_SEQ = 1, PAGED_BAD_PAGE = 2, PAGED_BAD_POSITION = 4, PAGED_BAD_VALUE = 8, PAGED_NO_PAGES = 16 };
 
 typedef __bf16 bf16;
 typedef _Float16 f16;

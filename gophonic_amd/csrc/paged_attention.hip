@@ -1,25 +1,26 @@
-// gphq_paged_attention: argument checks, the cut of a batch into tiles and splits, and the
-// join of split results. Kernels: paged_rows.hip and paged_chunk.hip.
+// gphq_paged_attention and gphq_paged8_attention: argument checks, the cut of a batch into tiles
+// and splits, and the join of split results. Kernels: paged_rows.hip and paged_chunk.hip,
+// paged8_rows.hip and paged8_chunk.hip.
 #include <math.h>
 
 #include <new>
 
 #include "lm_model.h"
-#include "paged_attention.h"
+#include "paged8.h"
 
 namespace gphq {
 
-int paged_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, PagedPool &pool, PagedBatch &batch) {
-    if (!kv || !b) return GPHQ_ERR_PAGED_SHAPE;
-    if (kv->dtype != GPHQ_DTYPE_F32 && kv->dtype != GPHQ_DTYPE_F16 && kv->dtype != GPHQ_DTYPE_BF16)
-        return GPHQ_ERR_UNSUPPORTED;
+namespace {
+
+// Checks of a pool whose values have `size` bytes, and of a batch.
+int pool_args(const gphq_paged_kv *kv, int64_t size, const gphq_paged_batch *b, PagedPool &pool, PagedBatch &batch) {
     if (kv->head_dim != 64 && kv->head_dim != 128) return GPHQ_ERR_UNSUPPORTED;
     if (kv->page_tokens < 16 || kv->page_tokens > GPHQ_PAGED_MAX_PAGE_TOKENS ||
         (kv->page_tokens & (kv->page_tokens - 1)))
         return GPHQ_ERR_UNSUPPORTED;
     if (kv->pages < 1 || kv->pages > INT32_MAX || kv->kv_heads < 1 || kv->kv_heads > GPHQ_PAGED_MAX_HEADS)
         return GPHQ_ERR_PAGED_SHAPE;
-    const int64_t size = kv->dtype == GPHQ_DTYPE_F32 ? 4 : 2, unit = 16 / size;
+    const int64_t unit = 16 / size;
     for (const int64_t s : {kv->page_stride, kv->token_stride, kv->head_stride})
         if (s < kv->head_dim || s % unit || s > INT64_MAX / (size * kv->pages)) return GPHQ_ERR_PAGED_SHAPE;
     if (kv->token_stride > INT32_MAX / (kv->page_tokens * size)) return GPHQ_ERR_PAGED_SHAPE;  // a page under 2 GiB
@@ -41,6 +42,28 @@ int paged_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, PagedPool &po
                        b->table_stride, (int)b->seqs, (int)b->rows, (int)std::min(b->max_rows, b->rows),
                        (int)b->max_len};
     if (batch.seqs == 0 || batch.max_rows == 0) batch.rows = 0;  // nothing to do
+    return GPHQ_OK;
+}
+
+}  // namespace
+
+int paged_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, PagedPool &pool, PagedBatch &batch) {
+    if (!kv || !b) return GPHQ_ERR_PAGED_SHAPE;
+    if (kv->dtype != GPHQ_DTYPE_F32 && kv->dtype != GPHQ_DTYPE_F16 && kv->dtype != GPHQ_DTYPE_BF16)
+        return GPHQ_ERR_UNSUPPORTED;
+    return pool_args(kv, kv->dtype == GPHQ_DTYPE_F32 ? 4 : 2, b, pool, batch);
+}
+
+int paged8_args(const gphq_paged8_kv *kv, const gphq_paged_batch *b, PagedPool &pool, Paged8Scales &scales,
+                PagedBatch &batch) {
+    if (!kv || !b) return GPHQ_ERR_PAGED_SHAPE;
+    if (kv->codes.dtype != GPHQ_DTYPE_I8 && kv->codes.dtype != GPHQ_DTYPE_E4M3) return GPHQ_ERR_UNSUPPORTED;
+    GPHQ_TRY(pool_args(&kv->codes, 1, b, pool, batch));
+    for (const int64_t s : {kv->scale_page_stride, kv->scale_head_stride})
+        if (s < kv->codes.page_tokens / kBlockTokens || s > INT64_MAX / (4 * kv->codes.pages)) return GPHQ_ERR_PAGED_SHAPE;
+    if (!kv->k_scales_dev || !kv->v_scales_dev || ((uintptr_t)kv->k_scales_dev | (uintptr_t)kv->v_scales_dev) % 4)
+        return GPHQ_ERR_PAGED_SHAPE;
+    scales = Paged8Scales{kv->k_scales_dev, kv->v_scales_dev, kv->scale_page_stride, kv->scale_head_stride};
     return GPHQ_OK;
 }
 
@@ -247,6 +270,15 @@ int attend(const AttnArgs &a, const AttnPlan &p, int hd, hipStream_t st) {
     return hd == 128 ? join_launch<RT, 128>(a, st) : join_launch<RT, 64>(a, st);
 }
 
+template <typename RT, typename C>
+int attend8(const Attn8Args &e, const AttnPlan &p, int hd, hipStream_t st) {
+    const AttnArgs &a = e.a;
+    if (p.big_tiles) GPHQ_TRY((attn8_chunk_launch<RT, C>(e, hd, p.big_splits, p.big_tiles, st)));
+    if (p.small_tiles) GPHQ_TRY((attn8_rows_launch<RT, C>(e, hd, p.small_splits, p.small_tiles, st)));
+    if (!small_count(p, a.b, a.heads) && !big_count(p, a.b, a.heads)) return GPHQ_OK;
+    return hd == 128 ? join_launch<RT, 128>(a, st) : join_launch<RT, 64>(a, st);
+}
+
 // The call's cut, refused where a launch would have too many blocks.
 int plan_of(const AttnArgs &a, const gphq_paged_kv *kv, AttnPlan &p) {
     const int64_t kvh = a.pool.kv_heads;
@@ -259,15 +291,20 @@ int plan_of(const AttnArgs &a, const gphq_paged_kv *kv, AttnPlan &p) {
     return join && join_units(a.b, a.heads, (int)kv->head_dim) / 8 > kMaxBlocks ? GPHQ_ERR_PAGED_SHAPE : GPHQ_OK;
 }
 
+int head_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, int64_t heads, int64_t window, AttnArgs &a) {
+    if (heads < 1 || heads > GPHQ_PAGED_MAX_HEADS || heads % kv->kv_heads || window < 0) return GPHQ_ERR_PAGED_SHAPE;
+    a.heads = (int)heads;
+    a.group = (int)(heads / kv->kv_heads);
+    a.window = window >= b->max_len ? 0 : (int)window;  // a window as long as any sequence hides nothing
+    return GPHQ_OK;
+}
+
 // The checks that the attention and its workspace size share.
 int attn_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, int row_dtype, int64_t heads, int64_t window,
               AttnArgs &a) {
     GPHQ_TRY(paged_args(kv, b, a.pool, a.b));
     if (row_dtype != GPHQ_DTYPE_F32 && row_dtype != kv->dtype) return GPHQ_ERR_UNSUPPORTED;
-    if (heads < 1 || heads > GPHQ_PAGED_MAX_HEADS || heads % kv->kv_heads || window < 0) return GPHQ_ERR_PAGED_SHAPE;
-    a.heads = (int)heads;
-    a.group = (int)(heads / kv->kv_heads);
-    a.window = window >= b->max_len ? 0 : (int)window;  // a window as long as any sequence hides nothing
+    GPHQ_TRY(head_args(kv, b, heads, window, a));
     const bool f16c = kv->dtype == GPHQ_DTYPE_F16;
     a.big_tile = 32 * (kv->dtype == GPHQ_DTYPE_F32 ? kChunkWaves<float, float>
                        : row_dtype == kv->dtype    ? (f16c ? kChunkWaves<f16, f16> : kChunkWaves<bf16, bf16>)
@@ -275,29 +312,27 @@ int attn_args(const gphq_paged_kv *kv, const gphq_paged_batch *b, int row_dtype,
     return GPHQ_OK;
 }
 
-}  // namespace
-}  // namespace gphq
+int attn8_args(const gphq_paged8_kv *kv, const gphq_paged_batch *b, int row_dtype, int64_t heads, int64_t window,
+               Attn8Args &e) {
+    GPHQ_TRY(paged8_args(kv, b, e.a.pool, e.s, e.a.b));
+    if (row_dtype != GPHQ_DTYPE_F32 && row_dtype != GPHQ_DTYPE_F16 && row_dtype != GPHQ_DTYPE_BF16)
+        return GPHQ_ERR_UNSUPPORTED;
+    GPHQ_TRY(head_args(&kv->codes, b, heads, window, e.a));
+    e.a.big_tile = 32 * (row_dtype == GPHQ_DTYPE_F32 ? kChunkWaves<float, f16> : kChunkWaves<f16, f16>);
+    return GPHQ_OK;
+}
 
-using namespace gphq;
-
-extern "C" {
-
-int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype,
-                                             int64_t heads, int64_t window) {
-    AttnArgs a{};
-    GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
+int64_t work_bytes_of(const AttnArgs &a, const gphq_paged_kv *kv) {
     if (a.b.rows == 0) return 0;
     AttnPlan p;
     GPHQ_TRY(plan_of(a, kv, p));
-    return (small_count(p, a.b, heads) + big_count(p, a.b, heads)) * (kv->head_dim + 2) * 4;
+    return (small_count(p, a.b, a.heads) + big_count(p, a.b, a.heads)) * (kv->head_dim + 2) * 4;
 }
 
-int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
-                         int64_t q_stride, int64_t heads, double scale, int64_t window, void *out, int64_t out_stride,
-                         void *work, int64_t work_bytes, void *stream) {
-    AttnArgs a{};
-    GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
-    const int64_t hd = kv->head_dim, size = row_dtype == GPHQ_DTYPE_F32 ? 4 : 2;
+// The rest of a call's checks and arguments; `p` is its cut. A batch without rows leaves a.b.rows 0.
+int call_args(const gphq_paged_kv *kv, int64_t size, const void *q, int64_t q_stride, double scale, void *out,
+              int64_t out_stride, void *work, int64_t work_bytes, AttnArgs &a, AttnPlan &p) {
+    const int64_t hd = kv->head_dim, heads = a.heads;
     if (!(fabs(scale) <= 1e30) || q_stride < heads * hd || out_stride < heads * hd || q_stride * size % 16 || out_stride * size % 16)
         return GPHQ_ERR_PAGED_SHAPE;
     if (a.b.rows == 0) return GPHQ_OK;
@@ -305,7 +340,6 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     if (spans_overlap(q, span_bytes(a.b.rows, q_stride, heads * hd, size), out,
                       span_bytes(a.b.rows, out_stride, heads * hd, size)))
         return GPHQ_ERR_OVERLAP;
-    AttnPlan p;
     GPHQ_TRY(plan_of(a, kv, p));
     const int64_t big = big_count(p, a.b, heads), small = small_count(p, a.b, heads);
     if (big + small && (!work || (uintptr_t)work % 16 || work_bytes < (big + small) * (hd + 2) * 4))
@@ -327,6 +361,32 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     a.split_big = p.big_len;
     a.q_sign = scale > 0 ? 1.0f : scale < 0 ? -1.0f : 0.0f;
     a.scale_log2 = scale == 0 ? 1.0f : (float)(fabs(scale) * 1.4426950408889634);
+    return GPHQ_OK;
+}
+
+}  // namespace
+}  // namespace gphq
+
+using namespace gphq;
+
+extern "C" {
+
+int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype,
+                                             int64_t heads, int64_t window) {
+    AttnArgs a{};
+    GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
+    return work_bytes_of(a, kv);
+}
+
+int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
+                         int64_t q_stride, int64_t heads, double scale, int64_t window, void *out, int64_t out_stride,
+                         void *work, int64_t work_bytes, void *stream) {
+    AttnArgs a{};
+    GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
+    AttnPlan p;
+    GPHQ_TRY(call_args(kv, row_dtype == GPHQ_DTYPE_F32 ? 4 : 2, q, q_stride, scale, out, out_stride, work, work_bytes, a, p));
+    if (a.b.rows == 0) return GPHQ_OK;
+    const int64_t hd = kv->head_dim;
     hipStream_t st = (hipStream_t)stream;
     if (row_dtype == GPHQ_DTYPE_F32) {
         if (kv->dtype == GPHQ_DTYPE_F32) return attend<float, float>(a, p, (int)hd, st);
@@ -337,16 +397,44 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     return attend<bf16, bf16>(a, p, (int)hd, st);
 }
 
+int64_t gphq_paged8_attention_workspace_bytes(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype,
+                                              int64_t heads, int64_t window) {
+    Attn8Args e{};
+    GPHQ_TRY(attn8_args(kv, batch, row_dtype, heads, window, e));
+    return work_bytes_of(e.a, &kv->codes);
+}
+
+int gphq_paged8_attention(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
+                          int64_t q_stride, int64_t heads, double scale, int64_t window, void *out, int64_t out_stride,
+                          void *work, int64_t work_bytes, void *stream) {
+    Attn8Args e{};
+    GPHQ_TRY(attn8_args(kv, batch, row_dtype, heads, window, e));
+    AttnPlan p;
+    GPHQ_TRY(call_args(&kv->codes, row_dtype == GPHQ_DTYPE_F32 ? 4 : 2, q, q_stride, scale, out, out_stride, work,
+                       work_bytes, e.a, p));
+    if (e.a.b.rows == 0) return GPHQ_OK;
+    const int hd = (int)kv->codes.head_dim;
+    hipStream_t st = (hipStream_t)stream;
+    const bool i8 = kv->codes.dtype == GPHQ_DTYPE_I8;
+    if (row_dtype == GPHQ_DTYPE_F32)
+        return i8 ? attend8<float, CodesI8>(e, p, hd, st) : attend8<float, CodesE4M3>(e, p, hd, st);
+    if (row_dtype == GPHQ_DTYPE_F16)
+        return i8 ? attend8<f16, CodesI8>(e, p, hd, st) : attend8<f16, CodesE4M3>(e, p, hd, st);
+    return i8 ? attend8<bf16, CodesI8>(e, p, hd, st) : attend8<bf16, CodesE4M3>(e, p, hd, st);
+}
+
 int gphq_paged_pool_new(const gphq_lm *lm, int64_t pages, int64_t page_tokens, int dtype, gphq_paged_pool **out) {
     if (!out) return GPHQ_ERR_DIMENSIONS;
     *out = nullptr;
     if (!lm) return GPHQ_ERR_WORKSPACE;
-    if (dtype != GPHQ_DTYPE_F32 && dtype != GPHQ_DTYPE_F16 && dtype != GPHQ_DTYPE_BF16) return GPHQ_ERR_UNSUPPORTED;
+    const bool codes = dtype == GPHQ_DTYPE_I8 || dtype == GPHQ_DTYPE_E4M3;
+    if (dtype != GPHQ_DTYPE_F32 && dtype != GPHQ_DTYPE_F16 && dtype != GPHQ_DTYPE_BF16 && !codes)
+        return GPHQ_ERR_UNSUPPORTED;
     if (page_tokens < 16 || page_tokens > GPHQ_PAGED_MAX_PAGE_TOKENS || (page_tokens & (page_tokens - 1)))
         return GPHQ_ERR_UNSUPPORTED;
     if (pages < 1 || pages > INT32_MAX) return GPHQ_ERR_PAGED_SHAPE;
     const gphq_lm_config &c = lm->cfg;
-    const int64_t token = lm->kvd * (dtype == GPHQ_DTYPE_F32 ? 4 : 2);
+    const int64_t token = lm->kvd * (dtype == GPHQ_DTYPE_F32 ? 4 : codes ? 1 : 2);
     if (pages > INT64_MAX / (token * page_tokens * c.layers)) return GPHQ_ERR_PAGED_SHAPE;
     gphq_paged_pool *p = new (std::nothrow) gphq_paged_pool();
     if (!p) return GPHQ_ERR_SCRATCH_LIMIT;
@@ -357,6 +445,11 @@ int gphq_paged_pool_new(const gphq_lm *lm, int64_t pages, int64_t page_tokens, i
     p->layer_bytes = token * page_tokens * pages;
     hipError_t e = hipMalloc((void **)&p->k, (size_t)(p->layer_bytes * c.layers));
     if (e == hipSuccess) e = hipMalloc((void **)&p->v, (size_t)(p->layer_bytes * c.layers));
+    if (codes) {
+        p->layer_scales = pages * c.kv_heads * (page_tokens / kBlockTokens);
+        if (e == hipSuccess) e = hipMalloc((void **)&p->k_scales, (size_t)(p->layer_scales * c.layers * 4));
+        if (e == hipSuccess) e = hipMalloc((void **)&p->v_scales, (size_t)(p->layer_scales * c.layers * 4));
+    }
     if (e != hipSuccess) {
         gphq_paged_pool_free(p);
         return hip_status(e);
@@ -369,6 +462,8 @@ void gphq_paged_pool_free(gphq_paged_pool *p) {
     if (!p) return;
     if (p->k) (void)hipFree(p->k);
     if (p->v) (void)hipFree(p->v);
+    if (p->k_scales) (void)hipFree(p->k_scales);
+    if (p->v_scales) (void)hipFree(p->v_scales);
     delete p;
 }
 
@@ -390,6 +485,17 @@ int gphq_paged_pool_layer(const gphq_paged_pool *p, int64_t layer, gphq_paged_kv
     return GPHQ_OK;
 }
 
+int gphq_paged_pool_layer8(const gphq_paged_pool *p, int64_t layer, gphq_paged8_kv *out) {
+    if (!p || !out) return GPHQ_ERR_PAGED_SHAPE;
+    if (!p->k_scales) return GPHQ_ERR_UNSUPPORTED;
+    GPHQ_TRY(gphq_paged_pool_layer(p, layer, &out->codes));
+    out->k_scales_dev = p->k_scales + layer * p->layer_scales;
+    out->v_scales_dev = p->v_scales + layer * p->layer_scales;
+    out->scale_head_stride = p->page_tokens / kBlockTokens;
+    out->scale_page_stride = out->scale_head_stride * p->lm->cfg.kv_heads;
+    return GPHQ_OK;
+}
+
 int gphq_paged_check(int32_t *bad_dev, void *stream) {
     if (!bad_dev) return GPHQ_ERR_PAGED_SHAPE;
     // All on the caller's stream: a call that follows on it finds the word cleared, not about to be.
@@ -400,7 +506,9 @@ int gphq_paged_check(int32_t *bad_dev, void *stream) {
     if (!bad) return GPHQ_OK;
     hipLaunchKernelGGL(paged_clear_kernel, dim3(1), dim3(1), 0, st, bad_dev, bad);
     GPHQ_TRY(launch_status());
-    return GPHQ_ERR_PAGED_BATCH;
+    if (bad & (PAGED_BAD_SEQ | PAGED_BAD_PAGE | PAGED_BAD_POSITION)) return GPHQ_ERR_PAGED_BATCH;
+    if (bad & PAGED_BAD_VALUE) return GPHQ_ERR_NON_FINITE;
+    return bad & PAGED_NO_PAGES ? GPHQ_ERR_PREFIX_FULL : GPHQ_ERR_PAGED_BATCH;
 }
 
 }  // extern "C"

@@ -1,0 +1,455 @@
+// gphq_probabilities and gphq_verify_drafts: from a head's logits to the tokens that a step keeps.
+#include <float.h>
+
+#include "paged.h"
+
+namespace gphq {
+namespace {
+
+constexpr int kThreads = 256, kPer = 16, kTile = kThreads * kPer;  // values of a row that a block takes at once
+
+// N neighbouring values from i on of a row of n: 16 bytes at a time where rows allow it (VEC).
+template <bool VEC, int N>
+__device__ __forceinline__ void load_row(const float *x, int i, int n, float fill, float (&v)[N]) {
+    if (VEC && i + N <= n) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {
+            const f32x4 q = *(const f32x4 *)(x + i + k);
+            v[k] = q.x, v[k + 1] = q.y, v[k + 2] = q.z, v[k + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = i + k < n ? x[i + k] : fill;
+    }
+}
+
+// ---- probabilities --------------------------------------------------------------
+
+struct ProbArgs {
+    const float *x, *temperatures;
+    float *out;
+    float2 *part;  // [rows][parts]: (largest, sum of exponentials against it), or (largest, its index) at t = 0
+    int64_t x_stride, out_stride;
+    int rows, n, parts, len;  // len: values of a part, a multiple of kTile
+};
+
+// log2(e) / t, 0 for a row that takes its largest value alone.
+__device__ __forceinline__ float rate_of(const ProbArgs &a, int row) {
+    const float t = a.temperatures ? a.temperatures[row] : 1.0f;
+    return t > 0.0f ? fminf(fmaxf(1.44269504088896340736f / t, FLT_MIN), FLT_MAX) : 0.0f;
+}
+
+// Joins two (largest, sum) pairs.
+__device__ __forceinline__ void join_sums(float &m, float &s, float m2, float s2, float rate) {
+    const float mx = fmaxf(m, m2), ref = mx == -INFINITY ? 0.0f : mx;
+    s = s * __builtin_amdgcn_exp2f((m - ref) * rate) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * rate);
+    m = mx;
+}
+// Joins two (largest, first index of it) pairs.
+__device__ __forceinline__ void join_first(float &m, int &i, float m2, int i2) {
+    if (m2 > m || (m2 == m && i2 < i)) m = m2, i = i2;
+}
+
+// A block's pairs to one, in a fixed order; the same in every thread.
+__device__ __forceinline__ void block_join(float &m, float &s, int &first, float rate) {
+    __shared__ float sm[4], ss[4];
+    __shared__ int si[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
+        const int i2 = __shfl_xor(first, d);
+        if (rate > 0.0f)
+            join_sums(m, s, m2, s2, rate);
+        else
+            join_first(m, first, m2, i2);
+    }
+    if (lane == 0) sm[wave] = m, ss[wave] = s, si[wave] = first;
+    __syncthreads();
+    m = sm[0], s = ss[0], first = si[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+        if (rate > 0.0f)
+            join_sums(m, s, sm[w], ss[w], rate);
+        else
+            join_first(m, first, sm[w], si[w]);
+    }
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void prob_parts_kernel(const ProbArgs a) {
+    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    const float *x = a.x + (int64_t)row * a.x_stride;
+    const float rate = rate_of(a, row);
+    const int end = min(a.n, (part + 1) * a.len);
+    float m = -INFINITY, s = 0.0f;
+    int first = INT32_MAX;
+    for (int i0 = part * a.len; i0 < end; i0 += kTile) {
+        float v[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; k += 4) {
+            float q[4];
+            load_row<VEC>(x, i0 + k * kThreads + 4 * threadIdx.x, end, -INFINITY, q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k + e] = q[e];
+        }
+        if (rate > 0.0f) {
+            float mx = m, sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) mx = fmaxf(mx, v[k]);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) sum += __builtin_amdgcn_exp2f((v[k] - ref) * rate);
+            s = s * __builtin_amdgcn_exp2f((m - ref) * rate) + sum;
+            m = mx;
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k)
+                if (v[k] > m) m = v[k], first = i0 + k / 4 * 4 * kThreads + 4 * threadIdx.x + k % 4;
+        }
+    }
+    block_join(m, s, first, rate);
+    if (threadIdx.x == 0) a.part[blockIdx.x] = make_float2(m, rate > 0.0f ? s : __builtin_bit_cast(float, first));
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void prob_write_kernel(const ProbArgs a) {
+    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    const float *x = a.x + (int64_t)row * a.x_stride;
+    float *out = a.out + (int64_t)row * a.out_stride;
+    const float rate = rate_of(a, row);
+    float m = -INFINITY, s = 0.0f;
+    int first = INT32_MAX;
+    for (int p = threadIdx.x; p < a.parts; p += kThreads) {
+        const float2 q = a.part[(int64_t)row * a.parts + p];
+        if (rate > 0.0f)
+            join_sums(m, s, q.x, q.y, rate);
+        else
+            join_first(m, first, q.x, __builtin_bit_cast(int, q.y));
+    }
+    block_join(m, s, first, rate);
+    const float ref = m == -INFINITY ? 0.0f : m, inv = s == 0.0f ? 0.0f : 1.0f / s;
+    const int end = min(a.n, (part + 1) * a.len);
+    for (int i0 = part * a.len; i0 < end; i0 += kTile) {
+#pragma unroll
+        for (int k = 0; k < kPer; k += 4) {
+            const int i = i0 + k * kThreads + 4 * threadIdx.x;
+            float q[4];
+            if (rate > 0.0f) {
+                load_row<VEC>(x, i, end, 0.0f, q);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[e] = __builtin_amdgcn_exp2f((q[e] - ref) * rate) * inv;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[e] = i + e == first ? 1.0f : 0.0f;
+            }
+            if (VEC && i + 4 <= end) {
+                *(f32x4 *)(out + i) = f32x4{q[0], q[1], q[2], q[3]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + e < end) out[i + e] = q[e];
+            }
+        }
+    }
+}
+
+// Parts of a row: about 2048 blocks in all.
+void prob_cut(int64_t rows, int64_t n, int &len, int &parts) {
+    const int64_t tiles = (n + kTile - 1) / kTile, per = std::max<int64_t>(1, tiles * rows / 2048);
+    len = (int)(std::min(per, tiles) * kTile);
+    parts = (int)((n + len - 1) / len);
+}
+
+// ---- drafts ---------------------------------------------------------------------
+
+struct VerifyArgs {
+    const int32_t *starts, *drafts, *lens;
+    const float *target, *draft, *accept_u, *sample_u;
+    int32_t *tokens, *accepted, *kept, *decided;  // decided: [seqs], of the workspace
+    double2 *sums;                                // [seqs][tiles]: of w, and of the target's row
+    int64_t target_stride, draft_stride;
+    int seqs, rows, n, tiles;
+};
+
+__device__ __forceinline__ double shfl_up_f64(double v, int d) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __shfl_up((int)(uint32_t)u, d), hi = __shfl_up((int)(uint32_t)(u >> 32), d);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Sum over the threads up to this one of a block, and over all, in a fixed order.
+__device__ __forceinline__ double block_scan(double v, double &total) {
+    __shared__ double lds[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double u = shfl_up_f64(v, d);
+        if (lane >= d) v += u;
+    }
+    __syncthreads();  // lds of the last scan has been read
+    if (lane == 63) lds[wave] = v;
+    __syncthreads();
+    double before = 0.0;
+    for (int w = 0; w < wave; ++w) before += lds[w];
+    total = lds[0] + lds[1] + lds[2] + lds[3];
+    return before + v;
+}
+
+__device__ __forceinline__ double weight(double v) { return v > 0.0 ? v : 0.0; }
+
+// This thread's kPer neighbouring weights of a tile: w, and the target's alone.
+struct Row {
+    const float *p, *q;  // q NULL: certain of x
+    int x;               // the draft; -1: w is the target's row
+};
+template <bool VEC>
+__device__ __forceinline__ void tile_weights(const VerifyArgs &a, const Row &r, int tile, double (&w)[kPer],
+                                             double (&t)[kPer]) {
+    const int i = tile * kTile + kPer * threadIdx.x;
+    float p[kPer], q[kPer];
+    load_row<VEC>(r.p, i, a.n, 0.0f, p);
+    if (r.q) load_row<VEC>(r.q, i, a.n, 0.0f, q);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        t[k] = weight(p[k]);
+        w[k] = r.x < 0 ? t[k] : r.q ? weight((double)p[k] - (double)q[k]) : i + k == r.x ? 0.0 : t[k];
+    }
+}
+
+__device__ __forceinline__ Row row_at(const VerifyArgs &a, int row, int last) {
+    Row r{a.target + (int64_t)row * a.target_stride, nullptr, -1};
+    if (row == last) return r;
+    const int x = a.drafts[row];
+    if (x < 0 || x >= a.n) return r;
+    r.x = x;
+    if (a.draft) r.q = a.draft + (int64_t)row * a.draft_stride;
+    return r;
+}
+
+// A sequence's rows [first, last]; false for one that has none or whose starts are bad.
+__device__ __forceinline__ bool rows_of(const VerifyArgs &a, int s, int &first, int &last) {
+    first = a.starts[s];
+    last = a.starts[s + 1] - 1;
+    return first >= 0 && last >= first && last < a.rows;
+}
+
+// The first row of [first, last) whose draft is not accepted, last if there is none; by each wavefront.
+__device__ __forceinline__ int decide(const VerifyArgs &a, int first, int last) {
+    const int lane = threadIdx.x & 63;
+    for (int r0 = first; r0 < last; r0 += 64) {
+        const int r = r0 + lane;
+        bool fails = false;
+        if (r < last) {
+            const int x = a.drafts[r];
+            const bool in = x >= 0 && x < a.n;
+            const double p = in ? a.target[(int64_t)r * a.target_stride + x] : 0.0;
+            const double q = !a.draft ? 1.0 : in ? a.draft[(int64_t)r * a.draft_stride + x] : 0.0;
+            fails = !in || !((double)a.accept_u[r] * q < p);
+        }
+        const uint64_t b = __ballot(fails);
+        if (b) return r0 + __builtin_ctzll(b);
+    }
+    return last;
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs a) {
+    const int s = blockIdx.x / a.tiles, tile = blockIdx.x - s * a.tiles;
+    int first, last;
+    if (!rows_of(a, s, first, last)) return;
+    const int row = decide(a, first, last);
+    const Row r = row_at(a, row, last);
+    double w[kPer], t[kPer], ws = 0.0, ts = 0.0;
+    tile_weights<VEC>(a, r, tile, w, t);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) ws += w[k], ts += t[k];
+    double wt, tt;
+    block_scan(ws, wt);
+    block_scan(ts, tt);
+    if (threadIdx.x == 0) {
+        a.sums[blockIdx.x] = double2{wt, tt};
+        if (tile == 0) a.decided[s] = row;
+    }
+}
+
+// One block a sequence: the tile in which the sum passes the number, then the token in it.
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyArgs a) {
+    const int s = blockIdx.x, tid = threadIdx.x;
+    int first, last;
+    if (!rows_of(a, s, first, last)) {
+        if (tid == 0) {
+            a.accepted[s] = first >= 0 && last == first - 1 && first <= a.rows ? 0 : -1;
+            if (a.kept) a.kept[s] = a.lens[s];
+        }
+        return;
+    }
+    const int row = a.decided[s];
+    Row r = row_at(a, row, last);
+    const double2 *sums = a.sums + (int64_t)s * a.tiles;
+    // Each thread sums a run of neighbouring tiles.
+    const int run = (a.tiles + kThreads - 1) / kThreads, t0 = min(tid * run, a.tiles), t1 = min(t0 + run, a.tiles);
+    double ws = 0.0, ts = 0.0, wt, tt;
+    for (int i = t0; i < t1; ++i) ws += sums[i].x, ts += sums[i].y;
+    double at = block_scan(ws, wt);
+    const double at_t = block_scan(ts, tt);
+    if (wt == 0.0) {  // no weight left: the target's row
+        r.x = -1;
+        at = at_t;
+        ws = ts;
+        wt = tt;
+    }
+    const float u = a.sample_u[s];
+    const double goal = (double)(u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f) * wt;
+    __shared__ int found, fallback;
+    if (tid == 0) found = INT32_MAX, fallback = -1;
+    __syncthreads();
+    double sum = at - ws;
+    for (int i = t0; i < t1; ++i) {
+        const double v = r.x < 0 ? sums[i].y : sums[i].x;
+        sum += v;
+        if (v > 0.0) {
+            if (sum > goal) atomicMin(&found, i);
+            atomicMax(&fallback, i);
+        }
+    }
+    __syncthreads();
+    const int tile = found < INT32_MAX ? found : fallback;
+    const bool any = found < INT32_MAX;
+    // The sum before that tile, from the thread that holds it.
+    __shared__ double before;
+    if (tile >= t0 && tile < t1) {
+        double b = at - ws;
+        for (int i = t0; i < tile; ++i) b += r.x < 0 ? sums[i].y : sums[i].x;
+        before = b;
+    }
+    __syncthreads();
+    int token = 0;
+    if (tile >= 0) {
+        const double b = before;
+        double w[kPer], t[kPer], mine = 0.0, total;
+        tile_weights<VEC>(a, r, tile, w, t);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) mine += w[k];
+        double c = b + (block_scan(mine, total) - mine);
+        if (tid == 0) found = INT32_MAX, fallback = -1;
+        __syncthreads();
+        int hit = INT32_MAX, end = -1;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            c += w[k];
+            if (w[k] > 0.0) {
+                end = tile * kTile + kPer * tid + k;
+                if (any && c > goal && hit == INT32_MAX) hit = end;
+            }
+        }
+        if (hit < INT32_MAX) atomicMin(&found, hit);
+        if (end >= 0) atomicMax(&fallback, end);
+        __syncthreads();
+        token = found < INT32_MAX ? found : max(fallback, 0);
+    }
+    for (int i = first + tid; i <= last; i += kThreads) {
+        const int v = i < row ? a.drafts[i] : i == row ? token : -1;
+        a.tokens[i] = v;
+    }
+    if (tid == 0) {
+        a.accepted[s] = row - first;
+        if (a.kept) a.kept[s] = a.lens[s] - (last - row);
+    }
+}
+
+int verify_tiles(int64_t n) { return (int)((n + kTile - 1) / kTile); }
+
+bool rows16(const void *p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 4 == 0; }
+
+}  // namespace
+}  // namespace gphq
+
+using namespace gphq;
+
+extern "C" {
+
+int64_t gphq_probabilities_workspace_bytes(int64_t rows, int64_t vocab) {
+    if (rows < 0 || rows > GPHQ_SAMPLE_MAX_ROWS || vocab < 0 || vocab > GPHQ_SAMPLE_MAX_VOCAB)
+        return GPHQ_ERR_DIMENSIONS;
+    if (rows == 0 || vocab == 0) return 0;
+    int len, parts;
+    prob_cut(rows, vocab, len, parts);
+    return (rows * parts * (int64_t)sizeof(float2) + 15) / 16 * 16;
+}
+
+int gphq_probabilities(const float *x, int64_t x_stride, const float *temperatures, float *out, int64_t out_stride,
+                       int64_t rows, int64_t vocab, void *work, int64_t work_bytes, void *stream) {
+    const int64_t need = gphq_probabilities_workspace_bytes(rows, vocab);
+    if (need < 0) return (int)need;
+    if (x_stride < vocab || out_stride < vocab || x_stride > INT64_MAX / 8 / GPHQ_SAMPLE_MAX_ROWS ||
+        out_stride > INT64_MAX / 8 / GPHQ_SAMPLE_MAX_ROWS)
+        return GPHQ_ERR_DIMENSIONS;
+    if (need == 0) return GPHQ_OK;
+    if (!x || !out || ((uintptr_t)x | (uintptr_t)out | (uintptr_t)temperatures) % 4) return GPHQ_ERR_DIMENSIONS;
+    if (!work || (uintptr_t)work % 16 || work_bytes < need) return GPHQ_ERR_DIMENSIONS;
+    if (!(x == out && x_stride == out_stride) &&
+        spans_overlap(x, span_bytes(rows, x_stride, vocab, 4), out, span_bytes(rows, out_stride, vocab, 4)))
+        return GPHQ_ERR_OVERLAP;
+    ProbArgs a{x, temperatures, out, (float2 *)work, x_stride, out_stride, (int)rows, (int)vocab, 0, 0};
+    prob_cut(rows, vocab, a.len, a.parts);
+    const dim3 grid((unsigned)(rows * a.parts));
+    hipStream_t st = (hipStream_t)stream;
+    const bool vec = rows16(x, x_stride) && rows16(out, out_stride);
+    if (vec)
+        hipLaunchKernelGGL(prob_parts_kernel<true>, grid, dim3(kThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL(prob_parts_kernel<false>, grid, dim3(kThreads), 0, st, a);
+    GPHQ_TRY(launch_status());
+    if (vec)
+        hipLaunchKernelGGL(prob_write_kernel<true>, grid, dim3(kThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL(prob_write_kernel<false>, grid, dim3(kThreads), 0, st, a);
+    return launch_status();
+}
+
+int64_t gphq_verify_drafts_workspace_bytes(int64_t seqs, int64_t vocab) {
+    if (seqs < 0 || seqs > GPHQ_PAGED_MAX_SEQS || vocab < 1 || vocab > GPHQ_SAMPLE_MAX_VOCAB ||
+        seqs * verify_tiles(vocab) > (1 << 23) - 1)
+        return GPHQ_ERR_DIMENSIONS;
+    return seqs * verify_tiles(vocab) * (int64_t)sizeof(double2) + (seqs * 4 + 15) / 16 * 16;
+}
+
+int gphq_verify_drafts(const int32_t *starts, const int32_t *drafts, const float *target, int64_t target_stride,
+                       const float *draft, int64_t draft_stride, const float *accept_u, const float *sample_u,
+                       int64_t seqs, int64_t rows, int64_t vocab, int32_t *tokens, int32_t *accepted,
+                       const int32_t *lens, int32_t *kept, void *work, int64_t work_bytes, void *stream) {
+    const int64_t need = gphq_verify_drafts_workspace_bytes(seqs, vocab);
+    if (need < 0) return (int)need;
+    if (rows < 0 || rows > GPHQ_SAMPLE_MAX_ROWS || target_stride < vocab || (draft && draft_stride < vocab) ||
+        target_stride > INT64_MAX / 8 / GPHQ_SAMPLE_MAX_ROWS || draft_stride > INT64_MAX / 8 / GPHQ_SAMPLE_MAX_ROWS)
+        return GPHQ_ERR_DIMENSIONS;
+    if (seqs == 0) return GPHQ_OK;
+    if (!starts || !accepted || !sample_u || (kept && !lens)) return GPHQ_ERR_DIMENSIONS;
+    if (rows && (!drafts || !target || !accept_u || !tokens)) return GPHQ_ERR_DIMENSIONS;
+    const uintptr_t bits = (uintptr_t)starts | (uintptr_t)drafts | (uintptr_t)target | (uintptr_t)draft |
+                           (uintptr_t)accept_u | (uintptr_t)sample_u | (uintptr_t)tokens | (uintptr_t)accepted |
+                           (uintptr_t)lens | (uintptr_t)kept;
+    if (bits % 4 || !work || (uintptr_t)work % 16 || work_bytes < need) return GPHQ_ERR_DIMENSIONS;
+    const int tiles = verify_tiles(vocab);
+    double2 *sums = (double2 *)work;
+    VerifyArgs a{starts, drafts,  lens, target, draft, accept_u, sample_u, tokens, accepted, kept,
+                 (int32_t *)(sums + seqs * tiles), sums, target_stride, draft_stride, (int)seqs, (int)rows, (int)vocab,
+                 tiles};
+    const dim3 grid((unsigned)(seqs * tiles));
+    hipStream_t st = (hipStream_t)stream;
+    const bool vec = rows16(target, target_stride) && (!draft || rows16(draft, draft_stride));
+    if (vec)
+        hipLaunchKernelGGL(verify_sums_kernel<true>, grid, dim3(kThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL(verify_sums_kernel<false>, grid, dim3(kThreads), 0, st, a);
+    GPHQ_TRY(launch_status());
+    if (vec)
+        hipLaunchKernelGGL(verify_pick_kernel<true>, dim3((unsigned)seqs), dim3(kThreads), 0, st, a);
+    else
+        hipLaunchKernelGGL(verify_pick_kernel<false>, dim3((unsigned)seqs), dim3(kThreads), 0, st, a);
+    return launch_status();
+}
+
+}  // extern "C"

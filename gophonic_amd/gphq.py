@@ -63,6 +63,8 @@ TAIL_MAX_ROWS = 256
 FMT_Q4, FMT_Q8, FMT_Q8B, FMT_Q8B_F32 = 4, 8, 9, 10
 PASS_FP16, PASS_INT8 = 0, 1  # gphq_prefill_set_arith
 DTYPE_BF16, DTYPE_F16, DTYPE_F32 = 1, 2, 3
+DTYPE_I8, DTYPE_E4M3 = 4, 5  # 8-bit codes of a paged cache
+PAGED_BLOCK_TOKENS = 16
 
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
@@ -208,6 +210,18 @@ SIGNATURES = {
     "gphq_paged_pool_layer": (ctypes.c_int, [_vp, _i64, _vp]),
     "gphq_prefill_paged": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "gphq_paged_check": (ctypes.c_int, [_vp, _vp]),
+    "gphq_paged_pool_layer8": (ctypes.c_int, [_vp, _i64, _vp]),
+    "gphq_paged8_append": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _i64, _i64, _vp, _vp, ctypes.c_double, _vp, _vp,
+                                          _i64, ctypes.c_double, _vp, _i64, _vp]),
+    "gphq_paged8_attention_workspace_bytes": (_i64, [_vp, _vp, ctypes.c_int, _i64, _i64]),
+    "gphq_paged8_attention": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _i64, _i64, ctypes.c_double, _i64, _vp, _i64,
+                                             _vp, _i64, _vp]),
+    "gphq_paged_plan": (ctypes.c_int, [_vp, _vp]),
+    "gphq_probabilities_workspace_bytes": (_i64, [_i64, _i64]),
+    "gphq_probabilities": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "gphq_verify_drafts_workspace_bytes": (_i64, [_i64, _i64]),
+    "gphq_verify_drafts": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp,
+                                          _vp, _vp, _i64, _vp]),
     "gphq_lora_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "gphq_lora_add": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64,
                                      _i64, _i64, _vp, _i64, _vp]),
@@ -1141,6 +1155,18 @@ class PagedBatch:
         return check(load().gphq_paged_check(ptr(self.bad), stream_handle(stream)))
 
 
+def _append_rows(kv, batch, qkv, q, heads, q_norm, k_norm, cos, sin):
+    """An append's tensors checked; the row strides of qkv and q."""
+    if qkv.dtype != q.dtype or (cos is None) != (sin is None):
+        check(ERR_PAGED_SHAPE)
+    for t, n in ((q_norm, kv.head_dim), (k_norm, kv.head_dim), (cos, 0), (sin, 0)):
+        _values(t, _torch.float32, n, ERR_PAGED_SHAPE)
+    if cos is not None and (cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != kv.head_dim // 2):
+        check(ERR_PAGED_SHAPE)
+    return (_rows2(qkv, batch.rows, (heads + 2 * kv.kv_heads) * kv.head_dim, ERR_PAGED_SHAPE),
+            _rows2(q, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE))
+
+
 def paged_append(kv, batch, qkv, q, heads, q_norm=None, k_norm=None, eps=1e-6, cos=None, sin=None, q_scale=1.0,
                  stream=None):
     """gphq_paged_append: qkv [rows][(heads + 2 KV heads) head_dim] rows to
@@ -1148,14 +1174,7 @@ def paged_append(kv, batch, qkv, q, heads, q_norm=None, k_norm=None, eps=1e-6, c
     q_norm, k_norm float32 [head_dim]; cos, sin float32 [positions][head_dim / 2]."""
     lib = load()
     _here(kv.k, batch.lens, qkv, q, q_norm, k_norm, cos, sin)
-    if qkv.dtype != q.dtype or (cos is None) != (sin is None):
-        check(ERR_PAGED_SHAPE)
-    for t, n in ((q_norm, kv.head_dim), (k_norm, kv.head_dim), (cos, 0), (sin, 0)):
-        _values(t, _torch.float32, n, ERR_PAGED_SHAPE)
-    if cos is not None and (cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != kv.head_dim // 2):
-        check(ERR_PAGED_SHAPE)
-    qs = _rows2(qkv, batch.rows, (heads + 2 * kv.kv_heads) * kv.head_dim, ERR_PAGED_SHAPE)
-    os_ = _rows2(q, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
+    qs, os_ = _append_rows(kv, batch, qkv, q, heads, q_norm, k_norm, cos, sin)
     return check(lib.gphq_paged_append(kv.ref, batch.ref, _dtype(qkv.dtype), ptr(qkv), qs, heads, ptr(q_norm),
                                        ptr(k_norm), eps, ptr(cos), ptr(sin), 0 if cos is None else cos.shape[0],
                                        q_scale, ptr(q), os_, stream_handle(stream)))
@@ -1195,6 +1214,208 @@ def paged_attention(kv, batch, q, out, heads, scale, window=0, work=None, stream
                                           os_, ptr(work), _scratch_bytes(work, ERR_PAGED_SHAPE), stream_handle(stream)))
 
 
+# ---- a paged cache held in 8 bits (gphq_paged8_*) --------------------------------
+
+
+class PagedKv8Desc(ctypes.Structure):
+    _fields_ = [("codes", PagedKvDesc), ("k_scales_dev", ctypes.c_void_p), ("v_scales_dev", ctypes.c_void_p),
+                ("scale_page_stride", ctypes.c_int64), ("scale_head_stride", ctypes.c_int64)]
+
+
+_CODES = {}
+
+
+def _code_dtype(t):
+    """The GPHQ_DTYPE_* code of a torch dtype whose values are 8-bit codes; ERR_UNSUPPORTED for another."""
+    if not _CODES:
+        import torch
+
+        _CODES.update({torch.int8: DTYPE_I8, torch.float8_e4m3fn: DTYPE_E4M3})
+    return _CODES.get(t) or check(ERR_UNSUPPORTED)
+
+
+class PagedKv8:
+    """gphq_paged8_kv: codes k and v as PagedKv's tensors, of torch.int8 or
+    torch.float8_e4m3fn, and their scales, float32 [pages][KV heads][page tokens
+    / 16] with the same strides, blocks of a page side by side."""
+
+    def __init__(self, k, v, k_scales, v_scales):
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
+            check(ERR_PAGED_SHAPE)
+        pages, tokens, heads, hd = k.shape
+        dtype = _code_dtype(k.dtype)
+        import torch
+
+        for t in (k_scales, v_scales):
+            if t.shape != (pages, heads, tokens // PAGED_BLOCK_TOKENS) or t.stride() != k_scales.stride():
+                check(ERR_PAGED_SHAPE)
+            if t.dtype != torch.float32 or (t.shape[2] > 1 and t.stride(2) != 1):
+                check(ERR_PAGED_SHAPE)
+        if any(t.device != k.device for t in (v, k_scales, v_scales)):
+            check(ERR_PAGED_SHAPE)
+        self.k, self.v, self.k_scales, self.v_scales, self.dtype = k, v, k_scales, v_scales, k.dtype
+        # The stride of a dimension of one is never taken: one that the checks allow.
+        ps, ts, hs = (s if n > 1 else hd for s, n in zip(k.stride()[:3], k.shape[:3]))
+        sps, shs = (s if n > 1 else k_scales.shape[2] for s, n in zip(k_scales.stride()[:2], k_scales.shape[:2]))
+        codes = PagedKvDesc(ptr(k), ptr(v), ps, ts, hs, pages, tokens, heads, hd, dtype, 0)
+        self.desc = PagedKv8Desc(codes, ptr(k_scales), ptr(v_scales), sps, shs)
+        self.ref = ctypes.byref(self.desc)
+        self.kv_heads, self.head_dim = heads, hd
+
+
+def paged8_append(kv, batch, qkv, q, heads, q_norm=None, k_norm=None, eps=1e-6, cos=None, sin=None, q_scale=1.0,
+                  stream=None):
+    """gphq_paged8_append: as paged_append, keys and values as 8-bit codes with
+    a scale for every 16 tokens and KV head (a PagedKv8). batch.check() raises
+    ERR_NON_FINITE where a value was not finite (its code is 0)."""
+    lib = load()
+    _here(kv.k, batch.lens, qkv, q, q_norm, k_norm, cos, sin)
+    qs, os_ = _append_rows(kv, batch, qkv, q, heads, q_norm, k_norm, cos, sin)
+    return check(lib.gphq_paged8_append(kv.ref, batch.ref, _dtype(qkv.dtype), ptr(qkv), qs, heads, ptr(q_norm),
+                                        ptr(k_norm), eps, ptr(cos), ptr(sin), 0 if cos is None else cos.shape[0],
+                                        q_scale, ptr(q), os_, stream_handle(stream)))
+
+
+def paged8_attention_workspace_bytes(kv, batch, dtype, heads, window=0):
+    n = load().gphq_paged8_attention_workspace_bytes(kv.ref, batch.ref, _dtype(dtype), heads, window)
+    return n if n >= 0 else check(n)
+
+
+def paged8_attention(kv, batch, q, out, heads, scale, window=0, work=None, stream=None):
+    """gphq_paged8_attention: as paged_attention, over a PagedKv8. work: a uint8
+    device tensor of paged8_attention_workspace_bytes, or None."""
+    lib = load()
+    _here(kv.k, batch.lens, q, out, work)
+    if q.dtype != out.dtype:
+        check(ERR_PAGED_SHAPE)
+    qs = _rows2(q, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
+    os_ = _rows2(out, batch.rows, heads * kv.head_dim, ERR_PAGED_SHAPE)
+    if work is None:
+        work = _work(paged8_attention_workspace_bytes(kv, batch, q.dtype, heads, window), q.device, stream)
+    return check(lib.gphq_paged8_attention(kv.ref, batch.ref, _dtype(q.dtype), ptr(q), qs, heads, scale, window,
+                                           ptr(out), os_, ptr(work), _scratch_bytes(work, ERR_PAGED_SHAPE),
+                                           stream_handle(stream)))
+
+
+# ---- the plan of a step (gphq_paged_plan) ----------------------------------------
+
+
+class PagedRequestsDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("held_dev", "count_dev", "taken_dev", "shared_dev", "table_dev", "free_dev", "free_count_dev",
+                 "starts_dev", "lens_dev", "taken_out_dev", "free_count_out_dev", "positions_dev", "sequences_dev",
+                 "slots_dev", "bad_dev")] + \
+               [(n, ctypes.c_int64) for n in
+                ("seqs", "table_stride", "free_len", "page_tokens", "rows", "max_rows", "max_len")]
+
+
+class PagedPlan:
+    """gphq_paged_plan over device tensors: held, count, taken (and shared) int32
+    [seqs], table int32 [seqs][entries], free int32 [pages] of which free_count
+    (int32 [1]) are free. Results, made here where not given: starts, lens,
+    taken_out, free_count_out, positions, sequences [rows] int32 and slots [rows]
+    int64 (False: not wanted). lens, taken_out and free_count_out may be held,
+    taken and free_count. run() plans a step from what the tensors hold then;
+    `batch` is the step's PagedBatch, whose check() also reports the plan."""
+
+    def __init__(self, held, count, taken, table, free, free_count, page_tokens, rows, max_rows, max_len, shared=None,
+                 starts=None, lens=None, taken_out=None, free_count_out=None, positions=None, sequences=None,
+                 slots=None):
+        import torch
+
+        seqs, i32 = held.numel(), torch.int32
+
+        def made(t, n, dtype=i32):
+            if t is None:
+                t = torch.zeros(n, dtype=dtype, device=held.device)
+            return None if t is False else t
+
+        starts, lens, taken_out = made(starts, seqs + 1), made(lens, seqs), made(taken_out, seqs)
+        free_count_out = made(free_count_out, 1)
+        positions, sequences = made(positions, rows), made(sequences, rows)
+        slots = made(slots, rows, torch.int64)
+        for t, n, dtype in ((held, seqs, i32), (count, seqs, i32), (taken, seqs, i32), (shared, seqs, i32),
+                            (free, 0, i32), (free_count, 1, i32), (starts, seqs + 1, i32), (lens, seqs, i32),
+                            (taken_out, seqs, i32), (free_count_out, 1, i32), (positions, rows, i32),
+                            (sequences, rows, i32), (slots, rows, torch.int64), (table, 0, i32)):
+            _values(t, dtype, n, ERR_PAGED_SHAPE)
+            if t is not None and t.device != held.device:
+                check(ERR_PAGED_SHAPE)
+        self.batch = PagedBatch(starts, lens, table, rows, max_rows, max_len)
+        self.held, self.count, self.taken, self.shared, self.table = held, count, taken, shared, table
+        self.free, self.free_count, self.free_count_out = free, free_count, free_count_out
+        self.starts, self.lens, self.taken_out = starts, lens, taken_out
+        self.positions, self.sequences, self.slots = positions, sequences, slots
+        self.desc = PagedRequestsDesc(*[ptr(t) for t in (held, count, taken, shared, table, free, free_count, starts,
+                                                         lens, taken_out, free_count_out, positions, sequences, slots,
+                                                         self.batch.bad)],
+                                      seqs, table.shape[1], free.numel(), page_tokens, rows, max_rows, max_len)
+        self.ref = ctypes.byref(self.desc)
+
+    def run(self, stream=None):
+        lib = load()
+        _here(self.held)
+        return check(lib.gphq_paged_plan(self.ref, stream_handle(stream)))
+
+
+# ---- tokens from logits (gphq_probabilities, gphq_verify_drafts) ------------------
+
+
+def probabilities_workspace_bytes(rows, vocab):
+    n = load().gphq_probabilities_workspace_bytes(rows, vocab)
+    return n if n >= 0 else check(n)
+
+
+def probabilities(logits, out, temperatures=None, work=None, stream=None):
+    """gphq_probabilities: out [rows][vocab] = softmax(logits[r] / temperatures[r]),
+    all float32; temperature 0: 1 at the first of the largest logits. out may be
+    logits itself."""
+    lib = load()
+    _here(logits, out, temperatures, work)
+    if logits.dim() != 2 or out.shape != logits.shape or logits.dtype != _torch.float32 or out.dtype != _torch.float32:
+        check(ERR_DIMENSIONS)
+    rows, vocab = logits.shape
+    _values(temperatures, _torch.float32, rows, ERR_DIMENSIONS)
+    xs, os_ = _rows2(logits, rows, vocab, ERR_DIMENSIONS), _rows2(out, rows, vocab, ERR_DIMENSIONS)
+    if work is None:
+        work = _work(probabilities_workspace_bytes(rows, vocab), logits.device, stream)
+    return check(lib.gphq_probabilities(ptr(logits), xs, ptr(temperatures), ptr(out), os_, rows, vocab, ptr(work),
+                                        _scratch_bytes(work, ERR_DIMENSIONS), stream_handle(stream)))
+
+
+def verify_drafts_workspace_bytes(seqs, vocab):
+    n = load().gphq_verify_drafts_workspace_bytes(seqs, vocab)
+    return n if n >= 0 else check(n)
+
+
+def verify_drafts(starts, drafts, target, draft, accept_u, sample_u, tokens, accepted, lens=None, kept=None, work=None,
+                  stream=None):
+    """gphq_verify_drafts: starts int32 [seqs + 1]; drafts and tokens int32
+    [rows]; target and draft (None: certain drafts) float32 [rows][vocab];
+    accept_u float32 [rows], sample_u float32 [seqs]; accepted, lens and kept
+    int32 [seqs]. tokens may be drafts, kept may be lens."""
+    lib = load()
+    _here(starts, drafts, target, draft, accept_u, sample_u, tokens, accepted, lens, kept, work)
+    if target.dim() != 2 or target.dtype != _torch.float32 or starts.numel() < 1 or (kept is not None and lens is None):
+        check(ERR_DIMENSIONS)
+    rows, vocab = target.shape
+    seqs = starts.numel() - 1
+    if draft is not None and (draft.shape != target.shape or draft.dtype != _torch.float32):
+        check(ERR_DIMENSIONS)
+    i32, f32 = _torch.int32, _torch.float32
+    for t, n, dtype in ((starts, 1, i32), (drafts, rows, i32), (accept_u, rows, f32), (sample_u, seqs, f32),
+                        (tokens, rows, i32), (accepted, seqs, i32), (lens, seqs, i32), (kept, seqs, i32)):
+        _values(t, dtype, n, ERR_DIMENSIONS)
+    ps = _rows2(target, rows, vocab, ERR_DIMENSIONS)
+    qs = 0 if draft is None else _rows2(draft, rows, vocab, ERR_DIMENSIONS)
+    if work is None:
+        work = _work(verify_drafts_workspace_bytes(seqs, vocab), target.device, stream)
+    return check(lib.gphq_verify_drafts(ptr(starts), ptr(drafts), ptr(target), ps, ptr(draft), qs, ptr(accept_u),
+                                        ptr(sample_u), seqs, rows, vocab, ptr(tokens), ptr(accepted), ptr(lens),
+                                        ptr(kept), ptr(work), _scratch_bytes(work, ERR_DIMENSIONS),
+                                        stream_handle(stream)))
+
+
 class _PoolMemory:
     """Device memory of a paged pool. A tensor made from it keeps this object, and so the pool, alive."""
 
@@ -1205,13 +1426,15 @@ class _PoolMemory:
 
 class PagedPool:
     """gphq_paged_pool: a model's layers' pages, for Prefill.paged and, layer
-    by layer, for paged_append and paged_attention. In the memory of the
+    by layer, for paged_append and paged_attention (dtype torch.int8 or
+    torch.float8_e4m3fn: codes with scales, for paged8_*). In the memory of the
     device that is current when it is made; close() ends its layers' tensors
     with it."""
 
     def __init__(self, lm, pages, page_tokens, dtype):
         h = ctypes.c_void_p()
-        check(load().gphq_paged_pool_new(lm.h, pages, page_tokens, _dtype(dtype), ctypes.byref(h)))
+        code = _code_dtype(dtype) if dtype.itemsize == 1 else _dtype(dtype)
+        check(load().gphq_paged_pool_new(lm.h, pages, page_tokens, code, ctypes.byref(h)))
         self.h, self.lm, self.dtype, self.device = h, lm, dtype, _torch.cuda.current_device()
 
     def close(self):
@@ -1226,17 +1449,28 @@ class PagedPool:
             pass
 
     def layer(self, i):
-        """PagedKv of layer i, its tensors views of the pool's memory."""
+        """PagedKv of layer i (PagedKv8 of a pool of 8-bit codes), its tensors views of the pool's memory."""
         import torch
 
-        d = PagedKvDesc()
-        check(load().gphq_paged_pool_layer(self.h, i, ctypes.byref(d)))
+        d, d8 = PagedKvDesc(), None
+        if self.dtype.itemsize == 1:
+            d8 = PagedKv8Desc()
+            check(load().gphq_paged_pool_layer8(self.h, i, ctypes.byref(d8)))
+            d = d8.codes
+        else:
+            check(load().gphq_paged_pool_layer(self.h, i, ctypes.byref(d)))
         shape = (d.pages, d.kv_heads, d.page_tokens, d.head_dim)
-        name = {DTYPE_F32: "<f4"}.get(d.dtype, "<i2")
-        # Asked for on another device than their memory's, the tensors would be copies.
-        k, v = (torch.as_tensor(_PoolMemory(self, a, shape, name), device=torch.device("cuda", self.device))
-                .view(self.dtype).transpose(1, 2) for a in (d.k_dev, d.v_dev))
-        return PagedKv(k, v)
+        name = {DTYPE_F32: "<f4", DTYPE_I8: "|i1", DTYPE_E4M3: "|i1"}.get(d.dtype, "<i2")
+
+        def view(address, shape, name):
+            # Asked for on another device than their memory's, the tensors would be copies.
+            return torch.as_tensor(_PoolMemory(self, address, shape, name), device=torch.device("cuda", self.device))
+
+        k, v = (view(a, shape, name).view(self.dtype).transpose(1, 2) for a in (d.k_dev, d.v_dev))
+        if d8 is None:
+            return PagedKv(k, v)
+        shape = (d.pages, d.kv_heads, d.page_tokens // PAGED_BLOCK_TOKENS)
+        return PagedKv8(k, v, *(view(a, shape, "<f4") for a in (d8.k_scales_dev, d8.v_scales_dev)))
 
 
 def lora_workspace_bytes(rows, k, max_rank):

@@ -630,18 +630,173 @@ int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq
 int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q_dev,
                          int64_t q_stride, int64_t heads, double scale, int64_t window, void *out_dev,
                          int64_t out_stride, void *work_dev, int64_t work_bytes, void *stream);
-/* Waits for the stream, and for no other; GPHQ_ERR_PAGED_BATCH if *bad_dev was
- * set, which is then cleared, on the stream. */
+/* Waits for the stream, and for no other; where *bad_dev was set, which is then
+ * cleared, on the stream: GPHQ_ERR_PAGED_BATCH for a sequence, page or position
+ * out of bounds, else GPHQ_ERR_NON_FINITE for a value that 8 bits cannot hold
+ * (gphq_paged8_append), else GPHQ_ERR_PREFIX_FULL where pages ran out
+ * (gphq_paged_plan). */
 int gphq_paged_check(int32_t *bad_dev, void *stream);
 
+/* ---- a paged cache held in 8 bits --------------------------------------------
+ * A pool as gphq_paged_kv's whose elements are codes of one byte (dtype
+ * GPHQ_DTYPE_I8: whole numbers -127 .. 127; GPHQ_DTYPE_E4M3: floating point of
+ * four exponent and three fraction bits, up to 448, no infinity), strides in
+ * bytes, and a scale for every block of GPHQ_PAGED_BLOCK_TOKENS neighbouring
+ * tokens and KV head: token t of page p has the value
+ *   scales[p * scale_page_stride + head * scale_head_stride + t / 16] * code,
+ * keys and values each with scales of their own. About half the memory, and
+ * half the bytes that attention reads, of a 16-bit pool. int8 codes are off by
+ * at most 1/254 of their block's largest value; e4m3 codes by at most 1/16 of
+ * the value itself (or 2^-10 of the scale), whatever else the block holds. */
+#define GPHQ_PAGED_BLOCK_TOKENS 16
+typedef struct gphq_paged8_kv {
+    gphq_paged_kv codes;
+    float *k_scales_dev, *v_scales_dev;
+    int64_t scale_page_stride, scale_head_stride; /* in scales, each >= page_tokens / 16 */
+} gphq_paged8_kv;
+
+/* gphq_paged_append into 8 bits; row_dtype F32, F16 or BF16 whatever the codes.
+ * Per block that receives tokens, m the largest magnitude among their values
+ * and top the largest code (127, 448):
+ *   a block that holds no earlier token of the sequence: scale = m / top;
+ *   one that does keeps its scale while m rounds to a code (m <= 127.5 scale,
+ *   464 scale), else the scale is doubled as often as that takes, and the
+ *   earlier tokens' codes are rounded to it (e4m3 codes lose nothing by it
+ *   above 2^-6 of the new scale; int8 codes stay within one step of the value).
+ *   code = value / scale, rounded to nearest, ties to even.
+ * Keys' norm and rotation, and all that decides a code, are 64-bit arithmetic:
+ * codes do not depend on the order of a sum, nor on how a batch is cut. (Tokens
+ * that come one by one may grow a scale that one call would have chosen at
+ * once.) Queries as gphq_paged_append's, in fp32. A value that is not finite
+ * becomes code 0 and sets *bad_dev (GPHQ_ERR_NON_FINITE). A block whose scale
+ * is not a positive finite number counts as empty: it gets a new one. Sequences
+ * may share pages whose 16-token blocks all lie before the call's tokens; two
+ * sequences of one call must not write the same block. Slots behind a
+ * sequence's last token keep their bytes. The rest as gphq_paged_append. */
+int gphq_paged8_append(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *qkv_dev,
+                       int64_t qkv_stride, int64_t heads, const float *q_norm_dev, const float *k_norm_dev, double eps,
+                       const float *cos_dev, const float *sin_dev, int64_t rope_rows, double q_scale, void *q_dev,
+                       int64_t q_stride, void *stream);
+
+/* gphq_paged_attention over an 8-bit pool: the same definition, with k and v the
+ * values that the codes stand for, the same arguments, masks, limits, workspace
+ * rules and order of sums; row_dtype F32, F16 or BF16 whatever the codes. Queries
+ * and the codes' products are taken as in an FP16 pool (fp32 rows keep 22 bits of
+ * a query value, relative to the row's largest), scales in fp32; probabilities
+ * times a block's scale keep 22 bits in sequences whose rows times heads /
+ * kv_heads are at most 64 and for fp32 rows, else they are rounded to 11. The two
+ * e4m3 codes that are no number, which append does not write, read as 480 and
+ * -480. Scales that a row sees should be finite; one that is not makes the row
+ * not finite, and reaches no other. */
+int64_t gphq_paged8_attention_workspace_bytes(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype,
+                                              int64_t heads, int64_t window);
+int gphq_paged8_attention(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q_dev,
+                          int64_t q_stride, int64_t heads, double scale, int64_t window, void *out_dev,
+                          int64_t out_stride, void *work_dev, int64_t work_bytes, void *stream);
+
+/* ---- the plan of a step --------------------------------------------------------
+ * What gphq_paged_batch describes, made on the device from the requests'
+ * lengths: pages taken from a list of free ones and given back to it, and where
+ * each new token goes. Per sequence s: `held` tokens that its pages hold and that
+ * are kept, `count` tokens that the step brings, `taken` entries of its table that
+ * name pages (the first ones), of which the first `shared` (NULL: none) are not its
+ * own to give back. With T = page_tokens, need = ceil((held + count) / T):
+ *   gives back entries max(need, min(shared, taken)) .. taken - 1: drafts that were
+ *   not accepted (held shrank), or a request that has ended (held = count = 0);
+ *   takes need - taken pages more.
+ * All that is given goes behind the list's free_count pages, in the order of the
+ * sequences and their entries; then pages are taken from the list's end, in the
+ * order of the sequences and their entries. Results:
+ *   starts[s] row of s's first new token, lens[s] = held + count: gphq_paged_batch's
+ *   taken_out[s], free_count_out (the list's pages now; it is changed in place)
+ *   positions[r], sequences[r], slots[r] = page * T + slot of row r (each NULL:
+ *   not wanted); -1 for rows behind the last sequence's.
+ * A sequence whose pages would not fit what the list holds, after the pages of those
+ * before it, fitting or not, takes none and brings no row in this step (lens = held;
+ * a later one that takes none still does), and sets *bad_dev
+ * (GPHQ_ERR_PREFIX_FULL); one whose rows would pass `rows` brings none, and a
+ * sequence with a negative number, taken past table_stride, count past max_rows or
+ * held + count past max_len is left alone, without rows; both set *bad_dev
+ * (GPHQ_ERR_PAGED_BATCH), as does a given page for which the list has no room
+ * (free_len), which is dropped. Table entries behind `taken` are left as they are.
+ * taken_out, lens and free_count_out may be the arrays taken, held and free_count
+ * themselves (a captured plan then goes on from step to step), and overlap nothing
+ * otherwise. Two calls on one list must not run at once. */
+typedef struct gphq_paged_requests {
+    const int32_t *held_dev, *count_dev, *taken_dev, *shared_dev; /* [seqs]; shared may be NULL */
+    int32_t *table_dev;                                          /* [seqs][table_stride] */
+    int32_t *free_dev;                                           /* [free_len] */
+    const int32_t *free_count_dev;
+    int32_t *starts_dev;                                         /* [seqs + 1] */
+    int32_t *lens_dev, *taken_out_dev;                           /* [seqs] */
+    int32_t *free_count_out_dev;
+    int32_t *positions_dev, *sequences_dev; /* [rows] or NULL */
+    int64_t *slots_dev;                     /* [rows] or NULL */
+    int32_t *bad_dev;                       /* or NULL */
+    int64_t seqs, table_stride, free_len, page_tokens, rows, max_rows, max_len;
+} gphq_paged_requests;
+int gphq_paged_plan(const gphq_paged_requests *r, void *stream);
+
+/* ---- tokens from logits -------------------------------------------------------
+ * No counterpart in the reference, which takes the largest logit. */
+#define GPHQ_SAMPLE_MAX_ROWS (1 << 20)
+#define GPHQ_SAMPLE_MAX_VOCAB (1 << 24)
+/* out[r][i] = exp((x[r][i] - max) / t) / sum over i, t = temperatures[r] (device
+ * f32[rows]; NULL: 1): rows of gphq_decode_batch_logits to probabilities. t = 0
+ * (and what is not above it, NaN included): 1 at the row's largest logit, the
+ * first of equal ones, 0 elsewhere. A row of -inf alone becomes 0; one with a
+ * NaN, or with +inf at t > 0, becomes NaN, at t = 0 +inf counts as a number and
+ * NaN as -inf. fp32, each exponential off by a few units in its last place and
+ * 2^-23 of (max - x) / t; sums in a fixed order. x and out may be the same rows
+ * (address and stride), and else must not overlap. work (16-byte aligned):
+ * gphq_probabilities_workspace_bytes, one per call that may run at the same time;
+ * strides in floats; rows best 16-byte aligned. */
+int64_t gphq_probabilities_workspace_bytes(int64_t rows, int64_t vocab);
+int gphq_probabilities(const float *x_dev, int64_t x_stride, const float *temperatures_dev, float *out_dev,
+                       int64_t out_stride, int64_t rows, int64_t vocab, void *work_dev, int64_t work_bytes,
+                       void *stream);
+/* Drafted tokens held against the target's probabilities. Sequence s has the rows
+ * a = starts[s] .. b = starts[s + 1] - 1 (device int32[seqs + 1]) and b - a drafts:
+ * row r < b of `target` [rows][vocab] are the probabilities of the token that drafts[r]
+ * (int32[rows]) proposes, row b of the one behind them all. `draft` [rows][vocab] are
+ * the proposer's own probabilities of the same tokens (row b is not read), NULL where
+ * it was certain (1 at the proposed token). With the random numbers accept_u[rows] and
+ * sample_u[seqs], both in 0 .. 1, without 1:
+ *   r counts up from a while accept_u[r] draft[r][x] < target[r][x], x = drafts[r], r < b;
+ *   tokens[a .. r - 1] = the drafts, accepted[s] = r - a;
+ *   tokens[r] = the first t with sum_{i <= t} w_i > sample_u[s] sum_i w_i, where
+ *     w = max(target[r] - draft[r], 0) at r < b (target[r] if that is 0 throughout),
+ *     w = target[b] at r = b;
+ *   tokens[r + 1 .. b] = -1.
+ * The tokens are then distributed as if they had been drawn from the target one by one.
+ * A sequence of one row is a token drawn from it. Comparisons and sums are 64-bit, in a
+ * fixed order. A draft outside the vocabulary is not accepted, and w is the target's
+ * row. Weights that are negative or NaN count as 0; where no t is found (all are 0, or
+ * the sum is infinite) the last t with a weight is taken, 0 if there is none.
+ * kept (may be NULL): kept[s] = lens[s] - (b - r), the tokens that stay in a cache of
+ * lens[s] with all drafts (gphq_paged_plan's held in the next step); may be lens.
+ * A sequence whose starts descend or leave 0 .. rows gets accepted -1, kept = lens;
+ * one without rows accepted 0. Rows outside all sequences are left alone. work:
+ * gphq_verify_drafts_workspace_bytes, 16-byte aligned, one per call that may run at
+ * the same time. tokens may be drafts itself. */
+int64_t gphq_verify_drafts_workspace_bytes(int64_t seqs, int64_t vocab);
+int gphq_verify_drafts(const int32_t *starts_dev, const int32_t *drafts_dev, const float *target_dev,
+                       int64_t target_stride, const float *draft_dev, int64_t draft_stride, const float *accept_u_dev,
+                       const float *sample_u_dev, int64_t seqs, int64_t rows, int64_t vocab, int32_t *tokens_dev,
+                       int32_t *accepted_dev, const int32_t *lens_dev, int32_t *kept_dev, void *work_dev,
+                       int64_t work_bytes, void *stream);
+
 /* A pool of one model's layers: `pages` pages of page_tokens tokens of every
- * layer, keys and values in head order, dtype as gphq_paged_kv. The caller
- * hands its page numbers out; page p of every layer belongs to the same tokens.
- * gphq_paged_pool_layer describes one layer's pages for the calls above. */
+ * layer, keys and values in head order, dtype as gphq_paged_kv or, with scales
+ * beside them, as gphq_paged8_kv. The caller hands its page numbers out; page p
+ * of every layer belongs to the same tokens. gphq_paged_pool_layer describes one
+ * layer's pages for the calls above, gphq_paged_pool_layer8 those of a pool of
+ * 8-bit codes (GPHQ_ERR_UNSUPPORTED for another). */
 typedef struct gphq_paged_pool gphq_paged_pool;
 int gphq_paged_pool_new(const gphq_lm *lm, int64_t pages, int64_t page_tokens, int dtype, gphq_paged_pool **out);
 void gphq_paged_pool_free(gphq_paged_pool *pool);
 int gphq_paged_pool_layer(const gphq_paged_pool *pool, int64_t layer, gphq_paged_kv *out);
+int gphq_paged_pool_layer8(const gphq_paged_pool *pool, int64_t layer, gphq_paged8_kv *out);
 
 /* ---- low-rank adapters beside a shared projection ------------------------------
  * No counterpart in the reference. After a projection of many requests' rows
@@ -823,7 +978,8 @@ int gphq_prefill_batch(gphq_prefill *ws, const gphq_prefix *shared, int64_t past
  * the one token of a decode step, to the past[s] its pages hold; `tokens` (host)
  * are theirs concatenated, table (host [count][table_stride]) their pages. Per
  * layer the pass projects, appends (gphq_paged_append with the layer's norms and
- * the model's rotation) and attends (gphq_paged_attention). Row s of hidden_dev
+ * the model's rotation) and attends (gphq_paged_attention), or, in a pool of 8-bit
+ * codes, gphq_paged8_append and gphq_paged8_attention. Row s of hidden_dev
  * [count][hidden] receives the post-final-norm state of sequence s's last
  * token. Tokens beyond the workspace's rows run as consecutive passes, in
  * order. Validation as gphq_prefill_batch's per sequence, then the table: a
@@ -987,6 +1143,9 @@ int gphq_gptq_quantize(const char *dir, const char *format, const gphq_lm_config
 #define GPHQ_DTYPE_BF16 1
 #define GPHQ_DTYPE_F16 2
 #define GPHQ_DTYPE_F32 3
+/* 8-bit codes of a paged cache (gphq_paged8_kv, gphq_paged_pool_new); no tensor of a checkpoint is read as these. */
+#define GPHQ_DTYPE_I8 4
+#define GPHQ_DTYPE_E4M3 5
 typedef struct gphq_checkpoint gphq_checkpoint;
 typedef struct gphq_mapping gphq_mapping;
 int gphq_checkpoint_open(const char *dir, gphq_checkpoint **out);
