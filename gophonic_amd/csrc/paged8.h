@@ -160,6 +160,25 @@ __device__ __forceinline__ unsigned pages8_step(const Attn8Args &e, Page8Walk &w
     return ok;
 }
 
+// Memory from p on, for loads whose places are a lane's 32-bit offset and a wavefront's.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, 0x7FFFFFFF, 0x00020000);
+}
+
+// Lane l's place among a step's N scales: block l % N's.
+template <int N>
+__device__ __forceinline__ int64_t lane_scale(const int64_t (&sat)[N]) {
+    const int b = threadIdx.x & (N - 1);
+    int64_t at = sat[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) at = b == i ? sat[i] : at;
+    return at;
+}
+// What lane i holds, wavefront-uniform.
+__device__ __forceinline__ float lane_value(float v, int i) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i));
+}
+
 // A scale at a wavefront-uniform place, by the scalar unit (nothing writes scales while attention reads them).
 __device__ __forceinline__ float uniform_scale(const float *p, int64_t at) {
     return *(const __attribute__((address_space(4))) float *)(uintptr_t)(p + at);
@@ -173,6 +192,17 @@ __device__ __forceinline__ int scale_exp(float s) { return s > 0.0f ? __builtin_
 // stay below 2^15; none is seen before kNoExp. What leaves the kernel has probabilities of at most 1.
 constexpr int kNoExp = -1000;
 constexpr int kDrop = 15;
+
+// Largest of a column's values, which lie in the four lanes lane % 16 + 16 i of a wavefront: rows
+// of 16 lanes, then halves, exchanged between two registers (the waits are those that the exchange
+// needs behind a vector instruction's result).
+__device__ __forceinline__ float column_max(float v) {
+    float w = v;
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+    w = v = fmaxf(v, w);
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+    return fmaxf(v, w);
+}
 
 template <typename RT, typename C>
 int attn8_rows_launch(const Attn8Args &a, int hd, int splits, int tiles, hipStream_t st);

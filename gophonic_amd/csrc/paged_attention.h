@@ -37,6 +37,7 @@ struct AttnArgs {
     int parts, small_parts, small_rows;
     int row_tiles;         // the row kernel's grid has this many tiles for every row; 0: all tiles for every sequence
     int small_cols;        // sequences of at most this many columns are the row kernel's
+    int small_tile;        // columns of the row kernel's tiles
     int big_tile;          // columns of the chunk kernel's tiles
     float q_sign;          // the sign of scale (0 if scale is 0), applied to the queries
     int split_small, split_big;  // keys per split in each kernel, multiples of 128

@@ -80,17 +80,23 @@ struct AttnPlan {
     int64_t small_units;  // tiles of the row kernel's grid
 };
 
-// Keys per split of `span` keys and how many splits that makes, for about `want` of them.
-void cut(int64_t span, int64_t want, int &len, int &splits) {
-    const int64_t steps = std::max<int64_t>(1, (span + 127) / 128);
+// What the row kernel of a call is like: columns of its tiles, keys that a block's wavefronts take
+// in one round, and up to how many keys a call is not split.
+struct RowKernel {
+    int tile, round, brief;
+};
+
+// Keys per split of `span` keys, a multiple of `unit`, and how many splits that makes, for about `want` of them.
+void cut(int64_t span, int64_t want, int unit, int &len, int &splits) {
+    const int64_t steps = std::max<int64_t>(1, (span + unit - 1) / unit);
     const int64_t n = std::min(std::max<int64_t>(want, 1), steps);
-    len = (int)((steps + n - 1) / n * 128);
+    len = (int)((steps + n - 1) / n * unit);
     splits = (int)((span + len - 1) / len);
     if (splits < 1) splits = 1;
 }
 
-// wide: fp32 pages. From host numbers alone, so a captured call keeps its cut whatever the lengths become.
-AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int big_tile, bool wide) {
+// From host numbers alone, so a captured call keeps its cut whatever the lengths become.
+AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int big_tile, const RowKernel &k) {
     AttnPlan p{};
     const int64_t cus = device_cus(), rows = b.rows, cols = (int64_t)b.max_rows * group;
     // Sequences of up to 64 columns run in the row kernel, in tiles of 16 that each read the
@@ -105,7 +111,7 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
     };
     if (p.small_cols && group <= p.small_cols) {
         p.small_rows = std::min(p.small_cols / group, b.max_rows);
-        p.small_tiles = (int)((std::min<int64_t>(cols, p.small_cols) + kSmallTile - 1) / kSmallTile);
+        p.small_tiles = (int)((std::min<int64_t>(cols, p.small_cols) + k.tile - 1) / k.tile);
         const int64_t units = std::min<int64_t>(b.seqs, rows) * p.small_tiles * kv_heads;
         // As many splits as leave one block on a CU: its four wavefronts keep enough loads in
         // flight, and a round more, begun or whole, costs more than it hides (16 bfloat16 rows of
@@ -113,7 +119,7 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         // with one and a half; fp32: 71.5, 74.7, 89.7). Short rows take no split: the second
         // launch costs more than the steps it saves up to 512 keys of 16 bits (one row: 8.2 us,
         // split 9.4; 768 keys: 10.3 and 9.3) and 256 of 32 (10.6 and 11.0; 384: 13.4 and 11.1).
-        const bool brief = span(kSmallTile) <= (wide ? 256 : 512);
+        const bool brief = span(k.tile) <= k.brief;
         // Beside longer sequences, which are the chunk kernel's, only some of the sequences are
         // this kernel's, in one tile mostly: twice as many splits of one tile each. Whole calls,
         // so and with the rule above: twelve sequences (three single rows) over up to 4000
@@ -124,14 +130,14 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         // The grid is by sequence, or by row where a batch has more room for sequences than rows (one
         // row of 40000 bfloat16 tokens, alone 26 us, among 2047 idle sequences 26 by row and 544 by
         // sequence). No more splits than a launch takes.
-        const int64_t row_tiles = (group + kSmallTile - 1) / kSmallTile;
+        const int64_t row_tiles = (group + k.tile - 1) / k.tile;
         p.small_units = (int64_t)b.seqs * p.small_tiles;
         if (rows * row_tiles < p.small_units) {
             p.small_units = rows * row_tiles;
             p.row_tiles = (int)row_tiles;
         }
         const int64_t most = kMaxBlocks / (p.small_units * kv_heads);
-        cut(span(kSmallTile), brief ? 1 : std::min(want, most), p.small_len, p.small_splits);
+        cut(span(k.tile), brief ? 1 : std::min(want, most), k.round, p.small_len, p.small_splits);
         if ((int64_t)b.seqs * p.small_rows > rows) p.small_rows = 0;  // at most `rows` sequences have any
     }
     if (cols > p.small_cols) {
@@ -150,7 +156,7 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         // alike or one alone: three of 83 to 234 FP16 rows over 6000 tokens 106 us, 94 with one
         // round, the six (one chunk) 106 and 88.
         const int64_t want = units >= slots ? 1 : (b.seqs == 1 ? 1 : 3) * slots / units;
-        cut(span(big_tile), want, p.big_len, p.big_splits);
+        cut(span(big_tile), want, 128, p.big_len, p.big_splits);
     }
     return p;
 }
@@ -183,7 +189,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
     if (row < s.start || row >= s.end || !seq_ok(a.b, s.start, s.end, s.len)) return;
     const int n = s.end - s.start, i = row - s.start, cols = n * a.group;
     const bool small = cols <= a.small_cols;
-    const int tm = small ? kSmallTile : a.big_tile, c0 = (i * a.group + head % a.group) / tm * tm;
+    const int tm = small ? a.small_tile : a.big_tile, c0 = (i * a.group + head % a.group) / tm * tm;
     const TileKeys k = tile_keys(n, s.len, c0 / a.group, min((c0 + tm - 1) / a.group, n - 1), a.window);
     const int all = head < a.heads ? tile_splits(k, small ? a.split_small : a.split_big) : 1;
     const int splits = all > 1 ? all : 0;  // (heads of a row may lie in different tiles)
@@ -280,9 +286,9 @@ int attend8(const Attn8Args &e, const AttnPlan &p, int hd, hipStream_t st) {
 }
 
 // The call's cut, refused where a launch would have too many blocks.
-int plan_of(const AttnArgs &a, const gphq_paged_kv *kv, AttnPlan &p) {
+int plan_of(const AttnArgs &a, const gphq_paged_kv *kv, const RowKernel &k, AttnPlan &p) {
     const int64_t kvh = a.pool.kv_heads;
-    p = attn_plan(a.b, (int)kvh, a.group, a.window, a.big_tile, kv->dtype == GPHQ_DTYPE_F32);
+    p = attn_plan(a.b, (int)kvh, a.group, a.window, a.big_tile, k);
     if (p.small_units * p.small_splits * kvh > kMaxBlocks ||
         (int64_t)p.big_tiles * p.big_splits * kvh > kMaxBlocks)
         return GPHQ_ERR_PAGED_SHAPE;
@@ -322,15 +328,24 @@ int attn8_args(const gphq_paged8_kv *kv, const gphq_paged_batch *b, int row_dtyp
     return GPHQ_OK;
 }
 
-int64_t work_bytes_of(const AttnArgs &a, const gphq_paged_kv *kv) {
+RowKernel row_kernel(const gphq_paged_kv *kv) { return {kSmallTile, 128, kv->dtype == GPHQ_DTYPE_F32 ? 256 : 512}; }
+// Over 8-bit pages up to 64 columns of a sequence go two sets of 16 to a tile; beside longer
+// sequences, which are the chunk kernel's, most of the row kernel's have one row. One row over 1024
+// tokens, eight KV heads: split 7.9 us and 3.4 for the join, unsplit 13.1.
+RowKernel row_kernel8(const AttnArgs &a) {
+    const int cols = a.b.max_rows * a.group;
+    return cols > 16 && cols <= 64 ? RowKernel{32, 256, 512} : RowKernel{16, 256, 512};
+}
+
+int64_t work_bytes_of(const AttnArgs &a, const gphq_paged_kv *kv, const RowKernel &k) {
     if (a.b.rows == 0) return 0;
     AttnPlan p;
-    GPHQ_TRY(plan_of(a, kv, p));
+    GPHQ_TRY(plan_of(a, kv, k, p));
     return (small_count(p, a.b, a.heads) + big_count(p, a.b, a.heads)) * (kv->head_dim + 2) * 4;
 }
 
 // The rest of a call's checks and arguments; `p` is its cut. A batch without rows leaves a.b.rows 0.
-int call_args(const gphq_paged_kv *kv, int64_t size, const void *q, int64_t q_stride, double scale, void *out,
+int call_args(const gphq_paged_kv *kv, const RowKernel &k, int64_t size, const void *q, int64_t q_stride, double scale, void *out,
               int64_t out_stride, void *work, int64_t work_bytes, AttnArgs &a, AttnPlan &p) {
     const int64_t hd = kv->head_dim, heads = a.heads;
     if (!(fabs(scale) <= 1e30) || q_stride < heads * hd || out_stride < heads * hd || q_stride * size % 16 || out_stride * size % 16)
@@ -340,7 +355,7 @@ int call_args(const gphq_paged_kv *kv, int64_t size, const void *q, int64_t q_st
     if (spans_overlap(q, span_bytes(a.b.rows, q_stride, heads * hd, size), out,
                       span_bytes(a.b.rows, out_stride, heads * hd, size)))
         return GPHQ_ERR_OVERLAP;
-    GPHQ_TRY(plan_of(a, kv, p));
+    GPHQ_TRY(plan_of(a, kv, k, p));
     const int64_t big = big_count(p, a.b, heads), small = small_count(p, a.b, heads);
     if (big + small && (!work || (uintptr_t)work % 16 || work_bytes < (big + small) * (hd + 2) * 4))
         return GPHQ_ERR_PAGED_SHAPE;
@@ -357,6 +372,7 @@ int call_args(const gphq_paged_kv *kv, int64_t size, const void *q, int64_t q_st
     a.part_ml = a.small_o + small * hd;
     a.small_ml = a.part_ml + 2 * big;
     a.small_cols = p.small_cols;
+    a.small_tile = k.tile;
     a.split_small = p.small_len;
     a.split_big = p.big_len;
     a.q_sign = scale > 0 ? 1.0f : scale < 0 ? -1.0f : 0.0f;
@@ -375,7 +391,7 @@ int64_t gphq_paged_attention_workspace_bytes(const gphq_paged_kv *kv, const gphq
                                              int64_t heads, int64_t window) {
     AttnArgs a{};
     GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
-    return work_bytes_of(a, kv);
+    return work_bytes_of(a, kv, row_kernel(kv));
 }
 
 int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
@@ -384,7 +400,8 @@ int gphq_paged_attention(const gphq_paged_kv *kv, const gphq_paged_batch *batch,
     AttnArgs a{};
     GPHQ_TRY(attn_args(kv, batch, row_dtype, heads, window, a));
     AttnPlan p;
-    GPHQ_TRY(call_args(kv, row_dtype == GPHQ_DTYPE_F32 ? 4 : 2, q, q_stride, scale, out, out_stride, work, work_bytes, a, p));
+    GPHQ_TRY(call_args(kv, row_kernel(kv), row_dtype == GPHQ_DTYPE_F32 ? 4 : 2, q, q_stride, scale, out, out_stride, work,
+                       work_bytes, a, p));
     if (a.b.rows == 0) return GPHQ_OK;
     const int64_t hd = kv->head_dim;
     hipStream_t st = (hipStream_t)stream;
@@ -401,7 +418,7 @@ int64_t gphq_paged8_attention_workspace_bytes(const gphq_paged8_kv *kv, const gp
                                               int64_t heads, int64_t window) {
     Attn8Args e{};
     GPHQ_TRY(attn8_args(kv, batch, row_dtype, heads, window, e));
-    return work_bytes_of(e.a, &kv->codes);
+    return work_bytes_of(e.a, &kv->codes, row_kernel8(e.a));
 }
 
 int gphq_paged8_attention(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
@@ -410,7 +427,7 @@ int gphq_paged8_attention(const gphq_paged8_kv *kv, const gphq_paged_batch *batc
     Attn8Args e{};
     GPHQ_TRY(attn8_args(kv, batch, row_dtype, heads, window, e));
     AttnPlan p;
-    GPHQ_TRY(call_args(&kv->codes, row_dtype == GPHQ_DTYPE_F32 ? 4 : 2, q, q_stride, scale, out, out_stride, work,
+    GPHQ_TRY(call_args(&kv->codes, row_kernel8(e.a), row_dtype == GPHQ_DTYPE_F32 ? 4 : 2, q, q_stride, scale, out, out_stride, work,
                        work_bytes, e.a, p));
     if (e.a.b.rows == 0) return GPHQ_OK;
     const int hd = (int)kv->codes.head_dim;

@@ -6,19 +6,29 @@
 namespace gphq {
 namespace {
 
-// One block's tile: 16 columns of a sequence and KV head over the keys [k0, k1).
+// One block's tile: 16 (or TM) columns of a sequence and KV head over the keys [k0, k1).
 struct RowTile {
     int seq, g, n, len, start, r0, r1, splits, split;
     int lo, hi, k0, k1, p0, p1;  // p0, p1: positions of the tile's first and last row
+    int c0;                      // the tile's first column
     // this lane's column
     int row, head, pos, first;
     bool live;
 };
 
+// Makes `col` this lane's column.
+__device__ __forceinline__ void row_column(const AttnArgs &a, RowTile &t, int col) {
+    t.live = col < t.n * a.group;
+    t.row = t.live ? col / a.group : t.r1;
+    t.head = t.g * a.group + (t.live ? col - t.row * a.group : 0);
+    t.pos = t.len - t.n + t.row;
+    t.first = a.window > 0 ? t.pos - a.window + 1 : 0;
+}
+
 // False where this block has nothing to do. BY_ROW: the grid has row_tiles tiles for every row (a
 // kernel of its own: both ways in one took 110 us instead of 108 in a call by sequence of one FP16
 // chunk and five single tokens over up to 6000 tokens).
-template <bool BY_ROW>
+template <bool BY_ROW, int TM = kSmallTile, int NT = 256>
 __device__ __forceinline__ bool row_tile(const AttnArgs &a, int tiles, int splits, RowTile &t) {
     int u = blockIdx.x;
     t.g = u % a.pool.kv_heads;
@@ -29,7 +39,7 @@ __device__ __forceinline__ bool row_tile(const AttnArgs &a, int tiles, int split
     if (BY_ROW) {
         // A row of group columns has up to row_tiles tiles of its own: n rows as many as their sequence
         // has, or more. The blocks share the check of all sequences, idle ones too.
-        for (unsigned s = blockIdx.x * 256 + threadIdx.x; s < (unsigned)a.b.seqs; s += gridDim.x * 256)
+        for (unsigned s = blockIdx.x * NT + threadIdx.x; s < (unsigned)a.b.seqs; s += gridDim.x * NT)
             if (!seq_ok(a.b, a.b.starts[s], a.b.starts[s + 1], a.b.lens[s])) paged_flag(a.b, PAGED_BAD_SEQ);
         const int row = u / a.row_tiles;
         const SeqRow s = find_seq(a.b, row);
@@ -52,9 +62,10 @@ __device__ __forceinline__ bool row_tile(const AttnArgs &a, int tiles, int split
     }
     t.n = end - t.start;
     const int cols = t.n * a.group;
-    if (cols > a.small_cols || ct * kSmallTile >= cols) return false;
-    t.r0 = ct * kSmallTile / a.group;
-    t.r1 = min((ct * kSmallTile + kSmallTile - 1) / a.group, t.n - 1);
+    if (cols > a.small_cols || ct * TM >= cols) return false;
+    t.c0 = ct * TM;
+    t.r0 = t.c0 / a.group;
+    t.r1 = min((t.c0 + TM - 1) / a.group, t.n - 1);
     const TileKeys k = tile_keys(t.n, t.len, t.r0, t.r1, a.window);
     t.lo = k.lo;
     t.hi = k.hi;
@@ -64,24 +75,23 @@ __device__ __forceinline__ bool row_tile(const AttnArgs &a, int tiles, int split
     t.k1 = min(t.k0 + a.split_small, k.hi);
     t.p0 = t.len - t.n + t.r0;
     t.p1 = t.len - t.n + t.r1;
-    const int col = ct * kSmallTile + (threadIdx.x & 15);
-    t.live = col < cols;
-    t.row = t.live ? col / a.group : t.r1;
-    t.head = t.g * a.group + (t.live ? col - t.row * a.group : 0);
-    t.pos = t.len - t.n + t.row;
-    t.first = a.window > 0 ? t.pos - a.window + 1 : 0;
+    row_column(a, t, t.c0 + (threadIdx.x & 15));
     return true;
 }
 
-// Joins the four wavefronts' (m, l, o) of a tile and writes the tile's rows, or its split
-// results. o[t][r] is column lane % 16, dim VD * (4 g4 + r) + t.
-template <typename RT, int HD>
+// Joins the (m, l, o) of the NW wavefronts that have the same 16 columns, NS such sets of them in a
+// block, and writes the columns' rows, or their split results. o[t][r] is column lane % 16, dim
+// VD * (4 g4 + r) + t. All threads take part.
+template <typename RT, int HD, int NW = 4, int NS = 1>
 __device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t, float m, float l,
                                             const f32x4 (&o)[HD / 16]) {
     constexpr int VD = HD / 16, LD = HD + 4;
-    __shared__ float so[4][16][LD];
-    __shared__ float sm[4][16], sl[4][16];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
+    __shared__ float set_o[NS][NW][16][LD];
+    __shared__ float set_m[NS][NW][16], set_l[NS][NW][16];
+    const int set = NS == 1 ? 0 : threadIdx.x / (64 * NW), tid = NS == 1 ? threadIdx.x : threadIdx.x % (64 * NW);
+    float(&so)[NW][16][LD] = set_o[set];
+    float(&sm)[NW][16] = set_m[set], (&sl)[NW][16] = set_l[set];
+    const int wave = tid >> 6, lane = threadIdx.x & 63, c = lane & 15, g4 = lane >> 4;
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     if (g4 == 0) {
@@ -95,21 +105,21 @@ __device__ __forceinline__ void rows_finish(const AttnArgs &a, const RowTile &t,
             *(f32x4 *)&so[wave][c][VD * (4 * g4 + r) + v] =
                 f32x4{o[v][r], o[v + 1][r], o[v + 2][r], o[v + 3][r]};
     // The column of thread i is i / 16: this lane's own numbers come from the lane holding it.
-    const int col = threadIdx.x >> 4, d = (threadIdx.x & 15) * VD;
+    const int col = tid >> 4 & 15, d = (tid & 15) * VD;
     const int from = col;  // lanes 0..15 of any wavefront hold columns 0..15
     const int row = __shfl(t.row, from), head = __shfl(t.head, from);
     const bool live = __shfl((int)t.live, from) != 0;
     __syncthreads();
-    if (!live) return;
+    if (!live || (NW > 4 && tid >= 256)) return;
     float M = sm[0][col];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) M = fmaxf(M, sm[w][col]);
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, sm[w][col]);
     const float ref = M == -INFINITY ? 0.0f : M;
     float L = 0.0f, v[VD];
 #pragma unroll
     for (int i = 0; i < VD; ++i) v[i] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
         const float e = __builtin_amdgcn_exp2f(sm[w][col] - ref);
         L += e * sl[w][col];
 #pragma unroll
