@@ -68,8 +68,10 @@ struct CodesE4M3 {
     static __device__ __forceinline__ int along(int w) {
         return half(__builtin_amdgcn_perm(0, w, 0x000C000C | B << 8 | (B + 1) << 24));
     }
+    // Codes in the upper bytes of both halves: shifted right with their sign, whose second copy is taken out.
     static __device__ __forceinline__ int half(int x) {
-        return (int)((unsigned)(x & 0x7F007F00) >> 1) | (x & (int)0x80008000);
+        typedef short s16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(int, __builtin_bit_cast(s16x2, x) >> (short)1) & (int)0xBFFFBFFF;
     }
 };
 
@@ -174,6 +176,14 @@ __device__ __forceinline__ int64_t lane_scale(const int64_t (&sat)[N]) {
     for (int i = 1; i < N; ++i) at = b == i ? sat[i] : at;
     return at;
 }
+// log2 of a block's scale of V in units of 2^ve, by which the exponents of its probabilities are
+// raised: 2^-60 for less (a scale of 0 among them), where FP16 probabilities become 0 and their
+// fp32 sum, taken back by 2^-log, still counts them.
+__device__ __forceinline__ float scale_log(float s, int ve) {
+    const float l = __builtin_amdgcn_logf(__builtin_amdgcn_ldexpf(s, -ve));
+    return l < -60.0f ? -60.0f : l;  // (not a maximum: a scale that is not a number stays one)
+}
+
 // What lane i holds, wavefront-uniform.
 __device__ __forceinline__ float lane_value(float v, int i) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i));

@@ -11,7 +11,20 @@ namespace {
 // block's 32 NW columns, K and V as rows of FP16 whose 16-byte pieces are permuted so that the
 // fragment reads fall on all banks; two LDS buffers, one barrier a step; S^T = K . Q^T and
 // O^T += V^T . P^T on v_mfma_f32_32x32x16_f16, V^T's fragments by transposing LDS reads. But a
-// step's codes come through registers, a step ahead, and are made FP16 once, on their way to LDS.
+// step's codes come through registers, a step ahead, and are made FP16 once, on their way to LDS;
+// and a step is multiplied 32 keys at a time, which leaves the registers for the pieces of fp32 rows
+// (64 at a time they spilled: one prompt of 4096 fp32 rows 402 us, 350 with this).
+//
+// With c the code, an exponent is s ks fac - m + log2(vs / 2^ve): V's scales are in the
+// exponents of the weights, and a block's sum of them is brought back by 2^-log for the
+// denominator.
+//
+// Bound by the vector instructions beside the matrix instructions, which overlap little: per 64 keys
+// and 32 columns a wavefront has about 360 of the first (1850 cycles with the exponentials) and 1024 cycles
+// of the second a piece. 512 FP16 rows of 32 heads over 16512 tokens: 195 us with the join, 0.70
+// PFLOP/s (the 16-bit kernel over FP16 pages 0.73); twelve sequences of up to 300 fp32 rows 119 us.
+// The next half's scores beside this half's exponentials in one wavefront's instructions, with V's
+// buffer tripled, took more registers than there are (340 and 331 us).
 template <typename RT, typename C, int HD, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attn8_chunk_kernel(const Attn8Args e, int tiles, int splits) {
     typedef Half<f16> H;
@@ -120,6 +133,90 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_chunk_kernel(const Attn8Args
     for (int i = 0; i < DT; ++i) o[i] = f32x16{};
     float m = -INFINITY, l = 0.0f;
     int ve = kNoExp;
+
+    // Scores of the 32 keys of half h of K's buffer: s[r] is key 8 (r / 4) + 4 hi + r % 4 of them.
+    auto scores = [&](int buf, int h, f32x16 &s) __attribute__((always_inline)) {
+        f32x16 low{};
+        s = f32x16{};
+#pragma unroll
+        for (int i = 0; i < QC; ++i) {
+            const int row = 32 * h + q;
+            const f16x8 kf = *(const f16x8 *)(Ks[buf] + row * HD + 8 * ((2 * i + hi) ^ k_swz(row & 15)));
+            s = H::mfma32(kf, qf[0][i], s);
+            if (NP == 2) low = H::mfma32(kf, qf[NP - 1][i], low);
+        }
+        if (NP == 2) s += low;
+    };
+    // The exponentials of 32 keys from kt on, whose blocks have the scales kb and vb and the bits ok;
+    // o is brought to their units. pf are the probabilities times V's scales in those units.
+    auto weigh = [&](f32x16 &s, int kt, const float *kb, const float *vb, unsigned ok, bool masked,
+                     f16x8 (&pf)[2][NP]) __attribute__((always_inline)) {
+        unsigned some = 3;  // the blocks of which the column sees any key
+        if (masked) {
+            some = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int key = kt + 8 * (r >> 2) + 4 * hi + (r & 3);
+                if (!(key <= t.pos && key >= t.first && (ok >> (r >> 3) & 1))) s[r] = -INFINITY;
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+                some |= kt + 16 * b <= t.pos && kt + 16 * b + 15 >= t.first && (ok >> b & 1) ? 1u << b : 0u;
+        }
+        float mx = some ? kLeast : -INFINITY, f[2];
+        int vx = ve;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            // (The factor of a block that the column does not see: any, so long as -inf times it stays that.)
+            const bool sees = !masked || (some >> b & 1);
+            f[b] = fac * kb[b];
+            f[b] = !sees ? 1.0f : f[b] < FLT_MIN ? FLT_MIN : f[b];  // (not a maximum: what is not a number stays that)
+            const int v = scale_exp(vb[b]);
+            vx = sees ? max(vx, v) : vx;
+            float big = s[8 * b];
+#pragma unroll
+            for (int r = 1; r < 8; ++r) big = fmaxf(big, s[8 * b + r]);
+            mx = fmaxf(mx, big * f[b]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const bool up = mx > m + kLag, grew = up || vx != ve;
+        const float mn = up ? mx : m;
+        const float ref = mn == -INFINITY ? 0.0f : mn - kLift<f16>;
+        float corr = __builtin_amdgcn_exp2f((m == -INFINITY ? m : m - kLift<f16>) - ref);
+        m = mn;
+        l *= corr;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const float raise = !masked || (some >> b & 1) ? scale_log(vb[b], vx) : 0.0f, from = raise - ref;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[8 * b + i], f[b], from));
+                sum += p;
+                f16 pc[NP];
+                split_pieces(p, pc);
+#pragma unroll
+                for (int n = 0; n < NP; ++n) pf[b][n][i] = pc[n];
+            }
+            l = fmaf(sum, __builtin_amdgcn_exp2f(-raise), l);
+        }
+        if (__any(grew)) {
+            corr = __builtin_amdgcn_ldexpf(corr, ve - vx);
+#pragma unroll
+            for (int i = 0; i < DT; ++i) o[i] *= corr;
+            ve = vx;
+        }
+    };
+    auto outputs = [&](int vbuf, int h, const f16x8 (&pf)[2][NP]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const f16x8 f = v_frag(vbuf, 2 * h + b, d);
+#pragma unroll
+                for (int n = 0; n < NP; ++n) o[d] = H::mfma32(f, pf[b][n], o[d]);
+            }
+    };
     unsigned ok = 0;
     if (t.k0 < t.k1) {
         pages8_start(a, w, t.seq, t.lo, t.hi, t.k0);
@@ -134,105 +231,19 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_chunk_kernel(const Attn8Args
 #pragma unroll
         for (int b = 0; b < NB; ++b) kn[b] = ks[b], vn[b] = vs[b];
         if (kt + KB < t.k1) ok = load(kt + KB);
-        if (kt >= t.w_hi || kt + KB <= t.w_lo) continue;
-        f32x16 s[2];
-        __builtin_amdgcn_s_setprio(1);
-        if (NP == 1) {
-            s[0] = s[1] = f32x16{};
 #pragma unroll
-            for (int i = 0; i < QC; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = 32 * h + q;
-                    const f16x8 kf = *(const f16x8 *)(Ks[buf] + row * HD + 8 * ((2 * i + hi) ^ k_swz(row & 15)));
-                    s[h] = H::mfma32(kf, qf[0][i], s[h]);
-                }
-        } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                f32x16 p[2] = {f32x16{}, f32x16{}};
-#pragma unroll
-                for (int i = 0; i < QC; ++i) {
-                    const int row = 32 * h + q;
-                    const f16x8 kf = *(const f16x8 *)(Ks[buf] + row * HD + 8 * ((2 * i + hi) ^ k_swz(row & 15)));
-                    p[0] = H::mfma32(kf, qf[0][i], p[0]);
-                    p[1] = H::mfma32(kf, qf[NP - 1][i], p[1]);
-                }
-                s[h] = p[0] + p[1];
-            }
-        }
-        __builtin_amdgcn_s_setprio(0);
-        // s[h][r] is key kt + 32 h + 8 (r / 4) + 4 hi + r % 4, of block 2 h + r / 8.
-        const bool masked =
-            kt + KB - 1 > t.p0 || kt < t.w_lo || (a.window > 0 && kt < t.p1 - a.window + 1) || okc != 15;
-        float mx = kLeast;
-        unsigned some = 15;  // the blocks of which the column sees any key
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[h][r] *= fac * kn[2 * h + (r >> 3)];
-        if (masked) {
-            some = 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int key = kt + 32 * h + 8 * (r >> 2) + 4 * hi + (r & 3);
-                    if (!(key <= t.pos && key >= t.first && (okc >> (2 * h + (r >> 3)) & 1))) s[h][r] = -INFINITY;
-                }
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-                some |= kt + 16 * b <= t.pos && kt + 16 * b + 15 >= t.first && (okc >> b & 1) ? 1u << b : 0u;
-            mx = some ? kLeast : -INFINITY;
-        }
-        int vx = ve;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int v = scale_exp(vn[b]);
-            vx = some >> b & 1 ? max(vx, v) : vx;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[h][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const bool grew = mx > m + kLag || vx != ve;
-        const float mn = mx > m + kLag ? mx : m;
-        const float ref = mn == -INFINITY ? 0.0f : mn - kLift<f16>;
-        float corr = __builtin_amdgcn_exp2f((m == -INFINITY ? m : m - kLift<f16>) - ref);
-        m = mn;
-        float sum = 0.0f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[h][r] = __builtin_amdgcn_exp2f(s[h][r] - ref);
-                sum += s[h][r];
-            }
-        l = l * corr + sum;
-        if (__any(grew)) {
-            corr = __builtin_amdgcn_ldexpf(corr, ve - vx);
-#pragma unroll
-            for (int i = 0; i < DT; ++i) o[i] *= corr;
-            ve = vx;
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const float scale = some >> b & 1 ? __builtin_amdgcn_ldexpf(vn[b], -ve) : 0.0f;
-            f16x8 pf[NP];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                f16 pc[NP];
-                weight_pieces(s[b >> 1][8 * (b & 1) + i], scale, pc);
-#pragma unroll
-                for (int n = 0; n < NP; ++n) pf[n][i] = pc[n];
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const f16x8 f = v_frag(buf, b, d);
-#pragma unroll
-                for (int n = 0; n < NP; ++n) o[d] = H::mfma32(f, pf[n], o[d]);
-            }
+        for (int h = 0; h < 2; ++h) {
+            const int kh = kt + 32 * h;
+            if (kh >= t.w_hi || kh + 32 <= t.w_lo) continue;
+            const unsigned okh = okc >> (2 * h) & 3;
+            f32x16 s;
+            f16x8 pf[2][NP];
+            __builtin_amdgcn_s_setprio(1);
+            scores(buf, h, s);
+            __builtin_amdgcn_s_setprio(0);
+            const bool masked = kh + 31 > t.p0 || kh < t.w_lo || (a.window > 0 && kh < t.p1 - a.window + 1) || okh != 3;
+            weigh(s, kh, kn + 2 * h, vn + 2 * h, okh, masked, pf);
+            outputs(buf, h, pf);
         }
     }
     const int down = ve - kDrop + C::kExp;
@@ -249,11 +260,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_chunk_kernel(const Attn8Args
 template <typename RT, typename C>
 int attn8_chunk_launch(const Attn8Args &e, int hd, int splits, int tiles, hipStream_t st) {
     const unsigned blocks = (unsigned)tiles * (unsigned)splits * (unsigned)e.a.pool.kv_heads;
-    constexpr int NW = kChunkWaves<RT, f16>;
-    if (hd == 128)
-        hipLaunchKernelGGL((attn8_chunk_kernel<RT, C, 128, NW>), dim3(blocks), dim3(64 * NW), 0, st, e, tiles, splits);
-    else
-        hipLaunchKernelGGL((attn8_chunk_kernel<RT, C, 64, NW>), dim3(blocks), dim3(64 * NW), 0, st, e, tiles, splits);
+    auto launch = [&](auto dim, auto waves) {
+        constexpr int HD = decltype(dim)::value, NW = decltype(waves)::value;
+        hipLaunchKernelGGL((attn8_chunk_kernel<RT, C, HD, NW>), dim3(blocks), dim3(64 * NW), 0, st, e, tiles, splits);
+    };
+    auto pick = [&](auto dim) {
+        if constexpr (kPieces<RT, f16> == 1)
+            if (e.a.big_tile == 256) return launch(dim, std::integral_constant<int, 8>{});
+        launch(dim, std::integral_constant<int, 4>{});
+    };
+    hd == 128 ? pick(std::integral_constant<int, 128>{}) : pick(std::integral_constant<int, 64>{});
     return launch_status();
 }
 

@@ -324,7 +324,11 @@ int attn8_args(const gphq_paged8_kv *kv, const gphq_paged_batch *b, int row_dtyp
     if (row_dtype != GPHQ_DTYPE_F32 && row_dtype != GPHQ_DTYPE_F16 && row_dtype != GPHQ_DTYPE_BF16)
         return GPHQ_ERR_UNSUPPORTED;
     GPHQ_TRY(head_args(&kv->codes, b, heads, window, e.a));
-    e.a.big_tile = 32 * (row_dtype == GPHQ_DTYPE_F32 ? kChunkWaves<float, f16> : kChunkWaves<f16, f16>);
+    // Tiles of eight wavefronts make a step's codes FP16 for twice the columns: 512 FP16 rows of four heads
+    // a KV head over 16512 tokens 220 us, with four wavefronts 245. Short sequences waste more of them (three
+    // of 83 to 234 rows over 6000 tokens 138 and 130 us), and fp32 rows gain nothing (4096: 349 and 350).
+    const bool wide = row_dtype != GPHQ_DTYPE_F32 && e.a.b.seqs && (int64_t)e.a.b.rows * e.a.group / e.a.b.seqs >= 1024;
+    e.a.big_tile = wide ? 256 : 128;
     return GPHQ_OK;
 }
 
