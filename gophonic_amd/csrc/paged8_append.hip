@@ -25,13 +25,21 @@ struct Append8Args {
     const float *qn, *kn, *cos, *sin;
     int64_t qkv_stride, q_stride;
     int rope_rows, heads;
-    int span;          // rows whose blocks one wavefront of the key and value part looks for
-    int q_parts;       // wavefronts of a row in the query part
+    int span, kv_parts;  // rows whose blocks one block of the key and value part looks for; blocks that share their heads
+    int q_parts;         // wavefronts of a row in the query part
     unsigned kv_blocks;  // blocks of the key and value part; the query part's come behind them
     double eps;
     float qscale;
 };
 
+// Another lane's value, by a DPP control that exchanges lanes of a row of 16.
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ double shfl_xor_f64(double v, int mask) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = __shfl_xor((int)(uint32_t)u, mask), hi = __shfl_xor((int)(uint32_t)(u >> 32), mask);
@@ -86,84 +94,94 @@ __device__ __forceinline__ void store_codes(char *p, int w) {
         *(uint16_t *)p = (uint16_t)w;
 }
 
-// The new tokens [n0, n1) of one block of a sequence, which stand in rows row .. of the batch,
-// for one KV head's keys or values. 16 lanes to a token, lane j holding values E j .. of both
-// halves (a rotary pair is in one lane), four tokens at a time: tokens 4 i + lane / 16.
+// The new tokens [n0, n1) of one block of a sequence, which stand in rows row .. of the batch:
+// keys and values of every kv_parts-th KV head from `part` on. A block's 256 threads take the 16
+// tokens, 16 lanes each, lane j of them holding values E j .. of both halves (a rotary pair is in one
+// lane); the wavefronts' largest magnitudes meet in LDS, in two places in turn, so that one barrier
+// a head is enough.
 template <typename RT, typename C, int HD>
-__device__ __forceinline__ void append_block(const Append8Args &a, int row, int n0, int n1, int page, bool key,
-                                             int head) {
+__device__ __forceinline__ void append_block(const Append8Args &a, int row, int n0, int n1, int page, int part) {
     constexpr int E = HD / 32;
-    const int lane = threadIdx.x & 63, j = lane & 15, slot = lane >> 4;
+    __shared__ double tops[2][4];
+    const int lane = threadIdx.x & 63, j = lane & 15, wave = threadIdx.x >> 6;
     const int b0 = n0 & ~(kBlockTokens - 1), kvh = a.pool.kv_heads;
-    const RT *src = (const RT *)a.qkv + (int64_t)(a.heads + (key ? 0 : kvh) + head) * HD + E * j;
-    const float *w = key ? a.kn : nullptr;
-    const bool rotate = key && a.cos;
-    float w0[E], w1[E];
-    if (w) {
-        load_vec(w + E * j, w0);
-        load_vec(w + HD / 2 + E * j, w1);
+    const int pos = b0 + (threadIdx.x >> 4);
+    const bool mine = pos >= n0 && pos < n1, earlier = pos < n0;
+    const int p = mine ? pos : n0;
+    const RT *src = (const RT *)a.qkv + (int64_t)(row + p - n0) * a.qkv_stride + (int64_t)a.heads * HD + E * j;
+    const int in = b0 & ((1 << a.pool.shift) - 1);
+    const int64_t code_at = (int64_t)page * a.pool.page_stride + (int64_t)(in + pos - b0) * a.pool.token_stride + E * j;
+    const int64_t scale_at = (int64_t)page * a.s.page_stride + in / kBlockTokens;
+    float x0[E], x1[E], w0[E], w1[E], cs[E], sn[E];
+    load_vec(src + (int64_t)part * HD, x0);
+    load_vec(src + (int64_t)part * HD + HD / 2, x1);
+    if (a.kn) {
+        load_vec(a.kn + E * j, w0);
+        load_vec(a.kn + HD / 2 + E * j, w1);
     }
-    double y[4][2 * E];
-    double most = 0.0;
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int pos = b0 + 4 * i + slot;
-        const bool mine = pos >= n0 && pos < n1;
-        const int p = mine ? pos : n0;
-        const RT *x = src + (int64_t)(row + p - n0) * a.qkv_stride;
-        float x0[E], x1[E];
-        load_vec(x, x0);
-        load_vec(x + HD / 2, x1);
-        double sum = 0.0;
+    if (a.cos) {
+        load_vec(a.cos + (int64_t)p * (HD / 2) + E * j, cs);
+        load_vec(a.sin + (int64_t)p * (HD / 2) + E * j, sn);
+    }
+    int turn = 0;
+    for (int item = part; item < 2 * kvh; item += a.kv_parts, turn ^= 1) {
+        const bool key = item < kvh;
+        const int head = key ? item : item - kvh;
+        char *codes = (char *)(key ? a.pool.k : a.pool.v) + code_at + (int64_t)head * a.pool.head_stride;
+        float *at = (key ? a.s.k : a.s.v) + scale_at + (int64_t)head * a.s.head_stride;
+        const float old = n0 > b0 ? *at : 0.0f;  // read by all before the barrier, written behind it
+        double y[2 * E], sum = 0.0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            y[i][e] = x0[e];
-            y[i][E + e] = x1[e];
-            sum += y[i][e] * y[i][e] + y[i][E + e] * y[i][E + e];
+            y[e] = x0[e];
+            y[E + e] = x1[e];
+            sum += y[e] * y[e] + y[E + e] * y[E + e];
         }
-        if (w) {
-#pragma unroll
-            for (int d = 1; d < 16; d *= 2) sum += shfl_xor_f64(sum, d);
+        if (item + a.kv_parts < 2 * kvh) {  // the next head's values, while these are worked on
+            load_vec(src + (int64_t)(item + a.kv_parts) * HD, x0);
+            load_vec(src + (int64_t)(item + a.kv_parts) * HD + HD / 2, x1);
+        }
+        if (key && a.kn) {
+            sum += dpp_f64<0xB1>(sum);
+            sum += dpp_f64<0x4E>(sum);
+            sum += dpp_f64<0x141>(sum);
+            sum += dpp_f64<0x140>(sum);
             const double inv = 1.0 / sqrt(sum / HD + a.eps);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                y[i][e] *= inv * w0[e];
-                y[i][E + e] *= inv * w1[e];
+                y[e] *= inv * w0[e];
+                y[E + e] *= inv * w1[e];
             }
         }
-        if (rotate) {
-            float cs[E], sn[E];
-            load_vec(a.cos + (int64_t)p * (HD / 2) + E * j, cs);
-            load_vec(a.sin + (int64_t)p * (HD / 2) + E * j, sn);
+        if (key && a.cos) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const double u = y[i][e], v = y[i][E + e];
-                y[i][e] = u * cs[e] - v * sn[e];
-                y[i][E + e] = v * cs[e] + u * sn[e];
+                const double u = y[e], v = y[E + e];
+                y[e] = u * cs[e] - v * sn[e];
+                y[E + e] = v * cs[e] + u * sn[e];
             }
         }
+        double most = 0.0;
+        bool odd = false;
 #pragma unroll
         for (int e = 0; e < 2 * E; ++e) {
-            const bool fine = fabs(y[i][e]) < (double)INFINITY;
+            const bool fine = fabs(y[e]) < (double)INFINITY;
             odd |= mine && !fine;
-            if (!fine) y[i][e] = 0.0;
-            most = mine ? fmax(most, fabs(y[i][e])) : most;
+            if (!fine) y[e] = 0.0;
+            most = mine ? fmax(most, fabs(y[e])) : most;
         }
-    }
-    if (odd) paged_flag(a.b, PAGED_BAD_VALUE);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) most = fmax(most, shfl_xor_f64(most, d));
+        if (odd) paged_flag(a.b, PAGED_BAD_VALUE);
+        most = fmax(most, dpp_f64<0xB1>(most));
+        most = fmax(most, dpp_f64<0x4E>(most));
+        most = fmax(most, dpp_f64<0x141>(most));
+        most = fmax(most, dpp_f64<0x140>(most));
+        most = fmax(most, shfl_xor_f64(most, 16));
+        most = fmax(most, shfl_xor_f64(most, 32));
+        if (lane == 0) tops[turn][wave] = most;
+        __syncthreads();
+        most = fmax(fmax(tops[turn][0], tops[turn][1]), fmax(tops[turn][2], tops[turn][3]));
 
-    const int in = b0 & ((1 << a.pool.shift) - 1);
-    char *codes = (char *)(key ? a.pool.k : a.pool.v) + (int64_t)page * a.pool.page_stride +
-                  (int64_t)head * a.pool.head_stride + (int64_t)in * a.pool.token_stride + E * j;
-    float *at = (key ? a.s.k : a.s.v) + (int64_t)page * a.s.page_stride + (int64_t)head * a.s.head_stride +
-                in / kBlockTokens;
-    float scale = most > 0.0 ? fmaxf((float)(most / C::kTop), 0x1p-126f) : 0.0f;
-    scale = fminf(scale, FLT_MAX);
-    if (n0 > b0) {
-        const float old = *at;
+        float scale = most > 0.0 ? fminf(fmaxf((float)(most / C::kTop), 0x1p-126f), FLT_MAX) : 0.0f;
         if (old > 0.0f && old < INFINITY) {
             const double r = most / ((double)C::kOver * old);
             int k = 0;
@@ -172,38 +190,30 @@ __device__ __forceinline__ void append_block(const Append8Args &a, int row, int 
                 k = __builtin_amdgcn_frexp_mant(r) == 0.5 ? e - 1 : e;
             }
             scale = __builtin_amdgcn_ldexpf(old, k);
-            if (k) {
+            if (k && earlier) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (b0 + 4 * i + slot >= n0) continue;
-                    char *p = codes + (int64_t)(4 * i + slot) * a.pool.token_stride;
+                for (int h = 0; h < 2; ++h) {
+                    double c[E];
+                    decode<C>(load_codes<E>(codes + h * (HD / 2)), c);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        double c[E];
-                        decode<C>(load_codes<E>(p + h * (HD / 2)), c);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) c[e] = ldexp(c[e], -k);
-                        store_codes<E>(p + h * (HD / 2), encode<C>(c));
-                    }
+                    for (int e = 0; e < E; ++e) c[e] = ldexp(c[e], -k);
+                    store_codes<E>(codes + h * (HD / 2), encode<C>(c));
                 }
             }
         }
-    }
-    if (lane == 0) *at = scale;
-    const double inv = scale > 0.0f ? 1.0 / (double)scale : 0.0;
+        if (threadIdx.x == 0) *at = scale;
+        const double inv = scale > 0.0f ? 1.0 / (double)scale : 0.0;
+        if (mine) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int pos = b0 + 4 * i + slot;
-        if (pos < n0 || pos >= n1) continue;
-        char *p = codes + (int64_t)(4 * i + slot) * a.pool.token_stride;
+            for (int h = 0; h < 2; ++h) {
+                double c[E];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            double c[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) c[e] = y[i][h * E + e] * inv;
-            store_codes<E>(p + h * (HD / 2), encode<C>(c));
+                for (int e = 0; e < E; ++e) c[e] = y[h * E + e] * inv;
+                store_codes<E>(codes + h * (HD / 2), encode<C>(c));
+            }
         }
     }
+    __syncthreads();  // the last heads' tops have been read
 }
 
 // What find_seq says of a row, checked: false (and flagged) for a row that no sequence brings.
@@ -222,17 +232,15 @@ __device__ __forceinline__ bool row_of(const PagedBatch &b, int row, SeqRow &s) 
     return true;
 }
 
-// One grid for both parts. Keys and values: a wavefront takes one head's keys or values of the
-// blocks whose first new token lies in `span` rows of the batch. Queries: a wavefront takes every
-// q_parts-th four heads of a row.
+// One grid for both parts. Keys and values: a block takes every kv_parts-th head's keys or values of
+// the 16-token blocks whose first new token lies in `span` rows of the batch. Queries: a wavefront
+// takes every q_parts-th four heads of a row.
 template <typename RT, typename C, int HD>
 __global__ __launch_bounds__(256) void paged8_append_kernel(const Append8Args a) {
     constexpr int E = HD / 32;
     const int lane = threadIdx.x & 63, j = lane & 15, slot = lane >> 4;
-    const int kvh = a.pool.kv_heads;
     if (blockIdx.x < a.kv_blocks) {
-        const int unit = uniform((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-        const int group = unit / (2 * kvh), item = unit - group * 2 * kvh;
+        const int group = blockIdx.x / a.kv_parts, part = blockIdx.x - group * a.kv_parts;
         const int r1 = min((group + 1) * a.span, a.b.rows);
         for (int row = group * a.span; row < r1;) {
             SeqRow s;
@@ -250,7 +258,7 @@ __global__ __launch_bounds__(256) void paged8_append_kernel(const Append8Args a)
             if (lead) {
                 const int page = a.b.table[s.seq * a.b.table_stride + (pos >> a.pool.shift)];
                 if (page >= 0 && page < a.pool.pages)
-                    append_block<RT, C, HD>(a, row, pos, n1, page, item < kvh, item < kvh ? item : item - kvh);
+                    append_block<RT, C, HD>(a, row, pos, n1, page, part);
                 else if (lane == 0)
                     paged_flag(a.b, PAGED_BAD_PAGE);
             }
@@ -261,6 +269,12 @@ __global__ __launch_bounds__(256) void paged8_append_kernel(const Append8Args a)
     const int unit = uniform((int)((blockIdx.x - a.kv_blocks) * 4 + (threadIdx.x >> 6)));
     const int row = unit / a.q_parts, part = unit - row * a.q_parts;
     if (row >= a.b.rows) return;
+    const RT *src = (const RT *)a.qkv + (int64_t)row * a.qkv_stride + E * j;
+    RT *dst = (RT *)a.q + (int64_t)row * a.q_stride + E * j;
+    int h = 4 * part + slot, hc = min(h, a.heads - 1);  // every lane takes part in the lane exchanges
+    float x0[E], x1[E];
+    load_vec(src + (int64_t)hc * HD, x0);
+    load_vec(src + (int64_t)hc * HD + HD / 2, x1);
     SeqRow s;
     if (!row_of(a.b, row, s)) return;
     const int pos = s.len - (s.end - row);
@@ -281,13 +295,18 @@ __global__ __launch_bounds__(256) void paged8_append_kernel(const Append8Args a)
         load_vec(a.qn + E * j, w0);
         load_vec(a.qn + HD / 2 + E * j, w1);
     }
-    const RT *src = (const RT *)a.qkv + (int64_t)row * a.qkv_stride + E * j;
-    RT *dst = (RT *)a.q + (int64_t)row * a.q_stride + E * j;
-    for (int h0 = 4 * part; h0 < a.heads; h0 += 4 * a.q_parts) {
-        const int h = h0 + slot, hc = min(h, a.heads - 1);  // every lane takes part in the lane exchanges
+    for (;;) {
         float y0[E], y1[E];
-        load_vec(src + (int64_t)hc * HD, y0);
-        load_vec(src + (int64_t)hc * HD + HD / 2, y1);
+#pragma unroll
+        for (int e = 0; e < E; ++e) y0[e] = x0[e], y1[e] = x1[e];
+        const int now = h;
+        h += 4 * a.q_parts;
+        const bool more = uniform(h - slot) < a.heads;
+        if (more) {  // the next heads' values, while these are worked on
+            hc = min(h, a.heads - 1);
+            load_vec(src + (int64_t)hc * HD, x0);
+            load_vec(src + (int64_t)hc * HD + HD / 2, x1);
+        }
         if (a.qn) {
             float v = 0.0f;
 #pragma unroll
@@ -308,15 +327,16 @@ __global__ __launch_bounds__(256) void paged8_append_kernel(const Append8Args a)
                 y1[e] = v * cs[e] + u * sn[e];
             }
         }
-        if (h < a.heads) {
+        if (now < a.heads) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 y0[e] *= a.qscale;
                 y1[e] *= a.qscale;
             }
-            store_vec(dst + (int64_t)h * HD, y0);
-            store_vec(dst + (int64_t)h * HD + HD / 2, y1);
+            store_vec(dst + (int64_t)now * HD, y0);
+            store_vec(dst + (int64_t)now * HD + HD / 2, y1);
         }
+        if (!more) break;
     }
 }
 
@@ -371,14 +391,15 @@ extern "C" int gphq_paged8_append(const gphq_paged8_kv *kv, const gphq_paged_bat
     a.eps = eps;
     a.qscale = (float)q_scale;
     const int64_t rows = a.b.rows;
-    // Rows that a wavefront looks through for blocks, and no more than 2^22 wavefronts.
-    a.span = (int)std::max<int64_t>(a.b.max_rows == 1 ? 1 : 4, (rows * 2 * kvh + (1 << 22) - 1) >> 22);
-    const int64_t kv_units = (rows + a.span - 1) / a.span * 2 * kvh;
-    // Wavefronts per row of queries: all of a row's heads at once while that leaves the chip
-    // short of wavefronts, else fewer, each over several groups of four.
-    const int64_t groups = (heads + 3) / 4, want = 32ll * device_cus();
+    // A single token's row is its block's; else four rows are looked through for the first of a block.
+    a.span = a.b.max_rows == 1 ? 1 : 4;
+    // Blocks that share a row group's heads: all while that leaves the chip short of wavefronts, else fewer.
+    const int64_t spans = (rows + a.span - 1) / a.span, want = 32ll * device_cus();
+    a.kv_parts = (int)std::min<int64_t>(2 * kvh, std::max<int64_t>(1, want / 4 / spans));
+    // Wavefronts per row of queries, likewise: of its heads four at a time.
+    const int64_t groups = (heads + 3) / 4;
     a.q_parts = (int)std::min<int64_t>(groups, std::max<int64_t>(1, (want + rows - 1) / rows));
-    a.kv_blocks = (unsigned)((kv_units + 3) / 4);
+    a.kv_blocks = (unsigned)(spans * a.kv_parts);
     const unsigned blocks = a.kv_blocks + (unsigned)((rows * a.q_parts + 3) / 4);
     hipStream_t st = (hipStream_t)stream;
     const bool i8 = kv->codes.dtype == GPHQ_DTYPE_I8;
