@@ -163,50 +163,62 @@ void prob_cut(int64_t rows, int64_t n, int &len, int &parts) {
 
 // ---- drafts ---------------------------------------------------------------------
 
+constexpr int kStretch = 64 * kPer;  // values of a row whose weights a wavefront sums
+
 struct VerifyArgs {
     const int32_t *starts, *drafts, *lens;
     const float *target, *draft, *accept_u, *sample_u;
-    int32_t *tokens, *accepted, *kept, *decided;  // decided: [seqs], of the workspace
-    double2 *sums;                                // [seqs][tiles]: of w, and of the target's row
+    int32_t *tokens, *accepted, *kept;
+    int2 *decided;   // [seqs]: the row that a sequence's token is taken from, and the draft not to be taken
+    double2 *sums;   // [seqs][stretches]: of w, and of the target's row
     int64_t target_stride, draft_stride;
-    int seqs, rows, n, tiles;
+    int seqs, rows, n, stretches;
 };
 
-__device__ __forceinline__ double shfl_up_f64(double v, int d) {
+template <int CTRL>
+__device__ __forceinline__ double shifted(double v) {  // 0 where the row of 16 lanes has no such lane
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __shfl_up((int)(uint32_t)u, d), hi = __shfl_up((int)(uint32_t)(u >> 32), d);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// Sum over the threads up to this one of a block, and over all, in a fixed order.
-__device__ __forceinline__ double block_scan(double v, double &total) {
-    __shared__ double lds[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double u = shfl_up_f64(v, d);
-        if (lane >= d) v += u;
-    }
-    __syncthreads();  // lds of the last scan has been read
-    if (lane == 63) lds[wave] = v;
-    __syncthreads();
-    double before = 0.0;
-    for (int w = 0; w < wave; ++w) before += lds[w];
-    total = lds[0] + lds[1] + lds[2] + lds[3];
-    return before + v;
+// Sum over the lanes up to this one of a wavefront, and over all, in a fixed order.
+__device__ __forceinline__ double wave_scan(double v, double &total) {
+    v += shifted<0x111>(v);
+    v += shifted<0x112>(v);
+    v += shifted<0x114>(v);
+    v += shifted<0x118>(v);
+    const double a = lane_f64(v, 15), b = lane_f64(v, 31), c = lane_f64(v, 47);
+    const int row = (threadIdx.x & 63) >> 4;
+    v += row == 0 ? 0.0 : row == 1 ? a : row == 2 ? a + b : (a + b) + c;
+    total = lane_f64(v, 63);
+    return v;
 }
 
 __device__ __forceinline__ double weight(double v) { return v > 0.0 ? v : 0.0; }
 
-// This thread's kPer neighbouring weights of a tile: w, and the target's alone.
+// The rows that a sequence's token is taken from.
 struct Row {
     const float *p, *q;  // q NULL: certain of x
     int x;               // the draft; -1: w is the target's row
 };
+__device__ __forceinline__ Row row_at(const VerifyArgs &a, int row, int x) {
+    return Row{a.target + (int64_t)row * a.target_stride,
+               x >= 0 && a.draft ? a.draft + (int64_t)row * a.draft_stride : nullptr, x};
+}
+
+// This lane's kPer neighbouring weights of a stretch: w, and the target's alone.
 template <bool VEC>
-__device__ __forceinline__ void tile_weights(const VerifyArgs &a, const Row &r, int tile, double (&w)[kPer],
-                                             double (&t)[kPer]) {
-    const int i = tile * kTile + kPer * threadIdx.x;
+__device__ __forceinline__ void stretch_weights(const VerifyArgs &a, const Row &r, int stretch, double (&w)[kPer],
+                                                double (&t)[kPer]) {
+    const int i = stretch * kStretch + kPer * (threadIdx.x & 63);
     float p[kPer], q[kPer];
     load_row<VEC>(r.p, i, a.n, 0.0f, p);
     if (r.q) load_row<VEC>(r.q, i, a.n, 0.0f, q);
@@ -216,15 +228,15 @@ __device__ __forceinline__ void tile_weights(const VerifyArgs &a, const Row &r, 
         w[k] = r.x < 0 ? t[k] : r.q ? weight((double)p[k] - (double)q[k]) : i + k == r.x ? 0.0 : t[k];
     }
 }
-
-__device__ __forceinline__ Row row_at(const VerifyArgs &a, int row, int last) {
-    Row r{a.target + (int64_t)row * a.target_stride, nullptr, -1};
-    if (row == last) return r;
-    const int x = a.drafts[row];
-    if (x < 0 || x >= a.n) return r;
-    r.x = x;
-    if (a.draft) r.q = a.draft + (int64_t)row * a.draft_stride;
-    return r;
+__device__ __forceinline__ double lane_sum(const double (&w)[kPer]) {
+    double s[kPer / 2];
+#pragma unroll
+    for (int k = 0; k < kPer / 2; ++k) s[k] = w[2 * k] + w[2 * k + 1];
+#pragma unroll
+    for (int n = kPer / 4; n > 0; n /= 2)
+#pragma unroll
+        for (int k = 0; k < n; ++k) s[k] = s[2 * k] + s[2 * k + 1];
+    return s[0];
 }
 
 // A sequence's rows [first, last]; false for one that has none or whose starts are bad.
@@ -234,132 +246,125 @@ __device__ __forceinline__ bool rows_of(const VerifyArgs &a, int s, int &first, 
     return first >= 0 && last >= first && last < a.rows;
 }
 
-// The first row of [first, last) whose draft is not accepted, last if there is none; by each wavefront.
-__device__ __forceinline__ int decide(const VerifyArgs &a, int first, int last) {
+// The first row of [first, last) whose draft is not accepted, last if there is none, and that
+// draft (-1: none of the vocabulary); by each wavefront.
+__device__ __forceinline__ int2 decide(const VerifyArgs &a, int first, int last) {
     const int lane = threadIdx.x & 63;
     for (int r0 = first; r0 < last; r0 += 64) {
         const int r = r0 + lane;
         bool fails = false;
+        int x = -1;
         if (r < last) {
-            const int x = a.drafts[r];
+            x = a.drafts[r];
             const bool in = x >= 0 && x < a.n;
             const double p = in ? a.target[(int64_t)r * a.target_stride + x] : 0.0;
             const double q = !a.draft ? 1.0 : in ? a.draft[(int64_t)r * a.draft_stride + x] : 0.0;
             fails = !in || !((double)a.accept_u[r] * q < p);
+            x = in ? x : -1;
         }
         const uint64_t b = __ballot(fails);
-        if (b) return r0 + __builtin_ctzll(b);
+        if (b) {
+            const int at = __builtin_ctzll(b);
+            return int2{r0 + at, __builtin_amdgcn_readlane(x, at)};
+        }
     }
-    return last;
+    return int2{last, -1};
 }
 
+// Four stretches of a sequence's row to a block, whose wavefronts have nothing to say to each
+// other. Bound by memory for many sequences, two rows of the vocabulary each (64 of 151936: 78 MB).
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyArgs a) {
-    const int s = blockIdx.x / a.tiles, tile = blockIdx.x - s * a.tiles;
+    const int blocks = (a.stretches + 3) / 4, s = blockIdx.x / blocks;
+    const int stretch = uniform((int)(blockIdx.x - s * blocks) * 4 + (int)(threadIdx.x >> 6));
     int first, last;
-    if (!rows_of(a, s, first, last)) return;
-    const int row = decide(a, first, last);
-    const Row r = row_at(a, row, last);
-    double w[kPer], t[kPer], ws = 0.0, ts = 0.0;
-    tile_weights<VEC>(a, r, tile, w, t);
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) ws += w[k], ts += t[k];
-    double wt, tt;
-    block_scan(ws, wt);
-    block_scan(ts, tt);
-    if (threadIdx.x == 0) {
-        a.sums[blockIdx.x] = double2{wt, tt};
-        if (tile == 0) a.decided[s] = row;
+    if (stretch >= a.stretches || !rows_of(a, s, first, last)) return;
+    const int2 at = decide(a, first, last);
+    double w[kPer], t[kPer], wt, tt;
+    stretch_weights<VEC>(a, row_at(a, at.x, at.y), stretch, w, t);
+    wave_scan(lane_sum(w), wt);
+    wave_scan(lane_sum(t), tt);
+    if ((threadIdx.x & 63) == 0) {
+        a.sums[(int64_t)s * a.stretches + stretch] = double2{wt, tt};
+        if (stretch == 0) a.decided[s] = at;
     }
 }
 
-// One block a sequence: the tile in which the sum passes the number, then the token in it.
+// One wavefront a sequence: the stretch in which the sum passes the number, then the token in it.
+// All latency: the stretches' sums 64 at a time, then one stretch's weights.
 template <bool VEC>
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(const VerifyArgs a) {
-    const int s = blockIdx.x, tid = threadIdx.x;
+__global__ __launch_bounds__(64) void verify_pick_kernel(const VerifyArgs a) {
+    const int s = blockIdx.x, lane = threadIdx.x;
     int first, last;
     if (!rows_of(a, s, first, last)) {
-        if (tid == 0) {
+        if (lane == 0) {
             a.accepted[s] = first >= 0 && last == first - 1 && first <= a.rows ? 0 : -1;
             if (a.kept) a.kept[s] = a.lens[s];
         }
         return;
     }
-    const int row = a.decided[s];
-    Row r = row_at(a, row, last);
-    const double2 *sums = a.sums + (int64_t)s * a.tiles;
-    // Each thread sums a run of neighbouring tiles.
-    const int run = (a.tiles + kThreads - 1) / kThreads, t0 = min(tid * run, a.tiles), t1 = min(t0 + run, a.tiles);
+    const int2 at = a.decided[s];
+    const float u = a.sample_u[s];
+    const double2 *sums = a.sums + (int64_t)s * a.stretches;
     double ws = 0.0, ts = 0.0, wt, tt;
-    for (int i = t0; i < t1; ++i) ws += sums[i].x, ts += sums[i].y;
-    double at = block_scan(ws, wt);
-    const double at_t = block_scan(ts, tt);
+    for (int i = lane; i < a.stretches; i += 64) ws += sums[i].x, ts += sums[i].y;
+    wave_scan(ws, wt);
+    wave_scan(ts, tt);
+    Row r = row_at(a, at.x, at.y);
     if (wt == 0.0) {  // no weight left: the target's row
-        r.x = -1;
-        at = at_t;
-        ws = ts;
+        r = row_at(a, at.x, -1);
         wt = tt;
     }
-    const float u = a.sample_u[s];
     const double goal = (double)(u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f) * wt;
-    __shared__ int found, fallback;
-    if (tid == 0) found = INT32_MAX, fallback = -1;
-    __syncthreads();
-    double sum = at - ws;
-    for (int i = t0; i < t1; ++i) {
-        const double v = r.x < 0 ? sums[i].y : sums[i].x;
-        sum += v;
-        if (v > 0.0) {
-            if (sum > goal) atomicMin(&found, i);
-            atomicMax(&fallback, i);
+    // The first stretch with a weight behind which the sum is over goal, else the last with a weight.
+    int stretch = -1;
+    bool any = false;
+    double before = 0.0, at_stretch = 0.0;
+    for (int i0 = 0; i0 < a.stretches && !any; i0 += 64) {
+        const int i = i0 + lane;
+        const double v = i < a.stretches ? (r.x < 0 ? sums[i].y : sums[i].x) : 0.0;
+        double total;
+        const double c = before + wave_scan(v, total);
+        const uint64_t over = __ballot(v > 0.0 && c > goal), some = __ballot(v > 0.0);
+        any = over != 0;
+        if (some) {
+            const int n = any ? __builtin_ctzll(over) : last_lane(some);
+            stretch = i0 + n;
+            at_stretch = lane_f64(c, n) - lane_f64(v, n);
         }
+        before += total;
     }
-    __syncthreads();
-    const int tile = found < INT32_MAX ? found : fallback;
-    const bool any = found < INT32_MAX;
-    // The sum before that tile, from the thread that holds it.
-    __shared__ double before;
-    if (tile >= t0 && tile < t1) {
-        double b = at - ws;
-        for (int i = t0; i < tile; ++i) b += r.x < 0 ? sums[i].y : sums[i].x;
-        before = b;
-    }
-    __syncthreads();
     int token = 0;
-    if (tile >= 0) {
-        const double b = before;
-        double w[kPer], t[kPer], mine = 0.0, total;
-        tile_weights<VEC>(a, r, tile, w, t);
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) mine += w[k];
-        double c = b + (block_scan(mine, total) - mine);
-        if (tid == 0) found = INT32_MAX, fallback = -1;
-        __syncthreads();
-        int hit = INT32_MAX, end = -1;
+    if (stretch >= 0) {
+        double w[kPer], t[kPer], total;
+        stretch_weights<VEC>(a, r, stretch, w, t);
+        const double mine = lane_sum(w);
+        double c = at_stretch + (wave_scan(mine, total) - mine);
+        int hit = -1, end = -1;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             c += w[k];
             if (w[k] > 0.0) {
-                end = tile * kTile + kPer * tid + k;
-                if (any && c > goal && hit == INT32_MAX) hit = end;
+                end = k;
+                if (hit < 0 && c > goal) hit = k;
             }
         }
-        if (hit < INT32_MAX) atomicMin(&found, hit);
-        if (end >= 0) atomicMax(&fallback, end);
-        __syncthreads();
-        token = found < INT32_MAX ? found : max(fallback, 0);
+        const uint64_t hits = __ballot(any && hit >= 0), ends = __ballot(end >= 0);
+        const int n = hits ? __builtin_ctzll(hits) : last_lane(ends);
+        token = stretch * kStretch + kPer * n + max(__builtin_amdgcn_readlane(hits ? hit : end, n), 0);
     }
-    for (int i = first + tid; i <= last; i += kThreads) {
-        const int v = i < row ? a.drafts[i] : i == row ? token : -1;
+    for (int i = first + lane; i <= last; i += 64) {
+        const int v = i < at.x ? a.drafts[i] : i == at.x ? token : -1;
         a.tokens[i] = v;
     }
-    if (tid == 0) {
-        a.accepted[s] = row - first;
-        if (a.kept) a.kept[s] = a.lens[s] - (last - row);
+    if (lane == 0) {
+        a.accepted[s] = at.x - first;
+        if (a.kept) a.kept[s] = a.lens[s] - (last - at.x);
     }
 }
 
-int verify_tiles(int64_t n) { return (int)((n + kTile - 1) / kTile); }
+int verify_stretches(int64_t n) { return (int)((n + kStretch - 1) / kStretch); }
+int64_t verify_blocks(int64_t seqs, int64_t n) { return seqs * ((verify_stretches(n) + 3) / 4); }
 
 bool rows16(const void *p, int64_t stride) { return (uintptr_t)p % 16 == 0 && stride % 4 == 0; }
 
@@ -411,9 +416,9 @@ int gphq_probabilities(const float *x, int64_t x_stride, const float *temperatur
 
 int64_t gphq_verify_drafts_workspace_bytes(int64_t seqs, int64_t vocab) {
     if (seqs < 0 || seqs > GPHQ_PAGED_MAX_SEQS || vocab < 1 || vocab > GPHQ_SAMPLE_MAX_VOCAB ||
-        seqs * verify_tiles(vocab) > (1 << 23) - 1)
+        verify_blocks(seqs, vocab) > (1 << 23) - 1)
         return GPHQ_ERR_DIMENSIONS;
-    return seqs * verify_tiles(vocab) * (int64_t)sizeof(double2) + (seqs * 4 + 15) / 16 * 16;
+    return seqs * verify_stretches(vocab) * (int64_t)sizeof(double2) + (seqs * (int64_t)sizeof(int2) + 15) / 16 * 16;
 }
 
 int gphq_verify_drafts(const int32_t *starts, const int32_t *drafts, const float *target, int64_t target_stride,
@@ -432,12 +437,12 @@ int gphq_verify_drafts(const int32_t *starts, const int32_t *drafts, const float
                            (uintptr_t)accept_u | (uintptr_t)sample_u | (uintptr_t)tokens | (uintptr_t)accepted |
                            (uintptr_t)lens | (uintptr_t)kept;
     if (bits % 4 || !work || (uintptr_t)work % 16 || work_bytes < need) return GPHQ_ERR_DIMENSIONS;
-    const int tiles = verify_tiles(vocab);
+    const int stretches = verify_stretches(vocab);
     double2 *sums = (double2 *)work;
-    VerifyArgs a{starts, drafts,  lens, target, draft, accept_u, sample_u, tokens, accepted, kept,
-                 (int32_t *)(sums + seqs * tiles), sums, target_stride, draft_stride, (int)seqs, (int)rows, (int)vocab,
-                 tiles};
-    const dim3 grid((unsigned)(seqs * tiles));
+    VerifyArgs a{starts, drafts, lens, target, draft, accept_u, sample_u, tokens, accepted, kept,
+                 (int2 *)(sums + seqs * stretches), sums, target_stride, draft_stride, (int)seqs, (int)rows, (int)vocab,
+                 stretches};
+    const dim3 grid((unsigned)verify_blocks(seqs, vocab));
     hipStream_t st = (hipStream_t)stream;
     const bool vec = rows16(target, target_stride) && (!draft || rows16(draft, draft_stride));
     if (vec)
@@ -446,9 +451,9 @@ int gphq_verify_drafts(const int32_t *starts, const int32_t *drafts, const float
         hipLaunchKernelGGL(verify_sums_kernel<false>, grid, dim3(kThreads), 0, st, a);
     GPHQ_TRY(launch_status());
     if (vec)
-        hipLaunchKernelGGL(verify_pick_kernel<true>, dim3((unsigned)seqs), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL(verify_pick_kernel<true>, dim3((unsigned)seqs), dim3(64), 0, st, a);
     else
-        hipLaunchKernelGGL(verify_pick_kernel<false>, dim3((unsigned)seqs), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL(verify_pick_kernel<false>, dim3((unsigned)seqs), dim3(64), 0, st, a);
     return launch_status();
 }
 

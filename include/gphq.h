@@ -686,8 +686,8 @@ int gphq_paged8_append(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, 
  * times a block's scale keep 22 bits in sequences whose rows times heads /
  * kv_heads are at most 64 and for fp32 rows, else they are rounded to 11. The two
  * e4m3 codes that are no number, which append does not write, read as 480 and
- * -480. Scales that a row sees should be finite; one that is not makes the row
- * not finite, and reaches no other. */
+ * -480. Scales that a row sees are 0 or positive numbers; one that is not finite
+ * makes the row not finite, and reaches no other. */
 int64_t gphq_paged8_attention_workspace_bytes(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype,
                                               int64_t heads, int64_t window);
 int gphq_paged8_attention(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q_dev,
@@ -775,8 +775,10 @@ int gphq_probabilities(const float *x_dev, int64_t x_stride, const float *temper
  * the sum is infinite) the last t with a weight is taken, 0 if there is none.
  * kept (may be NULL): kept[s] = lens[s] - (b - r), the tokens that stay in a cache of
  * lens[s] with all drafts (gphq_paged_plan's held in the next step); may be lens.
- * A sequence whose starts descend or leave 0 .. rows gets accepted -1, kept = lens;
- * one without rows accepted 0. Rows outside all sequences are left alone. work:
+ * A sequence whose starts descend or leave 0 .. rows gets accepted -1, kept = lens
+ * (a row that two sequences have, starts having descended between them, holds the
+ * token of either); one without rows accepted 0. Rows outside all sequences are left
+ * alone. work:
  * gphq_verify_drafts_workspace_bytes, 16-byte aligned, one per call that may run at
  * the same time. tokens may be drafts itself. */
 int64_t gphq_verify_drafts_workspace_bytes(int64_t seqs, int64_t vocab);
