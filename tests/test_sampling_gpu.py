@@ -312,8 +312,8 @@ def test_starts_that_are_no_rows():
         may = [{7} if w is None else set() for w in want]
         for s, (a, b) in enumerate(zip(starts, starts[1:])):
             mine, _ = verified([a, b], drafts, p, q, u, v[s:s + 1], 10)
-            for r, t in enumerate(mine):
-                may[r] |= set() if t is None else {t}
+            for row, t in enumerate(mine):
+                may[row] |= set() if t is None else {t}
         assert all(t in m for t, m in zip(tokens, may)), starts
         assert all(k == 50 for k, c in zip(kept, count) if c < 0)
 
