@@ -12,7 +12,7 @@
 namespace gphq {
 namespace {
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanFew = 256, kPlanMany = 1024;  // threads of the block, for up to as many sequences and for more
 
 struct PlanArgs {
     const int32_t *held, *count, *taken, *shared, *free_count;
@@ -26,8 +26,9 @@ __device__ __forceinline__ void plan_flag(const PlanArgs &a, int bit) {
     if (a.bad) atomicOr(a.bad, bit);
 }
 
-// Sum over the threads before this one, and over all, of a block of kPlanThreads.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t &total, int64_t (&lds)[kPlanThreads / 64]) {
+// Sum over the threads before this one, and over all, of a block of 64 NW.
+template <int NW>
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t &total, int64_t (&lds)[NW]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int64_t sum = v;
 #pragma unroll
@@ -40,7 +41,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t &total, int64_t
     __syncthreads();
     int64_t before = 0;
     total = 0;
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
+    for (int w = 0; w < NW; ++w) {
         before += w < wave ? lds[w] : 0;
         total += lds[w];
     }
@@ -72,10 +73,11 @@ __device__ __forceinline__ Request request(const PlanArgs &a, int s) {
 }
 
 // The last thread whose first place, of `first` (ascending), is at most k.
-__device__ __forceinline__ int owner(const int64_t (&first)[kPlanThreads], int64_t k) {
+template <int NT>
+__device__ __forceinline__ int owner(const int64_t (&first)[NT], int64_t k) {
     int at = 0;
 #pragma unroll
-    for (int d = kPlanThreads / 2; d > 0; d /= 2)
+    for (int d = NT / 2; d > 0; d /= 2)
         if (first[at + d] <= k) at += d;
     return at;
 }
@@ -117,22 +119,25 @@ __device__ __forceinline__ void map_rows(const PlanArgs &a, int row0) {
     if (a.slots) a.slots[row] = slot;
 }
 
-// One block: the prefix sums run over all sequences, 1024 at a time, and the pages of those are
+// One block: the prefix sums run over all sequences, NT at a time, and the pages of those are
 // moved by all threads, each finding the sequence of its page in the sums. With MAP it also maps
-// the rows.
-template <bool MAP>
-__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PlanArgs a) {
-    __shared__ int64_t lds[kPlanThreads / 64];
-    __shared__ int64_t first[kPlanThreads];
-    __shared__ int entry[kPlanThreads];
+// the rows. All latency, a chain of loads, sums and barriers: 32 requests 4.5 us (8.4 with 1024 threads and
+// a sum for each case that may come), 1000 requests
+// 9.0, and 3.3 for the rows in a grid of their own.
+template <bool MAP, int NT>
+__global__ __launch_bounds__(NT) void paged_plan_kernel(const PlanArgs a) {
+    __shared__ int64_t lds[NT / 64];
+    __shared__ int64_t first[NT];
+    __shared__ int entry[NT];
     const int tid = threadIdx.x;
     int64_t have = *a.free_count;
     if (have < 0 || have > a.free_len) {
         if (tid == 0) plan_flag(a, PAGED_BAD_PAGE);
         have = have < 0 ? 0 : a.free_len;
     }
-    for (int s0 = 0; s0 < a.seqs; s0 += kPlanThreads) {
-        const Request r = request(a, s0 + tid);
+    Request r{};
+    for (int s0 = 0; s0 < a.seqs; s0 += NT) {
+        r = request(a, s0 + tid);
         int64_t total;
         const int64_t gives = max(r.taken - r.keep, 0), at = block_scan(gives, total, lds);
         if (total) {
@@ -141,7 +146,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PlanArgs
             __syncthreads();
             const int64_t fit = min(total, a.free_len - have);
             if (fit < total && tid == 0) plan_flag(a, PAGED_BAD_PAGE);
-            for (int64_t k = tid; k < fit; k += kPlanThreads) {
+            for (int64_t k = tid; k < fit; k += NT) {
                 const int i = owner(first, k);
                 a.free[have + k] = a.table[(s0 + i) * a.table_stride + entry[i] + (k - first[i])];
             }
@@ -150,41 +155,44 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PlanArgs
         }
     }
     int64_t wanted = 0, used = 0, row_sum = 0, rows = 0;
-    for (int s0 = 0; s0 < a.seqs; s0 += kPlanThreads) {
+    for (int s0 = 0; s0 < a.seqs; s0 += NT) {
         const int s = s0 + tid;
         const bool mine = s < a.seqs;
-        const Request r = request(a, s);
+        if (a.seqs > NT) r = request(a, s);
         int64_t total;
         const int64_t wants = max(r.need - r.taken, 0), at = block_scan(wants, total, lds);
         const bool served = wants == 0 || wanted + at + wants <= have;
         first[tid] = at;
         entry[tid] = r.taken;
+        __syncthreads();
         // Those served are the first with wants: the pages taken are the first of all wanted.
-        int64_t got, unused;
-        block_scan(served ? wants : 0, got, lds);
-        for (int64_t k = tid; k < got; k += kPlanThreads) {
+        int64_t got = total;
+        if (wanted + total > have) block_scan(served ? wants : 0, got, lds);
+        for (int64_t k = tid; k < got; k += NT) {
             const int i = owner(first, k);
             a.table[(s0 + i) * a.table_stride + entry[i] + (k - first[i])] = a.free[have - 1 - wanted - k];
         }
         used += got;
         wanted += total;
+        __syncthreads();  // first and entry have been read
         int count = served ? r.count : 0;
-        const int64_t row_at = row_sum + block_scan(count, total, lds);
-        row_sum += total;
+        int64_t brought;
+        const int64_t row_before = block_scan(count, brought, lds), row_at = row_sum + row_before;
+        row_sum += brought;
         const bool fits = !count || row_at + count <= a.rows;
         if (mine) {
             if (!r.ok || !fits) plan_flag(a, PAGED_BAD_SEQ);
             if (!served) plan_flag(a, PAGED_NO_PAGES);
         }
         count = fits ? count : 0;
-        const int64_t start = rows + block_scan(count, unused, lds);
-        rows += unused;
+        int64_t start = rows + row_before;
+        if (row_sum > a.rows) start = rows + block_scan(count, brought, lds);  // some do not
+        rows += brought;
         if (mine) {
             a.starts[s + 1] = (int)(start + count);
             a.lens[s] = r.held + count;
             a.taken_out[s] = served ? r.keep : r.taken;
         }
-        __syncthreads();  // first and entry have been read
     }
     if (tid == 0) {
         a.starts[0] = 0;
@@ -192,7 +200,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PlanArgs
     }
     if (MAP) {
         __syncthreads();  // starts, lens and tables are written
-        for (int row0 = tid & ~63; row0 < a.rows; row0 += kPlanThreads) map_rows(a, row0);
+        for (int row0 = tid & ~63; row0 < a.rows; row0 += NT) map_rows(a, row0);
     }
 }
 
@@ -251,12 +259,18 @@ extern "C" int gphq_paged_plan(const gphq_paged_requests *r, void *stream) {
     a.shift = __builtin_ctzll((uint64_t)r->page_tokens);
     hipStream_t st = (hipStream_t)stream;
     const bool map = a.rows && (a.positions || a.sequences || a.slots);
-    if (map && a.rows <= kPlanThreads) {
-        hipLaunchKernelGGL(paged_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, st, a);
-        return launch_status();
-    }
-    hipLaunchKernelGGL(paged_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, st, a);
+    // A few rows are mapped by the block itself, more by a grid of their own.
+    const bool few = a.seqs <= kPlanFew, self = map && a.rows <= (few ? 1024 : 4096);
+    if (few && self)
+        hipLaunchKernelGGL((paged_plan_kernel<true, kPlanFew>), dim3(1), dim3(kPlanFew), 0, st, a);
+    else if (few)
+        hipLaunchKernelGGL((paged_plan_kernel<false, kPlanFew>), dim3(1), dim3(kPlanFew), 0, st, a);
+    else if (self)
+        hipLaunchKernelGGL((paged_plan_kernel<true, kPlanMany>), dim3(1), dim3(kPlanMany), 0, st, a);
+    else
+        hipLaunchKernelGGL((paged_plan_kernel<false, kPlanMany>), dim3(1), dim3(kPlanMany), 0, st, a);
     GPHQ_TRY(launch_status());
+    if (self) return GPHQ_OK;
     if (!map) return GPHQ_OK;
     hipLaunchKernelGGL(paged_map_kernel, dim3((unsigned)((a.rows + 255) / 256)), dim3(256), 0, st, a);
     return launch_status();

@@ -1086,16 +1086,32 @@ def _dtype(t):
 
 def _rows2(t, rows, width, err):
     """The row stride of a 2-D tensor of at least `rows` rows of `width` neighbouring values."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or shape[0] < rows or shape[1] < width or (stride[1] != 1 and shape[1] > 1):
+    shape = t.shape
+    if len(shape) != 2:
         check(err)
-    return stride[0] if shape[0] > 1 else max(stride[0], shape[1])
+    (n, w), (row, step) = shape, t.stride()
+    if n < rows or w < width or (step != 1 and w > 1):
+        check(err)
+    return row if n > 1 else max(row, w)
 
 
 def _values(t, dtype, n, err):
     """Refuses a tensor that is not n or more contiguous values of a type."""
-    if t is not None and (t.dtype != dtype or not t.is_contiguous() or t.numel() < n):
+    if t is not None and (t.dtype is not dtype or not t.is_contiguous() or t.numel() < n):
         check(err)
+
+
+def _all_values(err, *wanted):
+    """_values of several (tensor or None, type, n); their addresses."""
+    out = []
+    for t, dtype, n in wanted:
+        if t is None:
+            out.append(None)
+        elif t.dtype is not dtype or not t.is_contiguous() or t.numel() < n:
+            check(err)
+        else:
+            out.append(t.data_ptr())
+    return out
 
 
 def _here(*tensors):
@@ -1396,24 +1412,22 @@ def verify_drafts(starts, drafts, target, draft, accept_u, sample_u, tokens, acc
     int32 [seqs]. tokens may be drafts, kept may be lens."""
     lib = load()
     _here(starts, drafts, target, draft, accept_u, sample_u, tokens, accepted, lens, kept, work)
-    if target.dim() != 2 or target.dtype != _torch.float32 or starts.numel() < 1 or (kept is not None and lens is None):
+    i32, f32 = _torch.int32, _torch.float32
+    seqs = starts.numel() - 1
+    if target.dim() != 2 or target.dtype is not f32 or seqs < 0 or (kept is not None and lens is None):
         check(ERR_DIMENSIONS)
     rows, vocab = target.shape
-    seqs = starts.numel() - 1
-    if draft is not None and (draft.shape != target.shape or draft.dtype != _torch.float32):
+    if draft is not None and (draft.shape != target.shape or draft.dtype is not f32):
         check(ERR_DIMENSIONS)
-    i32, f32 = _torch.int32, _torch.float32
-    for t, n, dtype in ((starts, 1, i32), (drafts, rows, i32), (accept_u, rows, f32), (sample_u, seqs, f32),
-                        (tokens, rows, i32), (accepted, seqs, i32), (lens, seqs, i32), (kept, seqs, i32)):
-        _values(t, dtype, n, ERR_DIMENSIONS)
+    st, dr, au, su, tk, ac, ln, kp = _all_values(
+        ERR_DIMENSIONS, (starts, i32, 1), (drafts, i32, rows), (accept_u, f32, rows), (sample_u, f32, seqs),
+        (tokens, i32, rows), (accepted, i32, seqs), (lens, i32, seqs), (kept, i32, seqs))
     ps = _rows2(target, rows, vocab, ERR_DIMENSIONS)
-    qs = 0 if draft is None else _rows2(draft, rows, vocab, ERR_DIMENSIONS)
+    q, qs = (None, 0) if draft is None else (draft.data_ptr(), _rows2(draft, rows, vocab, ERR_DIMENSIONS))
     if work is None:
         work = _work(verify_drafts_workspace_bytes(seqs, vocab), target.device, stream)
-    return check(lib.gphq_verify_drafts(ptr(starts), ptr(drafts), ptr(target), ps, ptr(draft), qs, ptr(accept_u),
-                                        ptr(sample_u), seqs, rows, vocab, ptr(tokens), ptr(accepted), ptr(lens),
-                                        ptr(kept), ptr(work), _scratch_bytes(work, ERR_DIMENSIONS),
-                                        stream_handle(stream)))
+    return check(lib.gphq_verify_drafts(st, dr, target.data_ptr(), ps, q, qs, au, su, seqs, rows, vocab, tk, ac, ln, kp,
+                                        work.data_ptr(), _scratch_bytes(work, ERR_DIMENSIONS), stream_handle(stream)))
 
 
 class _PoolMemory:
