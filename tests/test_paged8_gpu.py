@@ -431,6 +431,83 @@ def test_rows_out_of_fp16_s_range(rt, mag):
     close(b, q, 2, scale, 0, attend(b, q, 2, scale))
 
 
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("hd,page,order", [(128, 16, "head"), (64, 64, "token")])
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("rt", ROWS, ids=ROW_IDS)
+def test_long_prompts(rt, kind, hd, page, order, window):
+    """Sequences of a thousand columns and more, whose tiles are the widest, split and whole."""
+    b = Batch8([(260, 700)], 1, hd, page, kind, order, seed=33)
+    q = b.randn(b.rows, 8 * hd).to(rt)
+    close(b, q, 8, hd ** -0.5, window, attend(b, q, 8, hd ** -0.5, window))
+    b = Batch8([(200, 200), (257, 300), (300, 301)], 2, hd, page, kind, order, seed=34)
+    q = b.randn(b.rows, 10 * hd).to(rt)
+    close(b, q, 10, hd ** -0.5, window, attend(b, q, 10, hd ** -0.5, window))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(32, 1), (64, 2), (17, 1), (33, 1), (64, 1), (65, 1), (128, 1)])
+@pytest.mark.parametrize("rt", ROWS, ids=ROW_IDS)
+def test_groups_of_every_size_among_idle_sequences(rt, heads, kv_heads):
+    """Single rows of more than one set of columns, in batches of few and of many sequences."""
+    for idle in (0, 150):
+        seqs = [(1, 300), (1, 33)] + [(0, 20)] * idle + [(1, 100)]
+        b = Batch8(seqs, kv_heads, 64, 16, I8, seed=35)
+        q = b.randn(b.rows, heads * 64).to(rt)
+        close(b, q, heads, 0.125, 0, attend(b, q, heads, 0.125))
+
+
+@pytest.mark.parametrize("heads,kv_heads,rows", [(4, 1, 4), (4, 1, 5), (4, 1, 8), (4, 1, 9), (4, 1, 16), (4, 1, 17), (8, 8, 64),
+                                                 (8, 8, 65), (5, 1, 6), (5, 1, 13)])
+@pytest.mark.parametrize("rt", ROWS, ids=ROW_IDS)
+def test_columns_on_both_sides_of_the_kernels(rt, heads, kv_heads, rows):
+    b = Batch8([(rows, 700), (1, 40)], kv_heads, 64, 16, E4M3, seed=36)
+    q = b.randn(b.rows, heads * 64).to(rt)
+    close(b, q, heads, 0.125, 0, attend(b, q, heads, 0.125))
+    b = Batch8([(rows, 700)], kv_heads, 64, 16, I8, seed=37)
+    q = b.randn(b.rows, heads * 64).to(rt)
+    close(b, q, heads, 0.125, 0, attend(b, q, heads, 0.125))
+
+
+def test_pages_of_4096_tokens_and_pools_of_one():
+    """The largest page, one page, one head: strides that are never taken."""
+    b = Batch8([(3, 700), (70, 4100)], 1, 64, 4096, I8, seed=38)
+    q = b.randn(b.rows, 2 * 64)
+    close(b, q, 2, 0.125, 0, attend(b, q, 2, 0.125))
+    qkv = b.randn(b.rows, 4 * 64)
+    kv, dev = b.device(gphq)
+    gphq.paged8_append(kv, dev, qkv.cuda(), torch.empty(b.rows, 128, device="cuda"), 2)
+    dev.check()
+    append64(b, qkv, 2, None, 0.0, None, None)
+    same_pool(kv, b)
+    k = torch.zeros(1, 16, 1, 64, dtype=torch.int8, device="cuda")
+    s = torch.zeros(1, 1, 1, device="cuda")
+    kv = gphq.PagedKv8(k, k.clone(), s, s.clone())
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    dev = gphq.PagedBatch(ints([0, 16]), ints([16]), ints([[0]]), 16, 16, 16)
+    qkv, q, out = torch.randn(16, 192, device="cuda"), torch.empty(16, 64, device="cuda"), torch.empty(16, 64, device="cuda")
+    gphq.paged8_append(kv, dev, qkv, q, 1)
+    gphq.paged8_attention(kv, dev, q, out, 1, 0.125)
+    dev.check()
+    x = values(kv.v.view(torch.uint8).cpu(), I8)[0, :, 0] * float(kv.v_scales)
+    assert (out[0].cpu().double() - x[0]).abs().max() <= 2.0 ** -20 * x[0].abs().max()
+
+
+def test_two_calls_at_once():
+    """Two streams over one pool, each with a workspace of its own."""
+    b = Batch8([(1, 3000), (1, 2500)], 2, 128, 16, I8, seed=39)
+    q = b.randn(b.rows, 8 * 128)
+    want = attend(b, q, 8, 0.1)
+    kv, dev = b.device(gphq)
+    qd = q.cuda()
+    streams, outs = [torch.cuda.Stream() for _ in (0, 1)], [torch.zeros(2, 1024, device="cuda") for _ in (0, 1)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, out in zip(streams, outs):
+            gphq.paged8_attention(kv, dev, qd, out, 8, 0.1, stream=st)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out.cpu(), want) for out in outs)
+
+
 def test_views_strides_another_stream_and_repeats():
     """Pages and scales that are views of larger pools, rows of wider buffers, a side stream; the same bits each time."""
     b = Batch8([(1, 700), (66, 90), (3, 40)], 2, 128, 32, I8, seed=30)
