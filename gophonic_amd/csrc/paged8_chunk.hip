@@ -22,7 +22,7 @@ namespace {
 // Bound by the vector instructions beside the matrix instructions, which overlap little: per 64 keys
 // and 32 columns a wavefront has about 360 of the first (1850 cycles with the exponentials) and 1024 cycles
 // of the second a piece. 512 FP16 rows of 32 heads over 16512 tokens: 195 us with the join, 0.70
-// PFLOP/s (the 16-bit kernel over FP16 pages 0.73); twelve sequences of up to 300 fp32 rows 119 us.
+// PFLOP/s (the 16-bit kernel over FP16 pages 0.73); twelve sequences of up to 300 fp32 rows 104 us.
 // The next half's scores beside this half's exponentials in one wavefront's instructions, with V's
 // buffer tripled, took more registers than there are (340 and 331 us).
 template <typename RT, typename C, int HD, int NW>

@@ -7,7 +7,9 @@
 namespace gphq {
 namespace {
 
-// Eight wavefronts take the tile's 32-key steps in turn, each on its own: everything goes from
+constexpr int row8_waves(int sets) { return sets == 1 ? 4 : 8; }
+
+// Four wavefronts, or eight with two sets, take the tile's 32-key steps in turn, each on its own: everything goes from
 // memory to registers, nothing through LDS. NC sets of 16 columns share what is loaded and made
 // FP16 of a step. On v_mfma_f32_16x16x32_f16, per block of 16 keys:
 //   S^T (16 keys x 16 columns) = K . Q^T; a lane loads 16 neighbouring codes of a key at once,
@@ -20,15 +22,16 @@ namespace {
 // anything but loads in their order.
 //
 // Bound by memory where a tile has one set of columns: two single rows over 36286 and 39946 tokens,
-// eight KV heads, bfloat16 rows: 26.4 us (141 MB, 5.3 TB/s). With two sets by what is done to the
+// eight KV heads, bfloat16 rows: 27.2 us (141 MB, 5.2 TB/s). With two sets by what is done to the
 // codes between memory and the matrix instructions, about 200 vector instructions a step for
 // the codes and 220 a set for its softmax: five rows each over the same caches 35.6 us. Loading a
-// step further ahead gained nothing (28.7 and 37.8 us); four wavefronts a block, twice as many
-// splits: 29.8 us; two sets as wavefronts of their own, each loading and converting: 44.9 us.
+// step further ahead gained nothing (28.7 and 37.8 us); two sets as wavefronts of their own, each
+// loading and converting: 44.9 us. What four and eight wavefronts cost is
+// said at the host's rule for their splits.
 template <typename RT, typename C, int HD, int NC, bool BY_ROW>
-__global__ __launch_bounds__(512) void attn8_rows_kernel(const Attn8Args e, int tiles, int splits) {
+__global__ __launch_bounds__(row8_waves(NC) * 64) void attn8_rows_kernel(const Attn8Args e, int tiles, int splits) {
     typedef Half<f16> H;
-    constexpr int NB = 2, NW = 8, STEP = 16 * NB, ROUND = NW * STEP, KQ = HD / 64, VD = HD / 16, VW = VD / 4;
+    constexpr int NB = 2, NW = row8_waves(NC), STEP = 16 * NB, ROUND = NW * STEP, KQ = HD / 64, VD = HD / 16, VW = VD / 4;
     constexpr int NP = kPieces<RT, f16>, PP = 2;  // pieces of a query value, of a probability
     const AttnArgs &a = e.a;
     RowTile t;
@@ -263,7 +266,7 @@ int attn8_rows_launch(const Attn8Args &e, int hd, int splits, int tiles, hipStre
     auto launch = [&](auto dim, auto sets, auto by_row) {
         constexpr int HD = decltype(dim)::value, NC = decltype(sets)::value;
         constexpr bool BY_ROW = decltype(by_row)::value;
-        hipLaunchKernelGGL((attn8_rows_kernel<RT, C, HD, NC, BY_ROW>), dim3(blocks), dim3(512), 0, st, e, tiles, splits);
+        hipLaunchKernelGGL((attn8_rows_kernel<RT, C, HD, NC, BY_ROW>), dim3(blocks), dim3(64 * row8_waves(NC)), 0, st, e, tiles, splits);
     };
     auto pick = [&](auto dim, auto sets) {
         a.row_tiles ? launch(dim, sets, std::true_type{}) : launch(dim, sets, std::false_type{});

@@ -81,9 +81,10 @@ struct AttnPlan {
 };
 
 // What the row kernel of a call is like: columns of its tiles, keys that a block's wavefronts take
-// in one round, and up to how many keys a call is not split.
+// in one round, up to how many keys a call is not split, how many blocks a CU holds, and how many
+// rounds of blocks the chunk kernel's tiles of several sequences are split into.
 struct RowKernel {
-    int tile, round, brief;
+    int tile, round, brief, blocks, rounds;
 };
 
 // Keys per split of `span` keys, a multiple of `unit`, and how many splits that makes, for about `want` of them.
@@ -113,7 +114,7 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         p.small_rows = std::min(p.small_cols / group, b.max_rows);
         p.small_tiles = (int)((std::min<int64_t>(cols, p.small_cols) + k.tile - 1) / k.tile);
         const int64_t units = std::min<int64_t>(b.seqs, rows) * p.small_tiles * kv_heads;
-        // As many splits as leave one block on a CU: its four wavefronts keep enough loads in
+        // As many splits as leave one block on a CU (k.blocks over 8-bit pages): its four wavefronts keep enough loads in
         // flight, and a round more, begun or whole, costs more than it hides (16 bfloat16 rows of
         // 2000 to 4095 tokens, eight KV heads: 39.4 us with one block a CU, 41.4 with two, 46.8
         // with one and a half; fp32: 71.5, 74.7, 89.7). Short rows take no split: the second
@@ -126,7 +127,7 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         // bfloat16 tokens 233 and 241 us, twenty (ten) up to 8000 274 and 355, six (five), FP16,
         // up to 6000 106 and 149, thirty (fifteen) up to 3000 FP16 tokens 123 and 136.
         const bool mixed = cols > p.small_cols;
-        const int64_t want = mixed ? 2 * cus / (units / p.small_tiles) : cus / units;
+        const int64_t want = mixed ? 2 * k.blocks * cus / (units / p.small_tiles) : k.blocks * cus / units;
         // The grid is by sequence, or by row where a batch has more room for sequences than rows (one
         // row of 40000 bfloat16 tokens, alone 26 us, among 2047 idle sequences 26 by row and 544 by
         // sequence). No more splits than a launch takes.
@@ -155,7 +156,7 @@ AttnPlan attn_plan(const PagedBatch &b, int kv_heads, int group, int window, int
         // that time), the twenty 274 and 535, the thirty 123 and 154. That loses where the chunks are
         // alike or one alone: three of 83 to 234 FP16 rows over 6000 tokens 106 us, 94 with one
         // round, the six (one chunk) 106 and 88.
-        const int64_t want = units >= slots ? 1 : (b.seqs == 1 ? 1 : 3) * slots / units;
+        const int64_t want = units >= slots ? 1 : (b.seqs == 1 ? 1 : k.rounds) * slots / units;
         cut(span(big_tile), want, 128, p.big_len, p.big_splits);
     }
     return p;
@@ -256,12 +257,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const AttnArgs a) {
 // Takes the bits that were reported out of a batch's word; one that another stream has set since stays.
 __global__ void paged_clear_kernel(int32_t *bad, int32_t reported) { atomicAnd(bad, ~reported); }
 
+// A call over 8-bit pages takes a block for each unit of its join up to this many. Four chunks of one
+// sequence each, more than eight splits, 1600 units: 6.2 us, a wavefront a unit 6.6; 3200: 10.3 and 10.1;
+// 5300: 13.4 and 10.7; twelve sequences of 16000 units in all 24.0 and 13.0. (Calls over wider pages,
+// whose splits are fewer, always take the block.)
+constexpr int64_t kWideJoin = 2048;
+
 int64_t join_units(const PagedBatch &b, int64_t heads, int hd) { return b.rows * ((heads * hd + 255) / 256); }
 
 template <typename RT, int HD>
-int join_launch(const AttnArgs &a, hipStream_t st) {
+int join_launch(const AttnArgs &a, int64_t most, hipStream_t st) {
     const int64_t units = join_units(a.b, a.heads, HD);
-    if (std::max(a.parts, a.small_parts) > 8 && units <= kMaxBlocks)
+    if (std::max(a.parts, a.small_parts) > 8 && units <= most)
         hipLaunchKernelGGL((paged_join_kernel<RT, HD, 4>), dim3((unsigned)units), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((paged_join_kernel<RT, HD, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
@@ -273,7 +280,7 @@ int attend(const AttnArgs &a, const AttnPlan &p, int hd, hipStream_t st) {
     if (p.big_tiles) GPHQ_TRY((attn_chunk_launch<RT, CT>(a, hd, p.big_splits, p.big_tiles, st)));
     if (p.small_tiles) GPHQ_TRY((attn_rows_launch<RT, CT>(a, hd, p.small_splits, p.small_tiles, st)));
     if (!small_count(p, a.b, a.heads) && !big_count(p, a.b, a.heads)) return GPHQ_OK;
-    return hd == 128 ? join_launch<RT, 128>(a, st) : join_launch<RT, 64>(a, st);
+    return hd == 128 ? join_launch<RT, 128>(a, kMaxBlocks, st) : join_launch<RT, 64>(a, kMaxBlocks, st);
 }
 
 template <typename RT, typename C>
@@ -282,7 +289,7 @@ int attend8(const Attn8Args &e, const AttnPlan &p, int hd, hipStream_t st) {
     if (p.big_tiles) GPHQ_TRY((attn8_chunk_launch<RT, C>(e, hd, p.big_splits, p.big_tiles, st)));
     if (p.small_tiles) GPHQ_TRY((attn8_rows_launch<RT, C>(e, hd, p.small_splits, p.small_tiles, st)));
     if (!small_count(p, a.b, a.heads) && !big_count(p, a.b, a.heads)) return GPHQ_OK;
-    return hd == 128 ? join_launch<RT, 128>(a, st) : join_launch<RT, 64>(a, st);
+    return hd == 128 ? join_launch<RT, 128>(a, kWideJoin, st) : join_launch<RT, 64>(a, kWideJoin, st);
 }
 
 // The call's cut, refused where a launch would have too many blocks.
@@ -332,13 +339,23 @@ int attn8_args(const gphq_paged8_kv *kv, const gphq_paged_batch *b, int row_dtyp
     return GPHQ_OK;
 }
 
-RowKernel row_kernel(const gphq_paged_kv *kv) { return {kSmallTile, 128, kv->dtype == GPHQ_DTYPE_F32 ? 256 : 512}; }
+RowKernel row_kernel(const gphq_paged_kv *kv) { return {kSmallTile, 128, kv->dtype == GPHQ_DTYPE_F32 ? 256 : 512, 1, 3}; }
 // Over 8-bit pages up to 64 columns of a sequence go two sets of 16 to a tile; beside longer
-// sequences, which are the chunk kernel's, most of the row kernel's have one row. One row over 1024
-// tokens, eight KV heads: split 7.9 us and 3.4 for the join, unsplit 13.1.
-RowKernel row_kernel8(const AttnArgs &a) {
-    const int cols = a.b.max_rows * a.group;
-    return cols > 16 && cols <= 64 ? RowKernel{32, 256, 512} : RowKernel{16, 256, 512};
+// sequences, which are the chunk kernel's, most of the row kernel's have one row. A tile of one set
+// has four wavefronts and two blocks to a CU, of two sets eight and one: more, shorter splits save
+// steps in turn where a call is short or its lengths differ, and few long ones where the work of a
+// step is what counts. One fp32 row over 1024 tokens, eight KV heads: four wavefronts 6.5 us (and 3.4
+// for the join), eight 8.0; over 3000 6.7 and 8.1; the single rows among thirty FP16 prompts 25.5 and
+// 35.2, among twenty fp32 ones 44.7 and 50.3; sixteen over 2000 to 4095 22.2 and 21.4, two bfloat16 over
+// 40k 27.2 and 26.4 (three blocks to a CU: 27.2 and 27.5). Five rows each over two of 40k, two sets:
+// four 41.3, eight 35.5. Unsplit, the first takes 13.1.
+// The chunk kernel's tiles of several sequences are cut into two rounds of blocks for fp32 rows and
+// three for 16-bit ones. Whole calls with one, two and three rounds: twelve sequences of up to 300 fp32
+// rows 201, 132, 148 us, twenty of up to 200 347, 236, 293, three 169, 181, 183; thirty of up to 100
+// FP16 rows 145, 129, 105, six bfloat16 62, 58, 57, three FP16 133, 145, 142.
+RowKernel row_kernel8(const AttnArgs &a, bool f32) {
+    const int cols = a.b.max_rows * a.group, rounds = f32 ? 2 : 3;
+    return cols > 16 && cols <= 64 ? RowKernel{32, 256, 512, 1, rounds} : RowKernel{16, 128, 512, 2, rounds};
 }
 
 int64_t work_bytes_of(const AttnArgs &a, const gphq_paged_kv *kv, const RowKernel &k) {
@@ -422,7 +439,7 @@ int64_t gphq_paged8_attention_workspace_bytes(const gphq_paged8_kv *kv, const gp
                                               int64_t heads, int64_t window) {
     Attn8Args e{};
     GPHQ_TRY(attn8_args(kv, batch, row_dtype, heads, window, e));
-    return work_bytes_of(e.a, &kv->codes, row_kernel8(e.a));
+    return work_bytes_of(e.a, &kv->codes, row_kernel8(e.a, row_dtype == GPHQ_DTYPE_F32));
 }
 
 int gphq_paged8_attention(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *q,
@@ -430,9 +447,9 @@ int gphq_paged8_attention(const gphq_paged8_kv *kv, const gphq_paged_batch *batc
                           void *work, int64_t work_bytes, void *stream) {
     Attn8Args e{};
     GPHQ_TRY(attn8_args(kv, batch, row_dtype, heads, window, e));
+    const bool f32 = row_dtype == GPHQ_DTYPE_F32;
     AttnPlan p;
-    GPHQ_TRY(call_args(&kv->codes, row_kernel8(e.a), row_dtype == GPHQ_DTYPE_F32 ? 4 : 2, q, q_stride, scale, out, out_stride, work,
-                       work_bytes, e.a, p));
+    GPHQ_TRY(call_args(&kv->codes, row_kernel8(e.a, f32), f32 ? 4 : 2, q, q_stride, scale, out, out_stride, work, work_bytes, e.a, p));
     if (e.a.b.rows == 0) return GPHQ_OK;
     const int hd = (int)kv->codes.head_dim;
     hipStream_t st = (hipStream_t)stream;
