@@ -658,7 +658,7 @@ typedef struct gphq_paged8_kv {
 /* gphq_paged_append into 8 bits; row_dtype F32, F16 or BF16 whatever the codes.
  * Per block that receives tokens, m the largest magnitude among their values
  * and top the largest code (127, 448):
- *   a block that holds no earlier token of the sequence: scale = m / top;
+ *   a block that holds no earlier token of the sequence: scale = m / top (2^-126 or more);
  *   one that does keeps its scale while m rounds to a code (m <= 127.5 scale,
  *   464 scale), else the scale is doubled as often as that takes, and the
  *   earlier tokens' codes are rounded to it (e4m3 codes lose nothing by it
@@ -667,12 +667,13 @@ typedef struct gphq_paged8_kv {
  * Keys' norm and rotation, and all that decides a code, are 64-bit arithmetic:
  * codes do not depend on the order of a sum, nor on how a batch is cut. (Tokens
  * that come one by one may grow a scale that one call would have chosen at
- * once.) Queries as gphq_paged_append's, in fp32. A value that is not finite
- * becomes code 0 and sets *bad_dev (GPHQ_ERR_NON_FINITE). A block whose scale
- * is not a positive finite number counts as empty: it gets a new one. Sequences
- * may share pages whose 16-token blocks all lie before the call's tokens; two
- * sequences of one call must not write the same block. Slots behind a
- * sequence's last token keep their bytes. The rest as gphq_paged_append. */
+ * once.) Queries as gphq_paged_append's, in fp32. A value that is not finite, or
+ * beyond fp32's range after norm and rotation, becomes code 0 and sets *bad_dev
+ * (GPHQ_ERR_NON_FINITE). A block whose scale is not a positive finite number
+ * counts as empty: it gets a new one. Sequences may share pages whose 16-token
+ * blocks all lie before the call's tokens; two sequences of one call must not
+ * write the same block. Slots behind a sequence's last token keep their bytes.
+ * The rest as gphq_paged_append. */
 int gphq_paged8_append(const gphq_paged8_kv *kv, const gphq_paged_batch *batch, int row_dtype, const void *qkv_dev,
                        int64_t qkv_stride, int64_t heads, const float *q_norm_dev, const float *k_norm_dev, double eps,
                        const float *cos_dev, const float *sin_dev, int64_t rope_rows, double q_scale, void *q_dev,

@@ -25,7 +25,9 @@ def encode(y, kind):
     """Codes (uint8 bytes) of float64 values in units of their scale: to nearest, ties to even."""
     if kind == I8:
         return y.round().clamp(-127, 127).to(torch.int8).view(torch.uint8)
-    return y.float().clamp(-448, 448).to(E4M3).view(torch.uint8)
+    exponent = torch.frexp(y)[1].clamp(min=-5)  # 2^(exponent - 1) at most |y|; 2^-9 is the smallest step
+    step = torch.ldexp(torch.ones_like(y), exponent - 4)
+    return ((y / step).round() * step).clamp(-448, 448).float().to(E4M3).view(torch.uint8)
 
 
 class Batch8(Batch):
@@ -148,7 +150,7 @@ def append64(b, qkv, heads, kn, eps, cos, sin, limit=None):
         pos = torch.arange(first, end)
         both = (rotated64(rows[:, heads:heads + G], kn, eps, cos, sin, pos), rows[:, heads + G:])
         for i, y in enumerate(both):
-            y = torch.where(y.isfinite(), y, 0.0)
+            y = torch.where(y.abs() <= torch.finfo(F32).max, y, 0.0)
             p = first
             while p < end:
                 lo = p // BLOCK * BLOCK
@@ -171,7 +173,6 @@ def append64(b, qkv, heads, kn, eps, cos, sin, limit=None):
                                 b.codes[i][at, slot:slot + p - lo, g] = encode(values(c, kind) * 2.0 ** -k, kind)
                             scale = grown
                         b.scales[i][at, g, slot // BLOCK] = scale
-                        inv = 1.0 / scale if scale else 0.0
-                        b.codes[i][at, slot + p - lo:slot + stop - lo, g] = encode(mine * inv, kind)
+                        b.codes[i][at, slot + p - lo:slot + stop - lo, g] = encode(mine / scale if scale else mine, kind)
                 p = stop
     b.refresh()

@@ -190,6 +190,62 @@ def test_values_that_are_not_finite(kind, bad):
         same_pool(kv, mine)
 
 
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_IDS)
+def test_keys_turned_past_fp32_s_range(kind):
+    """Finite keys whose rotation is above the largest fp32 number: code 0, reported, in a new block and in one with a
+    scale, which stays finite."""
+    rows = torch.zeros(3, 3 * 64)
+    rows[0, 64], rows[0, 64 + 32] = 3e38, -3e38  # a pair that a turn by 45 degrees makes (4.2e38, 0)
+    rows[1] = rows[0]
+    rows[1, 65] = 1e38
+    rows[2, 64:] = torch.linspace(-1, 1, 128)
+    half = torch.full((32, 32), 0.5 ** 0.5)
+    b = Batch8([(1, 20), (2, 2)], 1, 64, 16, kind, seed=6)
+    kv, dev = b.device(gphq)
+    gphq.paged8_append(kv, dev, rows.cuda(), torch.empty(3, 64, device="cuda"), 1, None, None, 0.0, half.cuda(), half.cuda())
+    with pytest.raises(gphq.GphqError) as e:
+        dev.check()
+    assert e.value.status == gphq.ERR_NON_FINITE
+    append64(b, rows, 1, None, 0.0, half, half)
+    same_pool(kv, b)
+    assert kv.k_scales[int(b.table[0, 1]), 0, 0].isfinite()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("scale", [49.0, 41.0, 2.0 ** 23 + 1])
+def test_values_between_two_codes(kind, scale):
+    """Quotients that lie between two codes, or so near to there that fp32 has no number between: 49 * (1 / 49) is not
+    1 in 64 bits, and (19 * 2^19 + 1) / (2^23 + 1) is 2^-26 of itself below 19 / 16."""
+    b = Batch8([(3, 20)], 1, 64, 16, kind, seed=7)
+    at = int(b.table[0, 1])
+    for s in b.scales:
+        s[at] = scale
+    if kind == I8:
+        ties = torch.arange(-62, 66).double() + 0.5
+    else:
+        codes = torch.arange(1, 127, dtype=torch.uint8).view(E4M3).double()
+        ties = torch.cat([(codes[1:] + codes[:-1]) / 2, torch.tensor([1.1875] * 3).double()])
+    y = ties * scale
+    below = (y - y.abs() * 2.0 ** -25).float()  # the fp32 number at most y, mostly
+    rows = torch.zeros(3, 3 * 64)
+    rows[0, 64:], rows[1, 64:], rows[2, 64:] = y.float(), -y.float(), below
+    kv, dev = b.device(gphq)
+    gphq.paged8_append(kv, dev, rows.cuda(), torch.empty(3, 64, device="cuda"), 1)
+    dev.check()
+    append64(b, rows, 1, None, 0.0, None, None)
+    same_pool(kv, b)
+    if kind == E4M3:  # to nearest, said another way: no other code is nearer, of two as near the even one
+        all_codes = torch.arange(0, 127, dtype=torch.uint8).view(E4M3).double()
+        for r in range(3):
+            x = (rows[r, 64:].double() / scale)[:, None]
+            d = (x.abs() - all_codes).abs()
+            near = d.min(1).values
+            even = (d == near[:, None]).long() * (2 - torch.arange(127) % 2)
+            want = even.argmax(1) + 128 * (x[:, 0] < 0)
+            got = torch.cat([b.codes[i][at, 1 + r, 0].long() for i in (0, 1)])
+            assert torch.equal(got, want)
+
+
 def test_append_in_place_of_the_queries():
     b = Batch8([(5, 9), (1, 20)], 2, 128, 16, I8, seed=3)
     heads, D = 8, 128
