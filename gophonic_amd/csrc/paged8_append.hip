@@ -245,10 +245,10 @@ __device__ __forceinline__ bool row_of(const PagedBatch &b, int row, SeqRow &s) 
 // the 16-token blocks whose first new token lies in `span` rows of the batch. Queries: a wavefront
 // takes every q_parts-th four heads of a row.
 //
-// Bound by memory, and by the chain of loads before it where rows are few: three fp32 prompts of
-// 3417 rows in all, 16 heads and 8 KV heads, 39.8 us (144 MB, 3.6 TB/s; a large copy makes 4.7); 64
-// single tokens 7.8 us. Of the former the 64-bit quotients cost 1.9 us. A wavefront a token and head,
-// with the block's values kept in LDS, took 54.0 us. Registers for more wavefronts a CU spilled: bounds
+// Bound by memory, and by the chain of loads before it where rows are few: five fp32 prompts of
+// 3417 rows in all, 32 heads and 8 KV heads, 39.8 us (144 MB, 3.6 TB/s; a large copy makes 4.7); 64
+// single tokens 7.8 us. Of the former the 64-bit quotients cost 1.9 us. A wavefront a block and
+// head, with all its 16 tokens in registers, took 54.0 us. Registers for more wavefronts a CU spilled: bounds
 // of 5, 6 and 8 to a SIMD unit 39.6, 55.4 and 72.6 us beside 37.9.
 template <typename RT, typename C, int HD>
 __global__ __launch_bounds__(256) void paged8_append_kernel(const Append8Args a) {

@@ -121,9 +121,9 @@ __device__ __forceinline__ void map_rows(const PlanArgs &a, int row0) {
 
 // One block: the prefix sums run over all sequences, NT at a time, and the pages of those are
 // moved by all threads, each finding the sequence of its page in the sums. With MAP it also maps
-// the rows. All latency, a chain of loads, sums and barriers: 32 requests 4.5 us (8.4 with 1024 threads and
-// a sum for each case that may come), 1000 requests
-// 9.0, and 3.3 for the rows in a grid of their own.
+// the rows. All latency, a chain of loads, sums and barriers: 32 requests 4.5 us (8.4 with 1024
+// threads and a sum for each case that may come), 1000 requests 9.0, and 3.3 for the rows in a grid of
+// their own.
 template <bool MAP, int NT>
 __global__ __launch_bounds__(NT) void paged_plan_kernel(const PlanArgs a) {
     __shared__ int64_t lds[NT / 64];
