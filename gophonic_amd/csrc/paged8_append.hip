@@ -25,7 +25,8 @@ struct Append8Args {
     const float *qn, *kn, *cos, *sin;
     int64_t qkv_stride, q_stride;
     int rope_rows, heads;
-    int span, kv_parts;  // rows whose blocks one block of the key and value part looks for; blocks that share their heads
+    int by_row;          // a block of the key and value part takes the 16-token block that a row begins, not a numbered one
+    int kv_parts;        // blocks that share a 16-token block's heads
     int q_parts;         // wavefronts of a row in the query part
     unsigned kv_blocks;  // blocks of the key and value part; the query part's come behind them
     double eps;
@@ -241,44 +242,66 @@ __device__ __forceinline__ bool row_of(const PagedBatch &b, int row, SeqRow &s) 
     return true;
 }
 
+// The 16-token blocks of a batch by numbers: a sequence's n tokens touch n / 16 + 2 of them at most
+// (rounded down), so those of sequence s get the numbers from starts[s] / 16 + 2 s on. False for a number
+// that no block has. Its first new token is in row `row`, at position pos, the block's last before n1.
+__device__ __forceinline__ bool block_of(const Append8Args &a, int number, SeqRow &s, int &row, int &pos, int &n1) {
+    const PagedBatch &b = a.b;
+    const int lane = threadIdx.x & 63;
+    int lo = 0, cnt = b.seqs;
+    while (cnt > 64) {
+        const int step = (cnt + 63) / 64, i = min(lane * step, cnt - 1);
+        const int at = last_lane(__ballot(lane * step < cnt && (b.starts[lo + i] >> 4) + 2 * (lo + i) <= number)) * step;
+        lo += at;
+        cnt = min(step, cnt - at);
+    }
+    const int i = lo + min(lane, cnt - 1);
+    const int s0 = b.starts[i], s1 = b.starts[i + 1], len = b.lens[i];
+    const int at = last_lane(__ballot(lane < cnt && (s0 >> 4) + 2 * i <= number));
+    s = SeqRow{lo + at, __builtin_amdgcn_readlane(s0, at), __builtin_amdgcn_readlane(s1, at),
+               __builtin_amdgcn_readlane(len, at)};
+    if (!seq_ok(b, s.start, s.end, s.len)) return false;  // (flagged by its rows' queries)
+    const int shift = s.len - (s.end - s.start), first = max(shift, 0), k = number - ((s.start >> 4) + 2 * s.seq);
+    const int end = a.cos ? min(s.len, a.rope_rows) : s.len;
+    if (k < 0) return false;
+    pos = k == 0 ? first : (first & ~(kBlockTokens - 1)) + k * kBlockTokens;
+    n1 = min((pos & ~(kBlockTokens - 1)) + kBlockTokens, end);
+    row = s.start + pos - shift;
+    return pos < end && find_seq(b, row).seq == s.seq;  // (not so where starts descend)
+}
+
+// The same by the row: false where it is not the first new one of a 16-token block, or cannot be placed.
+__device__ __forceinline__ bool block_at(const Append8Args &a, int row, SeqRow &s, int &pos, int &n1) {
+    if (!row_of(a.b, row, s)) return false;
+    const int shift = s.len - (s.end - s.start), end = a.cos ? min(s.len, a.rope_rows) : s.len;
+    pos = row - s.start + shift;
+    n1 = min((pos & ~(kBlockTokens - 1)) + kBlockTokens, end);
+    return pos >= 0 && pos < end && (pos == max(shift, 0) || pos % kBlockTokens == 0);
+}
+
 // One grid for both parts. Keys and values: a block takes every kv_parts-th head's keys or values of
-// the 16-token blocks whose first new token lies in `span` rows of the batch. Queries: a wavefront
-// takes every q_parts-th four heads of a row.
+// one 16-token block. Queries: a wavefront takes every q_parts-th four heads of a row.
 //
 // Bound by memory, and by the chain of loads before it where rows are few: five fp32 prompts of
-// 3417 rows in all, 32 heads and 8 KV heads, 39.8 us (144 MB, 3.6 TB/s; a large copy makes 4.7); 64
-// single tokens 7.8 us. Of the former the 64-bit quotients cost 1.9 us. A wavefront a block and
-// head, with all its 16 tokens in registers, took 54.0 us. Registers for more wavefronts a CU spilled: bounds
-// of 5, 6 and 8 to a SIMD unit 39.6, 55.4 and 72.6 us beside 37.9.
+// 3417 rows in all, 32 heads and 8 KV heads, 28.2 us with two sets of inputs, which the last-level cache
+// keeps in part (144 MB, 5.1 TB/s); 64 single tokens 7.1 us. The 64-bit quotients cost 1.9 us of the former.
+// A wavefront a block and head, with all its 16 tokens in registers, took 54.0 us when this took 37.9.
+// Registers for more wavefronts a CU spilled: bounds of 5, 6 and 8 to a SIMD unit 39.6, 55.4 and 72.6 us
+// beside those 37.9.
 template <typename RT, typename C, int HD>
 __global__ __launch_bounds__(256) void paged8_append_kernel(const Append8Args a) {
     constexpr int E = HD / 32;
     const int lane = threadIdx.x & 63, j = lane & 15, slot = lane >> 4;
     if (blockIdx.x < a.kv_blocks) {
         const int group = blockIdx.x / a.kv_parts, part = blockIdx.x - group * a.kv_parts;
-        const int r1 = min((group + 1) * a.span, a.b.rows);
-        for (int row = group * a.span; row < r1;) {
-            SeqRow s;
-            if (!row_of(a.b, row, s)) {
-                ++row;
-                continue;
-            }
-            const int pos = s.len - (s.end - row), first = max(s.len - (s.end - s.start), 0);
-            const int n1 = min((pos & ~(kBlockTokens - 1)) + kBlockTokens, a.cos ? min(s.len, a.rope_rows) : s.len);
-            const bool lead = pos == first || pos % kBlockTokens == 0;
-            if (pos < 0 || pos >= n1) {  // a row before token 0, or past the rotary table: flagged below
-                ++row;
-                continue;
-            }
-            if (lead) {
-                const int page = a.b.table[s.seq * a.b.table_stride + (pos >> a.pool.shift)];
-                if (page >= 0 && page < a.pool.pages)
-                    append_block<RT, C, HD>(a, row, pos, n1, page, part);
-                else if (lane == 0)
-                    paged_flag(a.b, PAGED_BAD_PAGE);
-            }
-            row += n1 - pos;
-        }
+        SeqRow s;
+        int row = group, pos, n1;
+        if (a.by_row ? !block_at(a, row, s, pos, n1) : !block_of(a, group, s, row, pos, n1)) return;
+        const int page = a.b.table[s.seq * a.b.table_stride + (pos >> a.pool.shift)];
+        if (page >= 0 && page < a.pool.pages)
+            append_block<RT, C, HD>(a, row, pos, n1, page, part);
+        else if (lane == 0)
+            paged_flag(a.b, PAGED_BAD_PAGE);
         return;
     }
     const int unit = uniform((int)((blockIdx.x - a.kv_blocks) * 4 + (threadIdx.x >> 6)));
@@ -406,10 +429,16 @@ extern "C" int gphq_paged8_append(const gphq_paged8_kv *kv, const gphq_paged_bat
     a.eps = eps;
     a.qscale = (float)q_scale;
     const int64_t rows = a.b.rows;
-    // A single token's row is its block's; else four rows are looked through for the first of a block.
-    a.span = a.b.max_rows == 1 ? 1 : 4;
-    // Blocks that share a row group's heads: all while that leaves the chip short of wavefronts, else fewer.
-    const int64_t spans = (rows + a.span - 1) / a.span, want = 32ll * device_cus();
+    // Blocks by their numbers, or by rows, each looking whether it is the first of one, where there are
+    // fewer rows (idle sequences have numbers, two each): 64 single tokens 7.8 us by rows, 7.9 by numbers;
+    // five sequences of four rows 5.8 and 5.0. Before numbers, with a block for every four rows, 3417 rows took
+    // 39.5 us (now 28.2), 512 rows 11.5 (7.1).
+    const int64_t numbers = rows / kBlockTokens + 2 * (int64_t)a.b.seqs;
+    a.by_row = rows <= numbers;
+    // Blocks that share a 16-token block's heads: all while that leaves the chip short of wavefronts, else
+    // fewer. With 8, 16, 24 and 32 wavefronts a CU wanted: 3417 rows 26.5, 28.2, 29.9, 32.5 us, forty
+    // sequences of up to 80 rows 15.2, 12.3, 13.0, 14.4, 32 of five 8.3, 7.6, 7.5, 7.2.
+    const int64_t spans = std::min(rows, numbers), want = 16ll * device_cus();
     a.kv_parts = (int)std::min<int64_t>(2 * kvh, std::max<int64_t>(1, want / 4 / spans));
     // Wavefronts per row of queries, likewise: of its heads four at a time.
     const int64_t groups = (heads + 3) / 4;

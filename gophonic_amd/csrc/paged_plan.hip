@@ -259,8 +259,11 @@ extern "C" int gphq_paged_plan(const gphq_paged_requests *r, void *stream) {
     a.shift = __builtin_ctzll((uint64_t)r->page_tokens);
     hipStream_t st = (hipStream_t)stream;
     const bool map = a.rows && (a.positions || a.sequences || a.slots);
-    // A few rows are mapped by the block itself, more by a grid of their own.
-    const bool few = a.seqs <= kPlanFew, self = map && a.rows <= (few ? 1024 : 4096);
+    // A few rows are mapped by the block itself, more by a grid of their own, whose launch costs less than
+    // the passes over them: 32 sequences of 32 rows 7.0 us and 3.6 + 2.8, of 64 rows 10.3 and 3.8 + 3.2, 500 of
+    // four 10.2 and 6.3 + 3.2, of one, 300, 8.1 and 6.2 + 2.6. Up to 256 sequences need 256 threads only: 256
+    // of one row 5.1 us, with 1024 threads 7.8.
+    const bool few = a.seqs <= kPlanFew, self = map && a.rows <= 1024;
     if (few && self)
         hipLaunchKernelGGL((paged_plan_kernel<true, kPlanFew>), dim3(1), dim3(kPlanFew), 0, st, a);
     else if (few)

@@ -157,7 +157,8 @@ __global__ __launch_bounds__(kThreads) void prob_write_kernel(const ProbArgs a) 
     }
 }
 
-// Parts of a row: about 2048 blocks in all.
+// Parts of a row: about 2048 blocks in all. 160 rows with 512, 1024, 2048 and 4096: 50.4, 48.2, 45.9 and
+// 45.1 us in the two kernels, 40 rows 15.7, 15.8, 16.3 and 16.0; one row has 38 in any case.
 void prob_cut(int64_t rows, int64_t n, int &len, int &parts) {
     const int64_t tiles = (n + kTile - 1) / kTile, per = std::max<int64_t>(1, tiles * rows / 2048);
     len = (int)(std::min(per, tiles) * kTile);

@@ -48,6 +48,7 @@ APPEND = [
     ([(1, n) for n in range(1, 71)], 4, 1, 64, 32, "token"),
     ([(130, 150), (1, 1), (33, 34)], 10, 2, 128, 128, "head"),
     ([(17, 17), (16, 32), (15, 31), (2, 17)], 2, 2, 64, 16, "head"),
+    ([(n % 8, n % 8 + n) for n in range(150)], 2, 1, 64, 32, "head"),
 ]
 
 
@@ -311,6 +312,45 @@ def test_bad_sequences_are_left_alone(starts, good):
     b.new = [starts[s + 1] - starts[s] if s in live else 0 for s in range(3)]
     append64(b, rows, 1, None, 0.0, None, None)
     same_pool(kv, b)
+
+
+@pytest.mark.parametrize("starts,good", [([0, 20, 40, 90], range(40)), ([0, 50, 50, 60], range(50, 60)),
+                                         ([-10, 20, 40, 60], range(20, 60)), ([0, 40, 20, 60], []),
+                                         ([2 ** 31 - 1, -2 ** 31, 40, 60], range(40, 60))])
+def test_bad_sequences_of_many_rows_are_left_alone(starts, good):
+    """The same where a sequence has more than a few rows."""
+    b = Batch8([(20, 50)] * 3, 2, 64, 16, I8, seed=6)
+    kv, _ = b.device(gphq)
+    dev = gphq.PagedBatch(*[torch.tensor(v, dtype=torch.int32, device="cuda") for v in (starts, b.lens)],
+                          torch.from_numpy(b.table).cuda(), 60, 20, 50)
+    q, good = torch.full((60, 128), 7.0, device="cuda"), list(good)
+    other = [r for r in range(60) if r not in good]
+    rows = b.randn(60, 6 * 64)
+    gphq.paged8_append(kv, dev, rows.cuda(), q, 2)
+    with pytest.raises(gphq.GphqError) as e:
+        dev.check()
+    assert e.value.status == gphq.ERR_PAGED_BATCH
+    assert (q[other] == 7).all() and (q[good] != 7).all()
+    live = [s for s in range(3) if starts[s] in good]
+    b.starts = [starts[s] if s in live else 0 for s in range(3)] + [60]
+    b.new = [starts[s + 1] - starts[s] if s in live else 0 for s in range(3)]
+    append64(b, rows, 2, None, 0.0, None, None)
+    same_pool(kv, b)
+
+
+def test_append_in_a_batch_of_many_idle_sequences():
+    """More sequences than the first search takes at once, most without rows; single tokens beside short prompts."""
+    seqs = [((0, 5), (1, 1 + n % 40), (0, 1), (n % 30, n % 30 + 7))[n % 4] if n % 11 == 0 else (0, 3) for n in range(5000)]
+    b = Batch8(seqs, 1, 64, 16, I8, seed=8)
+    rows = b.randn(b.rows, 3 * 64)
+    for few in (False, True):  # (fewer sequences than rows: blocks by their numbers; else by rows)
+        if few:
+            b = Batch8([s for s in seqs if s[0]], 1, 64, 16, I8, seed=8)
+        kv, dev = b.device(gphq)
+        gphq.paged8_append(kv, dev, rows.cuda(), torch.empty(b.rows, 64, device="cuda"), 1)
+        dev.check()
+        append64(b, rows, 1, None, 0.0, None, None)
+        same_pool(kv, b)
 
 
 # ---- attention ------------------------------------------------------------------
