@@ -1,5 +1,6 @@
 """The paged cache in 8 bits on the GPU: append and attention against their definitions in float64, over ragged batches
 whose unused bytes are arbitrary and whose unused scales are NaN."""
+import functools
 import math
 
 import numpy as np
@@ -35,6 +36,13 @@ def same_pool(kv, b):
         assert torch.equal(got, want), int((got != want).sum())
     for got, want in zip((kv.k_scales, kv.v_scales), b.scales):
         assert torch.equal(got.cpu().view(torch.int32), want.view(torch.int32))
+
+
+@functools.lru_cache(None)
+def two_streams():
+    """The file's streams. A process has more streams than hardware queues: each one more that a test takes changes which
+    of the streams of later tests share a queue, and wait for each other."""
+    return [torch.cuda.Stream() for _ in (0, 1)]
 
 
 # ---- append ---------------------------------------------------------------------
@@ -595,7 +603,7 @@ def test_two_calls_at_once():
     want = attend(b, q, 8, 0.1)
     kv, dev = b.device(gphq)
     qd = q.cuda()
-    streams, outs = [torch.cuda.Stream() for _ in (0, 1)], [torch.zeros(2, 1024, device="cuda") for _ in (0, 1)]
+    streams, outs = two_streams(), [torch.zeros(2, 1024, device="cuda") for _ in (0, 1)]
     torch.cuda.synchronize()
     for _ in range(20):
         for st, out in zip(streams, outs):
@@ -621,7 +629,7 @@ def test_views_strides_another_stream_and_repeats():
     wide = torch.zeros(b.rows, 4 * 128 + 32, device="cuda")
     wide[:, 16:16 + 512] = q.cuda()
     out = torch.zeros(b.rows, 512 + 64, device="cuda")
-    side = torch.cuda.Stream()
+    side = two_streams()[0]
     side.wait_stream(torch.cuda.current_stream())
     for _ in range(3):
         with torch.cuda.stream(side):
@@ -678,7 +686,7 @@ def test_captured_steps_follow_the_lengths():
         gphq.paged8_append(kv, dev, qkv, q, heads)
         gphq.paged8_attention(kv, dev, q, out, heads, 0.1, work=work)
 
-    side = torch.cuda.Stream()
+    side = two_streams()[0]
     side.wait_stream(torch.cuda.current_stream())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.stream(side):
