@@ -33,16 +33,31 @@ struct ProbArgs {
     int rows, n, parts, len;  // len: values of a part, a multiple of kTile
 };
 
-// log2(e) / t, 0 for a row that takes its largest value alone.
-__device__ __forceinline__ float rate_of(const ProbArgs &a, int row) {
+// log2(e) / t in two floats, 0 for a row that takes its largest value alone.
+struct Rate {
+    float hi, lo;
+};
+__device__ __forceinline__ Rate rate_of(const ProbArgs &a, int row) {
     const float t = a.temperatures ? a.temperatures[row] : 1.0f;
-    return t > 0.0f ? fminf(fmaxf(1.44269504088896340736f / t, FLT_MIN), FLT_MAX) : 0.0f;
+    if (!(t > 0.0f)) return Rate{0.0f, 0.0f};
+    constexpr float hi = 1.44269504088896340736f, lo = (float)(1.44269504088896340736 - (double)hi);
+    const float q = hi / t;
+    if (!(q >= FLT_MIN && q <= FLT_MAX)) return Rate{q < 1.0f ? FLT_MIN : FLT_MAX, 0.0f};
+    return Rate{q, (fmaf(-q, t, hi) + lo) / t};
+}
+// exp(d / t), d at most 0. The exponent's rounding, up to 2^-24 of it, is put back as a factor: one row of
+// 151936 is 1.3e-7 off its 64-bit values with it and 2.1e-7 without, which saves 0.6 of 5.0 us of a kernel
+// on one row and 2.8 of 48.8 us on 160.
+__device__ __forceinline__ float power(float d, Rate r) {
+    const float e = d * r.hi, rest = e > -160.0f ? fmaf(d, r.lo, fmaf(d, r.hi, -e)) : 0.0f;
+    const float p = __builtin_amdgcn_exp2f(e);
+    return fmaf(p, rest * 0.693147180559945309417f, p);
 }
 
 // Joins two (largest, sum) pairs.
-__device__ __forceinline__ void join_sums(float &m, float &s, float m2, float s2, float rate) {
+__device__ __forceinline__ void join_sums(float &m, float &s, float m2, float s2, Rate rate) {
     const float mx = fmaxf(m, m2), ref = mx == -INFINITY ? 0.0f : mx;
-    s = s * __builtin_amdgcn_exp2f((m - ref) * rate) + s2 * __builtin_amdgcn_exp2f((m2 - ref) * rate);
+    s = s * power(m - ref, rate) + s2 * power(m2 - ref, rate);
     m = mx;
 }
 // Joins two (largest, first index of it) pairs.
@@ -51,7 +66,7 @@ __device__ __forceinline__ void join_first(float &m, int &i, float m2, int i2) {
 }
 
 // A block's pairs to one, in a fixed order; the same in every thread.
-__device__ __forceinline__ void block_join(float &m, float &s, int &first, float rate) {
+__device__ __forceinline__ void block_join(float &m, float &s, int &first, Rate rate) {
     __shared__ float sm[4], ss[4];
     __shared__ int si[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -59,7 +74,7 @@ __device__ __forceinline__ void block_join(float &m, float &s, int &first, float
     for (int d = 1; d < 64; d *= 2) {
         const float m2 = __shfl_xor(m, d), s2 = __shfl_xor(s, d);
         const int i2 = __shfl_xor(first, d);
-        if (rate > 0.0f)
+        if (rate.hi > 0.0f)
             join_sums(m, s, m2, s2, rate);
         else
             join_first(m, first, m2, i2);
@@ -69,7 +84,7 @@ __device__ __forceinline__ void block_join(float &m, float &s, int &first, float
     m = sm[0], s = ss[0], first = si[0];
 #pragma unroll
     for (int w = 1; w < 4; ++w) {
-        if (rate > 0.0f)
+        if (rate.hi > 0.0f)
             join_sums(m, s, sm[w], ss[w], rate);
         else
             join_first(m, first, sm[w], si[w]);
@@ -77,13 +92,13 @@ __device__ __forceinline__ void block_join(float &m, float &s, int &first, float
 }
 
 // Two passes over a row: its parts' pairs, then all of them joined by every block, and the values. Bound by
-// memory, read twice and written once: 160 rows of 151936 (97 MB) 17.9 and 28.2 us, 53.1 in calls one behind
-// the other. One row 3.6 and 4.5 us, all latency: 38 blocks of 4096 values.
+// memory, read twice and written once: 160 rows of 151936 (97 MB) 19.8 and 29.0 us, 55.1 in calls one behind
+// the other. One row 4.2 and 5.0 us, all latency: 38 blocks of 4096 values.
 template <bool VEC>
 __global__ __launch_bounds__(kThreads) void prob_parts_kernel(const ProbArgs a) {
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     const float *x = a.x + (int64_t)row * a.x_stride;
-    const float rate = rate_of(a, row);
+    const Rate rate = rate_of(a, row);
     const int end = min(a.n, (part + 1) * a.len);
     float m = -INFINITY, s = 0.0f;
     int first = INT32_MAX;
@@ -96,14 +111,14 @@ __global__ __launch_bounds__(kThreads) void prob_parts_kernel(const ProbArgs a) 
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[k + e] = q[e];
         }
-        if (rate > 0.0f) {
+        if (rate.hi > 0.0f) {
             float mx = m, sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < kPer; ++k) mx = fmaxf(mx, v[k]);
             const float ref = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
-            for (int k = 0; k < kPer; ++k) sum += __builtin_amdgcn_exp2f((v[k] - ref) * rate);
-            s = s * __builtin_amdgcn_exp2f((m - ref) * rate) + sum;
+            for (int k = 0; k < kPer; ++k) sum += power(v[k] - ref, rate);
+            s = s * power(m - ref, rate) + sum;
             m = mx;
         } else {
 #pragma unroll
@@ -112,7 +127,7 @@ __global__ __launch_bounds__(kThreads) void prob_parts_kernel(const ProbArgs a) 
         }
     }
     block_join(m, s, first, rate);
-    if (threadIdx.x == 0) a.part[blockIdx.x] = make_float2(m, rate > 0.0f ? s : __builtin_bit_cast(float, first));
+    if (threadIdx.x == 0) a.part[blockIdx.x] = make_float2(m, rate.hi > 0.0f ? s : __builtin_bit_cast(float, first));
 }
 
 template <bool VEC>
@@ -120,12 +135,12 @@ __global__ __launch_bounds__(kThreads) void prob_write_kernel(const ProbArgs a) 
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     const float *x = a.x + (int64_t)row * a.x_stride;
     float *out = a.out + (int64_t)row * a.out_stride;
-    const float rate = rate_of(a, row);
+    const Rate rate = rate_of(a, row);
     float m = -INFINITY, s = 0.0f;
     int first = INT32_MAX;
     for (int p = threadIdx.x; p < a.parts; p += kThreads) {
         const float2 q = a.part[(int64_t)row * a.parts + p];
-        if (rate > 0.0f)
+        if (rate.hi > 0.0f)
             join_sums(m, s, q.x, q.y, rate);
         else
             join_first(m, first, q.x, __builtin_bit_cast(int, q.y));
@@ -138,10 +153,10 @@ __global__ __launch_bounds__(kThreads) void prob_write_kernel(const ProbArgs a) 
         for (int k = 0; k < kPer; k += 4) {
             const int i = i0 + k * kThreads + 4 * threadIdx.x;
             float q[4];
-            if (rate > 0.0f) {
+            if (rate.hi > 0.0f) {
                 load_row<VEC>(x, i, end, 0.0f, q);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) q[e] = __builtin_amdgcn_exp2f((q[e] - ref) * rate) * inv;
+                for (int e = 0; e < 4; ++e) q[e] = power(q[e] - ref, rate) * inv;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) q[e] = i + e == first ? 1.0f : 0.0f;
@@ -158,7 +173,8 @@ __global__ __launch_bounds__(kThreads) void prob_write_kernel(const ProbArgs a) 
 }
 
 // Parts of a row: about 2048 blocks in all. 160 rows with 512, 1024, 2048 and 4096: 50.4, 48.2, 45.9 and
-// 45.1 us in the two kernels, 40 rows 15.7, 15.8, 16.3 and 16.0; one row has 38 in any case.
+// 45.1 us in the two kernels (with exponents of one float), 40 rows 15.7, 15.8, 16.3 and 16.0; one row has
+// 38 in any case.
 void prob_cut(int64_t rows, int64_t n, int &len, int &parts) {
     const int64_t tiles = (n + kTile - 1) / kTile, per = std::max<int64_t>(1, tiles * rows / 2048);
     len = (int)(std::min(per, tiles) * kTile);
